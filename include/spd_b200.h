@@ -243,6 +243,87 @@ int spd_paged_decode_attn_noalloc(const void* q, void* k_pool, void* v_pool,
                                   const void* k_new, const void* v_new, int32_t* error_word,
                                   void* stream);
 
+/* ---- rotary positions, grouped heads, 4-bit cache ----------------------------------
+ * Operators for decoders whose attention rotates queries and keys by position and shares
+ * each key/value head between G = Hq / Hkv query heads.  No counterpart in the reference,
+ * whose models use learned positions and one key/value head per query head.
+ *
+ * 4-bit pool: uint8 [num_blocks][Hkv][page_bytes], page_bytes = spd_kv_int4_page_bytes(D,
+ * block_size).  A page holds one block's tokens of one head; with P = D / 64:
+ *   K codes  [P][block_size][32]   byte b: dimensions 2b (low 4 bits) and 2b + 1 of the plane
+ *   K params [P][block_size][2]    fp16 (scale, zero); a code c stands for c * scale + zero
+ *   V codes, V params              the same
+ * D in {64, 128, 256}; block_size in {8, 16, 32}. */
+size_t spd_kv_int4_page_bytes(int D, int block_size); /* 0: not supported */
+
+/* Rotates q and k by position and writes k and v into paged 16/32-bit pools.
+ *   q  [N][Hq][D] or NULL, k and v [N][Hkv][D]: N packed tokens, token and head strides in
+ *      elements, D contiguous (views of a packed q|k|v tensor)
+ *   q_out [N][Hq][D] contiguous; must not overlap q
+ *   cos_table, sin_table fp32 [max_pos][rot / 2]
+ *   cu_seqlens int32 [B + 1]: sequence b owns tokens [cu[b], cu[b + 1]); NULL: N == B and
+ *      token b belongs to sequence b (a decode step)
+ *   positions int32 [B]: position of each sequence's first token (< 0: sequence skipped)
+ *   With r = rot / 2 and angle i of the token's position:
+ *     y[i] = x[i] cos_i - x[j] sin_i,  y[j] = x[j] cos_i + x[i] sin_i,
+ *     j = i + r (interleaved == 0), or x[2i], x[2i + 1] (interleaved != 0);
+ *   dimensions >= rot pass through.  fp32 arithmetic, one rounding to dtype.
+ *   Tokens of skipped sequences, past cu[B], or whose position or block is out of range
+ *   (flagged in error_word) are not written; their rows of q_out are zero.
+ * Requires D % 8 == 0, rot % 16 == 0, rot <= D, 16-byte aligned pointers, strides and rows. */
+int spd_rope_kv_append(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k, int64_t k_stride_t,
+                       int64_t k_stride_h, const void* v, int64_t v_stride_t, int64_t v_stride_h, void* q_out,
+                       const float* cos_table, const float* sin_table, void* k_pool, void* v_pool,
+                       const int32_t* block_tables, const int32_t* positions, const int32_t* cu_seqlens, int N, int B,
+                       int Hq, int Hkv, int D, int rot, int interleaved, int max_pos, int block_size, int max_blocks,
+                       int num_blocks, int dtype, int32_t* error_word, void* stream);
+
+/* The same into a 4-bit pool.  Each token's 64 consecutive dimensions of a head share
+ *   scale = fp16((max - min) / 15), zero = fp16(min), saturated to the fp16 range;
+ *   code = clamp(rint((x - zero) / scale), 0, 15), 0 where scale is 0,
+ * of the fp32 rotated keys and of v.  A NaN makes its 64 values NaN. */
+int spd_rope_kv_append_int4(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k, int64_t k_stride_t,
+                            int64_t k_stride_h, const void* v, int64_t v_stride_t, int64_t v_stride_h, void* q_out,
+                            const float* cos_table, const float* sin_table, void* pool, const int32_t* block_tables,
+                            const int32_t* positions, const int32_t* cu_seqlens, int N, int B, int Hq, int Hkv, int D,
+                            int rot, int interleaved, int max_pos, int block_size, int max_blocks, int num_blocks,
+                            int dtype, int32_t* error_word, void* stream);
+
+/* Reads tokens of a 4-bit pool back as packed k and v of type dtype, [N][Hkv][D]: row
+ * cu_seqlens[b] + i is position starts[b] + i of sequence b (starts NULL: 0; < 0: a skipped
+ * sequence, whose rows are zero).  Rows past cu[B] are untouched; rows whose position or block is out of range are zero (flagged). */
+int spd_kv_gather_int4(const void* pool, const int32_t* block_tables, const int32_t* cu_seqlens, const int32_t* starts,
+                       void* k_out, void* v_out, int N, int B, int Hkv, int D, int block_size, int max_blocks,
+                       int num_blocks, int dtype, int32_t* error_word, void* stream);
+
+/* Single-token attention over a 4-bit pool with grouped heads: query head h attends key/value
+ * head h / (Hq / Hkv).
+ *   q, out [B][Hq][D]; context_lens int32 [B] tokens attended (<= 0: zeros).
+ * fp32 softmax and sums, output rounded to dtype.  The workspace follows the rules above
+ * (zero-filled once; one geometry, one stream at a time).  B <= 4096, Hq a multiple of Hkv. */
+size_t spd_paged_decode_attn_int4_workspace_size(int B, int Hq, int Hkv, int D, int block_size, int max_blocks,
+                                                 int dtype, int device);
+int spd_paged_decode_attn_int4(const void* q, const void* pool, const int32_t* block_tables,
+                               const int32_t* context_lens, void* out, int B, int Hq, int Hkv, int D, int block_size,
+                               int max_blocks, int num_blocks, float scale, int dtype, void* workspace,
+                               size_t workspace_bytes, void* stream);
+
+/* Attention of whole packed prompts on the tensor cores (dtype F16 or BF16):
+ *   q [Nq][Hq][D], k and v [Nk][Hkv][D] with token and head strides in elements, D contiguous;
+ *   out [Nq][Hq][D] contiguous.  Sequence b owns queries [cu_q[b], cu_q[b + 1]) and keys
+ *   [cu_k[b], cu_k[b + 1]); with causal != 0 its query i sees keys j <= i + Tk - Tq (the
+ *   keys of a cached prefix come first).  A query that sees no key gives zeros.  Rows of out
+ *   that belong to no sequence are untouched.
+ * fp32 scores, softmax statistics and accumulation; the weights are rounded to dtype.  Other
+ * sequences' values never reach a result, but within a sequence a non-finite v may turn
+ * earlier queries of the same 128-key step non-finite.
+ * Requires D % 8 == 0, D <= 128, scale > 0, Hq a multiple of Hkv, 16-byte aligned pointers and
+ * strides.  error_word: optional int32 device word receiving SPD_DEVERR_TIMEOUT. */
+int spd_prompt_attn(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k, int64_t k_stride_t,
+                    int64_t k_stride_h, const void* v, int64_t v_stride_t, int64_t v_stride_h, void* out,
+                    const int32_t* cu_q, const int32_t* cu_k, int Nq, int Nk, int B, int Hq, int Hkv, int D, int causal,
+                    float scale, int dtype, int32_t* error_word, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,546 @@
+// prompt_attn.cu — attention of whole packed prompts:
+//   out[i, h] = softmax_j(q[i, h] . k[j, h / G] * scale) . v[j, h / G]
+// for the queries i and keys j of each of B sequences packed along the token axis
+// (cu_q, cu_k: prefix sums of their lengths), with Hq = G * Hkv query heads.  A sequence may
+// have more keys than queries (a cached prefix); with `causal` query i sees the keys
+// j <= i + Tk - Tq, and a query that sees none gives zeros.
+//
+// Bounded by the tensor cores and, beside them, by the exponentials: a 128 x 128 score tile
+// at D = 128 is 8.4 MFLOP (about 1,020 cycles of an SM's dense 16-bit rate) and 16,384
+// exponentials (1,024 cycles of its special-function units); at D = 64 the exponentials
+// take twice the products' time.
+//
+// sm_100a design:
+// * A CTA owns two tiles of 128 query rows (A and B).  `pack` heads that share a key/value
+//   head sit in one tile (row = token * pack + head), so K and V are read once for all of
+//   them and short prompts fill the rows.
+// * Warp 0 loads Q, K and V tiles by TMA (3-D maps over [tokens][heads][D], any strides;
+//   128-byte swizzle); warp 1 issues tcgen05.mma: S = Q K^T into TMEM and O += P V with P
+//   read from TMEM (it overwrites S) and V as the MN-major operand, so nothing is transposed
+//   or written back to shared memory.
+// * Warps 4-7 and 8-11 are the softmax of tiles A and B: one row per thread, so the row
+//   maximum and sum need no shuffles.  While one tile's softmax runs, the tensor cores work on
+//   the other tile.  The running maximum is raised only when a score passes it by 8 (in
+//   log2), so O in TMEM is rescaled rarely; P is at most 2^8 and rounded to the input type
+//   (its 8 or 11 bits are what the tensor core takes), the row sum is taken in fp32 before
+//   the rounding.
+// * Rows of V past a sequence's last key are set to zero in shared memory before they are
+//   multiplied (P is zero there, but 0 * NaN is not), so what another sequence holds never
+//   reaches this one's result.
+// * Persistent: one CTA per SM walks the (tile, head) items; every wait is bounded.
+#include "spd_tc.cuh"
+
+namespace spd {
+namespace pa {
+using namespace tc;
+
+constexpr int BM = 128;  // query rows per tile (two tiles per CTA)
+constexpr int BN = 128;  // keys per step
+constexpr int kThreads = 384;
+constexpr float kLazy = 8.f;
+
+template <int DP> struct Cfg {
+  static constexpr int kBoxes = DP / 64;                  // 64-column boxes of a row
+  static constexpr int kTileBytes = 128 * DP * 2;         // one Q, K or V tile
+  static constexpr int kBoxBytes = 128 * 128;             // 128 rows of 128 bytes
+  static constexpr int kStages = DP == 128 ? 5 : 8;       // K and V tiles in flight
+  static constexpr int kBarBytes = 512;
+  static constexpr size_t kSmem = 1024 + (size_t)(2 + kStages) * kTileBytes + kBarBytes;
+  static constexpr uint32_t kTmemCols = 512;
+  static constexpr uint32_t kO = 256;                     // TMEM column of O_A; S_A at 0, S_B at 128
+};
+
+__device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+          smem_addr(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(smem_addr(bar))
+      : "memory");
+}
+
+// D[128 x N] (+)= A (TMEM, 16-bit pairs per column) * B (shared memory)
+__device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
+                                            uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// MN-major operand with 128-byte swizzle: 8 k-rows of 64 consecutive elements form a 1024-byte
+// atom; atoms follow each other along k (stride 1024) and 64-element blocks every kBoxBytes.
+__device__ __forceinline__ uint64_t smem_desc_mn(const void* tile, uint32_t block_bytes) {
+  const uint64_t addr = smem_addr(tile);
+  uint64_t d = 0;
+  d |= (addr >> 4) & 0x3FFFull;
+  d |= (uint64_t)(block_bytes >> 4) << 16;  // leading byte offset: next 64 elements
+  d |= (uint64_t)(1024 >> 4) << 32;         // stride byte offset: next 8 k-rows
+  d |= (uint64_t)1 << 46;
+  d |= (uint64_t)2 << 61;
+  return d;
+}
+
+__device__ __forceinline__ void tmem_ld32_nowait(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr)
+      : "memory");
+}
+// Waits for the loads issued so far; ties the 32 registers to the wait so that no use of them
+// is scheduled before it.
+__device__ __forceinline__ void tmem_ld_wait(uint32_t* r) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
+                 "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
+                 "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+               :
+               : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+      "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+      "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+      "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  if constexpr (std::is_same<T, __half>::value) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  } else {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+}
+
+// One unit of work: 2 x 128 query rows (tokens [tok0, tok0 + 256 / pack) of one sequence for
+// `pack` heads from h0).
+struct Item {
+  int q0, Tq, k0, Tk;  // the sequence's first query/key row and its lengths
+  int tok0;            // first token of the CTA's tiles within the sequence
+  int h0, kvh;
+  int n[2];            // key steps of tiles A and B
+};
+
+// The it-th item, found by the whole warp from the prefix sums; false past the last one.
+// Tiles of a sequence come last-first (the longest of a causal prompt first), heads fastest.
+__device__ __forceinline__ bool find_item(const PromptParams& p, int it, Item& w) {
+  const int lane = threadIdx.x & 31;
+  const int tokens = 2 * BM / p.pack, groups = p.Hq / p.pack;
+  const int tile = it / groups, grp = it % groups;
+  int before = 0, b = -1, lvl = 0;
+  for (int base = 0; base < p.B; base += 32) {
+    const int s = base + lane;
+    int q0 = 0, q1 = 0;
+    if (s < p.B) {
+      q0 = max(0, min(p.Nq, p.cu_q[s]));
+      q1 = max(q0, min(p.Nq, p.cu_q[s + 1]));
+    }
+    const int tiles = (q1 - q0 + tokens - 1) / tokens;
+    int incl = tiles;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += v;
+    }
+    const unsigned hit = __ballot_sync(0xffffffffu, tile < before + incl);
+    if (hit) {
+      const int src = __ffs(hit) - 1;
+      b = base + src;
+      const int excl = __shfl_sync(0xffffffffu, incl - tiles, src), n = __shfl_sync(0xffffffffu, tiles, src);
+      lvl = n - 1 - (tile - before - excl);
+      break;
+    }
+    before += __shfl_sync(0xffffffffu, incl, 31);
+  }
+  if (b < 0) return false;
+  w.q0 = max(0, min(p.Nq, p.cu_q[b]));
+  w.Tq = max(w.q0, min(p.Nq, p.cu_q[b + 1])) - w.q0;
+  w.k0 = max(0, min(p.Nk, p.cu_k[b]));
+  w.Tk = max(w.k0, min(p.Nk, p.cu_k[b + 1])) - w.k0;
+  w.tok0 = lvl * tokens;
+  w.h0 = grp * p.pack;
+  w.kvh = w.h0 / (p.Hq / p.Hkv);
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+    const int first = w.tok0 + x * (tokens / 2), last = min(w.Tq, first + tokens / 2) - 1;
+    int keys = 0;  // that the tile's last token sees
+    if (first < w.Tq) keys = p.causal ? min(w.Tk, last + 1 + w.Tk - w.Tq) : w.Tk;
+    w.n[x] = keys > 0 ? (keys + BN - 1) / BN : 0;
+  }
+  return true;
+}
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(kThreads, 1)
+    prompt_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+                       const __grid_constant__ CUtensorMap tm_v, const PromptParams p) {
+  using C = Cfg<DP>;
+  constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* smem = smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023);
+  unsigned char* q_tiles = smem;                        // [2]
+  unsigned char* kv_tiles = smem + 2 * C::kTileBytes;   // [kStages]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(kv_tiles + C::kStages * C::kTileBytes);
+  uint64_t* kv_full = bars;                    // [kStages]
+  uint64_t* kv_empty = kv_full + C::kStages;   // [kStages]
+  uint64_t* q_full = kv_empty + C::kStages;    // [2]
+  uint64_t* q_empty = q_full + 2;              // [2]
+  uint64_t* s_full = q_empty + 2;              // [2] scores ready (and all earlier products done)
+  uint64_t* p_full = s_full + 2;               // [2] weights written, output rescaled
+  uint64_t* o_full = p_full + 2;               // [2] output complete
+  uint64_t* o_empty = o_full + 2;              // [2] output read
+  uint64_t* done = o_empty + 2;                // every MMA has completed
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (warp == 1) tmem_alloc(tmem_slot, C::kTmemCols);
+  if (tid == 0) {
+    for (int s = 0; s < C::kStages; ++s) {
+      mbar_init(&kv_full[s], 1);
+      mbar_init(&kv_empty[s], 1);
+    }
+    for (int x = 0; x < 2; ++x) {
+      mbar_init(&q_full[x], 1);
+      mbar_init(&q_empty[x], 1);
+      mbar_init(&s_full[x], 1);
+      mbar_init(&p_full[x], 4);  // one arrival per warp
+      mbar_init(&o_full[x], 1);
+      mbar_init(&o_empty[x], 4);
+    }
+    mbar_init(done, 1);
+    fence_barrier_init();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  Item w;
+
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    if (warp == 0) {
+      // ---- TMA: Q tiles, then K and V tiles of each step, through one ring ------------------
+      const int half_tok = BM / p.pack;
+      int it = 0, s = 0, q_use[2] = {0, 0};
+      long long issued = 0;
+      bool ok = true;
+      auto load_kv = [&](const CUtensorMap* map, int kv_row) {
+        if (issued >= C::kStages)
+          ok = mbar_wait_bounded(&kv_empty[s], (uint32_t)(((issued / C::kStages) & 1) ^ 1), p.err, p.wait_ns);
+        if (!ok) return;
+        mbar_arrive_expect_tx(&kv_full[s], C::kTileBytes);
+        for (int c = 0; c < C::kBoxes; ++c)
+          tma_load_3d(kv_tiles + s * C::kTileBytes + c * C::kBoxBytes, map, 64 * c, w.kvh, kv_row, &kv_full[s]);
+        ++issued;
+        s = s + 1 == C::kStages ? 0 : s + 1;
+      };
+      for (it = blockIdx.x; ok && find_item(p, it, w); it += gridDim.x) {
+        if (lane == 0) {
+          const int n = max(w.n[0], w.n[1]);
+          auto load_q = [&](int x) {
+            if (!w.n[x] || !ok) return;
+            if (q_use[x] > 0) ok = mbar_wait_bounded(&q_empty[x], (uint32_t)((q_use[x] - 1) & 1), p.err, p.wait_ns);
+            if (!ok) return;
+            ++q_use[x];
+            mbar_arrive_expect_tx(&q_full[x], C::kTileBytes);
+            for (int c = 0; c < C::kBoxes; ++c)
+              tma_load_3d(q_tiles + x * C::kTileBytes + c * C::kBoxBytes, &tm_q, 64 * c, w.h0,
+                          w.q0 + w.tok0 + x * half_tok, &q_full[x]);
+          };
+          load_q(0);
+          for (int j = 0; j < n && ok; ++j) {
+            load_kv(&tm_k, w.k0 + j * BN);
+            if (j == 0) load_q(1);
+            if (ok) load_kv(&tm_v, w.k0 + j * BN);
+          }
+        }
+        ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
+      }
+      if (!ok && lane == 0) {  // let the copies in flight land before the CTA can exit
+        for (long long k = issued - 1; k >= 0 && k >= issued - C::kStages; --k)
+          (void)mbar_wait_bounded(&kv_full[k % C::kStages], (uint32_t)((k / C::kStages) & 1), nullptr);
+        for (int x = 0; x < 2; ++x)
+          if (q_use[x]) (void)mbar_wait_bounded(&q_full[x], (uint32_t)((q_use[x] - 1) & 1), nullptr);
+      }
+    } else if (warp == 1) {
+      // ---- MMA issuer -------------------------------------------------------------------
+      constexpr uint32_t idesc_s = instr_desc_f16(kBf16, BM, BN);
+      constexpr uint32_t idesc_o = instr_desc_f16(kBf16, BM, DP) | (1u << 16);  // B is MN-major
+      int q_use[2] = {0, 0}, p_use[2] = {0, 0}, o_use[2] = {0, 0};
+      long long got = 0;
+      bool ok = true;
+      for (int it = blockIdx.x; ok && find_item(p, it, w); it += gridDim.x) {
+        const int n = max(w.n[0], w.n[1]);
+        auto kv_wait = [&](long long k) {
+          return mbar_wait_bounded(&kv_full[k % C::kStages], (uint32_t)((k / C::kStages) & 1), p.err, p.wait_ns);
+        };
+        auto scores = [&](int x, long long kslot) {  // S_x = Q_x K^T
+          if (lane == 0) {
+            const unsigned char* kt = kv_tiles + (kslot % C::kStages) * C::kTileBytes;
+            const unsigned char* qt = q_tiles + x * C::kTileBytes;
+#pragma unroll
+            for (int c = 0; c < C::kBoxes; ++c) {
+              const uint64_t dq = smem_desc_sw128(qt + c * C::kBoxBytes), dk = smem_desc_sw128(kt + c * C::kBoxBytes);
+#pragma unroll
+              for (int k = 0; k < 4; ++k) umma_f16(tmem + x * BN, dq + 2 * k, dk + 2 * k, idesc_s, (c | k) != 0);
+            }
+            umma_commit(&s_full[x]);
+          }
+          __syncwarp();
+        };
+        // slots of this item: K_j at got + 2j, V_j at got + 2j + 1
+        for (int x = 0; x < 2 && ok; ++x) {
+          if (!w.n[x]) continue;
+          ok = mbar_wait_bounded(&q_full[x], (uint32_t)(q_use[x] & 1), p.err, p.wait_ns) && kv_wait(got);
+          ++q_use[x];
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          tc_fence_after();
+          scores(x, got);
+        }
+        if (ok && n && lane == 0) {
+          umma_commit(&kv_empty[got % C::kStages]);
+          for (int x = 0; x < 2; ++x)
+            if (w.n[x] == 1) umma_commit(&q_empty[x]);
+        }
+        for (int j = 0; j < n && ok; ++j) {
+          const long long vslot = got + 2 * j + 1, kslot = got + 2 * j + 2;
+          ok = __all_sync(0xffffffffu, kv_wait(vslot));
+          if (!ok) break;
+          unsigned char* vt = kv_tiles + (vslot % C::kStages) * C::kTileBytes;
+          const int valid = w.Tk - j * BN;
+          if (valid < BN) {  // zero the rows of V past the sequence's last key
+            for (int i = lane; i < (BN - valid) * 8; i += 32)
+              for (int c = 0; c < C::kBoxes; ++c)
+                *reinterpret_cast<uint4*>(vt + c * C::kBoxBytes + valid * 128 + i * 16) = make_uint4(0, 0, 0, 0);
+            fence_proxy_async_smem();
+            __syncwarp();
+          }
+          bool k_seen = false;
+          for (int x = 0; x < 2 && ok; ++x) {
+            if (j >= w.n[x]) continue;
+            if (j == 0 && o_use[x] > 0)
+              ok = mbar_wait_bounded(&o_empty[x], (uint32_t)((o_use[x] - 1) & 1), p.err, p.wait_ns);
+            ok = ok && mbar_wait_bounded(&p_full[x], (uint32_t)(p_use[x] & 1), p.err, p.wait_ns);
+            ++p_use[x];
+            const bool more = j + 1 < w.n[x];
+            if (more && !k_seen) {
+              ok = ok && kv_wait(kslot);
+              k_seen = true;
+            }
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            tc_fence_after();
+            if (lane == 0) {
+#pragma unroll
+              for (int k = 0; k < BN / 16; ++k)
+                umma_f16_ts(tmem + C::kO + x * DP, tmem + x * BN + 8 * k, smem_desc_mn(vt + k * 2048, C::kBoxBytes), idesc_o,
+                            (j | k) != 0);
+              if (!more) umma_commit(&o_full[x]);
+            }
+            __syncwarp();
+            if (more) {
+              scores(x, kslot);
+              if (j + 2 == w.n[x] && lane == 0) umma_commit(&q_empty[x]);
+            } else {
+              ++o_use[x];
+            }
+          }
+          if (ok && lane == 0) {
+            umma_commit(&kv_empty[vslot % C::kStages]);
+            if (j + 1 < n) umma_commit(&kv_empty[kslot % C::kStages]);
+          }
+          __syncwarp();
+        }
+        got += 2 * n;
+      }
+      if (lane == 0) {
+        umma_commit(done);
+        (void)mbar_wait_bounded(done, 0, p.err);
+      }
+      __syncwarp();
+    }
+  } else {
+    // ---- softmax and epilogue of tile x: thread = query row = TMEM lane --------------------
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+    const int x = (warp - 4) >> 2;
+    const int row = (warp & 3) * 32 + lane;
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t s_col = tmem + lanes + x * BN, o_col = tmem + lanes + C::kO + x * DP;
+    const int half_tok = BM / p.pack;
+    int s_use = 0, o_use = 0;
+    bool ok = true;
+    for (int it = blockIdx.x; ok && find_item(p, it, w); it += gridDim.x) {
+      const int tok = w.tok0 + x * half_tok + row / p.pack;  // of this row, within the sequence
+      const int first = w.tok0 + x * half_tok;
+      const int off = w.Tk - w.Tq;
+      // keys this row sees, and the fewest any row of the tile sees
+      const int limit = p.causal ? min(w.Tk, tok + 1 + off) : w.Tk;
+      const int least = p.causal ? min(w.Tk, first + 1 + off) : w.Tk;
+      float m = -INFINITY, l = 0.f;
+      const int n = w.n[x];
+      for (int j = 0; j < n; ++j) {
+        ok = __all_sync(0xffffffffu, mbar_wait_bounded(&s_full[x], (uint32_t)(s_use & 1), p.err, p.wait_ns));
+        ++s_use;
+        if (!ok) break;
+        tc_fence_after();
+        uint32_t s[BN];
+#pragma unroll
+        for (int c = 0; c < BN; c += 32) tmem_ld32_nowait(s_col + c, s + c);
+#pragma unroll
+        for (int c = 0; c < BN; c += 32) tmem_ld_wait(s + c);
+        const int base = j * BN;
+        if (base + BN > least) {
+          const int seen = limit - base;
+#pragma unroll
+          for (int c = 0; c < BN; ++c)
+            if (c >= seen) s[c] = 0xff800000u;  // -inf
+        }
+        float mx = -INFINITY;
+#pragma unroll
+        for (int c = 0; c < BN; ++c) mx = fmaxf(mx, __uint_as_float(s[c]));
+        mx *= p.scale_log2;
+        const bool raise = mx > m + kLazy;
+        if (__any_sync(0xffffffffu, raise)) {
+          const float mn = fmaxf(m, mx);
+          const float f = m == mn ? 1.f : ex2_approx(m - mn);
+          m = mn;
+          l *= f;
+          if (j > 0) {
+#pragma unroll 1
+            for (int c = 0; c < DP; c += 32) {
+              uint32_t o[32];
+              tmem_ld32_nowait(o_col + c, o);
+              tmem_ld_wait(o);
+#pragma unroll
+              for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
+              tmem_st32(o_col + c, o);
+            }
+          }
+        }
+        const float mm = m == -INFINITY ? 0.f : m;
+        float sum = 0.f;
+#pragma unroll
+        for (int c = 0; c < BN; c += 64) {
+          uint32_t pk[32];
+#pragma unroll
+          for (int k = 0; k < 32; ++k) {
+            const float a = ex2_approx(fmaf(__uint_as_float(s[c + 2 * k]), p.scale_log2, -mm));
+            const float b = ex2_approx(fmaf(__uint_as_float(s[c + 2 * k + 1]), p.scale_log2, -mm));
+            sum += a + b;
+            pk[k] = pack2<T>(a, b);
+          }
+          tmem_st32(s_col + c / 2, pk);
+        }
+        l += sum;
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[x]);
+      }
+      if (!ok) break;
+      T* out = reinterpret_cast<T*>(p.out) +
+               ((long long)(w.q0 + tok) * p.Hq + w.h0 + row % p.pack) * p.D;
+      const bool live = tok < w.Tq;
+      if (n > 0) {
+        ok = __all_sync(0xffffffffu, mbar_wait_bounded(&o_full[x], (uint32_t)(o_use & 1), p.err, p.wait_ns));
+        ++o_use;
+        if (!ok) break;
+        tc_fence_after();
+        const float r = l != 0.f ? 1.f / l : 0.f;  // a row that sees no key: zeros
+#pragma unroll
+        for (int c = 0; c < DP; c += 32) {
+          uint32_t o[32];
+          tmem_ld32_nowait(o_col + c, o);
+          tmem_ld_wait(o);
+#pragma unroll
+          for (int k = 0; k < 32; k += 8)
+            if (live && c + k < p.D) {
+              uint4 v;
+              v.x = pack2<T>(__uint_as_float(o[k]) * r, __uint_as_float(o[k + 1]) * r);
+              v.y = pack2<T>(__uint_as_float(o[k + 2]) * r, __uint_as_float(o[k + 3]) * r);
+              v.z = pack2<T>(__uint_as_float(o[k + 4]) * r, __uint_as_float(o[k + 5]) * r);
+              v.w = pack2<T>(__uint_as_float(o[k + 6]) * r, __uint_as_float(o[k + 7]) * r);
+              *reinterpret_cast<uint4*>(out + c + k) = v;
+            }
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&o_empty[x]);
+      } else if (live) {
+        for (int c = 0; c < p.D; c += 8) *reinterpret_cast<uint4*>(out + c) = make_uint4(0, 0, 0, 0);
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 1) tmem_dealloc(tmem, C::kTmemCols);
+}
+
+// [tokens][heads][D] of 16-bit elements with any token and head strides, box [rows][heads][64].
+static bool make_map3(CUtensorMap* map, const void* base, int D, int heads, int tokens, long long sh, long long st,
+                      int box_heads, int box_tokens, bool bf16) {
+  auto enc = encode_fn();
+  if (!enc) return false;
+  cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)heads, (cuuint64_t)tokens};
+  cuuint64_t strides[2] = {(cuuint64_t)sh * 2, (cuuint64_t)st * 2};
+  cuuint32_t box[3] = {64, (cuuint32_t)box_heads, (cuuint32_t)box_tokens};
+  cuuint32_t estr[3] = {1, 1, 1};
+  return enc(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(base),
+             dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+}  // namespace pa
+
+int prompt_attn_launch(PromptParams p, const void* q, const void* k, const void* v, long long q_st, long long q_sh,
+                       long long k_st, long long k_sh, long long v_st, long long v_sh, int dtype, int sms,
+                       cudaStream_t st) {
+  using namespace pa;
+  const bool bf16 = dtype == SPD_BF16;
+  if (p.Nk == 0)  // no key anywhere: every row is empty
+    return cudaMemsetAsync(p.out, 0, (size_t)p.Nq * p.Hq * p.D * 2, st) == cudaSuccess ? SPD_OK : SPD_ERR_CUDA;
+  // heads of one group in a tile: the largest power of two that divides G (up to 128)
+  const int G = p.Hq / p.Hkv;
+  p.pack = G & -G;
+  if (p.pack > BM) p.pack = BM;
+  CUtensorMap tq, tk, tv;
+  if (!make_map3(&tq, q, p.D, p.Hq, p.Nq, q_sh, q_st, p.pack, BM / p.pack, bf16) ||
+      !make_map3(&tk, k, p.D, p.Hkv, p.Nk, k_sh, k_st, 1, BN, bf16) ||
+      !make_map3(&tv, v, p.D, p.Hkv, p.Nk, v_sh, v_st, 1, BN, bf16))
+    return SPD_ERR_CUDA;
+  const int tokens = 2 * BM / p.pack;
+  const long long most = ((long long)p.Nq / tokens + p.B) * (p.Hq / p.pack);  // items at most
+  const dim3 grid((unsigned)(most < sms ? most : sms));
+  auto launch = [&](auto kfn, size_t smem) -> int {
+    if (cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
+      return SPD_ERR_CUDA;
+    kfn<<<grid, kThreads, smem, st>>>(tq, tk, tv, p);
+    return cudaPeekAtLastError() == cudaSuccess ? SPD_OK : SPD_ERR_CUDA;
+  };
+  auto by_d = [&](auto tag) -> int {
+    using T = decltype(tag);
+    return p.D <= 64 ? launch(prompt_attn_kernel<T, 64>, Cfg<64>::kSmem) : launch(prompt_attn_kernel<T, 128>, Cfg<128>::kSmem);
+  };
+  return bf16 ? by_d(__nv_bfloat16{}) : by_d(__half{});
+}
+
+}  // namespace spd

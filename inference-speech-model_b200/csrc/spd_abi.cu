@@ -9,6 +9,7 @@
 #include <cstring>
 #include <mutex>
 
+#include "spd_int4.cuh"
 #include "spd_params.cuh"
 
 namespace spd {
@@ -24,6 +25,13 @@ int linear_small_m_launch(const void* x, const void* w, const void* bias, void* 
 int cross_kv_project_launch(const void* enc_out, const void* w_kv, const void* b_kv, void* out,
                             const int32_t* slot_ids, int B, int T, int d_model, int L, int H, int D,
                             int T_out, int64_t out_slot_stride, int dtype, int* err, int sms, cudaStream_t st);
+int rope_append_launch(const RopeAppendParams& p, int dtype, bool int4_pool, cudaStream_t st);
+int gather_int4_launch(const GatherInt4Params& p, int dtype, cudaStream_t st);
+int decode_int4_chunk(int B, int Hq, int Hkv, int dtype, int max_ctx, int sms);
+int decode_int4_launch(const DecodeInt4Params& p, int D, int bs, cudaStream_t st);
+int prompt_attn_launch(PromptParams p, const void* q, const void* k, const void* v, long long q_st, long long q_sh,
+                       long long k_st, long long k_sh, long long v_st, long long v_sh, int dtype, int sms,
+                       cudaStream_t st);
 }  // namespace spd
 
 namespace {
@@ -75,6 +83,29 @@ int sm_count(int device) {
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+bool int4_shape_ok(int D, int block_size) {
+  return (D == 64 || D == 128 || D == 256) && (block_size == 8 || block_size == 16 || block_size == 32);
+}
+
+// The shared checks of the two rotating appends; `p` is filled but for the pools.
+int rope_append_check(const char* fn, const spd::RopeAppendParams& p, int dtype) {
+  const int eb = elem_bytes(dtype);
+  if (!eb) return fail(SPD_ERR_UNSUPPORTED, "%s: dtype %d not supported", fn, dtype);
+  if (!p.k || !p.v || !p.cos || !p.sin || !p.k_pool || !p.block_tables || !p.positions || (p.q && !p.q_out))
+    return fail(SPD_ERR_INVALID_ARG, "%s: null tensor pointer", fn);
+  if (p.N < 0 || p.B < 0 || p.Hkv <= 0 || (p.q && p.Hq <= 0) || p.D <= 0 || p.max_pos <= 0 || p.block_size <= 0 ||
+      p.max_blocks <= 0 || p.num_blocks <= 0 || (!p.cu_seqlens && p.N != p.B))
+    return fail(SPD_ERR_INVALID_ARG, "%s: bad sizes N=%d B=%d Hq=%d Hkv=%d D=%d", fn, p.N, p.B, p.Hq, p.Hkv, p.D);
+  if (p.D % 8 || p.rot <= 0 || p.rot % 16 || p.rot > p.D)
+    return fail(SPD_ERR_UNSUPPORTED, "%s: need D %% 8 == 0 and a rotated part that is a multiple of 16 up to D", fn);
+  for (long long s : {p.k_st, p.k_sh, p.v_st, p.v_sh, p.q ? p.q_st : 0ll, p.q ? p.q_sh : 0ll})
+    if ((s * eb) % 16) return fail(SPD_ERR_INVALID_ARG, "%s: strides must be multiples of 16 bytes", fn);
+  for (const void* t : {p.q, p.k, p.v, (const void*)p.q_out, (const void*)p.cos, (const void*)p.sin,
+                        (const void*)p.k_pool, (const void*)p.v_pool})
+    if (!aligned16(t)) return fail(SPD_ERR_INVALID_ARG, "%s: tensors must be 16-byte aligned", fn);
+  return SPD_OK;
+}
 
 bool head_dim_ok(int D) { return D == 16 || D == 32 || D == 64 || D == 128; }
 
@@ -383,6 +414,151 @@ int spd_cross_kv_project(const void* enc_out, const void* w_kv, const void* b_kv
                                               static_cast<cudaStream_t>(stream));
   if (rc == SPD_ERR_UNSUPPORTED) return fail(rc, "spd_cross_kv_project: shape not supported");
   if (rc != SPD_OK) return fail(rc, "spd_cross_kv_project: launch failed: %s", cudaGetErrorString(cudaGetLastError()));
+  return ok();
+}
+
+size_t spd_kv_int4_page_bytes(int D, int block_size) {
+  return int4_shape_ok(D, block_size) ? (size_t)spd::int4::page_bytes(D / spd::int4::kPlane, block_size) : 0;
+}
+
+int spd_rope_kv_append(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k, int64_t k_stride_t,
+                       int64_t k_stride_h, const void* v, int64_t v_stride_t, int64_t v_stride_h, void* q_out,
+                       const float* cos_table, const float* sin_table, void* k_pool, void* v_pool,
+                       const int32_t* block_tables, const int32_t* positions, const int32_t* cu_seqlens, int N, int B,
+                       int Hq, int Hkv, int D, int rot, int interleaved, int max_pos, int block_size, int max_blocks,
+                       int num_blocks, int dtype, int32_t* error_word, void* stream) {
+  const spd::RopeAppendParams p{q, k, v, q_stride_t, q_stride_h, k_stride_t, k_stride_h, v_stride_t, v_stride_h, q_out,
+                                cos_table, sin_table, k_pool, v_pool, block_tables, positions, cu_seqlens, N, B, Hq, Hkv,
+                                D, rot, interleaved, max_pos, block_size, max_blocks, num_blocks, error_word};
+  const int rc0 = rope_append_check("spd_rope_kv_append", p, dtype);
+  if (rc0 != SPD_OK) return rc0;
+  if (!v_pool) return fail(SPD_ERR_INVALID_ARG, "spd_rope_kv_append: null tensor pointer");
+  if (N == 0) return ok();
+  const int rc = spd::rope_append_launch(p, dtype, false, static_cast<cudaStream_t>(stream));
+  if (rc != SPD_OK) return fail(rc, "spd_rope_kv_append: launch failed: %s", cudaGetErrorString(cudaGetLastError()));
+  return ok();
+}
+
+int spd_rope_kv_append_int4(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k, int64_t k_stride_t,
+                            int64_t k_stride_h, const void* v, int64_t v_stride_t, int64_t v_stride_h, void* q_out,
+                            const float* cos_table, const float* sin_table, void* pool, const int32_t* block_tables,
+                            const int32_t* positions, const int32_t* cu_seqlens, int N, int B, int Hq, int Hkv, int D,
+                            int rot, int interleaved, int max_pos, int block_size, int max_blocks, int num_blocks,
+                            int dtype, int32_t* error_word, void* stream) {
+  const spd::RopeAppendParams p{q, k, v, q_stride_t, q_stride_h, k_stride_t, k_stride_h, v_stride_t, v_stride_h, q_out,
+                                cos_table, sin_table, pool, nullptr, block_tables, positions, cu_seqlens, N, B, Hq, Hkv,
+                                D, rot, interleaved, max_pos, block_size, max_blocks, num_blocks, error_word};
+  const int rc0 = rope_append_check("spd_rope_kv_append_int4", p, dtype);
+  if (rc0 != SPD_OK) return rc0;
+  if (!int4_shape_ok(D, block_size))
+    return fail(SPD_ERR_UNSUPPORTED, "spd_rope_kv_append_int4: head_dim %d / block_size %d not supported", D, block_size);
+  if (N == 0) return ok();
+  const int rc = spd::rope_append_launch(p, dtype, true, static_cast<cudaStream_t>(stream));
+  if (rc != SPD_OK)
+    return fail(rc, "spd_rope_kv_append_int4: launch failed: %s", cudaGetErrorString(cudaGetLastError()));
+  return ok();
+}
+
+int spd_kv_gather_int4(const void* pool, const int32_t* block_tables, const int32_t* cu_seqlens, const int32_t* starts,
+                       void* k_out, void* v_out, int N, int B, int Hkv, int D, int block_size, int max_blocks,
+                       int num_blocks, int dtype, int32_t* error_word, void* stream) {
+  if (!elem_bytes(dtype)) return fail(SPD_ERR_UNSUPPORTED, "spd_kv_gather_int4: dtype %d not supported", dtype);
+  if (!int4_shape_ok(D, block_size))
+    return fail(SPD_ERR_UNSUPPORTED, "spd_kv_gather_int4: head_dim %d / block_size %d not supported", D, block_size);
+  if (!pool || !block_tables || !cu_seqlens || !k_out || !v_out)
+    return fail(SPD_ERR_INVALID_ARG, "spd_kv_gather_int4: null tensor pointer");
+  if (N < 0 || B <= 0 || Hkv <= 0 || max_blocks <= 0 || num_blocks <= 0)
+    return fail(SPD_ERR_INVALID_ARG, "spd_kv_gather_int4: bad sizes");
+  if (!aligned16(pool) || !aligned16(k_out) || !aligned16(v_out))
+    return fail(SPD_ERR_INVALID_ARG, "spd_kv_gather_int4: tensors must be 16-byte aligned");
+  if (N == 0) return ok();
+  const spd::GatherInt4Params p{static_cast<const unsigned char*>(pool), block_tables, cu_seqlens, starts, k_out, v_out, N,
+                                B, Hkv, D, block_size, max_blocks, num_blocks, error_word};
+  const int rc = spd::gather_int4_launch(p, dtype, static_cast<cudaStream_t>(stream));
+  if (rc != SPD_OK) return fail(rc, "spd_kv_gather_int4: launch failed: %s", cudaGetErrorString(cudaGetLastError()));
+  return ok();
+}
+
+size_t spd_paged_decode_attn_int4_workspace_size(int B, int Hq, int Hkv, int D, int block_size, int max_blocks,
+                                                 int dtype, int device) {
+  const int sms = sm_count(device);
+  const long long max_ctx = (long long)max_blocks * block_size;
+  if (B <= 0 || Hkv <= 0 || Hq <= 0 || Hq % Hkv || !int4_shape_ok(D, block_size) || max_blocks <= 0 ||
+      max_ctx > INT32_MAX || sms <= 0)
+    return 0;
+  const int chunk = spd::decode_int4_chunk(B, Hq, Hkv, dtype, (int)max_ctx, sms);
+  const size_t splits = (size_t)((max_ctx + chunk - 1) / chunk);
+  return spd::kWsHeaderBytes + spd::round_up((size_t)B * Hq * 4, 256) +
+         spd::round_up((size_t)B * Hq * splits * (D + 4) * 4, 256);
+}
+
+int spd_paged_decode_attn_int4(const void* q, const void* pool, const int32_t* block_tables,
+                               const int32_t* context_lens, void* out, int B, int Hq, int Hkv, int D, int block_size,
+                               int max_blocks, int num_blocks, float scale, int dtype, void* workspace,
+                               size_t workspace_bytes, void* stream) {
+  if (!elem_bytes(dtype)) return fail(SPD_ERR_UNSUPPORTED, "spd_paged_decode_attn_int4: dtype %d not supported", dtype);
+  if (!q || !pool || !block_tables || !context_lens || !out)
+    return fail(SPD_ERR_INVALID_ARG, "spd_paged_decode_attn_int4: null tensor pointer");
+  if (!int4_shape_ok(D, block_size))
+    return fail(SPD_ERR_UNSUPPORTED, "spd_paged_decode_attn_int4: head_dim %d / block_size %d not supported", D,
+                block_size);
+  const long long max_ctx = (long long)max_blocks * block_size;
+  if (B <= 0 || B > 4096 || Hkv <= 0 || Hq <= 0 || Hq % Hkv || Hq > 4096 || max_blocks <= 0 || num_blocks <= 0 ||
+      max_ctx > INT32_MAX)
+    return fail(SPD_ERR_INVALID_ARG, "spd_paged_decode_attn_int4: bad sizes B=%d Hq=%d Hkv=%d max_blocks=%d", B, Hq, Hkv,
+                max_blocks);
+  if (!aligned16(q) || !aligned16(pool) || !aligned16(out))
+    return fail(SPD_ERR_INVALID_ARG, "spd_paged_decode_attn_int4: tensors must be 16-byte aligned");
+  const size_t need = spd_paged_decode_attn_int4_workspace_size(B, Hq, Hkv, D, block_size, max_blocks, dtype, -1);
+  if (!workspace || workspace_bytes < need || need == 0)
+    return fail(SPD_ERR_WORKSPACE, "spd_paged_decode_attn_int4: workspace %zu bytes, need %zu", workspace_bytes, need);
+  spd::DecodeInt4Params p{};
+  p.q = q; p.pool = static_cast<const unsigned char*>(pool); p.block_tables = block_tables;
+  p.context_lens = context_lens; p.out = out; p.dtype = dtype;
+  p.B = B; p.Hq = Hq; p.Hkv = Hkv; p.max_blocks = max_blocks; p.num_blocks = num_blocks;
+  p.chunk = spd::decode_int4_chunk(B, Hq, Hkv, dtype, (int)max_ctx, sm_count(-1));
+  p.splits = (int)((max_ctx + p.chunk - 1) / p.chunk);
+  p.scale_log2 = scale * 1.4426950408889634f;
+  p.wait_ns = g_wait_ns;
+  unsigned char* ws = static_cast<unsigned char*>(workspace);
+  p.err = reinterpret_cast<int*>(ws);
+  p.counters = reinterpret_cast<int*>(ws + spd::kWsHeaderBytes);
+  p.partials = reinterpret_cast<float*>(ws + spd::kWsHeaderBytes + spd::round_up((size_t)B * Hq * 4, 256));
+  const int rc = spd::decode_int4_launch(p, D, block_size, static_cast<cudaStream_t>(stream));
+  if (rc != SPD_OK)
+    return fail(rc, "spd_paged_decode_attn_int4: launch failed: %s", cudaGetErrorString(cudaGetLastError()));
+  return ok();
+}
+
+int spd_prompt_attn(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k, int64_t k_stride_t,
+                    int64_t k_stride_h, const void* v, int64_t v_stride_t, int64_t v_stride_h, void* out,
+                    const int32_t* cu_q, const int32_t* cu_k, int Nq, int Nk, int B, int Hq, int Hkv, int D, int causal,
+                    float scale, int dtype, int32_t* error_word, void* stream) {
+  if (dtype != SPD_F16 && dtype != SPD_BF16)
+    return fail(SPD_ERR_UNSUPPORTED, "spd_prompt_attn: dtype %d not supported (F16/BF16 only)", dtype);
+  if (Nq < 0 || Nk < 0 || B < 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || D <= 0)
+    return fail(SPD_ERR_INVALID_ARG, "spd_prompt_attn: bad sizes Nq=%d Nk=%d B=%d Hq=%d Hkv=%d D=%d", Nq, Nk, B, Hq, Hkv, D);
+  if (D % 8 || D > 128) return fail(SPD_ERR_UNSUPPORTED, "spd_prompt_attn: head_dim %d not supported", D);
+  if (!(scale > 0.f) || scale > 1e30f) return fail(SPD_ERR_INVALID_ARG, "spd_prompt_attn: scale must be positive");
+  if (Nq == 0 || B == 0) return ok();
+  if (!q || !out || !cu_q || !cu_k || (Nk && (!k || !v)))
+    return fail(SPD_ERR_INVALID_ARG, "spd_prompt_attn: null tensor pointer");
+  for (long long s : {(long long)q_stride_t, (long long)q_stride_h, (long long)k_stride_t, (long long)k_stride_h,
+                      (long long)v_stride_t, (long long)v_stride_h})
+    if (s < 0 || (s * 2) % 16) return fail(SPD_ERR_INVALID_ARG, "spd_prompt_attn: strides must be multiples of 16 bytes");
+  if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out))
+    return fail(SPD_ERR_INVALID_ARG, "spd_prompt_attn: tensors must be 16-byte aligned");
+  const int sms = sm_count(-1);
+  if (sms <= 0) return fail(SPD_ERR_CUDA, "spd_prompt_attn: no CUDA device");
+  spd::PromptParams p{};
+  p.out = out; p.cu_q = cu_q; p.cu_k = cu_k;
+  p.Nq = Nq; p.Nk = Nk; p.B = B; p.Hq = Hq; p.Hkv = Hkv; p.D = D; p.causal = causal != 0;
+  p.scale_log2 = scale * 1.4426950408889634f;
+  p.err = error_word;
+  p.wait_ns = g_wait_ns;
+  const int rc = spd::prompt_attn_launch(p, q, k, v, q_stride_t, q_stride_h, k_stride_t, k_stride_h, v_stride_t,
+                                         v_stride_h, dtype, sms, static_cast<cudaStream_t>(stream));
+  if (rc != SPD_OK) return fail(rc, "spd_prompt_attn: launch failed: %s", cudaGetErrorString(cudaGetLastError()));
   return ok();
 }
 

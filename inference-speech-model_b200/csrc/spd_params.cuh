@@ -86,4 +86,61 @@ struct GatherParams {
   int* err;
 };
 
+struct RopeAppendParams {  // rotation + K/V append (rope_kv_ops.cu)
+  const void* q;  // or null
+  const void* k;
+  const void* v;
+  long long q_st, q_sh, k_st, k_sh, v_st, v_sh;  // token and head strides (elements)
+  void* q_out;                                   // [N][Hq][D]
+  const float* cos;                              // [max_pos][rot / 2]
+  const float* sin;
+  void* k_pool;  // 16/32-bit pools, or the 4-bit pool with v_pool null
+  void* v_pool;
+  const int* block_tables;
+  const int* positions;   // [B]
+  const int* cu_seqlens;  // [B + 1] or null: token i belongs to sequence i
+  int N, B, Hq, Hkv, D, rot, interleaved, max_pos;
+  int block_size, max_blocks, num_blocks;
+  int* err;
+};
+
+struct GatherInt4Params {  // tokens of a 4-bit pool back as packed k, v (rope_kv_ops.cu)
+  const unsigned char* pool;
+  const int* block_tables;
+  const int* cu_seqlens;  // [B + 1]
+  const int* starts;      // [B] or null: 0
+  void* k_out;            // [N][Hkv][D]
+  void* v_out;
+  int N, B, Hkv, D, block_size, max_blocks, num_blocks;
+  int* err;
+};
+
+struct PromptParams {  // attention of packed prompts (prompt_attn.cu)
+  void* out;          // [Nq][Hq][D]
+  const int* cu_q;    // [B + 1]
+  const int* cu_k;    // [B + 1]
+  int Nq, Nk, B, Hq, Hkv, D, causal;
+  int pack;           // query heads of one key/value head that share a tile (a power of two)
+  float scale_log2;   // scale * log2(e)
+  int* err;
+  unsigned long long wait_ns;
+};
+
+struct DecodeInt4Params {  // single-token attention over a 4-bit pool (paged_decode_attn_int4.cu)
+  const void* q;
+  const unsigned char* pool;
+  const int* block_tables;
+  const int* context_lens;
+  void* out;
+  int dtype;
+  int B, Hq, Hkv, max_blocks, num_blocks;
+  int chunk;          // tokens per CTA
+  int splits;         // CTAs per (sequence, key/value head, head tile)
+  float scale_log2;   // scale * log2(e)
+  int* err;           // workspace error word
+  int* counters;      // [B * Hkv * head tiles] arrivals, left at zero
+  float* partials;    // [B * Hq][splits][D + 2]
+  unsigned long long wait_ns;
+};
+
 }  // namespace spd

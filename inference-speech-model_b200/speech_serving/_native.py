@@ -54,6 +54,16 @@ _SIGNATURES = {
     "spd_selftest_wait_timeout": (_i, [_vp, C.c_uint64, _vp]),
     "spd_paged_decode_attn_noalloc": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _f, _i, _vp, _vp,
                                            _vp, _vp]),
+    "spd_kv_int4_page_bytes": (_sz, [_i, _i]),
+    "spd_rope_kv_append": (_i, [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
+                                _vp] + [_i] * 12 + [_vp, _vp]),
+    "spd_rope_kv_append_int4": (_i, [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp,
+                                     _vp] + [_i] * 12 + [_vp, _vp]),
+    "spd_kv_gather_int4": (_i, [_vp] * 6 + [_i] * 8 + [_vp, _vp]),
+    "spd_paged_decode_attn_int4_workspace_size": (_sz, [_i] * 8),
+    "spd_paged_decode_attn_int4": (_i, [_vp] * 5 + [_i] * 7 + [_f, _i, _vp, _sz, _vp]),
+    "spd_prompt_attn": (_i, [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _vp] + [_i] * 7
+                        + [_f, _i, _vp, _vp]),
 }
 
 _lib = None

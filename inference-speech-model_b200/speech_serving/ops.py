@@ -1,4 +1,4 @@
-"""Torch-tensor front end of the five decode-path kernels (C ABI in include/spd_b200.h).
+"""Torch-tensor front end of the decode-path kernels (C ABI in include/spd_b200.h).
 
 Each function checks shapes, dtypes, devices and strides, then calls the extension
 through ctypes on ``torch.cuda.current_stream()`` (the capture stream inside
@@ -17,6 +17,13 @@ Ops and the reference code they replace:
   cross_kv_project        speech_serving/models.py:554-561
   linear                  the decode step's Linear layers (speech_serving/models.py:127-129,
                           :159, :178-180, :202, :205-207, :487)
+
+Ops without a counterpart in the reference, for decoders with rotary positions, grouped
+key/value heads and a 4-bit cache:
+  rope_kv_append, rope_kv_append_int4   rotate q and k, write k and v into a paged pool
+  kv_gather_int4                        cached tokens of a 4-bit pool as packed k and v
+  paged_decode_attention_int4           single-token attention over a 4-bit pool
+  prompt_attention                      attention of whole packed prompts
 """
 from __future__ import annotations
 
@@ -93,6 +100,16 @@ def _cached_workspace(kind: str, B: int, H: int, D: int, device: torch.device, m
               else cross_attn_workspace(B, H, D, device))
         _WORKSPACES[key] = ws
     return ws
+
+
+def decode_int4_workspace(B: int, Hq: int, Hkv: int, D: int, block_size: int, max_blocks: int, dtype: torch.dtype,
+                          device: torch.device) -> torch.Tensor:
+    """Zero-filled workspace for ``paged_decode_attention_int4`` (reusable on one stream)."""
+    idx = device.index if device.index is not None else torch.cuda.current_device()
+    n = N.load().spd_paged_decode_attn_int4_workspace_size(B, Hq, Hkv, D, block_size, max_blocks, dtype_code(dtype), idx)
+    if n == 0:
+        raise RuntimeError(f"decode_int4_workspace: unsupported geometry Hq={Hq} Hkv={Hkv} D={D} block_size={block_size}")
+    return torch.zeros(n, dtype=torch.uint8, device=device)
 
 
 def read_error_word(buf: torch.Tensor) -> int:
@@ -413,4 +430,286 @@ def argmax_rows(x: torch.Tensor, cols: Optional[int] = None, skip: Optional[torc
     rc = N.load().spd_argmax_rows(x.data_ptr(), rows, cols, ld, _ptr(skip), out.data_ptr(), dtype_code(x.dtype),
                                   _stream_handle())
     N.check(rc, "spd_argmax_rows")
+    return out
+
+
+# ----------------------------------------------------------------------------- rotary positions, 4-bit cache
+def kv_pool_int4(num_blocks: int, num_kv_heads: int, head_dim: int, block_size: int, device="cuda") -> torch.Tensor:
+    """A zero-filled 4-bit K/V pool, uint8 [num_blocks, num_kv_heads, page bytes]: one layer's
+    keys and values with a scale and a zero per token, head and 64 dimensions (4.5 bits a
+    value; page format in include/spd_b200.h).  head_dim 64, 128 or 256; block_size 8, 16
+    or 32."""
+    page = N.load().spd_kv_int4_page_bytes(head_dim, block_size)
+    if page == 0:
+        raise RuntimeError(f"kv_pool_int4: head_dim {head_dim} / block_size {block_size} not supported")
+    return torch.zeros((num_blocks, num_kv_heads, page), dtype=torch.uint8, device=device)
+
+
+def _int4_block_size(name: str, pool: torch.Tensor, Hkv: int, D: int) -> int:
+    if pool.dtype != torch.uint8 or pool.dim() != 3 or pool.shape[1] != Hkv or not pool.is_contiguous():
+        raise RuntimeError(f"{name}: pool must be a contiguous uint8 [num_blocks, {Hkv}, page bytes] tensor")
+    for bs in (8, 16, 32):
+        if N.load().spd_kv_int4_page_bytes(D, bs) == pool.shape[2]:
+            return bs
+    raise RuntimeError(f"{name}: pages of {pool.shape[2]} bytes fit no block size at head_dim {D}")
+
+
+def _tables(name: str, block_tables: torch.Tensor, B: int) -> int:
+    if block_tables.dim() != 2 or block_tables.shape[0] != B or block_tables.dtype != torch.int32 \
+            or not block_tables.is_contiguous():
+        raise RuntimeError(f"{name}: block_tables must be contiguous int32 [B, max_blocks]")
+    return block_tables.shape[1]
+
+
+def _int32_vector(name: str, what: str, t: torch.Tensor, n: int) -> None:
+    if t.dtype != torch.int32 or t.shape != (n,) or not t.is_contiguous():
+        raise RuntimeError(f"{name}: {what} must be a contiguous int32 [{n}] tensor")
+
+
+def _token_strides(name: str, what: str, t: torch.Tensor) -> Tuple[int, int]:
+    """Token and head strides of [N, H, D] with contiguous D; those of a dimension of one
+    entry, which nothing steps over, are taken as dense."""
+    n, H, D = t.shape
+    if t.stride(2) != 1 and D > 1:
+        raise RuntimeError(f"{name}: {what} needs a contiguous last dimension")
+    sh = t.stride(1) if H > 1 else D
+    return (t.stride(0) if n > 1 else sh * H), sh
+
+
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    def span(t):
+        last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
+        return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+    (a0, a1), (b0, b1) = span(a), span(b)
+    return a.numel() > 0 and b.numel() > 0 and a0 < b1 and b0 < a1
+
+
+def _rope_append(name, q, k, v, cos, sin, pools, block_tables, positions, cu_seqlens, interleaved, q_out, error_word,
+                 block_size, num_blocks):
+    dev = k.device
+    n, Hkv, D = k.shape
+    B = positions.shape[0] if positions.dim() == 1 else -1
+    _int32_vector(name, "positions", positions, B)
+    max_blocks = _tables(name, block_tables, B)
+    if cu_seqlens is None:
+        if n != B:
+            raise RuntimeError(f"{name}: without cu_seqlens one token per sequence is expected ({n} tokens, {B} sequences)")
+    else:
+        _int32_vector(name, "cu_seqlens", cu_seqlens, B + 1)
+    if cos.dtype != torch.float32 or cos.dim() != 2 or not cos.is_contiguous() or sin.shape != cos.shape \
+            or sin.dtype != cos.dtype or not sin.is_contiguous():
+        raise RuntimeError(f"{name}: cos and sin must be contiguous float32 [positions, rotated / 2] tables")
+    k_st, k_sh = _token_strides(name, "k", k)
+    v_st, v_sh = _token_strides(name, "v", v)
+    q_st = q_sh = Hq = 0
+    if q is not None:
+        if q.dim() != 3 or q.shape[0] != n or q.shape[2] != D or q.dtype != k.dtype:
+            raise RuntimeError(f"{name}: q {tuple(q.shape)} does not match k {tuple(k.shape)}")
+        Hq = q.shape[1]
+        q_st, q_sh = _token_strides(name, "q", q)
+        if q_out is None:
+            q_out = torch.empty((n, Hq, D), dtype=q.dtype, device=dev)
+        elif q_out.shape != q.shape or q_out.dtype != q.dtype or not q_out.is_contiguous() or _overlap(q, q_out):
+            raise RuntimeError(f"{name}: q_out must be a contiguous {tuple(q.shape)} tensor of q's dtype apart from q")
+    elif q_out is not None:
+        raise RuntimeError(f"{name}: q_out without q")
+    if error_word is not None and (error_word.dtype != torch.int32 or error_word.numel() < 1):
+        raise RuntimeError(f"{name}: error_word must be an int32 tensor")
+    rc = getattr(N.load(), "spd_" + name)(
+        _ptr(q), q_st, q_sh, k.data_ptr(), k_st, k_sh, v.data_ptr(), v_st, v_sh, _ptr(q_out), cos.data_ptr(),
+        sin.data_ptr(), *(t.data_ptr() for t in pools), block_tables.data_ptr(), positions.data_ptr(), _ptr(cu_seqlens),
+        n, B, Hq, Hkv, D, 2 * cos.shape[1], int(bool(interleaved)), cos.shape[0], block_size, max_blocks, num_blocks,
+        dtype_code(k.dtype), _ptr(error_word), _stream_handle())
+    N.check(rc, "spd_" + name)
+    return q_out
+
+
+def rope_kv_append(
+    q: Optional[torch.Tensor],
+    k: torch.Tensor,
+    v: torch.Tensor,
+    cos: torch.Tensor,
+    sin: torch.Tensor,
+    k_pool: torch.Tensor,
+    v_pool: torch.Tensor,
+    block_tables: torch.Tensor,
+    positions: torch.Tensor,
+    cu_seqlens: Optional[torch.Tensor] = None,
+    interleaved: bool = False,
+    q_out: Optional[torch.Tensor] = None,
+    error_word: Optional[torch.Tensor] = None,
+) -> Optional[torch.Tensor]:
+    """Rotates q and k by position and writes k and v into the paged pools; returns rotated q.
+
+    q [N, Hq, D] (or None), k and v [N, Hkv, D]: N packed tokens, any token and head strides
+    (views of a packed q|k|v projection), D contiguous; pools [num_blocks, block_size, Hkv, D].
+    cos, sin fp32 [max positions, rotated / 2]: the first ``rotated`` dimensions of a head turn,
+    as halves (i with i + rotated/2) or, ``interleaved``, as neighbours (2i with 2i + 1).
+    positions int32 [B]: position of each sequence's first token here (< 0 skips it);
+    cu_seqlens int32 [B + 1]: its tokens are [cu[b], cu[b + 1]), or None for one token per
+    sequence (a decode step).  Rows of q for tokens that are not written come back as zeros."""
+    name = "rope_kv_append"
+    _require_cuda(name, q, k, v, cos, sin, k_pool, v_pool, block_tables, positions, cu_seqlens, q_out, error_word)
+    if k.dim() != 3 or v.shape != k.shape or v.dtype != k.dtype:
+        raise RuntimeError(f"{name}: k and v must be [N, Hkv, D] of one shape and dtype")
+    for t in (k_pool, v_pool):
+        if t.dim() != 4 or t.shape[2:] != k.shape[1:] or t.shape != k_pool.shape or t.dtype != k.dtype \
+                or not t.is_contiguous():
+            raise RuntimeError(f"{name}: pools must be contiguous [num_blocks, block_size, Hkv, D] of k's dtype")
+    return _rope_append(name, q, k, v, cos, sin, (k_pool, v_pool), block_tables, positions, cu_seqlens, interleaved,
+                        q_out, error_word, k_pool.shape[1], k_pool.shape[0])
+
+
+def rope_kv_append_int4(
+    q: Optional[torch.Tensor],
+    k: torch.Tensor,
+    v: torch.Tensor,
+    cos: torch.Tensor,
+    sin: torch.Tensor,
+    pool: torch.Tensor,
+    block_tables: torch.Tensor,
+    positions: torch.Tensor,
+    cu_seqlens: Optional[torch.Tensor] = None,
+    interleaved: bool = False,
+    q_out: Optional[torch.Tensor] = None,
+    error_word: Optional[torch.Tensor] = None,
+) -> Optional[torch.Tensor]:
+    """``rope_kv_append`` into a 4-bit pool (``kv_pool_int4``): the rotated keys (in fp32) and
+    the values are quantised per token, head and 64 dimensions as they are written."""
+    name = "rope_kv_append_int4"
+    _require_cuda(name, q, k, v, cos, sin, pool, block_tables, positions, cu_seqlens, q_out, error_word)
+    if k.dim() != 3 or v.shape != k.shape or v.dtype != k.dtype:
+        raise RuntimeError(f"{name}: k and v must be [N, Hkv, D] of one shape and dtype")
+    bs = _int4_block_size(name, pool, k.shape[1], k.shape[2])
+    return _rope_append(name, q, k, v, cos, sin, (pool,), block_tables, positions, cu_seqlens, interleaved, q_out,
+                        error_word, bs, pool.shape[0])
+
+
+def kv_gather_int4(
+    pool: torch.Tensor,
+    block_tables: torch.Tensor,
+    cu_seqlens: torch.Tensor,
+    total: int,
+    head_dim: int,
+    dtype: torch.dtype,
+    starts: Optional[torch.Tensor] = None,
+    k_out: Optional[torch.Tensor] = None,
+    v_out: Optional[torch.Tensor] = None,
+    error_word: Optional[torch.Tensor] = None,
+) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Tokens of a 4-bit pool as packed k and v [total, Hkv, D] of ``dtype``: rows
+    [cu_seqlens[b], cu_seqlens[b + 1]) are positions starts[b], starts[b] + 1, ... of sequence b
+    (starts None: from 0).  ``total`` is cu_seqlens[B], known to the caller on the host."""
+    name = "kv_gather_int4"
+    dev = _require_cuda(name, pool, block_tables, cu_seqlens, starts, k_out, v_out, error_word)
+    bs = _int4_block_size(name, pool, pool.shape[1] if pool.dim() == 3 else -1, head_dim)
+    B = cu_seqlens.shape[0] - 1 if cu_seqlens.dim() == 1 else -1
+    _int32_vector(name, "cu_seqlens", cu_seqlens, B + 1)
+    if starts is not None:
+        _int32_vector(name, "starts", starts, B)
+    max_blocks = _tables(name, block_tables, B)
+    shape = (int(total), pool.shape[1], head_dim)
+    k_out = torch.empty(shape, dtype=dtype, device=dev) if k_out is None else k_out
+    v_out = torch.empty(shape, dtype=dtype, device=dev) if v_out is None else v_out
+    for t in (k_out, v_out):
+        if tuple(t.shape) != shape or t.dtype != dtype or not t.is_contiguous():
+            raise RuntimeError(f"{name}: outputs must be contiguous {shape} tensors of {dtype}")
+    rc = N.load().spd_kv_gather_int4(pool.data_ptr(), block_tables.data_ptr(), cu_seqlens.data_ptr(), _ptr(starts),
+                                     k_out.data_ptr(), v_out.data_ptr(), shape[0], B, shape[1], head_dim, bs, max_blocks,
+                                     pool.shape[0], dtype_code(dtype), _ptr(error_word), _stream_handle())
+    N.check(rc, "spd_kv_gather_int4")
+    return k_out, v_out
+
+
+def paged_decode_attention_int4(
+    q: torch.Tensor,
+    pool: torch.Tensor,
+    block_tables: torch.Tensor,
+    context_lens: torch.Tensor,
+    scale: Optional[float] = None,
+    out: Optional[torch.Tensor] = None,
+    workspace: Optional[torch.Tensor] = None,
+) -> torch.Tensor:
+    """Single-token attention over a 4-bit pool with grouped heads.
+
+    q [B, Hq, D]; pool from ``kv_pool_int4`` with Hkv heads (Hq a multiple of it; query head h
+    reads head h // (Hq // Hkv)); block_tables int32 [B, max_blocks]; context_lens int32 [B]
+    tokens attended (<= 0 gives zeros).  Returns out [B, Hq, D]."""
+    name = "paged_decode_attention_int4"
+    dev = _require_cuda(name, q, pool, block_tables, context_lens, out, workspace)
+    if q.dim() != 3 or not q.is_contiguous():
+        raise RuntimeError(f"{name}: q must be a contiguous [B, Hq, D] tensor")
+    B, Hq, D = q.shape
+    Hkv = pool.shape[1] if pool.dim() == 3 else -1
+    bs = _int4_block_size(name, pool, Hkv, D)
+    if Hkv <= 0 or Hq % Hkv:
+        raise RuntimeError(f"{name}: {Hq} query heads do not divide over {Hkv} key/value heads")
+    max_blocks = _tables(name, block_tables, B)
+    _int32_vector(name, "context_lens", context_lens, B)
+    if out is None:
+        out = torch.empty_like(q)
+    elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous():
+        raise RuntimeError(f"{name}: out must be a contiguous {tuple(q.shape)} tensor of q's dtype")
+    code = dtype_code(q.dtype)
+    if B == 0:
+        return out
+    if workspace is None:
+        key = ("int4", B, Hq, Hkv, D, bs, max_blocks, code, dev, _stream_handle())
+        workspace = _WORKSPACES.get(key)
+        if workspace is None:
+            workspace = _WORKSPACES[key] = decode_int4_workspace(B, Hq, Hkv, D, bs, max_blocks, q.dtype, dev)
+    if scale is None:
+        scale = 1.0 / math.sqrt(D)
+    rc = N.load().spd_paged_decode_attn_int4(
+        q.data_ptr(), pool.data_ptr(), block_tables.data_ptr(), context_lens.data_ptr(), out.data_ptr(), B, Hq, Hkv, D,
+        bs, max_blocks, pool.shape[0], float(scale), code, workspace.data_ptr(), workspace.numel(), _stream_handle())
+    N.check(rc, "spd_paged_decode_attn_int4")
+    return out
+
+
+def prompt_attention(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    cu_seqlens_q: torch.Tensor,
+    cu_seqlens_k: Optional[torch.Tensor] = None,
+    causal: bool = True,
+    scale: Optional[float] = None,
+    out: Optional[torch.Tensor] = None,
+    error_word: Optional[torch.Tensor] = None,
+) -> torch.Tensor:
+    """Attention of whole packed prompts (fp16 / bf16, D a multiple of 8 up to 128).
+
+    q [Nq, Hq, D], k and v [Nk, Hkv, D]: tokens of all sequences packed, any token and head
+    strides, D contiguous; cu_seqlens_q / cu_seqlens_k int32 [B + 1] (keys default to the
+    queries' lengths).  With ``causal`` query i of a sequence sees the keys j <= i + Tk - Tq, so
+    keys of a cached prefix come first; a query that sees no key gives zeros.  Rows that belong
+    to no sequence are left as they are in ``out``.  Returns out [Nq, Hq, D]."""
+    name = "prompt_attention"
+    _require_cuda(name, q, k, v, cu_seqlens_q, cu_seqlens_k, out, error_word)
+    if q.dim() != 3 or k.dim() != 3 or v.shape != k.shape or q.shape[2] != k.shape[2]:
+        raise RuntimeError(f"{name}: q [Nq, Hq, D] and k, v [Nk, Hkv, D] expected")
+    if k.dtype != q.dtype or v.dtype != q.dtype:
+        raise RuntimeError(f"{name}: q, k and v must share a dtype")
+    (Nq, Hq, D), (Nk, Hkv, _) = q.shape, k.shape
+    if Hkv == 0 or Hq % Hkv:
+        raise RuntimeError(f"{name}: {Hq} query heads do not divide over {Hkv} key/value heads")
+    B = cu_seqlens_q.shape[0] - 1 if cu_seqlens_q.dim() == 1 else -1
+    _int32_vector(name, "cu_seqlens_q", cu_seqlens_q, B + 1)
+    if cu_seqlens_k is None:
+        cu_seqlens_k = cu_seqlens_q
+    else:
+        _int32_vector(name, "cu_seqlens_k", cu_seqlens_k, B + 1)
+    if out is None:
+        out = torch.empty((Nq, Hq, D), dtype=q.dtype, device=q.device)
+    elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous():
+        raise RuntimeError(f"{name}: out must be a contiguous {tuple(q.shape)} tensor of q's dtype")
+    if scale is None:
+        scale = 1.0 / math.sqrt(D)
+    strides = [x for what, t in (("q", q), ("k", k), ("v", v)) for x in _token_strides(name, what, t)]
+    rc = N.load().spd_prompt_attn(
+        q.data_ptr(), *strides[0:2], k.data_ptr(), *strides[2:4], v.data_ptr(), *strides[4:6], out.data_ptr(),
+        cu_seqlens_q.data_ptr(), cu_seqlens_k.data_ptr(), Nq, Nk, B, Hq, Hkv, D, int(bool(causal)), float(scale),
+        dtype_code(q.dtype), _ptr(error_word), _stream_handle())
+    N.check(rc, "spd_prompt_attn")
     return out
