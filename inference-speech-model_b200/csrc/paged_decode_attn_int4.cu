@@ -321,6 +321,8 @@ __global__ void __launch_bounds__(kThreads) decode_int4_kernel(const DecodeInt4P
         }
     }
     const float wscale = pow2(6 - lift);
+    constexpr float mid = 7.5f;
+    const float unscale = mid * pow2(lift - 6);
 
     // ---- output ------------------------------------------------------------------------
 #pragma unroll
@@ -343,10 +345,14 @@ __global__ void __launch_bounds__(kThreads) decode_int4_kernel(const DecodeInt4P
           b1 = movmatrix_trans(pack_split(pr[1] * sb));
           zacc[pl][0] += pr[0] * a.y + pr[1] * bq.y;
         } else {
-          b0 = movmatrix_trans(pack_half(pr[0] * sa, pr[C - 1] * sa));
-          b1 = movmatrix_trans(pack_half(pr[C] * sb, pr[2 * C - 1] * sb));
-          zacc[pl][0] += pr[0] * a.y + pr[C] * bq.y;
-          zacc[pl][C - 1] += pr[C - 1] * a.y + pr[2 * C - 1] * bq.y;
+          // what the rounding of a weight takes from the middle code (7.5) is put back, so that
+          // its error meets codes of both signs, as an output's own rounding would
+          const uint32_t ha = pack_half(pr[0] * sa, pr[C - 1] * sa), hb = pack_half(pr[C] * sb, pr[2 * C - 1] * sb);
+          b0 = movmatrix_trans(ha);
+          b1 = movmatrix_trans(hb);
+          const float2 ra = unpack_half(ha), rb = unpack_half(hb);
+          zacc[pl][0] += pr[0] * (a.y + mid * a.x) - ra.x * unscale + pr[C] * (bq.y + mid * bq.x) - rb.x * unscale;
+          zacc[pl][C - 1] += pr[C - 1] * (a.y + mid * a.x) - ra.y * unscale + pr[2 * C - 1] * (bq.y + mid * bq.x) - rb.y * unscale;
         }
         const unsigned char* vb_ = buf + kHalf + pl * BS * int4::kRowBytes + 4 * g;
         const uint32_t w0 = *reinterpret_cast<const uint32_t*>(vb_ + place(sub * 16 + tok_v0));
@@ -467,6 +473,13 @@ __global__ void __launch_bounds__(kThreads) decode_int4_kernel(const DecodeInt4P
   }
 }
 
+template <int P, int BS, bool SPLIT>
+int launch(const DecodeInt4Params& p, dim3 grid, cudaStream_t st) {
+  if (!allow_smem<decode_int4_kernel<P, BS, SPLIT>>(smem_bytes<P>())) return SPD_ERR_CUDA;
+  decode_int4_kernel<P, BS, SPLIT><<<grid, kThreads, smem_bytes<P>(), st>>>(p);
+  return cudaPeekAtLastError() == cudaSuccess ? SPD_OK : SPD_ERR_CUDA;
+}
+
 }  // namespace dec4
 
 // Heads per column tile: four with two columns each, or eight.
@@ -486,19 +499,13 @@ int decode_int4_launch(const DecodeInt4Params& p, int D, int bs, cudaStream_t st
   using namespace dec4;
   const int G = p.Hq / p.Hkv, kHeads = dec4_heads(p.dtype, G);
   const dim3 grid((unsigned)p.splits, (unsigned)(p.Hkv * ((G + kHeads - 1) / kHeads)), (unsigned)p.B);
-  auto launch = [&](auto kfn, size_t smem) -> int {
-    if (cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
-      return SPD_ERR_CUDA;
-    kfn<<<grid, kThreads, smem, st>>>(p);
-    return cudaPeekAtLastError() == cudaSuccess ? SPD_OK : SPD_ERR_CUDA;
-  };
   auto by_bs = [&](auto planes, auto split) -> int {
     constexpr int P = decltype(planes)::value;
     constexpr bool S = decltype(split)::value;
     switch (bs) {
-      case 8: return launch(decode_int4_kernel<P, 8, S>, smem_bytes<P>());
-      case 16: return launch(decode_int4_kernel<P, 16, S>, smem_bytes<P>());
-      case 32: return launch(decode_int4_kernel<P, 32, S>, smem_bytes<P>());
+      case 8: return launch<P, 8, S>(p, grid, st);
+      case 16: return launch<P, 16, S>(p, grid, st);
+      case 32: return launch<P, 32, S>(p, grid, st);
       default: return SPD_ERR_UNSUPPORTED;
     }
   };

@@ -509,6 +509,14 @@ static bool make_map3(CUtensorMap* map, const void* base, int D, int heads, int 
              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+template <typename T, int DP>
+static int launch(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const PromptParams& p, dim3 grid,
+                  cudaStream_t st) {
+  if (!allow_smem<prompt_attn_kernel<T, DP>>(Cfg<DP>::kSmem)) return SPD_ERR_CUDA;
+  prompt_attn_kernel<T, DP><<<grid, kThreads, Cfg<DP>::kSmem, st>>>(tq, tk, tv, p);
+  return cudaPeekAtLastError() == cudaSuccess ? SPD_OK : SPD_ERR_CUDA;
+}
+
 }  // namespace pa
 
 int prompt_attn_launch(PromptParams p, const void* q, const void* k, const void* v, long long q_st, long long q_sh,
@@ -530,15 +538,9 @@ int prompt_attn_launch(PromptParams p, const void* q, const void* k, const void*
   const int tokens = 2 * BM / p.pack;
   const long long most = ((long long)p.Nq / tokens + p.B) * (p.Hq / p.pack);  // items at most
   const dim3 grid((unsigned)(most < sms ? most : sms));
-  auto launch = [&](auto kfn, size_t smem) -> int {
-    if (cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
-      return SPD_ERR_CUDA;
-    kfn<<<grid, kThreads, smem, st>>>(tq, tk, tv, p);
-    return cudaPeekAtLastError() == cudaSuccess ? SPD_OK : SPD_ERR_CUDA;
-  };
   auto by_d = [&](auto tag) -> int {
     using T = decltype(tag);
-    return p.D <= 64 ? launch(prompt_attn_kernel<T, 64>, Cfg<64>::kSmem) : launch(prompt_attn_kernel<T, 128>, Cfg<128>::kSmem);
+    return p.D <= 64 ? launch<T, 64>(tq, tk, tv, p, grid, st) : launch<T, 128>(tq, tk, tv, p, grid, st);
   };
   return bf16 ? by_d(__nv_bfloat16{}) : by_d(__half{});
 }

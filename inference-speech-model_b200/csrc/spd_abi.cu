@@ -25,8 +25,8 @@ int linear_small_m_launch(const void* x, const void* w, const void* bias, void* 
 int cross_kv_project_launch(const void* enc_out, const void* w_kv, const void* b_kv, void* out,
                             const int32_t* slot_ids, int B, int T, int d_model, int L, int H, int D,
                             int T_out, int64_t out_slot_stride, int dtype, int* err, int sms, cudaStream_t st);
-int rope_append_launch(const RopeAppendParams& p, int dtype, bool int4_pool, cudaStream_t st);
-int gather_int4_launch(const GatherInt4Params& p, int dtype, cudaStream_t st);
+int rope_append_launch(const RopeAppendParams& p, int dtype, bool int4_pool, int sms, cudaStream_t st);
+int gather_int4_launch(const GatherInt4Params& p, int dtype, int sms, cudaStream_t st);
 int decode_int4_chunk(int B, int Hq, int Hkv, int dtype, int max_ctx, int sms);
 int decode_int4_launch(const DecodeInt4Params& p, int D, int bs, cudaStream_t st);
 int prompt_attn_launch(PromptParams p, const void* q, const void* k, const void* v, long long q_st, long long q_sh,
@@ -434,7 +434,9 @@ int spd_rope_kv_append(const void* q, int64_t q_stride_t, int64_t q_stride_h, co
   if (rc0 != SPD_OK) return rc0;
   if (!v_pool) return fail(SPD_ERR_INVALID_ARG, "spd_rope_kv_append: null tensor pointer");
   if (N == 0) return ok();
-  const int rc = spd::rope_append_launch(p, dtype, false, static_cast<cudaStream_t>(stream));
+  const int sms = sm_count(-1);
+  if (sms <= 0) return fail(SPD_ERR_CUDA, "spd_rope_kv_append: no CUDA device");
+  const int rc = spd::rope_append_launch(p, dtype, false, sms, static_cast<cudaStream_t>(stream));
   if (rc != SPD_OK) return fail(rc, "spd_rope_kv_append: launch failed: %s", cudaGetErrorString(cudaGetLastError()));
   return ok();
 }
@@ -453,7 +455,9 @@ int spd_rope_kv_append_int4(const void* q, int64_t q_stride_t, int64_t q_stride_
   if (!int4_shape_ok(D, block_size))
     return fail(SPD_ERR_UNSUPPORTED, "spd_rope_kv_append_int4: head_dim %d / block_size %d not supported", D, block_size);
   if (N == 0) return ok();
-  const int rc = spd::rope_append_launch(p, dtype, true, static_cast<cudaStream_t>(stream));
+  const int sms = sm_count(-1);
+  if (sms <= 0) return fail(SPD_ERR_CUDA, "spd_rope_kv_append_int4: no CUDA device");
+  const int rc = spd::rope_append_launch(p, dtype, true, sms, static_cast<cudaStream_t>(stream));
   if (rc != SPD_OK)
     return fail(rc, "spd_rope_kv_append_int4: launch failed: %s", cudaGetErrorString(cudaGetLastError()));
   return ok();
@@ -474,7 +478,9 @@ int spd_kv_gather_int4(const void* pool, const int32_t* block_tables, const int3
   if (N == 0) return ok();
   const spd::GatherInt4Params p{static_cast<const unsigned char*>(pool), block_tables, cu_seqlens, starts, k_out, v_out, N,
                                 B, Hkv, D, block_size, max_blocks, num_blocks, error_word};
-  const int rc = spd::gather_int4_launch(p, dtype, static_cast<cudaStream_t>(stream));
+  const int sms = sm_count(-1);
+  if (sms <= 0) return fail(SPD_ERR_CUDA, "spd_kv_gather_int4: no CUDA device");
+  const int rc = spd::gather_int4_launch(p, dtype, sms, static_cast<cudaStream_t>(stream));
   if (rc != SPD_OK) return fail(rc, "spd_kv_gather_int4: launch failed: %s", cudaGetErrorString(cudaGetLastError()));
   return ok();
 }

@@ -2,9 +2,24 @@
 // Passed to kernels by value (they live in the constant parameter bank).
 #pragma once
 
+#include <atomic>
+
 #include "spd_common.cuh"
 
 namespace spd {
+
+// Raises kernel K's dynamic shared-memory limit, once per device (one bit each).
+template <auto K>
+inline bool allow_smem(size_t bytes) {
+  static std::atomic<unsigned long long> seen{0};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return false;
+  const unsigned long long bit = 1ull << (dev & 63);
+  if (seen.load(std::memory_order_relaxed) & bit) return true;
+  if (cudaFuncSetAttribute(K, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) != cudaSuccess) return false;
+  seen.fetch_or(bit, std::memory_order_relaxed);
+  return true;
+}
 
 struct PagedParams {
   const void* q;
