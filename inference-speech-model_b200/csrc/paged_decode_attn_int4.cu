@@ -23,12 +23,14 @@
 //   each head takes two columns, the value and its rounding remainder, so q and p keep 22
 //   bits; with more, q keeps 11 bits (exact for fp16 and bf16 queries) and p 11.
 //
-// Work split: one CTA per (chunk of tokens, key/value head, sequence); each of its four
-// warps takes every fourth step of 64 tokens, fed by its own ring of shared-memory stages
-// (one bulk copy per page, issued by the lanes in parallel, no CTA-wide barrier in the
-// loop), with a running maximum that is raised only when a score passes it by 8 (p <= 2^8).
-// The warps' results are joined in shared memory, and the chunks' by the last CTA of a
-// (sequence, head) to arrive.
+// Work split, short block tables (up to kWholeTokens): one CTA per (sequence, key/value head tile).
+// Work split, longer ones: the steps (64 tokens) of all sequences and key/value heads are laid end to end
+// and shared equally among as many CTAs as are resident at once, whatever the lengths; a CTA's
+// share may begin and end inside a (sequence, head).  Its four warps take every fourth step,
+// each fed by its own ring of shared-memory stages (one bulk copy per page, issued by the lanes
+// in parallel, running ahead over segment ends), with a running maximum that is raised only
+// when a score passes it by 8 (p <= 2^8).  At a segment's end the warps are joined in shared
+// memory; segments that span CTAs are joined by the last of them to arrive.
 #include "spd_int4.cuh"
 #include "spd_params.cuh"
 
@@ -37,12 +39,34 @@ namespace dec4 {
 
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
-constexpr int kStep = 64;  // tokens per warp step
+constexpr int kWholeTokens = 2048;
+constexpr int kMaxCtas = 4;  // per SM (sizes the workspace's partial slots)
 constexpr float kLazy = 8.f;  // log2 units a score may pass the reference maximum by
 
-template <int P> constexpr int stages() { return P == 1 ? 4 : 3; }
-template <int P> constexpr int step_bytes() { return int4::page_bytes(P, kStep); }
-template <int P> constexpr size_t smem_bytes() { return (size_t)kWarps * stages<P>() * step_bytes<P>() + 1024; }
+#ifndef DEC4_ST1
+#define DEC4_ST1 3
+#define DEC4_SP1 64
+#define DEC4_ST2 2
+#define DEC4_SP2 64
+#define DEC4_MB 1
+#endif
+template <int P> constexpr int step_tokens() { return P == 4 ? 32 : P == 2 ? DEC4_SP2 : DEC4_SP1; }  // tokens per warp step
+template <int P> constexpr int stages() { return P == 1 ? DEC4_ST1 : P == 2 ? DEC4_ST2 : 2; }
+template <int P> constexpr int step_bytes() { return int4::page_bytes(P, step_tokens<P>()); }
+template <int P> constexpr int ring_bytes() { return kWarps * stages<P>() * step_bytes<P>(); }
+// the ring, then the warps' results [kWarps][heads][D] of a segment
+template <int P, bool SPLIT> constexpr size_t smem_bytes() {
+  return (size_t)ring_bytes<P>() + kWarps * (SPLIT ? 4 : 8) * P * int4::kPlane * 4;
+}
+
+// D += A * B (m16n8k16, fp16 in, fp32 accumulation).  Not volatile: the compiler may interleave the
+// chains of different accumulators, which hides each product's latency.
+__device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                    uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
 
 __device__ __forceinline__ uint32_t movmatrix_trans(uint32_t a) {
   uint32_t d;
@@ -60,6 +84,21 @@ __device__ __forceinline__ uint32_t pack_split(float x) {
 }
 __device__ __forceinline__ float2 unpack_half(uint32_t v) { return __half22float2(*reinterpret_cast<const __half2*>(&v)); }
 __device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }  // -126 <= e <= 127
+
+// P consecutive (scale, zero) pairs of one token
+template <int P>
+__device__ __forceinline__ void load_par(const float2* at, float2 (&v)[P]) {
+  if constexpr (P == 1) {
+    v[0] = *at;
+  } else {
+#pragma unroll
+    for (int i = 0; i < P; i += 2) {
+      const float4 x = *reinterpret_cast<const float4*>(at + i);
+      v[i] = make_float2(x.x, x.y);
+      v[i + 1] = make_float2(x.z, x.w);
+    }
+  }
+}
 
 // 16 consecutive query elements as fp32
 __device__ __forceinline__ void load_q16(const void* q, int dtype, long long at, float* o) {
@@ -80,79 +119,202 @@ __device__ __forceinline__ void store_out4(void* out, int dtype, long long at, f
   }
 }
 
+// A run of steps of one (sequence, head tile) inside a CTA's share.
+struct Segment {
+  int b, y;      // sequence; key/value head * tiles + tile
+  int step0, n;  // first step and number of steps here
+  int total;     // steps of the whole sequence
+};
+
 // P: planes (D / 64); BS: block size; SPLIT: two columns per head.
 template <int P, int BS, bool SPLIT>
-__global__ void __launch_bounds__(kThreads) decode_int4_kernel(const DecodeInt4Params p) {
+__global__ void __launch_bounds__(kThreads, P == 4 ? 1 : DEC4_MB) decode_int4_kernel(const DecodeInt4Params p) {
   constexpr int D = P * int4::kPlane;
   constexpr int kHeads = SPLIT ? 4 : 8;  // heads per column tile
-  constexpr int kStages = stages<P>();
+  constexpr int kStages = stages<P>(), kStep = step_tokens<P>(), kSubs = kStep / 16;
   constexpr int kPage = int4::page_bytes(P, BS), kHalf = int4::half_bytes(P, BS);
   constexpr int kPages = kStep / BS;
   constexpr int kParams = P * BS * int4::kRowBytes;  // offset of the parameters in a half page
+  constexpr int kRow = D + 4;  // floats per partial row: D values, m, l, two unused
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ __align__(8) uint64_t bars[kWarps][kStages];
   __shared__ float stat_m[kWarps][8], stat_l[kWarps][8];
-  __shared__ int last_flag;
+  __shared__ int scan[kWarps], last_flag;
+  // [kWarps][kHeads][D]: a warp's result at a segment's end; before it, the warp's parameters of
+  // the step at hand, (scale, zero) [K, V][tokens][P]
+  float* joined = reinterpret_cast<float*>(smem + ring_bytes<P>());
+  int* prefix = reinterpret_cast<int*>(smem + smem_bytes<P, SPLIT>());  // [B + 1] steps before each sequence
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int g = lane >> 2, t = lane & 3;
-  const int b = blockIdx.z, split = blockIdx.x;
   const int G = p.Hq / p.Hkv;
-  const int tiles = (G + kHeads - 1) / kHeads;
-  const int kvh = (int)blockIdx.y / tiles, tile = (int)blockIdx.y % tiles;
-  const int heads = min(kHeads, G - tile * kHeads);  // of this tile
-  const long long head0 = (long long)b * p.Hq + kvh * G + tile * kHeads;  // row of q and out
+  const int tiles = (G + kHeads - 1) / kHeads, Y = p.Hkv * tiles;
 
-  int ctx = p.context_lens[b];
-  if ((long long)ctx > (long long)p.max_blocks * BS) {
-    if (tid == 0) set_error(p.err, SPD_DEVERR_LENGTH);
-    ctx = p.max_blocks * BS;
+  auto ctx_of = [&](int b) {
+    const int c = p.context_lens[b];
+    return (long long)c > (long long)p.max_blocks * BS ? p.max_blocks * BS : c < 0 ? 0 : c;
+  };
+  auto zeros = [&](int b, int h0, int n) {  // a sequence without a context
+    for (int i = tid; i < n * D / 4; i += kThreads)
+      store_out4(p.out, p.dtype, ((long long)b * p.Hq + h0) * D + i * 4, make_float4(0.f, 0.f, 0.f, 0.f));
+  };
+  long long W = 0, u0 = 0, u1 = 0;  // steps of all; this CTA's share [u0, u1) of them
+  int ctas = 0;
+  bool narrow = true;
+  Segment seg{};
+  if (p.whole) {
+    // ---- one (sequence, head tile) per CTA -----------------------------------------------------
+    seg.b = blockIdx.x / Y;
+    seg.y = blockIdx.x - seg.b * Y;
+    const int c = p.context_lens[seg.b];
+    if ((long long)c > (long long)p.max_blocks * BS && tid == 0) set_error(p.err, SPD_DEVERR_LENGTH);
+    seg.total = seg.n = (ctx_of(seg.b) + kStep - 1) / kStep;
+    u1 = seg.n;
+    if (seg.n == 0) {
+      const int tile = seg.y % tiles;
+      zeros(seg.b, seg.y / tiles * G + tile * kHeads, min(kHeads, G - tile * kHeads));
+      return;
+    }
+  } else {
+    // ---- steps before each sequence --------------------------------------------------------
+    int base = 0;
+    for (int b0 = 0; b0 < p.B; b0 += kThreads) {
+      const int b = b0 + tid;
+      int n = 0;
+      if (b < p.B) {
+        n = (ctx_of(b) + kStep - 1) / kStep;
+        if (blockIdx.x == 0 && (long long)p.context_lens[b] > (long long)p.max_blocks * BS)
+          set_error(p.err, SPD_DEVERR_LENGTH);
+      }
+      int incl = n;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += v;
+      }
+      if (lane == 31) scan[warp] = incl;
+      __syncthreads();
+      int before = base, all = 0;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        if (w < warp) before += scan[w];
+        all += scan[w];
+      }
+      if (b < p.B) prefix[b] = before + incl - n;
+      base += all;
+      __syncthreads();
+    }
+    if (tid == 0) prefix[p.B] = base;
+    __syncthreads();
+    if (blockIdx.x == 0)
+      for (int b = 0; b < p.B; ++b)
+        if (prefix[b + 1] == prefix[b]) zeros(b, 0, p.Hq);
+    // ---- this CTA's share ------------------------------------------------------------------
+    W = (long long)base * Y;
+    ctas = (int)min((long long)gridDim.x, W);  // a few steps spread over as many CTAs
+    if ((int)blockIdx.x >= ctas) return;
+    narrow = W <= 0x7fffffff / (ctas + 1);
   }
-  if (ctx <= 0) {
-    if (split == 0)
-      for (int i = tid; i < heads * D / 4; i += kThreads)
-        store_out4(p.out, p.dtype, head0 * D + i * 4, make_float4(0.f, 0.f, 0.f, 0.f));
-    return;
+  // c * W / ctas, and the CTA whose share holds unit u; in 32 bits where the products fit
+  auto share = [&](int c) {
+    return narrow ? (long long)((unsigned)c * (unsigned)W / (unsigned)ctas) : range_start(c, ctas, W);
+  };
+  auto cta_of = [&](long long u) {
+    return narrow ? (int)((((unsigned)u + 1) * (unsigned)ctas + (unsigned)W - 1) / (unsigned)W) - 1
+                  : cta_of_unit(u, ctas, W);
+  };
+  if (!p.whole) {
+    u0 = share(blockIdx.x);
+    u1 = share(blockIdx.x + 1);
+    seg.b = upper_index_i32(prefix, p.B, narrow ? (long long)((unsigned)u0 / (unsigned)Y) : u0 / Y);
+    seg.total = prefix[seg.b + 1] - prefix[seg.b];
+    const long long r = u0 - (long long)prefix[seg.b] * Y;
+    seg.y = narrow ? (int)((unsigned)r / (unsigned)seg.total) : (int)(r / seg.total);
+    seg.step0 = (int)(r - (long long)seg.y * seg.total);
+    seg.n = (int)min((long long)(seg.total - seg.step0), u1 - u0);
   }
-  const int t0 = split * p.chunk;
-  if (t0 >= ctx) return;
-  const int t1 = min(ctx, t0 + p.chunk);
-  const int nsplit = (ctx + p.chunk - 1) / p.chunk;
-  const int steps = (t1 - t0 + kStep - 1) / kStep;
-  const int my_steps = steps > warp ? (steps - warp + kWarps - 1) / kWarps : 0;
+  auto next = [&](Segment& s, long long u) {  // the segment after s, which begins at unit u < u1
+    if (++s.y == Y) {
+      s.y = 0;
+      do ++s.b; while (prefix[s.b + 1] == prefix[s.b]);
+      s.total = prefix[s.b + 1] - prefix[s.b];
+    }
+    s.step0 = 0;
+    s.n = (int)min((long long)s.total, u1 - u);
+  };
 
   unsigned char* ring = smem + (size_t)warp * kStages * step_bytes<P>();
-  const int* table = p.block_tables + (long long)b * p.max_blocks;
-  const unsigned char* pool_h = p.pool + (long long)kvh * kPage;
-  const long long block_stride = (long long)p.Hkv * kPage;
   const uint64_t policy = l2_policy_evict_first();
   if (lane == 0) {
     for (int s = 0; s < kStages; ++s) mbar_init(&bars[warp][s], 1);
     fence_barrier_init();
   }
   __syncwarp();
-  // Copies the pages of this warp's i-th step into its stage.
-  auto issue = [&](int i) {
-    const int tok = t0 + (warp + i * kWarps) * kStep;
-    const int n = min(kPages, (t1 - tok + BS - 1) / BS);
-    uint64_t* bar = &bars[warp][i % kStages];
-    if (lane == 0) mbar_arrive_expect_tx(bar, (uint32_t)(n * kPage));
+
+  // The copies run ahead of the arithmetic over this warp's steps of all segments: `ahead` is
+  // the segment of the next step to fetch, `id` this lane's page of that step (its table entry is
+  // loaded one step early).
+  Segment ahead = seg;
+  long long ahead_u = u0;
+  int ahead_i = warp, id = -1, ahead_pages = 0, fetched = 0, ahead_ctx = ctx_of(ahead.b);
+  bool more = true;
+  auto look_up = [&]() {
+    while (more && ahead_i >= ahead.n) {
+      ahead_u += ahead.n;
+      ahead_i = warp;
+      if (ahead_u >= u1) {
+        more = false;
+      } else {
+        next(ahead, ahead_u);
+        ahead_ctx = ctx_of(ahead.b);
+      }
+    }
+    if (!more) return;
+    const int tok = (ahead.step0 + ahead_i) * kStep;
+    ahead_pages = min(kPages, (ahead_ctx - tok + BS - 1) / BS);
+    id = lane < ahead_pages ? p.block_tables[(long long)ahead.b * p.max_blocks + tok / BS + lane] : 0;
+  };
+  auto fetch = [&]() {
+    if (!more) return;
+    const int st = fetched % kStages;
+    if (lane == 0) mbar_arrive_expect_tx(&bars[warp][st], (uint32_t)(ahead_pages * kPage));
     __syncwarp();
-    if (lane < n) {
-      int id = table[tok / BS + lane];
+    if (lane < ahead_pages) {
       if (id < 0 || id >= p.num_blocks) {
         set_error(p.err, SPD_DEVERR_BLOCK_ID);
         id = 0;
       }
-      bulk_copy_g2s_hint(ring + (size_t)(i % kStages) * step_bytes<P>() + lane * kPage, pool_h + id * block_stride, kPage,
-                         bar, policy);
+      bulk_copy_g2s_hint(ring + (size_t)st * step_bytes<P>() + lane * kPage,
+                         p.pool + ((long long)id * p.Hkv + ahead.y / tiles) * kPage, kPage, &bars[warp][st], policy);
     }
+    ++fetched;
+    ahead_i += kWarps;
+    look_up();
   };
-  for (int i = 0; i < kStages && i < my_steps; ++i) issue(i);
+  look_up();
+  for (int i = 0; i < kStages; ++i) fetch();
+
+  // Row r of an 8-token group holds token r ^ (r >> 2): with it both the rows that a
+  // half-warp reads for the scores (r = 0..3, 4..7) and those that a warp reads for the output
+  // (even or odd r) fall on four different quarters of the 32 banks.
+  const int tok_k = g ^ (g >> 2);
+  const int tok_v0 = (2 * t) ^ (t >> 1), tok_v1 = (2 * t + 1) ^ (t >> 1);
+  auto place = [](int tok) { return (tok / BS) * kPage + (tok % BS) * int4::kRowBytes; };
+
+  constexpr int C = SPLIT ? 1 : 2;  // heads of this lane's two columns
+  static_assert(2 * kStep * P * 2 <= kHeads * D, "the parameters fit in the warp's result");
+  float2* par = reinterpret_cast<float2*>(joined + warp * kHeads * D);
+  int used = 0;
+  bool fine = true;
+  for (long long u = u0; u < u1; ) {
+  const int tile = seg.y % tiles, kvh = seg.y / tiles;
+  const int heads = min(kHeads, G - tile * kHeads);  // of this tile
+  const long long head0 = (long long)seg.b * p.Hq + kvh * G + tile * kHeads;  // row of q and out
+  const int ctx = ctx_of(seg.b);
 
   // ---- the query fragments: column g, k = this lane's 16 dimensions of each plane --------
   uint32_t qb[P][4][2];
-  float fa, fb, qsa[P], qsb[P];  // score factors and sums of q of this lane's columns 2t, 2t + 1
+  float f, qsa[P], qsb[P];  // score factor, and sums of q of this lane's columns 2t, 2t + 1
   {
     const int hq = SPLIT ? g >> 1 : g;
     float qv[P][16];
@@ -166,15 +328,15 @@ __global__ void __launch_bounds__(kThreads) decode_int4_kernel(const DecodeInt4P
       qs[pl] = 0.f;
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        amax = fmaxf(amax, fabsf(qv[pl][i]));
+        const float a = fabsf(qv[pl][i]);
+        amax = fmaxf(amax, a < INFINITY ? a : 0.f);
         qs[pl] += qv[pl][i];
       }
       qs[pl] += __shfl_xor_sync(0xffffffffu, qs[pl], 1);
       qs[pl] += __shfl_xor_sync(0xffffffffu, qs[pl], 2);
       qs[pl] *= p.scale_log2;
     }
-    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+    amax = warp_max(amax);  // of the tile's finite queries
     // |q| * 2^k < 2^11; k is limited so that both 2^k and 2^(24 - k) are normal numbers
     const int k = amax > 0.f ? max(-100, min(100, 10 - ((__float_as_int(amax) >> 23) - 127))) : 0;
     const float up = pow2(k);
@@ -194,9 +356,7 @@ __global__ void __launch_bounds__(kThreads) decode_int4_kernel(const DecodeInt4P
         qb[pl][s][0] = pack_half(x[0], x[1]);
         qb[pl][s][1] = pack_half(x[2] * 0.0625f, x[3] * 0.0625f);  // meets codes that read as 16c
       }
-    const float f = pow2(24 - k) * p.scale_log2;
-    fa = __shfl_sync(0xffffffffu, f, 8 * t);
-    fb = __shfl_sync(0xffffffffu, f, 8 * t + 4);
+    f = pow2(24 - k) * p.scale_log2;
 #pragma unroll
     for (int pl = 0; pl < P; ++pl) {
       qsa[pl] = __shfl_sync(0xffffffffu, qs[pl], 8 * t);
@@ -204,7 +364,6 @@ __global__ void __launch_bounds__(kThreads) decode_int4_kernel(const DecodeInt4P
     }
   }
 
-  constexpr int C = SPLIT ? 1 : 2;  // heads of this lane's two columns
   float o[P][4][4], zacc[P][C], l[C], m[C];
 #pragma unroll
   for (int c = 0; c < C; ++c) {
@@ -219,140 +378,177 @@ __global__ void __launch_bounds__(kThreads) decode_int4_kernel(const DecodeInt4P
     for (int i = 0; i < 16; ++i) o[pl][i >> 2][i & 3] = 0.f;
   int lift = -15;  // exponent of the largest value scale seen; weights carry 2^(6 - lift)
 
-  // Row r of an 8-token group holds token r ^ (r >> 2): with it both the rows that a
-  // half-warp reads for the scores (r = 0..3, 4..7) and those that a warp reads for the output
-  // (even or odd r) fall on four different quarters of the 32 banks.
-  const int tok_k = g ^ (g >> 2);
-  const int tok_v0 = (2 * t) ^ (t >> 1), tok_v1 = (2 * t + 1) ^ (t >> 1);
-  auto place = [](int tok) { return (tok / BS) * kPage + (tok % BS) * int4::kRowBytes; };
-
-  int i = 0;
-  for (; i < my_steps; ++i) {
-    const int st = i % kStages;
-    const bool ok = mbar_wait_bounded(&bars[warp][st], (uint32_t)((i / kStages) & 1), p.err, p.wait_ns);
-    if (!__all_sync(0xffffffffu, ok)) break;
+  for (int i = warp; i < seg.n && fine; i += kWarps) {
+    const int st = used % kStages;
+    const bool ok = mbar_wait_bounded(&bars[warp][st], (uint32_t)((used / kStages) & 1), p.err, p.wait_ns);
+    fine = __all_sync(0xffffffffu, ok);
+    if (!fine) break;
+    ++used;
     const unsigned char* buf = ring + (size_t)st * step_bytes<P>();
-    const int left = t1 - (t0 + (warp + i * kWarps) * kStep);  // valid tokens of this step (>= 1)
+    const int left = ctx - (seg.step0 + i) * kStep;  // valid tokens of this step (>= 1)
 
-    // ---- scores ----------------------------------------------------------------------
-    float sc[4][2 * C];      // per 16 tokens: tokens tok_k and tok_k + 8 of each head
-    uint32_t vp[4][2][P];    // the value parameters of those tokens, zero past the end
-    uint32_t smax = 0;
+    // ---- the tokens' parameters, once per token: to fp32 with all factors multiplied in ----
+    // (scale * f, zero) of K and (scale * 2^(6 - lift), zero) of V, zero past the end; lane = token
+    uint32_t raw[kStep / 32][2 * P], top = 0;
 #pragma unroll
-    for (int sub = 0; sub < 4; ++sub) {
-#pragma unroll
-      for (int c = 0; c < 2 * C; ++c) sc[sub][c] = 0.f;
-      const int ta = sub * 16 + tok_k, tb = ta + 8;
-      const bool va = ta < left, vb = tb < left;
+    for (int h = 0; h < kStep / 32; ++h) {
+      const int tok = h * 32 + lane;
+      const unsigned char* at = buf + (tok / BS) * kPage + kParams + (tok % BS) * int4::kParamBytes;
 #pragma unroll
       for (int pl = 0; pl < P; ++pl) {
-        const uint2 wa = *reinterpret_cast<const uint2*>(buf + place(ta) + pl * BS * int4::kRowBytes + 8 * t);
-        const uint2 wb = *reinterpret_cast<const uint2*>(buf + place(tb) + pl * BS * int4::kRowBytes + 8 * t);
-        float acc[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int w = 0; w < 2; ++w) {
-          const uint32_t xa = w ? wa.y : wa.x, xb = w ? wb.y : wb.x;
-          mma_16816<__half>(acc, xa & 0x000F000Fu, xb & 0x000F000Fu, xa & 0x00F000F0u, xb & 0x00F000F0u, qb[pl][2 * w][0],
-                            qb[pl][2 * w][1]);
-          mma_16816<__half>(acc, (xa >> 8) & 0x000F000Fu, (xb >> 8) & 0x000F000Fu, (xa >> 8) & 0x00F000F0u,
-                            (xb >> 8) & 0x00F000F0u, qb[pl][2 * w + 1][0], qb[pl][2 * w + 1][1]);
-        }
-        const int pa = (ta / BS) * kPage + kParams + (pl * BS + ta % BS) * int4::kParamBytes;
-        const int pb = (tb / BS) * kPage + kParams + (pl * BS + tb % BS) * int4::kParamBytes;
-        const float2 ka = unpack_half(*reinterpret_cast<const uint32_t*>(buf + pa));
-        const float2 kb = unpack_half(*reinterpret_cast<const uint32_t*>(buf + pb));
-        if (SPLIT) {
-          sc[sub][0] += fa * ka.x * (acc[0] + acc[1]) + qsa[pl] * ka.y;
-          sc[sub][1] += fa * kb.x * (acc[2] + acc[3]) + qsa[pl] * kb.y;
-        } else {
-          sc[sub][0] += fa * ka.x * acc[0] + qsa[pl] * ka.y;
-          sc[sub][C - 1] += fb * ka.x * acc[1] + qsb[pl] * ka.y;
-          sc[sub][C] += fa * kb.x * acc[2] + qsa[pl] * kb.y;
-          sc[sub][2 * C - 1] += fb * kb.x * acc[3] + qsb[pl] * kb.y;
-        }
-        vp[sub][0][pl] = va ? *reinterpret_cast<const uint32_t*>(buf + kHalf + pa) : 0u;
-        vp[sub][1][pl] = vb ? *reinterpret_cast<const uint32_t*>(buf + kHalf + pb) : 0u;
-        smax = max(smax, max(vp[sub][0][pl] & 0x7FFFu, vp[sub][1][pl] & 0x7FFFu));
-      }
-#pragma unroll
-      for (int c = 0; c < C; ++c) {
-        if (!va) sc[sub][c] = -INFINITY;
-        if (!vb) sc[sub][C + c] = -INFINITY;
+        const bool in = tok < left;
+        raw[h][pl] = in ? *reinterpret_cast<const uint32_t*>(at + pl * BS * int4::kParamBytes) : 0u;
+        raw[h][P + pl] = in ? *reinterpret_cast<const uint32_t*>(at + kHalf + pl * BS * int4::kParamBytes) : 0u;
+        top = max(top, raw[h][P + pl] & 0x7FFFu);
       }
     }
-
-    // ---- running maximum and weight exponent: raised for the whole warp when needed --------
-    float mx[C];
-#pragma unroll
-    for (int c = 0; c < C; ++c) {
-      mx[c] = -INFINITY;
-#pragma unroll
-      for (int sub = 0; sub < 4; ++sub) mx[c] = fmaxf(mx[c], fmaxf(sc[sub][c], sc[sub][C + c]));
-#pragma unroll
-      for (int x = 4; x < 32; x <<= 1) mx[c] = fmaxf(mx[c], __shfl_xor_sync(0xffffffffu, mx[c], x));
-    }
-    const int new_lift = min(15, (int)(__reduce_max_sync(0xffffffffu, smax) >> 10) - 15);
-    bool raise = new_lift > lift;
-#pragma unroll
-    for (int c = 0; c < C; ++c) raise |= mx[c] > m[c] + kLazy;
-    if (__any_sync(0xffffffffu, raise)) {
-      const int up = max(lift, new_lift);
+    if (__any_sync(0xffffffffu, (int)(top >> 10) - 15 > lift)) {  // a larger value scale than any before
+      const int up = min(15, (int)(__reduce_max_sync(0xffffffffu, top) >> 10) - 15);
       const float w = pow2(lift - up);
       lift = up;
-      float f[C];
+#pragma unroll
+      for (int pl = 0; pl < P; ++pl)
+#pragma unroll
+        for (int k = 0; k < 16; ++k) o[pl][k >> 2][k & 3] *= w;
+    }
+    const float wscale = pow2(6 - lift);
+#pragma unroll
+    for (int h = 0; h < kStep / 32; ++h)
+#pragma unroll
+      for (int pl = 0; pl < P; ++pl) {
+        const float2 kp = unpack_half(raw[h][pl]), vp = unpack_half(raw[h][P + pl]);
+        par[(h * 32 + lane) * P + pl] = make_float2(kp.x * f, kp.y);
+        par[(kStep + h * 32 + lane) * P + pl] = make_float2(vp.x * wscale, vp.y);
+      }
+    __syncwarp();
+
+    // ---- scores ----------------------------------------------------------------------
+    // products of all 16-token tiles and planes first, their accumulator chains interleaved
+    float acc[kSubs][P][4];
+    {
+      uint2 wa[kSubs][P], wb[kSubs][P];
+#pragma unroll
+      for (int sub = 0; sub < kSubs; ++sub)
+#pragma unroll
+        for (int pl = 0; pl < P; ++pl) {
+          const unsigned char* at = buf + pl * BS * int4::kRowBytes + 8 * t;
+          wa[sub][pl] = *reinterpret_cast<const uint2*>(at + place(sub * 16 + tok_k));
+          wb[sub][pl] = *reinterpret_cast<const uint2*>(at + place(sub * 16 + 8 + tok_k));
+#pragma unroll
+          for (int i = 0; i < 4; ++i) acc[sub][pl][i] = 0.f;
+        }
+#pragma unroll
+      for (int s = 0; s < 4; ++s)
+#pragma unroll
+        for (int sub = 0; sub < kSubs; ++sub)
+#pragma unroll
+          for (int pl = 0; pl < P; ++pl) {
+            uint32_t xa = s < 2 ? wa[sub][pl].x : wa[sub][pl].y, xb = s < 2 ? wb[sub][pl].x : wb[sub][pl].y;
+            if (s & 1) xa >>= 8, xb >>= 8;
+            mma(acc[sub][pl], xa & 0x000F000Fu, xb & 0x000F000Fu, xa & 0x00F000F0u, xb & 0x00F000F0u, qb[pl][s][0],
+                qb[pl][s][1]);
+          }
+    }
+    float sc[kSubs][2 * C];  // per 16 tokens: tokens tok_k and tok_k + 8 of each head
+#pragma unroll
+    for (int sub = 0; sub < kSubs; ++sub) {
+      const int ta = sub * 16 + tok_k, tb = ta + 8;
+      float2 ka[P], kb[P];
+      load_par<P>(par + ta * P, ka);
+      load_par<P>(par + tb * P, kb);
+#pragma unroll
+      for (int pl = 0; pl < P; ++pl) {
+        const float* a = acc[sub][pl];
+        auto add = [&](int i, float x, float2 kp, float qs) {
+          sc[sub][i] = fmaf(kp.x, x, pl ? fmaf(kp.y, qs, sc[sub][i]) : kp.y * qs);
+        };
+        if (SPLIT) {
+          add(0, a[0] + a[1], ka[pl], qsa[pl]);
+          add(C, a[2] + a[3], kb[pl], qsa[pl]);
+        } else {
+          add(0, a[0], ka[pl], qsa[pl]);
+          add(C - 1, a[1], ka[pl], qsb[pl]);
+          add(C, a[2], kb[pl], qsa[pl]);
+          add(2 * C - 1, a[3], kb[pl], qsb[pl]);
+        }
+      }
+      if (left < kStep)  // the sequence's last step
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+          if (ta >= left) sc[sub][c] = -INFINITY;
+          if (tb >= left) sc[sub][C + c] = -INFINITY;
+        }
+    }
+
+    // ---- running maximum: raised when a score passes it by kLazy -----------------------------
+    float mx[C];
+    bool raise = false;
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      mx[c] = fmaxf(sc[0][c], sc[0][C + c]);
+#pragma unroll
+      for (int sub = 1; sub < kSubs; ++sub) mx[c] = fmaxf(mx[c], fmaxf(sc[sub][c], sc[sub][C + c]));
+      raise |= mx[c] > m[c] + kLazy;
+    }
+    if (__any_sync(0xffffffffu, raise)) {
+      float fm[C];
 #pragma unroll
       for (int c = 0; c < C; ++c) {
-        const float mn = fmaxf(m[c], mx[c]);
-        f[c] = m[c] == mn ? 1.f : ex2_approx(m[c] - mn);  // also when both are -inf
-        m[c] = mn;
-        l[c] *= f[c];
 #pragma unroll
-        for (int pl = 0; pl < P; ++pl) zacc[pl][c] *= f[c];
-        f[c] *= w;
+        for (int x = 4; x < 32; x <<= 1) mx[c] = fmaxf(mx[c], __shfl_xor_sync(0xffffffffu, mx[c], x));
+        const float mn = fmaxf(m[c], mx[c]);
+        fm[c] = m[c] == mn ? 1.f : ex2_approx(m[c] - mn);  // also when both are -inf
+        m[c] = mn;
+        l[c] *= fm[c];
+#pragma unroll
+        for (int pl = 0; pl < P; ++pl) zacc[pl][c] *= fm[c];
       }
 #pragma unroll
       for (int pl = 0; pl < P; ++pl)
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          o[pl][k][0] *= f[0];
-          o[pl][k][1] *= f[C - 1];
-          o[pl][k][2] *= f[0];
-          o[pl][k][3] *= f[C - 1];
+          o[pl][k][0] *= fm[0];
+          o[pl][k][1] *= fm[C - 1];
+          o[pl][k][2] *= fm[0];
+          o[pl][k][3] *= fm[C - 1];
         }
     }
-    const float wscale = pow2(6 - lift);
-    constexpr float mid = 7.5f;
-    const float unscale = mid * pow2(lift - 6);
+    float mm[C];  // a head whose scores are all -inf so far keeps m = -inf: its weights are 0
+#pragma unroll
+    for (int c = 0; c < C; ++c) mm[c] = m[c] == -INFINITY ? 0.f : m[c];
 
     // ---- output ------------------------------------------------------------------------
 #pragma unroll
-    for (int sub = 0; sub < 4; ++sub) {
+    for (int sub = 0; sub < kSubs; ++sub) {
+      const int ta = sub * 16 + tok_k, tb = ta + 8;
+      float2 va[P], vb[P];
+      load_par<P>(par + (kStep + ta) * P, va);
+      load_par<P>(par + (kStep + tb) * P, vb);
       float pr[2 * C];
 #pragma unroll
       for (int c = 0; c < C; ++c) {
-        // a head whose scores are all -inf so far keeps m = -inf: its weights are 0
-        pr[c] = ex2_approx(sc[sub][c] - (m[c] == -INFINITY ? 0.f : m[c]));
-        pr[C + c] = ex2_approx(sc[sub][C + c] - (m[c] == -INFINITY ? 0.f : m[c]));
+        pr[c] = ex2_approx(sc[sub][c] - mm[c]);
+        pr[C + c] = ex2_approx(sc[sub][C + c] - mm[c]);
         l[c] += pr[c] + pr[C + c];
       }
 #pragma unroll
       for (int pl = 0; pl < P; ++pl) {
-        const float2 a = unpack_half(vp[sub][0][pl]), bq = unpack_half(vp[sub][1][pl]);
-        const float sa = a.x * wscale, sb = bq.x * wscale;
         uint32_t b0, b1;
         if (SPLIT) {
-          b0 = movmatrix_trans(pack_split(pr[0] * sa));
-          b1 = movmatrix_trans(pack_split(pr[1] * sb));
-          zacc[pl][0] += pr[0] * a.y + pr[1] * bq.y;
+          b0 = movmatrix_trans(pack_split(pr[0] * va[pl].x));
+          b1 = movmatrix_trans(pack_split(pr[1] * vb[pl].x));
+          zacc[pl][0] += pr[0] * va[pl].y + pr[1] * vb[pl].y;
         } else {
           // what the rounding of a weight takes from the middle code (7.5) is put back, so that
           // its error meets codes of both signs, as an output's own rounding would
-          const uint32_t ha = pack_half(pr[0] * sa, pr[C - 1] * sa), hb = pack_half(pr[C] * sb, pr[2 * C - 1] * sb);
+          const float unscale = 7.5f * pow2(lift - 6);
+          const float w0 = pr[0] * va[pl].x, w1 = pr[C - 1] * va[pl].x, w2 = pr[C] * vb[pl].x, w3 = pr[2 * C - 1] * vb[pl].x;
+          const uint32_t ha = pack_half(w0, w1), hb = pack_half(w2, w3);
           b0 = movmatrix_trans(ha);
           b1 = movmatrix_trans(hb);
           const float2 ra = unpack_half(ha), rb = unpack_half(hb);
-          zacc[pl][0] += pr[0] * (a.y + mid * a.x) - ra.x * unscale + pr[C] * (bq.y + mid * bq.x) - rb.x * unscale;
-          zacc[pl][C - 1] += pr[C - 1] * (a.y + mid * a.x) - ra.y * unscale + pr[2 * C - 1] * (bq.y + mid * bq.x) - rb.y * unscale;
+          zacc[pl][0] += pr[0] * va[pl].y + pr[C] * vb[pl].y + unscale * ((w0 - ra.x) + (w2 - rb.x));
+          zacc[pl][C - 1] += pr[C - 1] * va[pl].y + pr[2 * C - 1] * vb[pl].y + unscale * ((w1 - ra.y) + (w3 - rb.y));
         }
         const unsigned char* vb_ = buf + kHalf + pl * BS * int4::kRowBytes + 4 * g;
         const uint32_t w0 = *reinterpret_cast<const uint32_t*>(vb_ + place(sub * 16 + tok_v0));
@@ -362,19 +558,16 @@ __global__ void __launch_bounds__(kThreads) decode_int4_kernel(const DecodeInt4P
         // dimensions 8g..8g+3 (lo) and 8g+4..8g+7 (hi) of a pair of tokens per register
         uint32_t lo0 = __byte_perm(w0, w1, 0x5410), hi0 = __byte_perm(w0, w1, 0x7632);
         uint32_t lo1 = __byte_perm(w2, w3, 0x5410), hi1 = __byte_perm(w2, w3, 0x7632);
-        mma_16816<__half>(o[pl][0], lo0 & 0x000F000Fu, hi0 & 0x000F000Fu, lo1 & 0x000F000Fu, hi1 & 0x000F000Fu, b0, b1);
-        mma_16816<__half>(o[pl][1], lo0 & 0x00F000F0u, hi0 & 0x00F000F0u, lo1 & 0x00F000F0u, hi1 & 0x00F000F0u, b0, b1);
+        mma(o[pl][0], lo0 & 0x000F000Fu, hi0 & 0x000F000Fu, lo1 & 0x000F000Fu, hi1 & 0x000F000Fu, b0, b1);
+        mma(o[pl][1], lo0 & 0x00F000F0u, hi0 & 0x00F000F0u, lo1 & 0x00F000F0u, hi1 & 0x00F000F0u, b0, b1);
         lo0 >>= 8; hi0 >>= 8; lo1 >>= 8; hi1 >>= 8;
-        mma_16816<__half>(o[pl][2], lo0 & 0x000F000Fu, hi0 & 0x000F000Fu, lo1 & 0x000F000Fu, hi1 & 0x000F000Fu, b0, b1);
-        mma_16816<__half>(o[pl][3], lo0 & 0x00F000F0u, hi0 & 0x00F000F0u, lo1 & 0x00F000F0u, hi1 & 0x00F000F0u, b0, b1);
+        mma(o[pl][2], lo0 & 0x000F000Fu, hi0 & 0x000F000Fu, lo1 & 0x000F000Fu, hi1 & 0x000F000Fu, b0, b1);
+        mma(o[pl][3], lo0 & 0x00F000F0u, hi0 & 0x00F000F0u, lo1 & 0x00F000F0u, hi1 & 0x00F000F0u, b0, b1);
       }
     }
-    __syncwarp();  // every lane has read this stage
-    if (i + kStages < my_steps) issue(i + kStages);
+    __syncwarp();  // every lane has read this stage and these parameters
+    fetch();
   }
-  if (i < my_steps)  // a wait gave up: let this warp's copies in flight land before the CTA can exit
-    for (int k = i; k < my_steps && k < i + kStages; ++k)
-      (void)mbar_wait_bounded(&bars[warp][k % kStages], (uint32_t)((k / kStages) & 1), nullptr);
 
   // ---- join the warps ---------------------------------------------------------------------
 #pragma unroll
@@ -385,8 +578,8 @@ __global__ void __launch_bounds__(kThreads) decode_int4_kernel(const DecodeInt4P
 #pragma unroll
       for (int pl = 0; pl < P; ++pl) zacc[pl][c] += __shfl_xor_sync(0xffffffffu, zacc[pl][c], x);
     }
+  float* mine = joined + warp * kHeads * D;
   __syncwarp();
-  float* mine = reinterpret_cast<float*>(ring);  // [head][D]; the ring is drained
   {
     // out of the fp16 scaling: 2^24 / 2^(6 - lift), and / 16 where the codes read as 16c
     const float f1 = pow2(18 + lift), f16 = pow2(14 + lift);
@@ -415,7 +608,9 @@ __global__ void __launch_bounds__(kThreads) decode_int4_kernel(const DecodeInt4P
       }
   }
   __syncthreads();
-  constexpr int kRow = D + 4;  // floats per partial row: D values, m, l, two unused
+  const bool whole = seg.step0 == 0 && seg.n == seg.total;
+  // a CTA has at most two segments that others share: the one it begins in and the one it ends in
+  float* slot = p.partials + (size_t)(2 * blockIdx.x + (seg.step0 == 0 ? 1 : 0)) * kHeads * kRow;
   for (int e = tid; e < heads * D / 4; e += kThreads) {
     const int h = e / (D / 4), d = (e % (D / 4)) * 4;
     float mm = -INFINITY;
@@ -425,58 +620,89 @@ __global__ void __launch_bounds__(kThreads) decode_int4_kernel(const DecodeInt4P
     float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
-      if (steps <= w) break;  // a warp without a step
       const float f = stat_m[w][h] == mm ? 1.f : ex2_approx(stat_m[w][h] - mm);
-      const float4 v = *reinterpret_cast<const float4*>(smem + (size_t)w * kStages * step_bytes<P>() + (h * D + d) * 4);
+      const float4 v = *reinterpret_cast<const float4*>(joined + (w * kHeads + h) * D + d);
       ll += f * stat_l[w][h];
       s.x += f * v.x; s.y += f * v.y; s.z += f * v.z; s.w += f * v.w;
     }
-    if (nsplit == 1) {
+    if (whole) {
       const float r = ll != 0.f ? 1.f / ll : 0.f;  // no weight at all: zeros
       store_out4(p.out, p.dtype, (head0 + h) * D + d, make_float4(s.x * r, s.y * r, s.z * r, s.w * r));
     } else {
-      float* row = p.partials + ((head0 + h) * p.splits + split) * kRow;
+      float* row = slot + h * kRow;
       *reinterpret_cast<float4*>(row + d) = s;
       if (d == 0) *reinterpret_cast<float2*>(row + D) = make_float2(mm, ll);
     }
   }
-  if (nsplit == 1) return;
-
-  // ---- join the chunks: the last CTA of this (sequence, head tile) to arrive ---------------
-  __threadfence();
-  __syncthreads();
-  if (tid == 0) {
-    int* counter = p.counters + (long long)b * gridDim.y + blockIdx.y;
-    const int n = atomicAdd(counter, 1);
-    last_flag = n == nsplit - 1;
-    if (last_flag) *counter = 0;
-  }
-  __syncthreads();
-  if (!last_flag) return;
-  __threadfence();
-  for (int e = tid; e < heads * D / 4; e += kThreads) {
-    const int h = e / (D / 4), d = (e % (D / 4)) * 4;
-    const float* rows = p.partials + (head0 + h) * p.splits * kRow;
-    float mm = -INFINITY;
-    for (int s = 0; s < nsplit; ++s) mm = fmaxf(mm, __ldcg(rows + s * kRow + D));
-    float ll = 0.f;
-    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int s = 0; s < nsplit; ++s) {
-      const float2 st = __ldcg(reinterpret_cast<const float2*>(rows + s * kRow + D));
-      const float4 v = __ldcg(reinterpret_cast<const float4*>(rows + s * kRow + d));
-      const float f = st.x == mm ? 1.f : ex2_approx(st.x - mm);
-      ll += f * st.y;
-      a.x += f * v.x; a.y += f * v.y; a.z += f * v.z; a.w += f * v.w;
+  if (!whole) {
+    // ---- join the CTAs of this segment: the last one to arrive -----------------------------
+    const long long start = (long long)prefix[seg.b] * Y + (long long)seg.y * seg.total;
+    const int first = cta_of(start), last = cta_of(start + seg.total - 1);
+    __threadfence();
+    __syncthreads();
+    if (tid == 0) {
+      int* counter = p.counters + (long long)seg.b * Y + seg.y;
+      const int n = atomicAdd(counter, 1);
+      last_flag = n == last - first;
+      if (last_flag) *counter = 0;
     }
-    const float r = ll != 0.f ? 1.f / ll : 0.f;
-    store_out4(p.out, p.dtype, (head0 + h) * D + d, make_float4(a.x * r, a.y * r, a.z * r, a.w * r));
+    __syncthreads();
+    if (last_flag) {
+      __threadfence();
+      // the part of CTA c: it begins in this segment in all but the first one
+      auto part = [&](int c, int h) {
+        return p.partials + ((size_t)(2 * c + (c == first ? 1 : 0)) * kHeads + h) * kRow;
+      };
+      for (int e = tid; e < heads * D / 4; e += kThreads) {
+        const int h = e / (D / 4), d = (e % (D / 4)) * 4;
+        float mm = -INFINITY, ll = 0.f;
+        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+        for (int c = first; c <= last; ++c) mm = fmaxf(mm, __ldcg(part(c, h) + D));
+#pragma unroll 8
+        for (int c = first; c <= last; ++c) {
+          const float* row = part(c, h);
+          const float2 st = __ldcg(reinterpret_cast<const float2*>(row + D));
+          const float4 v = __ldcg(reinterpret_cast<const float4*>(row + d));
+          const float f = st.x == mm ? 1.f : ex2_approx(st.x - mm);
+          ll += f * st.y;
+          a.x += f * v.x; a.y += f * v.y; a.z += f * v.z; a.w += f * v.w;
+        }
+        const float r = ll != 0.f ? 1.f / ll : 0.f;
+        store_out4(p.out, p.dtype, (head0 + h) * D + d, make_float4(a.x * r, a.y * r, a.z * r, a.w * r));
+      }
+    }
   }
+  __syncthreads();  // the joined results have been read before the next segment's are written
+  u += seg.n;
+  if (u < u1) next(seg, u);
+  }
+  // a wait that gave up: let this warp's copies in flight land before the CTA can exit
+  for (; used < fetched; ++used)
+    (void)mbar_wait_bounded(&bars[warp][used % kStages], (uint32_t)((used / kStages) & 1), nullptr);
 }
 
 template <int P, int BS, bool SPLIT>
-int launch(const DecodeInt4Params& p, dim3 grid, cudaStream_t st) {
-  if (!allow_smem<decode_int4_kernel<P, BS, SPLIT>>(smem_bytes<P>())) return SPD_ERR_CUDA;
-  decode_int4_kernel<P, BS, SPLIT><<<grid, kThreads, smem_bytes<P>(), st>>>(p);
+int launch(const DecodeInt4Params& p, int sms, cudaStream_t st) {
+  const size_t smem = smem_bytes<P, SPLIT>() + ((size_t)p.B + 1) * 4;
+  if (!allow_smem<decode_int4_kernel<P, BS, SPLIT>>(smem_bytes<P, SPLIT>() + 4097 * 4)) return SPD_ERR_CUDA;
+  if (p.whole) {
+    const int G = p.Hq / p.Hkv, kHeads = SPLIT ? 4 : 8;
+    const unsigned n = (unsigned)(p.B * p.Hkv * ((G + kHeads - 1) / kHeads));
+    decode_int4_kernel<P, BS, SPLIT><<<n, kThreads, smem_bytes<P, SPLIT>(), st>>>(p);
+    return cudaPeekAtLastError() == cudaSuccess ? SPD_OK : SPD_ERR_CUDA;
+  }
+  // as many CTAs as fit at once: by registers (found once) and by shared memory (228 KB an SM,
+  // 1 KB and the static part taken per CTA)
+  static const int by_regs = [] {
+    int n = 0;
+    return cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, decode_int4_kernel<P, BS, SPLIT>, kThreads,
+                                                         smem_bytes<P, SPLIT>()) == cudaSuccess && n > 0 ? n : 1;
+  }();
+  int per_sm = (int)(228 * 1024 / (smem + 2048));
+  per_sm = per_sm < 1 ? 1 : per_sm > by_regs ? by_regs : per_sm;
+  if (per_sm > kMaxCtas) per_sm = kMaxCtas;
+  decode_int4_kernel<P, BS, SPLIT><<<sms * per_sm, kThreads, smem, st>>>(p);
   return cudaPeekAtLastError() == cudaSuccess ? SPD_OK : SPD_ERR_CUDA;
 }
 
@@ -485,27 +711,22 @@ int launch(const DecodeInt4Params& p, dim3 grid, cudaStream_t st) {
 // Heads per column tile: four with two columns each, or eight.
 static int dec4_heads(int dtype, int G) { return (dtype == SPD_F32 || G <= 4) ? 4 : 8; }
 
-// Tokens per CTA: enough CTAs for four rounds of two per SM, each at least one step per warp
-// and at most 4096 tokens (which bounds what the slowest CTA of a ragged batch does alone).
-int decode_int4_chunk(int B, int Hq, int Hkv, int dtype, int max_ctx, int sms) {
-  const int G = Hq / Hkv, kHeads = dec4_heads(dtype, G);
-  const long long pairs = (long long)B * Hkv * ((G + kHeads - 1) / kHeads);
-  const long long unit = dec4::kWarps * dec4::kStep;
-  long long c = ((long long)max_ctx * pairs / (sms * 8) + unit - 1) / unit * unit;
-  return (int)(c < unit ? unit : c > 4096 ? 4096 : c);
+// Bytes of partial results: two slots per CTA.
+size_t decode_int4_partial_bytes(int Hq, int Hkv, int D, int dtype, int sms) {
+  return (size_t)sms * dec4::kMaxCtas * 2 * dec4_heads(dtype, Hq / Hkv) * (D + 4) * 4;
 }
 
-int decode_int4_launch(const DecodeInt4Params& p, int D, int bs, cudaStream_t st) {
+int decode_int4_launch(DecodeInt4Params p, int D, int bs, int sms, cudaStream_t st) {
   using namespace dec4;
-  const int G = p.Hq / p.Hkv, kHeads = dec4_heads(p.dtype, G);
-  const dim3 grid((unsigned)p.splits, (unsigned)(p.Hkv * ((G + kHeads - 1) / kHeads)), (unsigned)p.B);
+  p.whole = (long long)p.max_blocks * bs <= kWholeTokens;
+  const int kHeads = dec4_heads(p.dtype, p.Hq / p.Hkv);
   auto by_bs = [&](auto planes, auto split) -> int {
     constexpr int P = decltype(planes)::value;
     constexpr bool S = decltype(split)::value;
     switch (bs) {
-      case 8: return launch<P, 8, S>(p, grid, st);
-      case 16: return launch<P, 16, S>(p, grid, st);
-      case 32: return launch<P, 32, S>(p, grid, st);
+      case 8: return launch<P, 8, S>(p, sms, st);
+      case 16: return launch<P, 16, S>(p, sms, st);
+      case 32: return launch<P, 32, S>(p, sms, st);
       default: return SPD_ERR_UNSUPPORTED;
     }
   };

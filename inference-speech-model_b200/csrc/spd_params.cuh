@@ -149,12 +149,11 @@ struct DecodeInt4Params {  // single-token attention over a 4-bit pool (paged_de
   void* out;
   int dtype;
   int B, Hq, Hkv, max_blocks, num_blocks;
-  int chunk;          // tokens per CTA
-  int splits;         // CTAs per (sequence, key/value head, head tile)
+  int whole;          // one CTA per (sequence, head tile)
   float scale_log2;   // scale * log2(e)
   int* err;           // workspace error word
   int* counters;      // [B * Hkv * head tiles] arrivals, left at zero
-  float* partials;    // [B * Hq][splits][D + 2]
+  float* partials;    // two slots per CTA of [heads of a tile][D + 4]
   unsigned long long wait_ns;
 };
 
