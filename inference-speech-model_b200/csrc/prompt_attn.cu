@@ -58,14 +58,42 @@ __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, i
       : "memory");
 }
 
-// D[128 x N] (+)= A (TMEM, 16-bit pairs per column) * B (shared memory)
-__device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
-                                            uint32_t accumulate) {
+// One lane of a converged warp (the same one each time).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t is;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(is));
+  return is != 0;
+}
+
+// Four products of 16 k each, issued back to back: an operand's descriptors are its first one plus
+// a constant, so that the issue takes fewer cycles than the products (64 each at N = 128).
+// D[128 x N] (+)= A B, both in shared memory: k advances by 32 bytes inside the swizzle row.
+__device__ __forceinline__ void umma4_ss(uint32_t d_tmem, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
+      "{\n\t.reg .pred p;\n\t.reg .b64 a1, a2, a3, b1, b2, b3;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
-      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      "add.s64 a1, %1, 2;\n\tadd.s64 a2, %1, 4;\n\tadd.s64 a3, %1, 6;\n\t"
+      "add.s64 b1, %2, 2;\n\tadd.s64 b2, %2, 4;\n\tadd.s64 b3, %2, 6;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], a1, b1, %3, 1;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], a2, b2, %3, 1;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], a3, b3, %3, 1;\n\t}" ::"r"(d_tmem),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// D[128 x N] (+)= A B with A in TMEM (16-bit pairs, 8 columns per 16 k) and B MN-major: 16 k-rows
+// of 128 bytes further.
+__device__ __forceinline__ void umma4_ts(uint32_t d_tmem, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b32 a1, a2, a3;\n\t.reg .b64 b1, b2, b3;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "add.u32 a1, %1, 8;\n\tadd.u32 a2, %1, 16;\n\tadd.u32 a3, %1, 24;\n\t"
+      "add.s64 b1, %2, 128;\n\tadd.s64 b2, %2, 256;\n\tadd.s64 b3, %2, 384;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [a1], b1, %3, 1;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [a2], b2, %3, 1;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [a3], b3, %3, 1;\n\t}" ::"r"(d_tmem),
+      "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
       : "memory");
 }
 
@@ -126,6 +154,81 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   } else {
     const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&h);
+  }
+}
+
+// ---- pairs of fp32 in one instruction ----------------------------------------------------
+typedef unsigned long long f32x2;
+__device__ __forceinline__ f32x2 pair(float a, float b) {
+  f32x2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 unpair(f32x2 v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+  f32x2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+  f32x2 d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+
+// 2^x of a pair on the fp32 pipes, for x <= 100; below -125 it stays at 2^-125.  x is split into a
+// whole number n (adding 1.5 * 2^23 rounds it to the low bits) and f in [-1/2, 1/2]; 2^f is a
+// polynomial whose largest relative error is least (fitted by the Remez exchange to 2^f on that
+// interval: 7.5e-5 at degree 3, 2.6e-6 at degree 4), and n is added to its exponent field.  The
+// special-function unit gives 4 results a cycle and quarter SM, a quarter of what the softmax
+// needs; degree 3 is under a bf16 weight's rounding (2^-9), degree 4 under fp16's (2^-12).
+template <int DEG>
+__device__ __forceinline__ float2 exp2_poly(f32x2 x) {
+  float2 v = unpair(x);
+  x = pair(fmaxf(v.x, -125.f), fmaxf(v.y, -125.f));
+  const f32x2 t = add2(x, pair(12582912.f, 12582912.f));
+  const f32x2 f = fma2(add2(t, pair(-12582912.f, -12582912.f)), pair(-1.f, -1.f), x);
+  f32x2 q;
+  if constexpr (DEG == 3) {
+    q = fma2(pair(0.0551716691f, 0.0551716691f), f, pair(0.242611122f, 0.242611122f));
+    q = fma2(q, f, pair(0.693260985f, 0.693260985f));
+    q = fma2(q, f, pair(0.999928074f, 0.999928074f));
+  } else {
+    q = fma2(pair(0.00957010191f, 0.00957010191f), f, pair(0.0559178603f, 0.0559178603f));
+    q = fma2(q, f, pair(0.240247448f, 0.240247448f));
+    q = fma2(q, f, pair(0.693121815f, 0.693121815f));
+    q = fma2(q, f, pair(0.999999261f, 0.999999261f));
+  }
+  const float2 n = unpair(t), p = unpair(q);
+  return make_float2(__uint_as_float(__float_as_uint(p.x) + (__float_as_uint(n.x) << 23)),
+                     __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(n.y) << 23)));
+}
+
+#ifndef PA_EMU
+#define PA_EMU 4
+#endif
+// Weights of 64 keys: p = 2^(s * c - m) rounded to T and packed, sums added.  EXACT: all on the
+// special-function unit, so that a masked score (-inf) gives an exact zero; otherwise PA_EMU of
+// each 8 pairs go to the polynomial.
+template <typename T, bool EXACT>
+__device__ __forceinline__ void weights64(const uint32_t* s, f32x2 c, f32x2 neg_m, uint32_t* pk, f32x2 (&sum)[2]) {
+  constexpr int kDeg = std::is_same<T, __half>::value ? 4 : 3;
+#pragma unroll
+  for (int k = 0; k < 32; ++k) {
+    const f32x2 x = fma2(pair(__uint_as_float(s[2 * k]), __uint_as_float(s[2 * k + 1])), c, neg_m);
+    float2 e;
+    if (!EXACT && (k * PA_EMU) % 8 < PA_EMU) {  // spread evenly
+      e = exp2_poly<kDeg>(x);
+    } else {
+      const float2 v = unpair(x);
+      e = make_float2(ex2_approx(v.x), ex2_approx(v.y));
+    }
+    sum[k & 1] = add2(sum[k & 1], pair(e.x, e.y));
+    pk[k] = pack2<T>(e.x, e.y);
   }
 }
 
@@ -203,8 +306,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* q_full = kv_empty + C::kStages;    // [2]
   uint64_t* q_empty = q_full + 2;              // [2]
   uint64_t* s_full = q_empty + 2;              // [2] scores ready (and all earlier products done)
-  uint64_t* p_full = s_full + 2;               // [2] weights written, output rescaled
-  uint64_t* o_full = p_full + 2;               // [2] output complete
+  uint64_t* p_full = s_full + 2;               // [2 tiles][2 halves] weights written (and the output rescaled)
+  uint64_t* o_full = p_full + 4;               // [2] output complete
   uint64_t* o_empty = o_full + 2;              // [2] output read
   uint64_t* done = o_empty + 2;                // every MMA has completed
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
@@ -220,7 +323,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&q_full[x], 1);
       mbar_init(&q_empty[x], 1);
       mbar_init(&s_full[x], 1);
-      mbar_init(&p_full[x], 4);  // one arrival per warp
+      mbar_init(&p_full[2 * x], 4);  // one arrival per warp
+      mbar_init(&p_full[2 * x + 1], 4);
       mbar_init(&o_full[x], 1);
       mbar_init(&o_empty[x], 4);
     }
@@ -282,6 +386,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     } else if (warp == 1) {
       // ---- MMA issuer -------------------------------------------------------------------
       constexpr uint32_t idesc_s = instr_desc_f16(kBf16, BM, BN);
+      // descriptors of the first Q tile, and of the ring's first tile as K and as V
+      const uint64_t q_desc = smem_desc_sw128(q_tiles), kv_desc = smem_desc_sw128(kv_tiles),
+                     v_desc = smem_desc_mn(kv_tiles, C::kBoxBytes);
       constexpr uint32_t idesc_o = instr_desc_f16(kBf16, BM, DP) | (1u << 16);  // B is MN-major
       int q_use[2] = {0, 0}, p_use[2] = {0, 0}, o_use[2] = {0, 0};
       long long got = 0;
@@ -292,15 +399,12 @@ __global__ void __launch_bounds__(kThreads, 1)
           return mbar_wait_bounded(&kv_full[k % C::kStages], (uint32_t)((k / C::kStages) & 1), p.err, p.wait_ns);
         };
         auto scores = [&](int x, long long kslot) {  // S_x = Q_x K^T
-          if (lane == 0) {
-            const unsigned char* kt = kv_tiles + (kslot % C::kStages) * C::kTileBytes;
-            const unsigned char* qt = q_tiles + x * C::kTileBytes;
+          if (elect_one()) {
+            const uint64_t dq = q_desc + (uint64_t)(x * (C::kTileBytes >> 4));
+            const uint64_t dk = kv_desc + (uint64_t)((int)(kslot % C::kStages) * (C::kTileBytes >> 4));
 #pragma unroll
-            for (int c = 0; c < C::kBoxes; ++c) {
-              const uint64_t dq = smem_desc_sw128(qt + c * C::kBoxBytes), dk = smem_desc_sw128(kt + c * C::kBoxBytes);
-#pragma unroll
-              for (int k = 0; k < 4; ++k) umma_f16(tmem + x * BN, dq + 2 * k, dk + 2 * k, idesc_s, (c | k) != 0);
-            }
+            for (int c = 0; c < C::kBoxes; ++c)
+              umma4_ss(tmem + x * BN, dq + c * (C::kBoxBytes >> 4), dk + c * (C::kBoxBytes >> 4), idesc_s, c != 0);
             umma_commit(&s_full[x]);
           }
           __syncwarp();
@@ -315,7 +419,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           tc_fence_after();
           scores(x, got);
         }
-        if (ok && n && lane == 0) {
+        if (ok && n && elect_one()) {
           umma_commit(&kv_empty[got % C::kStages]);
           for (int x = 0; x < 2; ++x)
             if (w.n[x] == 1) umma_commit(&q_empty[x]);
@@ -338,8 +442,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (j >= w.n[x]) continue;
             if (j == 0 && o_use[x] > 0)
               ok = mbar_wait_bounded(&o_empty[x], (uint32_t)((o_use[x] - 1) & 1), p.err, p.wait_ns);
-            ok = ok && mbar_wait_bounded(&p_full[x], (uint32_t)(p_use[x] & 1), p.err, p.wait_ns);
-            ++p_use[x];
+            ok = ok && mbar_wait_bounded(&p_full[2 * x], (uint32_t)(p_use[x] & 1), p.err, p.wait_ns);
             const bool more = j + 1 < w.n[x];
             if (more && !k_seen) {
               ok = ok && kv_wait(kslot);
@@ -347,23 +450,28 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
+            // O_x += P_x V over 64 keys
+            const uint64_t dv = v_desc + (uint64_t)((int)(vslot % C::kStages) * (C::kTileBytes >> 4));
             tc_fence_after();
-            if (lane == 0) {
-#pragma unroll
-              for (int k = 0; k < BN / 16; ++k)
-                umma_f16_ts(tmem + C::kO + x * DP, tmem + x * BN + 8 * k, smem_desc_mn(vt + k * 2048, C::kBoxBytes), idesc_o,
-                            (j | k) != 0);
+            if (elect_one()) umma4_ts(tmem + C::kO + x * DP, tmem + x * BN, dv, idesc_o, j != 0);
+            __syncwarp();
+            ok = __all_sync(0xffffffffu, mbar_wait_bounded(&p_full[2 * x + 1], (uint32_t)(p_use[x] & 1), p.err, p.wait_ns));
+            ++p_use[x];
+            if (!ok) break;
+            tc_fence_after();
+            if (elect_one()) {
+              umma4_ts(tmem + C::kO + x * DP, tmem + x * BN + 32, dv + 4 * 128, idesc_o, 1);
               if (!more) umma_commit(&o_full[x]);
             }
             __syncwarp();
             if (more) {
               scores(x, kslot);
-              if (j + 2 == w.n[x] && lane == 0) umma_commit(&q_empty[x]);
+              if (j + 2 == w.n[x] && elect_one()) umma_commit(&q_empty[x]);
             } else {
               ++o_use[x];
             }
           }
-          if (ok && lane == 0) {
+          if (ok && elect_one()) {
             umma_commit(&kv_empty[vslot % C::kStages]);
             if (j + 1 < n) umma_commit(&kv_empty[kslot % C::kStages]);
           }
@@ -371,10 +479,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         got += 2 * n;
       }
-      if (lane == 0) {
-        umma_commit(done);
-        (void)mbar_wait_bounded(done, 0, p.err);
-      }
+      __syncwarp();
+      if (elect_one()) umma_commit(done);
+      (void)mbar_wait_bounded(done, 0, p.err);
       __syncwarp();
     }
   } else {
@@ -402,21 +509,41 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!ok) break;
         tc_fence_after();
         uint32_t s[BN];
-#pragma unroll
-        for (int c = 0; c < BN; c += 32) tmem_ld32_nowait(s_col + c, s + c);
-#pragma unroll
-        for (int c = 0; c < BN; c += 32) tmem_ld_wait(s + c);
+        tmem_ld32_nowait(s_col, s);
+        tmem_ld32_nowait(s_col + 32, s + 32);
+        tmem_ld_wait(s);
+        tmem_ld_wait(s + 32);
+        tmem_ld32_nowait(s_col + 64, s + 64);
+        tmem_ld32_nowait(s_col + 96, s + 96);
         const int base = j * BN;
-        if (base + BN > least) {
+        const bool edge = base + BN > least;  // some row of the tile does not see all of these keys
+        if (edge) {
+          tmem_ld_wait(s + 64);
+          tmem_ld_wait(s + 96);
           const int seen = limit - base;
 #pragma unroll
           for (int c = 0; c < BN; ++c)
             if (c >= seen) s[c] = 0xff800000u;  // -inf
         }
-        float mx = -INFINITY;
+        float mx4[4];
 #pragma unroll
-        for (int c = 0; c < BN; ++c) mx = fmaxf(mx, __uint_as_float(s[c]));
-        mx *= p.scale_log2;
+        for (int i = 0; i < 4; ++i) mx4[i] = __uint_as_float(s[i]);
+#pragma unroll
+        for (int c = 4; c < 64; c += 8)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            mx4[i] = c + 4 + i < 64 ? fmaxf(fmaxf(mx4[i], __uint_as_float(s[c + i])), __uint_as_float(s[c + 4 + i]))
+                                    : fmaxf(mx4[i], __uint_as_float(s[c + i]));
+        if (!edge) {
+          tmem_ld_wait(s + 64);
+          tmem_ld_wait(s + 96);
+        }
+#pragma unroll
+        for (int c = 64; c < BN; c += 8)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            mx4[i] = fmaxf(fmaxf(mx4[i], __uint_as_float(s[c + i])), __uint_as_float(s[c + 4 + i]));
+        const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * p.scale_log2;
         const bool raise = mx > m + kLazy;
         if (__any_sync(0xffffffffu, raise)) {
           const float mn = fmaxf(m, mx);
@@ -436,24 +563,22 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
         const float mm = m == -INFINITY ? 0.f : m;
-        float sum = 0.f;
+        const f32x2 c2 = pair(p.scale_log2, p.scale_log2), nm2 = pair(-mm, -mm);
+        f32x2 sum[2] = {pair(0.f, 0.f), pair(0.f, 0.f)};
+        // in two halves, each handed to the tensor cores when it is written
 #pragma unroll
-        for (int c = 0; c < BN; c += 64) {
+        for (int h = 0; h < 2; ++h) {
           uint32_t pk[32];
-#pragma unroll
-          for (int k = 0; k < 32; ++k) {
-            const float a = ex2_approx(fmaf(__uint_as_float(s[c + 2 * k]), p.scale_log2, -mm));
-            const float b = ex2_approx(fmaf(__uint_as_float(s[c + 2 * k + 1]), p.scale_log2, -mm));
-            sum += a + b;
-            pk[k] = pack2<T>(a, b);
-          }
-          tmem_st32(s_col + c / 2, pk);
+          if (edge) weights64<T, true>(s + 64 * h, c2, nm2, pk, sum);
+          else weights64<T, false>(s + 64 * h, c2, nm2, pk, sum);
+          tmem_st32(s_col + 32 * h, pk);
+          tmem_st_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&p_full[2 * x + h]);
         }
-        l += sum;
-        tmem_st_wait();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[x]);
+        const float2 t2 = unpair(add2(sum[0], sum[1]));
+        l += t2.x + t2.y;
       }
       if (!ok) break;
       T* out = reinterpret_cast<T*>(p.out) +
