@@ -232,6 +232,23 @@ __device__ __forceinline__ void weights64(const uint32_t* s, f32x2 c, f32x2 neg_
   }
 }
 
+// Position in a ring of stages: the slot, and how often the ring has come round.
+struct Ring {
+  int slot = 0, round = 0;
+  __device__ __forceinline__ uint32_t phase() const { return (uint32_t)(round & 1); }
+  __device__ __forceinline__ void next(int stages) {
+    if (++slot == stages) slot = 0, ++round;
+  }
+  __device__ __forceinline__ void back(int stages) {
+    if (--slot < 0) slot = stages - 1, --round;
+  }
+  __device__ __forceinline__ void skip(int n, int stages) {
+    slot += n;
+    round += slot / stages;
+    slot %= stages;
+  }
+};
+
 // One unit of work: 2 x 128 query rows (tokens [tok0, tok0 + 256 / pack) of one sequence for
 // `pack` heads from h0).
 struct Item {
@@ -309,7 +326,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* p_full = s_full + 2;               // [2 tiles][2 halves] weights written (and the output rescaled)
   uint64_t* o_full = p_full + 4;               // [2] output complete
   uint64_t* o_empty = o_full + 2;              // [2] output read
-  uint64_t* done = o_empty + 2;                // every MMA has completed
+  uint64_t* v_landed = o_empty + 2;            // a V tile with rows past the last key is there
+  uint64_t* v_fixed = v_landed + 1;            // and those rows are zero
+  uint64_t* done = v_fixed + 1;                // every MMA has completed
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -328,6 +347,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&o_full[x], 1);
       mbar_init(&o_empty[x], 4);
     }
+    mbar_init(v_landed, 1);
+    mbar_init(v_fixed, 1);
     mbar_init(done, 1);
     fence_barrier_init();
   }
@@ -342,20 +363,19 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (warp == 0) {
       // ---- TMA: Q tiles, then K and V tiles of each step, through one ring ------------------
       const int half_tok = BM / p.pack;
-      int it = 0, s = 0, q_use[2] = {0, 0};
-      long long issued = 0;
+      int q_use[2] = {0, 0};
+      Ring ring;
       bool ok = true;
       auto load_kv = [&](const CUtensorMap* map, int kv_row) {
-        if (issued >= C::kStages)
-          ok = mbar_wait_bounded(&kv_empty[s], (uint32_t)(((issued / C::kStages) & 1) ^ 1), p.err, p.wait_ns);
+        if (ring.round) ok = mbar_wait_bounded(&kv_empty[ring.slot], ring.phase() ^ 1u, p.err, p.wait_ns);
         if (!ok) return;
-        mbar_arrive_expect_tx(&kv_full[s], C::kTileBytes);
+        mbar_arrive_expect_tx(&kv_full[ring.slot], C::kTileBytes);
         for (int c = 0; c < C::kBoxes; ++c)
-          tma_load_3d(kv_tiles + s * C::kTileBytes + c * C::kBoxBytes, map, 64 * c, w.kvh, kv_row, &kv_full[s]);
-        ++issued;
-        s = s + 1 == C::kStages ? 0 : s + 1;
+          tma_load_3d(kv_tiles + ring.slot * C::kTileBytes + c * C::kBoxBytes, map, 64 * c, w.kvh, kv_row,
+                      &kv_full[ring.slot]);
+        ring.next(C::kStages);
       };
-      for (it = blockIdx.x; ok && find_item(p, it, w); it += gridDim.x) {
+      for (int it = blockIdx.x; ok && find_item(p, it, w); it += gridDim.x) {
         if (lane == 0) {
           const int n = max(w.n[0], w.n[1]);
           auto load_q = [&](int x) {
@@ -378,111 +398,128 @@ __global__ void __launch_bounds__(kThreads, 1)
         ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
       }
       if (!ok && lane == 0) {  // let the copies in flight land before the CTA can exit
-        for (long long k = issued - 1; k >= 0 && k >= issued - C::kStages; --k)
-          (void)mbar_wait_bounded(&kv_full[k % C::kStages], (uint32_t)((k / C::kStages) & 1), nullptr);
+        for (int k = 0; k < C::kStages; ++k) {
+          ring.back(C::kStages);
+          if (ring.round >= 0) (void)mbar_wait_bounded(&kv_full[ring.slot], ring.phase(), nullptr);
+        }
         for (int x = 0; x < 2; ++x)
           if (q_use[x]) (void)mbar_wait_bounded(&q_full[x], (uint32_t)((q_use[x] - 1) & 1), nullptr);
       }
     } else if (warp == 1) {
-      // ---- MMA issuer -------------------------------------------------------------------
+      // ---- MMA issuer: one lane, with nothing but waits and issues in its step -----------------
       constexpr uint32_t idesc_s = instr_desc_f16(kBf16, BM, BN);
+      constexpr uint32_t idesc_o = instr_desc_f16(kBf16, BM, DP) | (1u << 16);  // B is MN-major
+      constexpr uint32_t kTile16 = C::kTileBytes >> 4, kBox16 = C::kBoxBytes >> 4;
       // descriptors of the first Q tile, and of the ring's first tile as K and as V
       const uint64_t q_desc = smem_desc_sw128(q_tiles), kv_desc = smem_desc_sw128(kv_tiles),
                      v_desc = smem_desc_mn(kv_tiles, C::kBoxBytes);
-      constexpr uint32_t idesc_o = instr_desc_f16(kBf16, BM, DP) | (1u << 16);  // B is MN-major
-      int q_use[2] = {0, 0}, p_use[2] = {0, 0}, o_use[2] = {0, 0};
-      long long got = 0;
+      const bool leader = elect_one();
+      const int leader_lane = __ffs(__ballot_sync(0xffffffffu, leader)) - 1;
+      uint32_t q_ph[2] = {0, 0}, p_ph[2] = {0, 0}, o_ph[2] = {1, 1}, fix_ph = 0;
+      Ring ring;
       bool ok = true;
+      auto wait = [&](uint64_t* bar, uint32_t phase) {
+        if (ok) ok = mbar_wait_bounded(bar, phase, p.err, p.wait_ns);
+      };
+      auto scores = [&](int x, int slot) {  // S_x = Q_x K^T
+#pragma unroll
+        for (int c = 0; c < C::kBoxes; ++c)
+          umma4_ss(tmem + x * BN, q_desc + (uint64_t)(x * kTile16 + c * kBox16), kv_desc + (uint64_t)(slot * kTile16 + c * kBox16),
+                   idesc_s, c != 0);
+        umma_commit(&s_full[x]);
+      };
       for (int it = blockIdx.x; ok && find_item(p, it, w); it += gridDim.x) {
         const int n = max(w.n[0], w.n[1]);
-        auto kv_wait = [&](long long k) {
-          return mbar_wait_bounded(&kv_full[k % C::kStages], (uint32_t)((k / C::kStages) & 1), p.err, p.wait_ns);
-        };
-        auto scores = [&](int x, long long kslot) {  // S_x = Q_x K^T
-          if (elect_one()) {
-            const uint64_t dq = q_desc + (uint64_t)(x * (C::kTileBytes >> 4));
-            const uint64_t dk = kv_desc + (uint64_t)((int)(kslot % C::kStages) * (C::kTileBytes >> 4));
+        if (n > 0 && leader) {
+          int kslot = ring.slot;
+          wait(&kv_full[kslot], ring.phase());
+          ring.next(C::kStages);
 #pragma unroll
-            for (int c = 0; c < C::kBoxes; ++c)
-              umma4_ss(tmem + x * BN, dq + c * (C::kBoxBytes >> 4), dk + c * (C::kBoxBytes >> 4), idesc_s, c != 0);
-            umma_commit(&s_full[x]);
-          }
-          __syncwarp();
-        };
-        // slots of this item: K_j at got + 2j, V_j at got + 2j + 1
-        for (int x = 0; x < 2 && ok; ++x) {
-          if (!w.n[x]) continue;
-          ok = mbar_wait_bounded(&q_full[x], (uint32_t)(q_use[x] & 1), p.err, p.wait_ns) && kv_wait(got);
-          ++q_use[x];
-          ok = __all_sync(0xffffffffu, ok);
-          if (!ok) break;
-          tc_fence_after();
-          scores(x, got);
-        }
-        if (ok && n && elect_one()) {
-          umma_commit(&kv_empty[got % C::kStages]);
           for (int x = 0; x < 2; ++x)
-            if (w.n[x] == 1) umma_commit(&q_empty[x]);
-        }
-        for (int j = 0; j < n && ok; ++j) {
-          const long long vslot = got + 2 * j + 1, kslot = got + 2 * j + 2;
-          ok = __all_sync(0xffffffffu, kv_wait(vslot));
-          if (!ok) break;
-          unsigned char* vt = kv_tiles + (vslot % C::kStages) * C::kTileBytes;
-          const int valid = w.Tk - j * BN;
-          if (valid < BN) {  // zero the rows of V past the sequence's last key
-            for (int i = lane; i < (BN - valid) * 8; i += 32)
-              for (int c = 0; c < C::kBoxes; ++c)
-                *reinterpret_cast<uint4*>(vt + c * C::kBoxBytes + valid * 128 + i * 16) = make_uint4(0, 0, 0, 0);
-            fence_proxy_async_smem();
-            __syncwarp();
-          }
-          bool k_seen = false;
-          for (int x = 0; x < 2 && ok; ++x) {
-            if (j >= w.n[x]) continue;
-            if (j == 0 && o_use[x] > 0)
-              ok = mbar_wait_bounded(&o_empty[x], (uint32_t)((o_use[x] - 1) & 1), p.err, p.wait_ns);
-            ok = ok && mbar_wait_bounded(&p_full[2 * x], (uint32_t)(p_use[x] & 1), p.err, p.wait_ns);
-            const bool more = j + 1 < w.n[x];
-            if (more && !k_seen) {
-              ok = ok && kv_wait(kslot);
-              k_seen = true;
-            }
-            ok = __all_sync(0xffffffffu, ok);
-            if (!ok) break;
-            // O_x += P_x V over 64 keys
-            const uint64_t dv = v_desc + (uint64_t)((int)(vslot % C::kStages) * (C::kTileBytes >> 4));
-            tc_fence_after();
-            if (elect_one()) umma4_ts(tmem + C::kO + x * DP, tmem + x * BN, dv, idesc_o, j != 0);
-            __syncwarp();
-            ok = __all_sync(0xffffffffu, mbar_wait_bounded(&p_full[2 * x + 1], (uint32_t)(p_use[x] & 1), p.err, p.wait_ns));
-            ++p_use[x];
-            if (!ok) break;
-            tc_fence_after();
-            if (elect_one()) {
-              umma4_ts(tmem + C::kO + x * DP, tmem + x * BN + 32, dv + 4 * 128, idesc_o, 1);
-              if (!more) umma_commit(&o_full[x]);
-            }
-            __syncwarp();
-            if (more) {
+            if (w.n[x]) {
+              wait(&q_full[x], q_ph[x]);
+              q_ph[x] ^= 1;
+              if (!ok) break;
+              tc_fence_after();
               scores(x, kslot);
-              if (j + 2 == w.n[x] && elect_one()) umma_commit(&q_empty[x]);
-            } else {
-              ++o_use[x];
+              if (w.n[x] == 1) umma_commit(&q_empty[x]);
             }
+          umma_commit(&kv_empty[kslot]);
+          for (int j = 0; j < n && ok; ++j) {
+            const int vslot = ring.slot;
+            wait(&kv_full[vslot], ring.phase());
+            ring.next(C::kStages);
+            const bool ragged = w.Tk - j * BN < BN;
+            if (ragged && ok) mbar_arrive(v_landed);
+            kslot = ring.slot;
+            if (j + 1 < n) {
+              wait(&kv_full[kslot], ring.phase());
+              ring.next(C::kStages);
+            }
+            if (ragged) {  // the rows past the last key are zero
+              wait(v_fixed, fix_ph);
+              fix_ph ^= 1;
+            }
+            const uint64_t dv = v_desc + (uint64_t)(vslot * kTile16);
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              if (j >= w.n[x] || !ok) continue;
+              if (j == 0) {
+                wait(&o_empty[x], o_ph[x]);  // passes at once the first time
+                o_ph[x] ^= 1;
+              }
+              // O_x += P_x V, each half of the keys when its weights are there
+              wait(&p_full[2 * x], p_ph[x]);
+              if (!ok) continue;
+              tc_fence_after();
+              umma4_ts(tmem + C::kO + x * DP, tmem + x * BN, dv, idesc_o, j != 0);
+              wait(&p_full[2 * x + 1], p_ph[x]);
+              p_ph[x] ^= 1;
+              if (!ok) continue;
+              tc_fence_after();
+              umma4_ts(tmem + C::kO + x * DP, tmem + x * BN + 32, dv + 4 * 128, idesc_o, 1);
+              if (j + 1 < w.n[x]) {
+                scores(x, kslot);
+                if (j + 2 == w.n[x]) umma_commit(&q_empty[x]);
+              } else {
+                umma_commit(&o_full[x]);
+              }
+            }
+            umma_commit(&kv_empty[vslot]);
+            if (j + 1 < n) umma_commit(&kv_empty[kslot]);
           }
-          if (ok && elect_one()) {
-            umma_commit(&kv_empty[vslot % C::kStages]);
-            if (j + 1 < n) umma_commit(&kv_empty[kslot % C::kStages]);
-          }
-          __syncwarp();
         }
-        got += 2 * n;
+        __syncwarp();
+        ok = __shfl_sync(0xffffffffu, (int)ok, leader_lane) != 0;
       }
+      if (leader) umma_commit(done);
       __syncwarp();
-      if (elect_one()) umma_commit(done);
       (void)mbar_wait_bounded(done, 0, p.err);
       __syncwarp();
+    } else if (warp == 2) {
+      // ---- rows of V past a sequence's last key: zero, before they are multiplied ----------------
+      // (told by the MMA lane that the tile is there: this warp does not follow the ring's phases)
+      Ring ring;
+      uint32_t ph = 0;
+      bool ok = true;
+      for (int it = blockIdx.x; ok && find_item(p, it, w); it += gridDim.x) {
+        const int n = max(w.n[0], w.n[1]), valid = w.Tk - (n - 1) * BN;
+        if (n == 0) continue;
+        ring.skip(2 * n - 1, C::kStages);
+        if (valid < BN) {
+          ok = __all_sync(0xffffffffu, mbar_wait_bounded(v_landed, ph, p.err, p.wait_ns));
+          if (!ok) break;
+          ph ^= 1;
+          unsigned char* vt = kv_tiles + ring.slot * C::kTileBytes;
+          for (int i = lane; i < (BN - valid) * 8; i += 32)
+            for (int c = 0; c < C::kBoxes; ++c)
+              *reinterpret_cast<uint4*>(vt + c * C::kBoxBytes + valid * 128 + i * 16) = make_uint4(0, 0, 0, 0);
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(v_fixed);
+        }
+        ring.skip(1, C::kStages);
+      }
     }
   } else {
     // ---- softmax and epilogue of tile x: thread = query row = TMEM lane --------------------
