@@ -155,6 +155,7 @@ __global__ void __launch_bounds__(kThreads, P == 4 ? 1 : DEC4_MB) decode_int4_ke
     return (long long)c > (long long)p.max_blocks * BS ? p.max_blocks * BS : c < 0 ? 0 : c;
   };
   auto zeros = [&](int b, int h0, int n) {  // a sequence without a context
+#pragma unroll 1
     for (int i = tid; i < n * D / 4; i += kThreads)
       store_out4(p.out, p.dtype, ((long long)b * p.Hq + h0) * D + i * 4, make_float4(0.f, 0.f, 0.f, 0.f));
   };
@@ -178,6 +179,7 @@ __global__ void __launch_bounds__(kThreads, P == 4 ? 1 : DEC4_MB) decode_int4_ke
   } else {
     // ---- steps before each sequence --------------------------------------------------------
     int base = 0;
+#pragma unroll 1
     for (int b0 = 0; b0 < p.B; b0 += kThreads) {
       const int b = b0 + tid;
       int n = 0;
@@ -207,6 +209,7 @@ __global__ void __launch_bounds__(kThreads, P == 4 ? 1 : DEC4_MB) decode_int4_ke
     if (tid == 0) prefix[p.B] = base;
     __syncthreads();
     if (blockIdx.x == 0)
+#pragma unroll 1
       for (int b = 0; b < p.B; ++b)
         if (prefix[b + 1] == prefix[b]) zeros(b, 0, p.Hq);
     // ---- this CTA's share ------------------------------------------------------------------
@@ -236,6 +239,7 @@ __global__ void __launch_bounds__(kThreads, P == 4 ? 1 : DEC4_MB) decode_int4_ke
   auto next = [&](Segment& s, long long u) {  // the segment after s, which begins at unit u < u1
     if (++s.y == Y) {
       s.y = 0;
+#pragma unroll 1
       do ++s.b; while (prefix[s.b + 1] == prefix[s.b]);
       s.total = prefix[s.b + 1] - prefix[s.b];
     }
@@ -259,6 +263,7 @@ __global__ void __launch_bounds__(kThreads, P == 4 ? 1 : DEC4_MB) decode_int4_ke
   int ahead_i = warp, id = -1, ahead_pages = 0, fetched = 0, ahead_ctx = ctx_of(ahead.b);
   bool more = true;
   auto look_up = [&]() {
+#pragma unroll 1
     while (more && ahead_i >= ahead.n) {
       ahead_u += ahead.n;
       ahead_i = warp;
@@ -292,6 +297,7 @@ __global__ void __launch_bounds__(kThreads, P == 4 ? 1 : DEC4_MB) decode_int4_ke
     look_up();
   };
   look_up();
+#pragma unroll 1
   for (int i = 0; i < kStages; ++i) fetch();
 
   // Row r of an 8-token group holds token r ^ (r >> 2): with it both the rows that a
@@ -306,6 +312,7 @@ __global__ void __launch_bounds__(kThreads, P == 4 ? 1 : DEC4_MB) decode_int4_ke
   float2* par = reinterpret_cast<float2*>(joined + warp * kHeads * D);
   int used = 0;
   bool fine = true;
+#pragma unroll 1
   for (long long u = u0; u < u1; ) {
   const int tile = seg.y % tiles, kvh = seg.y / tiles;
   const int heads = min(kHeads, G - tile * kHeads);  // of this tile
@@ -378,9 +385,10 @@ __global__ void __launch_bounds__(kThreads, P == 4 ? 1 : DEC4_MB) decode_int4_ke
     for (int i = 0; i < 16; ++i) o[pl][i >> 2][i & 3] = 0.f;
   int lift = -15;  // exponent of the largest value scale seen; weights carry 2^(6 - lift)
 
+#pragma unroll 1
   for (int i = warp; i < seg.n && fine; i += kWarps) {
     const int st = used % kStages;
-    const bool ok = mbar_wait_bounded(&bars[warp][st], (uint32_t)((used / kStages) & 1), p.err, p.wait_ns);
+    const bool ok = mbar_wait_suspend(&bars[warp][st], (uint32_t)((used / kStages) & 1), p.err, p.wait_ns);
     fine = __all_sync(0xffffffffu, ok);
     if (!fine) break;
     ++used;
@@ -611,6 +619,7 @@ __global__ void __launch_bounds__(kThreads, P == 4 ? 1 : DEC4_MB) decode_int4_ke
   const bool whole = seg.step0 == 0 && seg.n == seg.total;
   // a CTA has at most two segments that others share: the one it begins in and the one it ends in
   float* slot = p.partials + (size_t)(2 * blockIdx.x + (seg.step0 == 0 ? 1 : 0)) * kHeads * kRow;
+#pragma unroll 1
   for (int e = tid; e < heads * D / 4; e += kThreads) {
     const int h = e / (D / 4), d = (e % (D / 4)) * 4;
     float mm = -INFINITY;
@@ -653,6 +662,7 @@ __global__ void __launch_bounds__(kThreads, P == 4 ? 1 : DEC4_MB) decode_int4_ke
       auto part = [&](int c, int h) {
         return p.partials + ((size_t)(2 * c + (c == first ? 1 : 0)) * kHeads + h) * kRow;
       };
+#pragma unroll 1
       for (int e = tid; e < heads * D / 4; e += kThreads) {
         const int h = e / (D / 4), d = (e % (D / 4)) * 4;
         float mm = -INFINITY, ll = 0.f;
@@ -678,8 +688,9 @@ __global__ void __launch_bounds__(kThreads, P == 4 ? 1 : DEC4_MB) decode_int4_ke
   if (u < u1) next(seg, u);
   }
   // a wait that gave up: let this warp's copies in flight land before the CTA can exit
+#pragma unroll 1
   for (; used < fetched; ++used)
-    (void)mbar_wait_bounded(&bars[warp][used % kStages], (uint32_t)((used / kStages) & 1), nullptr);
+    (void)mbar_wait_suspend(&bars[warp][used % kStages], (uint32_t)((used / kStages) & 1), nullptr);
 }
 
 template <int P, int BS, bool SPLIT>

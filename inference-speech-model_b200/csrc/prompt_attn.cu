@@ -208,12 +208,11 @@ __device__ __forceinline__ float2 exp2_poly(f32x2 x) {
                      __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(n.y) << 23)));
 }
 
-#ifndef PA_EMU
-#define PA_EMU 4
-#endif
+constexpr int kPoly = 2;  // of 8 pairs, to the polynomial
 // Weights of 64 keys: p = 2^(s * c - m) rounded to T and packed, sums added.  EXACT: all on the
-// special-function unit, so that a masked score (-inf) gives an exact zero; otherwise PA_EMU of
-// each 8 pairs go to the polynomial.
+// special-function unit, so that a masked score (-inf) gives an exact zero; otherwise kPoly of
+// each 8 pairs go to the polynomial (0: 492 us, 2: 484 us, 4: 496 us for 8192 causal tokens, 32 / 8
+// heads of 128; the polynomial's six packed fp32 instructions soon cost more than they free).
 template <typename T, bool EXACT>
 __device__ __forceinline__ void weights64(const uint32_t* s, f32x2 c, f32x2 neg_m, uint32_t* pk, f32x2 (&sum)[2]) {
   constexpr int kDeg = std::is_same<T, __half>::value ? 4 : 3;
@@ -221,7 +220,7 @@ __device__ __forceinline__ void weights64(const uint32_t* s, f32x2 c, f32x2 neg_
   for (int k = 0; k < 32; ++k) {
     const f32x2 x = fma2(pair(__uint_as_float(s[2 * k]), __uint_as_float(s[2 * k + 1])), c, neg_m);
     float2 e;
-    if (!EXACT && (k * PA_EMU) % 8 < PA_EMU) {  // spread evenly
+    if (!EXACT && (k * kPoly) % 8 < kPoly) {  // spread evenly
       e = exp2_poly<kDeg>(x);
     } else {
       const float2 v = unpair(x);
@@ -367,7 +366,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       Ring ring;
       bool ok = true;
       auto load_kv = [&](const CUtensorMap* map, int kv_row) {
-        if (ring.round) ok = mbar_wait_bounded(&kv_empty[ring.slot], ring.phase() ^ 1u, p.err, p.wait_ns);
+        if (ring.round) ok = mbar_wait_suspend(&kv_empty[ring.slot], ring.phase() ^ 1u, p.err, p.wait_ns);
         if (!ok) return;
         mbar_arrive_expect_tx(&kv_full[ring.slot], C::kTileBytes);
         for (int c = 0; c < C::kBoxes; ++c)
@@ -380,7 +379,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           const int n = max(w.n[0], w.n[1]);
           auto load_q = [&](int x) {
             if (!w.n[x] || !ok) return;
-            if (q_use[x] > 0) ok = mbar_wait_bounded(&q_empty[x], (uint32_t)((q_use[x] - 1) & 1), p.err, p.wait_ns);
+            if (q_use[x] > 0) ok = mbar_wait_suspend(&q_empty[x], (uint32_t)((q_use[x] - 1) & 1), p.err, p.wait_ns);
             if (!ok) return;
             ++q_use[x];
             mbar_arrive_expect_tx(&q_full[x], C::kTileBytes);
@@ -400,10 +399,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!ok && lane == 0) {  // let the copies in flight land before the CTA can exit
         for (int k = 0; k < C::kStages; ++k) {
           ring.back(C::kStages);
-          if (ring.round >= 0) (void)mbar_wait_bounded(&kv_full[ring.slot], ring.phase(), nullptr);
+          if (ring.round >= 0) (void)mbar_wait_suspend(&kv_full[ring.slot], ring.phase(), nullptr);
         }
         for (int x = 0; x < 2; ++x)
-          if (q_use[x]) (void)mbar_wait_bounded(&q_full[x], (uint32_t)((q_use[x] - 1) & 1), nullptr);
+          if (q_use[x]) (void)mbar_wait_suspend(&q_full[x], (uint32_t)((q_use[x] - 1) & 1), nullptr);
       }
     } else if (warp == 1) {
       // ---- MMA issuer: one lane, with nothing but waits and issues in its step -----------------
@@ -419,7 +418,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       Ring ring;
       bool ok = true;
       auto wait = [&](uint64_t* bar, uint32_t phase) {
-        if (ok) ok = mbar_wait_bounded(bar, phase, p.err, p.wait_ns);
+        if (ok) ok = mbar_wait_suspend(bar, phase, p.err, p.wait_ns);
       };
       auto scores = [&](int x, int slot) {  // S_x = Q_x K^T
 #pragma unroll
@@ -494,7 +493,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (leader) umma_commit(done);
       __syncwarp();
-      (void)mbar_wait_bounded(done, 0, p.err);
+      (void)mbar_wait_suspend(done, 0, p.err);
       __syncwarp();
     } else if (warp == 2) {
       // ---- rows of V past a sequence's last key: zero, before they are multiplied ----------------
@@ -507,7 +506,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (n == 0) continue;
         ring.skip(2 * n - 1, C::kStages);
         if (valid < BN) {
-          ok = __all_sync(0xffffffffu, mbar_wait_bounded(v_landed, ph, p.err, p.wait_ns));
+          ok = __all_sync(0xffffffffu, mbar_wait_suspend(v_landed, ph, p.err, p.wait_ns));
           if (!ok) break;
           ph ^= 1;
           unsigned char* vt = kv_tiles + ring.slot * C::kTileBytes;
@@ -541,7 +540,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       float m = -INFINITY, l = 0.f;
       const int n = w.n[x];
       for (int j = 0; j < n; ++j) {
-        ok = __all_sync(0xffffffffu, mbar_wait_bounded(&s_full[x], (uint32_t)(s_use & 1), p.err, p.wait_ns));
+        ok = __all_sync(0xffffffffu, mbar_wait_suspend(&s_full[x], (uint32_t)(s_use & 1), p.err, p.wait_ns));
         ++s_use;
         if (!ok) break;
         tc_fence_after();
@@ -622,7 +621,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                ((long long)(w.q0 + tok) * p.Hq + w.h0 + row % p.pack) * p.D;
       const bool live = tok < w.Tq;
       if (n > 0) {
-        ok = __all_sync(0xffffffffu, mbar_wait_bounded(&o_full[x], (uint32_t)(o_use & 1), p.err, p.wait_ns));
+        ok = __all_sync(0xffffffffu, mbar_wait_suspend(&o_full[x], (uint32_t)(o_use & 1), p.err, p.wait_ns));
         ++o_use;
         if (!ok) break;
         tc_fence_after();

@@ -228,6 +228,38 @@ __device__ __forceinline__ bool mbar_wait_bounded(uint64_t* bar, uint32_t parity
   }
 }
 
+// As mbar_wait_bounded, for kernels whose other warps compute while this one waits: each try may
+// suspend the thread for up to kSuspendNs (it wakes when the phase completes), so that a waiting
+// warp takes next to no issue slots.  The clock is read after every try.
+constexpr uint32_t kSuspendNs = 100000;
+__device__ __forceinline__ bool mbar_try_wait_suspend(uint64_t* bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(done)
+      : "r"(smem_addr(bar)), "r"(parity), "r"(kSuspendNs)
+      : "memory");
+  return done != 0;
+}
+__device__ __forceinline__ bool mbar_wait_more(uint64_t* bar, uint32_t parity, int* err, unsigned long long limit_ns) {
+  const unsigned long long t0 = global_ns();
+#pragma unroll 1
+  while (!mbar_try_wait_suspend(bar, parity))
+    if (global_ns() - t0 > limit_ns) {
+      set_error(err, SPD_DEVERR_TIMEOUT);
+      return false;
+    }
+  return true;
+}
+
+// instruction-cache room is worth more than a call there.
+__device__ __forceinline__ bool mbar_wait_suspend(uint64_t* bar, uint32_t parity, int* err,
+                                                  unsigned long long limit_ns = SPD_WAIT_NS) {
+  return mbar_try_wait_suspend(bar, parity) || mbar_wait_more(bar, parity, err, limit_ns);
+}
+
 // 2^x by the hardware approximation (ex2.approx.ftz: results below 2^-126 are 0, which for
 // softmax weights relative to the running maximum is exact enough); 2^-inf = 0.
 __device__ __forceinline__ float ex2_approx(float x) {
