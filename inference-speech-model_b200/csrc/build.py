@@ -6,6 +6,8 @@ Every ``*.cu`` file in this directory is compiled to an object with
 ``-gencode arch=compute_100a,code=sm_100a -lineinfo -O3`` (in parallel), then linked
 into ``../lib/libspd_b200.so`` with the CUDA runtime linked statically, so the library
 carries no dependency on the CUDA runtime that the host process happens to load.
+``torch_binding.cpp`` becomes the CPython module ``../lib/spd_torch.so`` beside it (g++,
+torch's headers; it holds no kernel).
 Objects are rebuilt only when a source or header is newer than them.
 
 ``python build.py --trace`` builds the trace variant instead: the same sources with
@@ -29,6 +31,7 @@ PKG = HERE.parent
 REPO = PKG.parent
 OBJ_DIR = PKG / "_build"
 LIB = PKG / "lib" / "libspd_b200.so"
+BINDING = PKG / "lib" / "spd_torch.so"  # CPython module over torch's headers (torch_binding.cpp)
 TRACE_OBJ_DIR = OBJ_DIR / "trace"
 TRACE_LIB = PKG / "lib" / "libspd_b200_trace.so"
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -50,6 +53,31 @@ def _stale(obj: Path, deps: list[Path]) -> bool:
     return any(d.stat().st_mtime > t for d in deps)
 
 
+def build_binding(force: bool = False) -> Path:
+    """Compiles torch_binding.cpp (no kernels) into ``../lib/spd_torch.so``."""
+    import sysconfig
+
+    import torch
+
+    src = HERE / "torch_binding.cpp"
+    if not force and not _stale(BINDING, [src, REPO / "include" / "spd_b200.h"]):
+        return BINDING
+    BINDING.parent.mkdir(parents=True, exist_ok=True)
+    root = Path(torch.__file__).resolve().parent
+    cuda = Path(nvcc()).resolve().parent.parent
+    cmd = [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", "-I", str(REPO / "include"),
+           "-I", str(root / "include"), "-I", str(root / "include" / "torch" / "csrc" / "api" / "include"),
+           "-I", str(cuda / "include"), "-I", sysconfig.get_paths()["include"], str(src), "-o", str(BINDING),
+           "-L", str(root / "lib"), "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda",
+           f"-Wl,-rpath,{root / 'lib'}"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        sys.stderr.write(r.stdout + r.stderr)
+        raise RuntimeError("g++ failed for: torch_binding.cpp")
+    return BINDING
+
+
 def build(verbose: bool = False, force: bool = False, trace: bool = False) -> Path:
     obj_dir, lib = (TRACE_OBJ_DIR, TRACE_LIB) if trace else (OBJ_DIR, LIB)
     flags = NVCC_FLAGS + (["-DSPD_TRACE_BUILD"] if trace else [])
@@ -68,6 +96,7 @@ def build(verbose: bool = False, force: bool = False, trace: bool = False) -> Pa
         src, cmd = job
         r = subprocess.run(cmd, capture_output=True, text=True)
         return src, r
+    binding = None if trace else cf.ThreadPoolExecutor(max_workers=1).submit(build_binding, force)
     failed = []
     with cf.ThreadPoolExecutor(max_workers=max(1, min(len(jobs), os.cpu_count() or 4))) as ex:
         for src, r in ex.map(run, jobs):
@@ -75,6 +104,8 @@ def build(verbose: bool = False, force: bool = False, trace: bool = False) -> Pa
                 sys.stderr.write(r.stdout + r.stderr)
             if r.returncode != 0:
                 failed.append(src.name)
+    if binding is not None:
+        binding.result()
     if failed:
         raise RuntimeError(f"nvcc failed for: {', '.join(failed)}")
     objs = [obj_dir / (s.stem + ".o") for s in sources]

@@ -88,6 +88,35 @@ def load() -> C.CDLL:
     return lib
 
 
+# CPython module that hands torch tensors to the C ABI without ctypes (csrc/torch_binding.cpp)
+BINDING_PATH = _PKG_ROOT / "lib" / "spd_torch.so"
+_binding = None
+
+
+def binding():
+    """Loads the torch binding once and gives it the addresses of the library's functions."""
+    global _binding
+    if _binding is not None:
+        return _binding
+    import importlib.machinery
+    import importlib.util
+
+    import torch  # noqa: F401  (its libraries are what the module links to)
+
+    lib = load()
+    if not BINDING_PATH.exists():
+        raise RuntimeError(
+            f"spd_torch.so not found at {BINDING_PATH}; build it with "
+            "`python inference-speech-model_b200/csrc/build.py` (there is no other path)"
+        )
+    loader = importlib.machinery.ExtensionFileLoader("spd_torch", str(BINDING_PATH))
+    module = importlib.util.module_from_spec(importlib.util.spec_from_loader("spd_torch", loader))
+    loader.exec_module(module)
+    module.setup({name: C.cast(getattr(lib, name), C.c_void_p).value for name in _SIGNATURES})
+    _binding = module
+    return module
+
+
 def exported_symbols() -> list[str]:
     return list(_SIGNATURES)
 

@@ -447,116 +447,8 @@ def kv_pool_int4(num_blocks: int, num_kv_heads: int, head_dim: int, block_size: 
 
 
 # The ops below are called once per layer of a decode step, whose kernels take a few
-# microseconds: their checks read each property of a tensor once and build no message or
-# object unless a check fails.
-_INT4_PAGES = {}  # (head_dim, page bytes) -> block size
-_I32 = torch.int32
-
-
-def _current_device(name: str, first: torch.Tensor, *rest: Optional[torch.Tensor]) -> None:
-    """All tensors on the current CUDA device (the one whose current stream is launched on)."""
-    dev = first.get_device()
-    for t in rest:
-        if t is not None and t.get_device() != dev:
-            dev = -1 if dev < 0 or t.get_device() < 0 else -2
-            break
-    if dev == -1:
-        raise RuntimeError(f"{name}: CUDA tensors required (the B200 kernels have no CPU fallback)")
-    if dev != torch._C._cuda_getDevice():
-        raise RuntimeError(f"{name}: all tensors must be on the current CUDA device")
-
-
-def _int4_block_size(name: str, pool: torch.Tensor, Hkv: int, D: int) -> int:
-    if pool.dtype is not torch.uint8 or pool.dim() != 3 or pool.shape[1] != Hkv or not pool.is_contiguous():
-        raise RuntimeError(f"{name}: pool must be a contiguous uint8 [num_blocks, {Hkv}, page bytes] tensor")
-    key = (D, pool.shape[2])
-    bs = _INT4_PAGES.get(key)
-    if bs is None:
-        bs = next((b for b in (8, 16, 32) if N.load().spd_kv_int4_page_bytes(D, b) == key[1]), 0)
-        if not bs:
-            raise RuntimeError(f"{name}: pages of {key[1]} bytes fit no block size at head_dim {D}")
-        _INT4_PAGES[key] = bs
-    return bs
-
-
-def _table_columns(name: str, block_tables: torch.Tensor, B: int) -> int:
-    shape = block_tables.shape
-    if len(shape) != 2 or shape[0] != B or block_tables.dtype is not _I32 or not block_tables.is_contiguous():
-        raise RuntimeError(f"{name}: block_tables must be contiguous int32 [B, max_blocks]")
-    return shape[1]
-
-
-def _int32_vector(name: str, what: str, t: torch.Tensor, n: int) -> None:
-    if t.dtype is not _I32 or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous():
-        raise RuntimeError(f"{name}: {what} must be a contiguous int32 [{n}] tensor")
-
-
-def _token_strides(name: str, what: str, t: torch.Tensor, n: int, H: int, D: int) -> Tuple[int, int]:
-    """Token and head strides of [n, H, D] with contiguous D; those of a dimension of one
-    entry, which nothing steps over, are taken as dense."""
-    st, sh, sd = t.stride()
-    if sd != 1 and D > 1:
-        raise RuntimeError(f"{name}: {what} needs a contiguous last dimension")
-    if H == 1:
-        sh = D
-    return (st if n > 1 else sh * H), sh
-
-
-def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
-    def span(t):
-        last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
-        return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
-    (a0, a1), (b0, b1) = span(a), span(b)
-    return a.numel() > 0 and b.numel() > 0 and a0 < b1 and b0 < a1
-
-
-def _kv_shape(name: str, k: torch.Tensor, v: torch.Tensor):
-    shape = k.shape
-    if len(shape) != 3 or v.shape != shape or v.dtype is not k.dtype:
-        raise RuntimeError(f"{name}: k and v must be [N, Hkv, D] of one shape and dtype")
-    return shape
-
-
-def _rope_append(name, fn, q, k, v, shape, cos, sin, pools, block_tables, positions, cu_seqlens, interleaved, q_out,
-                 error_word, block_size, num_blocks):
-    n, Hkv, D = shape
-    B = positions.shape[0] if positions.dim() == 1 else -1
-    _int32_vector(name, "positions", positions, B)
-    max_blocks = _table_columns(name, block_tables, B)
-    if cu_seqlens is not None:
-        _int32_vector(name, "cu_seqlens", cu_seqlens, B + 1)
-    elif n != B:
-        raise RuntimeError(f"{name}: without cu_seqlens one token per sequence is expected ({n} tokens, {B} sequences)")
-    cs = cos.shape
-    if cos.dtype is not torch.float32 or sin.dtype is not torch.float32 or len(cs) != 2 or sin.shape != cs \
-            or not (cos.is_contiguous() and sin.is_contiguous()):
-        raise RuntimeError(f"{name}: cos and sin must be contiguous float32 [positions, rotated / 2] tables")
-    k_st, k_sh = _token_strides(name, "k", k, n, Hkv, D)
-    v_st, v_sh = _token_strides(name, "v", v, n, Hkv, D)
-    q_st = q_sh = Hq = 0
-    q_ptr = out_ptr = None
-    if q is not None:
-        qs = q.shape
-        if len(qs) != 3 or qs[0] != n or qs[2] != D or q.dtype is not k.dtype:
-            raise RuntimeError(f"{name}: q {tuple(qs)} does not match k {tuple(shape)}")
-        Hq = qs[1]
-        q_st, q_sh = _token_strides(name, "q", q, n, Hq, D)
-        if q_out is None:
-            q_out = q.new_empty(qs)
-        elif q_out.shape != qs or q_out.dtype is not q.dtype or not q_out.is_contiguous() or _overlap(q, q_out):
-            raise RuntimeError(f"{name}: q_out must be a contiguous {tuple(qs)} tensor of q's dtype apart from q")
-        q_ptr, out_ptr = q.data_ptr(), q_out.data_ptr()
-    elif q_out is not None:
-        raise RuntimeError(f"{name}: q_out without q")
-    if error_word is not None and (error_word.dtype is not _I32 or error_word.numel() < 1):
-        raise RuntimeError(f"{name}: error_word must be an int32 tensor")
-    rc = fn(q_ptr, q_st, q_sh, k.data_ptr(), k_st, k_sh, v.data_ptr(), v_st, v_sh, out_ptr, cos.data_ptr(), sin.data_ptr(),
-            *pools, block_tables.data_ptr(), positions.data_ptr(), None if cu_seqlens is None else cu_seqlens.data_ptr(),
-            n, B, Hq, Hkv, D, 2 * cs[1], 1 if interleaved else 0, cs[0], block_size, max_blocks, num_blocks,
-            dtype_code(k.dtype), _ptr(error_word), _stream_handle())
-    if rc:
-        N.check(rc, "spd_" + name)
-    return q_out
+# microseconds: their checks and their calls are made in the torch binding
+# (csrc/torch_binding.cpp), which raises RuntimeError with the reason of a refusal.
 
 
 def rope_kv_append(
@@ -583,15 +475,8 @@ def rope_kv_append(
     positions int32 [B]: position of each sequence's first token here (< 0 skips it);
     cu_seqlens int32 [B + 1]: its tokens are [cu[b], cu[b + 1]), or None for one token per
     sequence (a decode step).  Rows of q for tokens that are not written come back as zeros."""
-    name = "rope_kv_append"
-    _current_device(name, k, q, v, cos, sin, k_pool, v_pool, block_tables, positions, cu_seqlens, q_out, error_word)
-    shape = _kv_shape(name, k, v)
-    ps = k_pool.shape
-    if len(ps) != 4 or ps[2] != shape[1] or ps[3] != shape[2] or v_pool.shape != ps or k_pool.dtype is not k.dtype \
-            or v_pool.dtype is not k.dtype or not (k_pool.is_contiguous() and v_pool.is_contiguous()):
-        raise RuntimeError(f"{name}: pools must be contiguous [num_blocks, block_size, Hkv, D] of k's dtype")
-    return _rope_append(name, N.load().spd_rope_kv_append, q, k, v, shape, cos, sin, (k_pool.data_ptr(), v_pool.data_ptr()),
-                        block_tables, positions, cu_seqlens, interleaved, q_out, error_word, ps[1], ps[0])
+    return N.binding().rope_kv_append(q, k, v, cos, sin, k_pool, v_pool, block_tables, positions, cu_seqlens, interleaved,
+                                      q_out, error_word)
 
 
 def rope_kv_append_int4(
@@ -610,12 +495,8 @@ def rope_kv_append_int4(
 ) -> Optional[torch.Tensor]:
     """``rope_kv_append`` into a 4-bit pool (``kv_pool_int4``): the rotated keys (in fp32) and
     the values are quantised per token, head and 64 dimensions as they are written."""
-    name = "rope_kv_append_int4"
-    _current_device(name, k, q, v, cos, sin, pool, block_tables, positions, cu_seqlens, q_out, error_word)
-    shape = _kv_shape(name, k, v)
-    bs = _int4_block_size(name, pool, shape[1], shape[2])
-    return _rope_append(name, N.load().spd_rope_kv_append_int4, q, k, v, shape, cos, sin, (pool.data_ptr(),), block_tables,
-                        positions, cu_seqlens, interleaved, q_out, error_word, bs, pool.shape[0])
+    return N.binding().rope_kv_append_int4(q, k, v, cos, sin, pool, None, block_tables, positions, cu_seqlens, interleaved,
+                                           q_out, error_word)
 
 
 def kv_gather_int4(
@@ -633,29 +514,7 @@ def kv_gather_int4(
     """Tokens of a 4-bit pool as packed k and v [total, Hkv, D] of ``dtype``: rows
     [cu_seqlens[b], cu_seqlens[b + 1]) are positions starts[b], starts[b] + 1, ... of sequence b
     (starts None: from 0).  ``total`` is cu_seqlens[B], known to the caller on the host."""
-    name = "kv_gather_int4"
-    _current_device(name, pool, block_tables, cu_seqlens, starts, k_out, v_out, error_word)
-    bs = _int4_block_size(name, pool, pool.shape[1] if pool.dim() == 3 else -1, head_dim)
-    B = cu_seqlens.shape[0] - 1 if cu_seqlens.dim() == 1 else -1
-    _int32_vector(name, "cu_seqlens", cu_seqlens, B + 1)
-    if starts is not None:
-        _int32_vector(name, "starts", starts, B)
-    max_blocks = _table_columns(name, block_tables, B)
-    shape = (int(total), pool.shape[1], head_dim)
-    if k_out is None and v_out is None:
-        k_out, v_out = pool.new_empty((2,) + shape, dtype=dtype).unbind(0)
-    else:
-        k_out = pool.new_empty(shape, dtype=dtype) if k_out is None else k_out
-        v_out = pool.new_empty(shape, dtype=dtype) if v_out is None else v_out
-        for t in (k_out, v_out):
-            if tuple(t.shape) != shape or t.dtype is not dtype or not t.is_contiguous():
-                raise RuntimeError(f"{name}: outputs must be contiguous {shape} tensors of {dtype}")
-    rc = N.load().spd_kv_gather_int4(pool.data_ptr(), block_tables.data_ptr(), cu_seqlens.data_ptr(), _ptr(starts),
-                                     k_out.data_ptr(), v_out.data_ptr(), shape[0], B, shape[1], head_dim, bs, max_blocks,
-                                     pool.shape[0], dtype_code(dtype), _ptr(error_word), _stream_handle())
-    if rc:
-        N.check(rc, "spd_kv_gather_int4")
-    return k_out, v_out
+    return N.binding().kv_gather_int4(pool, block_tables, cu_seqlens, total, head_dim, dtype, starts, k_out, v_out, error_word)
 
 
 def paged_decode_attention_int4(
@@ -672,38 +531,8 @@ def paged_decode_attention_int4(
     q [B, Hq, D]; pool from ``kv_pool_int4`` with Hkv heads (Hq a multiple of it; query head h
     reads head h // (Hq // Hkv)); block_tables int32 [B, max_blocks]; context_lens int32 [B]
     tokens attended (<= 0 gives zeros).  Returns out [B, Hq, D]."""
-    name = "paged_decode_attention_int4"
-    _current_device(name, q, pool, block_tables, context_lens, out, workspace)
-    if q.dim() != 3 or not q.is_contiguous():
-        raise RuntimeError(f"{name}: q must be a contiguous [B, Hq, D] tensor")
-    B, Hq, D = q.shape
-    Hkv = pool.shape[1] if pool.dim() == 3 else -1
-    bs = _int4_block_size(name, pool, Hkv, D)
-    if Hkv <= 0 or Hq % Hkv:
-        raise RuntimeError(f"{name}: {Hq} query heads do not divide over {Hkv} key/value heads")
-    max_blocks = _table_columns(name, block_tables, B)
-    _int32_vector(name, "context_lens", context_lens, B)
-    if out is None:
-        out = torch.empty_like(q)
-    elif out.shape != q.shape or out.dtype is not q.dtype or not out.is_contiguous():
-        raise RuntimeError(f"{name}: out must be a contiguous {tuple(q.shape)} tensor of q's dtype")
-    code = dtype_code(q.dtype)
-    if B == 0:
-        return out
-    stream = _stream_handle()
-    if workspace is None:
-        key = ("int4", B, Hq, Hkv, D, bs, max_blocks, code, q.get_device(), stream)
-        workspace = _WORKSPACES.get(key)
-        if workspace is None:
-            workspace = _WORKSPACES[key] = decode_int4_workspace(B, Hq, Hkv, D, bs, max_blocks, q.dtype, q.device)
-    if scale is None:
-        scale = 1.0 / math.sqrt(D)
-    rc = N.load().spd_paged_decode_attn_int4(
-        q.data_ptr(), pool.data_ptr(), block_tables.data_ptr(), context_lens.data_ptr(), out.data_ptr(), B, Hq, Hkv, D,
-        bs, max_blocks, pool.shape[0], float(scale), code, workspace.data_ptr(), workspace.numel(), stream)
-    if rc:
-        N.check(rc, "spd_paged_decode_attn_int4")
-    return out
+    return N.binding().paged_decode_attention_int4(q, pool, block_tables, context_lens,
+                                                   q.shape[-1] ** -0.5 if scale is None else scale, out, workspace)
 
 
 def prompt_attention(
@@ -724,35 +553,5 @@ def prompt_attention(
     queries' lengths).  With ``causal`` query i of a sequence sees the keys j <= i + Tk - Tq, so
     keys of a cached prefix come first; a query that sees no key gives zeros.  Rows that belong
     to no sequence are left as they are in ``out``.  Returns out [Nq, Hq, D]."""
-    name = "prompt_attention"
-    _current_device(name, q, k, v, cu_seqlens_q, cu_seqlens_k, out, error_word)
-    qs, ks, dtype = q.shape, k.shape, q.dtype
-    if len(qs) != 3 or len(ks) != 3 or v.shape != ks or qs[2] != ks[2]:
-        raise RuntimeError(f"{name}: q [Nq, Hq, D] and k, v [Nk, Hkv, D] expected")
-    if k.dtype is not dtype or v.dtype is not dtype:
-        raise RuntimeError(f"{name}: q, k and v must share a dtype")
-    (Nq, Hq, D), (Nk, Hkv, _) = qs, ks
-    if Hkv == 0 or Hq % Hkv:
-        raise RuntimeError(f"{name}: {Hq} query heads do not divide over {Hkv} key/value heads")
-    B = cu_seqlens_q.shape[0] - 1 if cu_seqlens_q.dim() == 1 else -1
-    _int32_vector(name, "cu_seqlens_q", cu_seqlens_q, B + 1)
-    if cu_seqlens_k is None:
-        cu_seqlens_k = cu_seqlens_q
-    elif cu_seqlens_k is not cu_seqlens_q:
-        _int32_vector(name, "cu_seqlens_k", cu_seqlens_k, B + 1)
-    if out is None:
-        out = q.new_empty(qs)
-    elif out.shape != qs or out.dtype is not dtype or not out.is_contiguous():
-        raise RuntimeError(f"{name}: out must be a contiguous {tuple(qs)} tensor of q's dtype")
-    if scale is None:
-        scale = 1.0 / math.sqrt(D)
-    q_st, q_sh = _token_strides(name, "q", q, Nq, Hq, D)
-    k_st, k_sh = _token_strides(name, "k", k, Nk, Hkv, D)
-    v_st, v_sh = _token_strides(name, "v", v, Nk, Hkv, D)
-    rc = N.load().spd_prompt_attn(
-        q.data_ptr(), q_st, q_sh, k.data_ptr(), k_st, k_sh, v.data_ptr(), v_st, v_sh, out.data_ptr(),
-        cu_seqlens_q.data_ptr(), cu_seqlens_k.data_ptr(), Nq, Nk, B, Hq, Hkv, D, 1 if causal else 0, float(scale),
-        dtype_code(dtype), _ptr(error_word), _stream_handle())
-    if rc:
-        N.check(rc, "spd_prompt_attn")
-    return out
+    return N.binding().prompt_attention(q, k, v, cu_seqlens_q, cu_seqlens_k, causal,
+                                        q.shape[-1] ** -0.5 if scale is None else scale, out, error_word)
