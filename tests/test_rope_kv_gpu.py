@@ -179,6 +179,18 @@ def test_tokens_past_the_last_sequence_are_left_alone():
     assert (k[[0, 4]] == 7).all() and (v[[0, 4]] == 7).all() and (k[1:4] != 7).any()
 
 
+def test_gather_into_outputs_aligned_to_16_bytes_only():
+    c = Case([5, 40], [0, 3], 2, 2, 128, 128, 16, torch.bfloat16, False)
+    pool = ops.kv_pool_int4(c.blocks, 2, 128, 16)
+    cu = c.cu.to(DEV)
+    ops.rope_kv_append_int4(None, c.dk, c.dv, *c.args, pool, *c.where, cu_seqlens=cu)
+    want = ops.kv_gather_int4(pool, c.where[0], cu, 45, 128, torch.bfloat16, starts=c.where[1])
+    n = 45 * 2 * 128
+    k, v = (torch.empty(n + 8, dtype=torch.bfloat16, device=DEV)[8:].view(45, 2, 128) for _ in range(2))
+    ops.kv_gather_int4(pool, c.where[0], cu, 45, 128, torch.bfloat16, starts=c.where[1], k_out=k, v_out=v)
+    assert torch.equal(k, want[0]) and torch.equal(v, want[1])
+
+
 def test_pool_beyond_two_gigabytes():
     """Offsets past 2^31 bytes: the last block of a large pool."""
     D, bs, H = 128, 32, 8
