@@ -23,41 +23,36 @@
 //   each head takes two columns, the value and its rounding remainder, so q and p keep 22
 //   bits; with more, q keeps 11 bits (exact for fp16 and bf16 queries) and p 11.
 //
-// Work split, short block tables (up to kWholeTokens): one CTA per (sequence, key/value head tile).
-// Work split, longer ones: the steps (64 tokens) of all sequences and key/value heads are laid end to end
-// and shared equally among as many CTAs as are resident at once, whatever the lengths; a CTA's
-// share may begin and end inside a (sequence, head).  Its four warps take every fourth step,
-// each fed by its own ring of shared-memory stages (one bulk copy per page, issued by the lanes
-// in parallel, running ahead over segment ends), with a running maximum that is raised only
-// when a score passes it by 8 (p <= 2^8).  At a segment's end the warps are joined in shared
-// memory; segments that span CTAs are joined by the last of them to arrive.
+// Work split: one CTA per (sequence, key/value head tile, chunk of tokens).  A CTA's four warps take
+// every fourth step of 64 tokens, each fed by its own ring of shared-memory stages (one bulk copy per
+// page, issued by the lanes in parallel, no CTA-wide barrier in the loop), with a running maximum that
+// is raised only when a score passes it by 8 (p <= 2^8).  The warps are joined in shared memory, the
+// chunks of a (sequence, head tile) by the last CTA to arrive, which adds them in their order: the
+// result does not depend on who that is.
+// Measured: 32 contexts of 1,000 to 32,000 tokens, 32/8 heads of 128, bf16 (582 MB of pool): 126 us,
+// 4.6 TB/s, 0.70 of a plain copy's rate.  Copies alone take 108 us in this form, the arithmetic alone
+// 125: the two share the SM's issue slots.  128 contexts of up to 3,900, 12 heads of 64: 66 us; one
+// of 32,000: 17.5 us; one of 448: 5.3 us, most of it the latency of table, page and join.
 #include "spd_int4.cuh"
 #include "spd_params.cuh"
+
+#include <algorithm>
 
 namespace spd {
 namespace dec4 {
 
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
-constexpr int kWholeTokens = 2048;
-constexpr int kMaxCtas = 4;  // per SM (sizes the workspace's partial slots)
 constexpr float kLazy = 8.f;  // log2 units a score may pass the reference maximum by
 
-#ifndef DEC4_ST1
-#define DEC4_ST1 3
-#define DEC4_SP1 64
-#define DEC4_ST2 2
-#define DEC4_SP2 64
-#define DEC4_MB 1
-#endif
-template <int P> constexpr int step_tokens() { return P == 4 ? 32 : P == 2 ? DEC4_SP2 : DEC4_SP1; }  // tokens per warp step
-template <int P> constexpr int stages() { return P == 1 ? DEC4_ST1 : P == 2 ? DEC4_ST2 : 2; }
+// Tokens per warp step, stages per warp and CTAs per SM: as many warps as their registers allow.  At
+// D = 128 12 warps an SM, each with two stages of 9,216 bytes (8 warps with three: 139 us for the 32
+// contexts above in place of 126); at D = 64 16 warps (12: 70 us for the 128 contexts, 66 with 16).
+template <int P> constexpr int step_tokens() { return P == 4 ? 32 : 64; }
+template <int P> constexpr int stages() { return P == 1 ? 3 : 2; }
+template <int P> constexpr int ctas_per_sm() { return P == 1 ? 4 : P == 2 ? 3 : 2; }
 template <int P> constexpr int step_bytes() { return int4::page_bytes(P, step_tokens<P>()); }
 template <int P> constexpr int ring_bytes() { return kWarps * stages<P>() * step_bytes<P>(); }
-// the ring, then the warps' results [kWarps][heads][D] of a segment
-template <int P, bool SPLIT> constexpr size_t smem_bytes() {
-  return (size_t)ring_bytes<P>() + kWarps * (SPLIT ? 4 : 8) * P * int4::kPlane * 4;
-}
 
 // D += A * B (m16n8k16, fp16 in, fp32 accumulation).  Not volatile: the compiler may interleave the
 // chains of different accumulators, which hides each product's latency.
@@ -119,16 +114,9 @@ __device__ __forceinline__ void store_out4(void* out, int dtype, long long at, f
   }
 }
 
-// A run of steps of one (sequence, head tile) inside a CTA's share.
-struct Segment {
-  int b, y;      // sequence; key/value head * tiles + tile
-  int step0, n;  // first step and number of steps here
-  int total;     // steps of the whole sequence
-};
-
 // P: planes (D / 64); BS: block size; SPLIT: two columns per head.
 template <int P, int BS, bool SPLIT>
-__global__ void __launch_bounds__(kThreads, P == 4 ? 1 : DEC4_MB) decode_int4_kernel(const DecodeInt4Params p) {
+__global__ void __launch_bounds__(kThreads, ctas_per_sm<P>()) decode_int4_kernel(const DecodeInt4Params p) {
   constexpr int D = P * int4::kPlane;
   constexpr int kHeads = SPLIT ? 4 : 8;  // heads per column tile
   constexpr int kStages = stages<P>(), kStep = step_tokens<P>(), kSubs = kStep / 16;
@@ -139,113 +127,41 @@ __global__ void __launch_bounds__(kThreads, P == 4 ? 1 : DEC4_MB) decode_int4_ke
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ __align__(8) uint64_t bars[kWarps][kStages];
   __shared__ float stat_m[kWarps][8], stat_l[kWarps][8];
-  __shared__ int scan[kWarps], last_flag;
-  // [kWarps][kHeads][D]: a warp's result at a segment's end; before it, the warp's parameters of
-  // the step at hand, (scale, zero) [K, V][tokens][P]
-  float* joined = reinterpret_cast<float*>(smem + ring_bytes<P>());
-  int* prefix = reinterpret_cast<int*>(smem + smem_bytes<P, SPLIT>());  // [B + 1] steps before each sequence
+  __shared__ int last_flag;
+  __shared__ float* joined[kWarps];  // where each warp left its result, [heads][D]
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int g = lane >> 2, t = lane & 3;
   const int G = p.Hq / p.Hkv;
   const int tiles = (G + kHeads - 1) / kHeads, Y = p.Hkv * tiles;
 
-  auto ctx_of = [&](int b) {
-    const int c = p.context_lens[b];
-    return (long long)c > (long long)p.max_blocks * BS ? p.max_blocks * BS : c < 0 ? 0 : c;
-  };
-  auto zeros = [&](int b, int h0, int n) {  // a sequence without a context
-#pragma unroll 1
-    for (int i = tid; i < n * D / 4; i += kThreads)
-      store_out4(p.out, p.dtype, ((long long)b * p.Hq + h0) * D + i * 4, make_float4(0.f, 0.f, 0.f, 0.f));
-  };
-  long long W = 0, u0 = 0, u1 = 0;  // steps of all; this CTA's share [u0, u1) of them
-  int ctas = 0;
-  bool narrow = true;
-  Segment seg{};
-  if (p.whole) {
-    // ---- one (sequence, head tile) per CTA -----------------------------------------------------
-    seg.b = blockIdx.x / Y;
-    seg.y = blockIdx.x - seg.b * Y;
-    const int c = p.context_lens[seg.b];
-    if ((long long)c > (long long)p.max_blocks * BS && tid == 0) set_error(p.err, SPD_DEVERR_LENGTH);
-    seg.total = seg.n = (ctx_of(seg.b) + kStep - 1) / kStep;
-    u1 = seg.n;
-    if (seg.n == 0) {
-      const int tile = seg.y % tiles;
-      zeros(seg.b, seg.y / tiles * G + tile * kHeads, min(kHeads, G - tile * kHeads));
-      return;
-    }
-  } else {
-    // ---- steps before each sequence --------------------------------------------------------
-    int base = 0;
-#pragma unroll 1
-    for (int b0 = 0; b0 < p.B; b0 += kThreads) {
-      const int b = b0 + tid;
-      int n = 0;
-      if (b < p.B) {
-        n = (ctx_of(b) + kStep - 1) / kStep;
-        if (blockIdx.x == 0 && (long long)p.context_lens[b] > (long long)p.max_blocks * BS)
-          set_error(p.err, SPD_DEVERR_LENGTH);
-      }
-      int incl = n;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, incl, o);
-        if (lane >= o) incl += v;
-      }
-      if (lane == 31) scan[warp] = incl;
-      __syncthreads();
-      int before = base, all = 0;
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
-        if (w < warp) before += scan[w];
-        all += scan[w];
-      }
-      if (b < p.B) prefix[b] = before + incl - n;
-      base += all;
-      __syncthreads();
-    }
-    if (tid == 0) prefix[p.B] = base;
-    __syncthreads();
-    if (blockIdx.x == 0)
-#pragma unroll 1
-      for (int b = 0; b < p.B; ++b)
-        if (prefix[b + 1] == prefix[b]) zeros(b, 0, p.Hq);
-    // ---- this CTA's share ------------------------------------------------------------------
-    W = (long long)base * Y;
-    ctas = (int)min((long long)gridDim.x, W);  // a few steps spread over as many CTAs
-    if ((int)blockIdx.x >= ctas) return;
-    narrow = W <= 0x7fffffff / (ctas + 1);
+  // all heads of a sequence's chunk together: their pages lie side by side
+  const int y = (int)(blockIdx.x % (unsigned)Y), rest = (int)(blockIdx.x / (unsigned)Y);
+  const int chunk = rest % p.chunks, b = rest / p.chunks;
+  const int tile = y % tiles, kvh = y / tiles;
+  const int heads = min(kHeads, G - tile * kHeads);  // of this tile
+  const long long head0 = (long long)b * p.Hq + kvh * G + tile * kHeads;  // row of q and out
+  int ctx = p.context_lens[b];
+  if ((long long)ctx > (long long)p.max_blocks * BS) {
+    if (tid == 0) set_error(p.err, SPD_DEVERR_LENGTH);
+    ctx = p.max_blocks * BS;
   }
-  // c * W / ctas, and the CTA whose share holds unit u; in 32 bits where the products fit
-  auto share = [&](int c) {
-    return narrow ? (long long)((unsigned)c * (unsigned)W / (unsigned)ctas) : range_start(c, ctas, W);
-  };
-  auto cta_of = [&](long long u) {
-    return narrow ? (int)((((unsigned)u + 1) * (unsigned)ctas + (unsigned)W - 1) / (unsigned)W) - 1
-                  : cta_of_unit(u, ctas, W);
-  };
-  if (!p.whole) {
-    u0 = share(blockIdx.x);
-    u1 = share(blockIdx.x + 1);
-    seg.b = upper_index_i32(prefix, p.B, narrow ? (long long)((unsigned)u0 / (unsigned)Y) : u0 / Y);
-    seg.total = prefix[seg.b + 1] - prefix[seg.b];
-    const long long r = u0 - (long long)prefix[seg.b] * Y;
-    seg.y = narrow ? (int)((unsigned)r / (unsigned)seg.total) : (int)(r / seg.total);
-    seg.step0 = (int)(r - (long long)seg.y * seg.total);
-    seg.n = (int)min((long long)(seg.total - seg.step0), u1 - u0);
-  }
-  auto next = [&](Segment& s, long long u) {  // the segment after s, which begins at unit u < u1
-    if (++s.y == Y) {
-      s.y = 0;
+  if (ctx <= 0) {
+    if (chunk == 0)
 #pragma unroll 1
-      do ++s.b; while (prefix[s.b + 1] == prefix[s.b]);
-      s.total = prefix[s.b + 1] - prefix[s.b];
-    }
-    s.step0 = 0;
-    s.n = (int)min((long long)s.total, u1 - u);
-  };
+      for (int i = tid; i < heads * D / 4; i += kThreads)
+        store_out4(p.out, p.dtype, head0 * D + i * 4, make_float4(0.f, 0.f, 0.f, 0.f));
+    return;
+  }
+  // the sequence's own chunks: as many as there are CTAs for it, but of `least` tokens or more
+  const int size = max(p.least, ((ctx + p.chunks - 1) / p.chunks + kStep - 1) / kStep * kStep);
+  const long long first = (long long)chunk * size;
+  if (first >= ctx) return;
+  const int t0 = (int)first;
+  const int t1 = ctx - t0 > size ? t0 + size : ctx;
+  const int parts = (ctx - 1) / size + 1;
+  const int steps = (t1 - t0 + kStep - 1) / kStep;
+  const int* table = p.block_tables + (long long)b * p.max_blocks;
 
   unsigned char* ring = smem + (size_t)warp * kStages * step_bytes<P>();
   const uint64_t policy = l2_policy_evict_first();
@@ -255,45 +171,32 @@ __global__ void __launch_bounds__(kThreads, P == 4 ? 1 : DEC4_MB) decode_int4_ke
   }
   __syncwarp();
 
-  // The copies run ahead of the arithmetic over this warp's steps of all segments: `ahead` is
-  // the segment of the next step to fetch, `id` this lane's page of that step (its table entry is
-  // loaded one step early).
-  Segment ahead = seg;
-  long long ahead_u = u0;
-  int ahead_i = warp, id = -1, ahead_pages = 0, fetched = 0, ahead_ctx = ctx_of(ahead.b);
-  bool more = true;
+  // Copies run ahead of the arithmetic: `id` is this lane's page of the step `ahead` that is fetched next
+  // (its table entry is loaded one step early).
+  const unsigned char* pool_h = p.pool + (long long)kvh * kPage;
+  const long long block_stride = (long long)p.Hkv * kPage;
+  int ahead = warp, id = 0, pages = 0, fetched = 0;
   auto look_up = [&]() {
-#pragma unroll 1
-    while (more && ahead_i >= ahead.n) {
-      ahead_u += ahead.n;
-      ahead_i = warp;
-      if (ahead_u >= u1) {
-        more = false;
-      } else {
-        next(ahead, ahead_u);
-        ahead_ctx = ctx_of(ahead.b);
-      }
-    }
-    if (!more) return;
-    const int tok = (ahead.step0 + ahead_i) * kStep;
-    ahead_pages = min(kPages, (ahead_ctx - tok + BS - 1) / BS);
-    id = lane < ahead_pages ? p.block_tables[(long long)ahead.b * p.max_blocks + tok / BS + lane] : 0;
+    if (ahead >= steps) return;
+    const int tok = t0 + ahead * kStep;
+    pages = min(kPages, (t1 - tok + BS - 1) / BS);
+    id = lane < pages ? __ldg(table + tok / BS + lane) : 0;
   };
   auto fetch = [&]() {
-    if (!more) return;
+    if (ahead >= steps) return;
     const int st = fetched % kStages;
-    if (lane == 0) mbar_arrive_expect_tx(&bars[warp][st], (uint32_t)(ahead_pages * kPage));
+    if (lane == 0) mbar_arrive_expect_tx(&bars[warp][st], (uint32_t)(pages * kPage));
     __syncwarp();
-    if (lane < ahead_pages) {
+    if (lane < pages) {
       if (id < 0 || id >= p.num_blocks) {
         set_error(p.err, SPD_DEVERR_BLOCK_ID);
         id = 0;
       }
-      bulk_copy_g2s_hint(ring + (size_t)st * step_bytes<P>() + lane * kPage,
-                         p.pool + ((long long)id * p.Hkv + ahead.y / tiles) * kPage, kPage, &bars[warp][st], policy);
+      bulk_copy_g2s_hint(ring + (size_t)st * step_bytes<P>() + lane * kPage, pool_h + id * block_stride, kPage,
+                         &bars[warp][st], policy);
     }
     ++fetched;
-    ahead_i += kWarps;
+    ahead += kWarps;
     look_up();
   };
   look_up();
@@ -308,16 +211,9 @@ __global__ void __launch_bounds__(kThreads, P == 4 ? 1 : DEC4_MB) decode_int4_ke
   auto place = [](int tok) { return (tok / BS) * kPage + (tok % BS) * int4::kRowBytes; };
 
   constexpr int C = SPLIT ? 1 : 2;  // heads of this lane's two columns
-  static_assert(2 * kStep * P * 2 <= kHeads * D, "the parameters fit in the warp's result");
-  float2* par = reinterpret_cast<float2*>(joined + warp * kHeads * D);
+  static_assert(kHeads * D * 4 <= step_bytes<P>(), "a segment's result fits in a stage");
   int used = 0;
   bool fine = true;
-#pragma unroll 1
-  for (long long u = u0; u < u1; ) {
-  const int tile = seg.y % tiles, kvh = seg.y / tiles;
-  const int heads = min(kHeads, G - tile * kHeads);  // of this tile
-  const long long head0 = (long long)seg.b * p.Hq + kvh * G + tile * kHeads;  // row of q and out
-  const int ctx = ctx_of(seg.b);
 
   // ---- the query fragments: column g, k = this lane's 16 dimensions of each plane --------
   uint32_t qb[P][4][2];
@@ -386,28 +282,25 @@ __global__ void __launch_bounds__(kThreads, P == 4 ? 1 : DEC4_MB) decode_int4_ke
   int lift = -15;  // exponent of the largest value scale seen; weights carry 2^(6 - lift)
 
 #pragma unroll 1
-  for (int i = warp; i < seg.n && fine; i += kWarps) {
+  for (int i = warp; i < steps && fine; i += kWarps) {
     const int st = used % kStages;
     const bool ok = mbar_wait_suspend(&bars[warp][st], (uint32_t)((used / kStages) & 1), p.err, p.wait_ns);
     fine = __all_sync(0xffffffffu, ok);
     if (!fine) break;
     ++used;
-    const unsigned char* buf = ring + (size_t)st * step_bytes<P>();
-    const int left = ctx - (seg.step0 + i) * kStep;  // valid tokens of this step (>= 1)
+    unsigned char* buf = ring + (size_t)st * step_bytes<P>();
+    const int left = t1 - (t0 + i * kStep);  // valid tokens of this step (>= 1)
 
-    // ---- the tokens' parameters, once per token: to fp32 with all factors multiplied in ----
-    // (scale * f, zero) of K and (scale * 2^(6 - lift), zero) of V, zero past the end; lane = token
-    uint32_t raw[kStep / 32][2 * P], top = 0;
+    // ---- the values' parameters, lane = token: zero past the end; the largest scale -----------
+    uint32_t raw[kStep / 32][P], top = 0;
 #pragma unroll
     for (int h = 0; h < kStep / 32; ++h) {
       const int tok = h * 32 + lane;
-      const unsigned char* at = buf + (tok / BS) * kPage + kParams + (tok % BS) * int4::kParamBytes;
+      const unsigned char* at = buf + kHalf + (tok / BS) * kPage + kParams + (tok % BS) * int4::kParamBytes;
 #pragma unroll
       for (int pl = 0; pl < P; ++pl) {
-        const bool in = tok < left;
-        raw[h][pl] = in ? *reinterpret_cast<const uint32_t*>(at + pl * BS * int4::kParamBytes) : 0u;
-        raw[h][P + pl] = in ? *reinterpret_cast<const uint32_t*>(at + kHalf + pl * BS * int4::kParamBytes) : 0u;
-        top = max(top, raw[h][P + pl] & 0x7FFFu);
+        raw[h][pl] = tok < left ? *reinterpret_cast<const uint32_t*>(at + pl * BS * int4::kParamBytes) : 0u;
+        top = max(top, raw[h][pl] & 0x7FFFu);
       }
     }
     if (__any_sync(0xffffffffu, (int)(top >> 10) - 15 > lift)) {  // a larger value scale than any before
@@ -420,15 +313,6 @@ __global__ void __launch_bounds__(kThreads, P == 4 ? 1 : DEC4_MB) decode_int4_ke
         for (int k = 0; k < 16; ++k) o[pl][k >> 2][k & 3] *= w;
     }
     const float wscale = pow2(6 - lift);
-#pragma unroll
-    for (int h = 0; h < kStep / 32; ++h)
-#pragma unroll
-      for (int pl = 0; pl < P; ++pl) {
-        const float2 kp = unpack_half(raw[h][pl]), vp = unpack_half(raw[h][P + pl]);
-        par[(h * 32 + lane) * P + pl] = make_float2(kp.x * f, kp.y);
-        par[(kStep + h * 32 + lane) * P + pl] = make_float2(vp.x * wscale, vp.y);
-      }
-    __syncwarp();
 
     // ---- scores ----------------------------------------------------------------------
     // products of all 16-token tiles and planes first, their accumulator chains interleaved
@@ -445,6 +329,19 @@ __global__ void __launch_bounds__(kThreads, P == 4 ? 1 : DEC4_MB) decode_int4_ke
 #pragma unroll
           for (int i = 0; i < 4; ++i) acc[sub][pl][i] = 0.f;
         }
+      // The key codes are in registers: over them go the values' parameters as fp32, (scale *
+      // 2^(6 - lift), zero) of P planes per token.
+      __syncwarp();
+#pragma unroll
+      for (int h = 0; h < kStep / 32; ++h) {
+        const int tok = h * 32 + lane;
+        float2* par = reinterpret_cast<float2*>(buf + (tok / BS) * kPage + (tok % BS) * (8 * P));
+#pragma unroll
+        for (int pl = 0; pl < P; ++pl) {
+          const float2 v = unpack_half(raw[h][pl]);
+          par[pl] = make_float2(v.x * wscale, v.y);
+        }
+      }
 #pragma unroll
       for (int s = 0; s < 4; ++s)
 #pragma unroll
@@ -461,23 +358,25 @@ __global__ void __launch_bounds__(kThreads, P == 4 ? 1 : DEC4_MB) decode_int4_ke
 #pragma unroll
     for (int sub = 0; sub < kSubs; ++sub) {
       const int ta = sub * 16 + tok_k, tb = ta + 8;
-      float2 ka[P], kb[P];
-      load_par<P>(par + ta * P, ka);
-      load_par<P>(par + tb * P, kb);
 #pragma unroll
       for (int pl = 0; pl < P; ++pl) {
         const float* a = acc[sub][pl];
+        const unsigned char* at = buf + kParams + pl * BS * int4::kParamBytes;
+        float2 ka = unpack_half(*reinterpret_cast<const uint32_t*>(at + (ta / BS) * kPage + (ta % BS) * int4::kParamBytes));
+        float2 kb = unpack_half(*reinterpret_cast<const uint32_t*>(at + (tb / BS) * kPage + (tb % BS) * int4::kParamBytes));
+        ka.x *= f;
+        kb.x *= f;
         auto add = [&](int i, float x, float2 kp, float qs) {
           sc[sub][i] = fmaf(kp.x, x, pl ? fmaf(kp.y, qs, sc[sub][i]) : kp.y * qs);
         };
         if (SPLIT) {
-          add(0, a[0] + a[1], ka[pl], qsa[pl]);
-          add(C, a[2] + a[3], kb[pl], qsa[pl]);
+          add(0, a[0] + a[1], ka, qsa[pl]);
+          add(C, a[2] + a[3], kb, qsa[pl]);
         } else {
-          add(0, a[0], ka[pl], qsa[pl]);
-          add(C - 1, a[1], ka[pl], qsb[pl]);
-          add(C, a[2], kb[pl], qsa[pl]);
-          add(2 * C - 1, a[3], kb[pl], qsb[pl]);
+          add(0, a[0], ka, qsa[pl]);
+          add(C - 1, a[1], ka, qsb[pl]);
+          add(C, a[2], kb, qsa[pl]);
+          add(2 * C - 1, a[3], kb, qsb[pl]);
         }
       }
       if (left < kStep)  // the sequence's last step
@@ -526,12 +425,13 @@ __global__ void __launch_bounds__(kThreads, P == 4 ? 1 : DEC4_MB) decode_int4_ke
     for (int c = 0; c < C; ++c) mm[c] = m[c] == -INFINITY ? 0.f : m[c];
 
     // ---- output ------------------------------------------------------------------------
+    __syncwarp();  // the values' parameters are written
 #pragma unroll
     for (int sub = 0; sub < kSubs; ++sub) {
       const int ta = sub * 16 + tok_k, tb = ta + 8;
       float2 va[P], vb[P];
-      load_par<P>(par + (kStep + ta) * P, va);
-      load_par<P>(par + (kStep + tb) * P, vb);
+      load_par<P>(reinterpret_cast<const float2*>(buf + (ta / BS) * kPage + (ta % BS) * (8 * P)), va);
+      load_par<P>(reinterpret_cast<const float2*>(buf + (tb / BS) * kPage + (tb % BS) * (8 * P)), vb);
       float pr[2 * C];
 #pragma unroll
       for (int c = 0; c < C; ++c) {
@@ -573,9 +473,15 @@ __global__ void __launch_bounds__(kThreads, P == 4 ? 1 : DEC4_MB) decode_int4_ke
         mma(o[pl][3], lo0 & 0x00F000F0u, hi0 & 0x00F000F0u, lo1 & 0x00F000F0u, hi1 & 0x00F000F0u, b0, b1);
       }
     }
-    __syncwarp();  // every lane has read this stage and these parameters
+    // every lane has read this stage; what it wrote there comes before the next copy into it
+    fence_proxy_async_smem();
+    __syncwarp();
     fetch();
   }
+  // a wait that gave up: let this warp's copies in flight land
+#pragma unroll 1
+  for (; used < fetched; ++used)
+    (void)mbar_wait_suspend(&bars[warp][used % kStages], (uint32_t)((used / kStages) & 1), nullptr);
 
   // ---- join the warps ---------------------------------------------------------------------
 #pragma unroll
@@ -586,9 +492,10 @@ __global__ void __launch_bounds__(kThreads, P == 4 ? 1 : DEC4_MB) decode_int4_ke
 #pragma unroll
       for (int pl = 0; pl < P; ++pl) zacc[pl][c] += __shfl_xor_sync(0xffffffffu, zacc[pl][c], x);
     }
-  float* mine = joined + warp * kHeads * D;
-  __syncwarp();
-  {
+  const bool had_step = warp < steps;
+  float* mine = reinterpret_cast<float*>(ring);  // the ring is drained
+  if (lane == 0) joined[warp] = mine;
+  if (had_step) {
     // out of the fp16 scaling: 2^24 / 2^(6 - lift), and / 16 where the codes read as 16c
     const float f1 = pow2(18 + lift), f16 = pow2(14 + lift);
 #pragma unroll
@@ -616,104 +523,71 @@ __global__ void __launch_bounds__(kThreads, P == 4 ? 1 : DEC4_MB) decode_int4_ke
       }
   }
   __syncthreads();
-  const bool whole = seg.step0 == 0 && seg.n == seg.total;
-  // a CTA has at most two segments that others share: the one it begins in and the one it ends in
-  float* slot = p.partials + (size_t)(2 * blockIdx.x + (seg.step0 == 0 ? 1 : 0)) * kHeads * kRow;
 #pragma unroll 1
   for (int e = tid; e < heads * D / 4; e += kThreads) {
     const int h = e / (D / 4), d = (e % (D / 4)) * 4;
     float mm = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) mm = fmaxf(mm, stat_m[w][h]);
+    for (int w = 0; w < kWarps; ++w)
+      if (w < steps) mm = fmaxf(mm, stat_m[w][h]);
     float ll = 0.f;
     float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
+      if (w >= steps) break;  // a warp without a step
       const float f = stat_m[w][h] == mm ? 1.f : ex2_approx(stat_m[w][h] - mm);
-      const float4 v = *reinterpret_cast<const float4*>(joined + (w * kHeads + h) * D + d);
+      const float4 v = *reinterpret_cast<const float4*>(joined[w] + h * D + d);
       ll += f * stat_l[w][h];
       s.x += f * v.x; s.y += f * v.y; s.z += f * v.z; s.w += f * v.w;
     }
-    if (whole) {
+    if (parts == 1) {
       const float r = ll != 0.f ? 1.f / ll : 0.f;  // no weight at all: zeros
       store_out4(p.out, p.dtype, (head0 + h) * D + d, make_float4(s.x * r, s.y * r, s.z * r, s.w * r));
     } else {
-      float* row = slot + h * kRow;
+      float* row = p.partials + ((head0 + h) * p.chunks + chunk) * kRow;
       *reinterpret_cast<float4*>(row + d) = s;
       if (d == 0) *reinterpret_cast<float2*>(row + D) = make_float2(mm, ll);
     }
   }
-  if (!whole) {
-    // ---- join the CTAs of this segment: the last one to arrive -----------------------------
-    const long long start = (long long)prefix[seg.b] * Y + (long long)seg.y * seg.total;
-    const int first = cta_of(start), last = cta_of(start + seg.total - 1);
-    __threadfence();
-    __syncthreads();
-    if (tid == 0) {
-      int* counter = p.counters + (long long)seg.b * Y + seg.y;
-      const int n = atomicAdd(counter, 1);
-      last_flag = n == last - first;
-      if (last_flag) *counter = 0;
-    }
-    __syncthreads();
-    if (last_flag) {
-      __threadfence();
-      // the part of CTA c: it begins in this segment in all but the first one
-      auto part = [&](int c, int h) {
-        return p.partials + ((size_t)(2 * c + (c == first ? 1 : 0)) * kHeads + h) * kRow;
-      };
-#pragma unroll 1
-      for (int e = tid; e < heads * D / 4; e += kThreads) {
-        const int h = e / (D / 4), d = (e % (D / 4)) * 4;
-        float mm = -INFINITY, ll = 0.f;
-        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-        for (int c = first; c <= last; ++c) mm = fmaxf(mm, __ldcg(part(c, h) + D));
-#pragma unroll 8
-        for (int c = first; c <= last; ++c) {
-          const float* row = part(c, h);
-          const float2 st = __ldcg(reinterpret_cast<const float2*>(row + D));
-          const float4 v = __ldcg(reinterpret_cast<const float4*>(row + d));
-          const float f = st.x == mm ? 1.f : ex2_approx(st.x - mm);
-          ll += f * st.y;
-          a.x += f * v.x; a.y += f * v.y; a.z += f * v.z; a.w += f * v.w;
-        }
-        const float r = ll != 0.f ? 1.f / ll : 0.f;
-        store_out4(p.out, p.dtype, (head0 + h) * D + d, make_float4(a.x * r, a.y * r, a.z * r, a.w * r));
-      }
-    }
+  if (parts == 1) return;
+
+  // ---- join the chunks: the last CTA of this (sequence, head tile) to arrive ---------------
+  __threadfence();
+  __syncthreads();
+  if (tid == 0) {
+    int* counter = p.counters + (long long)b * Y + y;
+    last_flag = atomicAdd(counter, 1) == parts - 1;
+    if (last_flag) *counter = 0;
   }
-  __syncthreads();  // the joined results have been read before the next segment's are written
-  u += seg.n;
-  if (u < u1) next(seg, u);
-  }
-  // a wait that gave up: let this warp's copies in flight land before the CTA can exit
+  __syncthreads();
+  if (!last_flag) return;
+  __threadfence();
 #pragma unroll 1
-  for (; used < fetched; ++used)
-    (void)mbar_wait_suspend(&bars[warp][used % kStages], (uint32_t)((used / kStages) & 1), nullptr);
+  for (int e = tid; e < heads * D / 4; e += kThreads) {
+    const int h = e / (D / 4), d = (e % (D / 4)) * 4;
+    const float* rows = p.partials + (head0 + h) * p.chunks * kRow;
+    float mm = -INFINITY, ll = 0.f;
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+    for (int c = 0; c < parts; ++c) mm = fmaxf(mm, __ldcg(rows + (long long)c * kRow + D));
+#pragma unroll 8
+    for (int c = 0; c < parts; ++c) {
+      const float* row = rows + (long long)c * kRow;
+      const float2 st = __ldcg(reinterpret_cast<const float2*>(row + D));
+      const float4 v = __ldcg(reinterpret_cast<const float4*>(row + d));
+      const float f = st.x == mm ? 1.f : ex2_approx(st.x - mm);
+      ll += f * st.y;
+      a.x += f * v.x; a.y += f * v.y; a.z += f * v.z; a.w += f * v.w;
+    }
+    const float r = ll != 0.f ? 1.f / ll : 0.f;
+    store_out4(p.out, p.dtype, (head0 + h) * D + d, make_float4(a.x * r, a.y * r, a.z * r, a.w * r));
+  }
 }
 
 template <int P, int BS, bool SPLIT>
-int launch(const DecodeInt4Params& p, int sms, cudaStream_t st) {
-  const size_t smem = smem_bytes<P, SPLIT>() + ((size_t)p.B + 1) * 4;
-  if (!allow_smem<decode_int4_kernel<P, BS, SPLIT>>(smem_bytes<P, SPLIT>() + 4097 * 4)) return SPD_ERR_CUDA;
-  if (p.whole) {
-    const int G = p.Hq / p.Hkv, kHeads = SPLIT ? 4 : 8;
-    const unsigned n = (unsigned)(p.B * p.Hkv * ((G + kHeads - 1) / kHeads));
-    decode_int4_kernel<P, BS, SPLIT><<<n, kThreads, smem_bytes<P, SPLIT>(), st>>>(p);
-    return cudaPeekAtLastError() == cudaSuccess ? SPD_OK : SPD_ERR_CUDA;
-  }
-  // as many CTAs as fit at once: by registers (found once) and by shared memory (228 KB an SM,
-  // 1 KB and the static part taken per CTA)
-  static const int by_regs = [] {
-    int n = 0;
-    return cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, decode_int4_kernel<P, BS, SPLIT>, kThreads,
-                                                         smem_bytes<P, SPLIT>()) == cudaSuccess && n > 0 ? n : 1;
-  }();
-  int per_sm = (int)(228 * 1024 / (smem + 2048));
-  per_sm = per_sm < 1 ? 1 : per_sm > by_regs ? by_regs : per_sm;
-  if (per_sm > kMaxCtas) per_sm = kMaxCtas;
-  decode_int4_kernel<P, BS, SPLIT><<<sms * per_sm, kThreads, smem, st>>>(p);
+int launch(const DecodeInt4Params& p, unsigned grid, cudaStream_t st) {
+  if (!allow_smem<decode_int4_kernel<P, BS, SPLIT>>(ring_bytes<P>())) return SPD_ERR_CUDA;
+  decode_int4_kernel<P, BS, SPLIT><<<grid, kThreads, ring_bytes<P>(), st>>>(p);
   return cudaPeekAtLastError() == cudaSuccess ? SPD_OK : SPD_ERR_CUDA;
 }
 
@@ -721,23 +595,41 @@ int launch(const DecodeInt4Params& p, int sms, cudaStream_t st) {
 
 // Heads per column tile: four with two columns each, or eight.
 static int dec4_heads(int dtype, int G) { return (dtype == SPD_F32 || G <= 4) ? 4 : 8; }
-
-// Bytes of partial results: two slots per CTA.
-size_t decode_int4_partial_bytes(int Hq, int Hkv, int D, int dtype, int sms) {
-  return (size_t)sms * dec4::kMaxCtas * 2 * dec4_heads(dtype, Hq / Hkv) * (D + 4) * 4;
+static long long dec4_tiles(int Hq, int Hkv, int dtype) {
+  const int G = Hq / Hkv, heads = dec4_heads(dtype, G);
+  return (long long)Hkv * ((G + heads - 1) / heads);
 }
 
-int decode_int4_launch(DecodeInt4Params p, int D, int bs, int sms, cudaStream_t st) {
+// CTAs for each (sequence, head tile), from the longest contexts that the tables hold.  With up to 2048
+// tokens for each CTA slot of the device all CTAs run at once, in chunks of 1024 tokens (four steps a
+// warp) or more: less makes the join cost more than it saves (one context of 32,000 tokens, 8 key/value
+// heads of 128: 17.5 us in chunks of 1024, 20.6 of 640, 22.0 of 1536; one of 448, 12 heads of 64:
+// 5.3 us in one chunk, 7.1 in two).  Beyond that, chunks of 2048 to 4096 tokens, half a slot's share
+// within these: the SMs' rates differ by up to a third, and CTAs that are dealt out as slots fall free
+// even that out (the 32 contexts above: one equal share per slot 132 us, chunks of 512 tokens 192, 1024
+// 146, 2048 126, 4096 128; the 128 contexts: 97, 102, 80, 70, 66).
+Int4Split decode_int4_split(int B, int Hq, int Hkv, int D, int dtype, int max_ctx, int sms) {
   using namespace dec4;
-  p.whole = (long long)p.max_blocks * bs <= kWholeTokens;
-  const int kHeads = dec4_heads(p.dtype, p.Hq / p.Hkv);
+  constexpr int kLeast = 1024, kChunk = 2048;
+  const int per_sm = D == 64 ? ctas_per_sm<1>() : D == 128 ? ctas_per_sm<2>() : ctas_per_sm<4>();
+  const long long slots = (long long)sms * per_sm, pairs = B * dec4_tiles(Hq, Hkv, dtype);
+  const long long share = max_ctx * pairs / slots;  // tokens
+  if (share <= kChunk) return {(int)std::max(1ll, std::min(slots / pairs, (max_ctx + kLeast - 1ll) / kLeast)), kLeast};
+  const long long c = std::min(std::max(share / 2, (long long)kChunk), 2ll * kChunk);
+  return {(int)((max_ctx + c - 1) / c), kChunk};
+}
+
+int decode_int4_launch(const DecodeInt4Params& p, int D, int bs, cudaStream_t st) {
+  using namespace dec4;
+  const long long grid = (long long)p.chunks * p.B * dec4_tiles(p.Hq, p.Hkv, p.dtype);
+  if (grid > 0x7fffffffll) return SPD_ERR_UNSUPPORTED;
   auto by_bs = [&](auto planes, auto split) -> int {
     constexpr int P = decltype(planes)::value;
     constexpr bool S = decltype(split)::value;
     switch (bs) {
-      case 8: return launch<P, 8, S>(p, sms, st);
-      case 16: return launch<P, 16, S>(p, sms, st);
-      case 32: return launch<P, 32, S>(p, sms, st);
+      case 8: return launch<P, 8, S>(p, (unsigned)grid, st);
+      case 16: return launch<P, 16, S>(p, (unsigned)grid, st);
+      case 32: return launch<P, 32, S>(p, (unsigned)grid, st);
       default: return SPD_ERR_UNSUPPORTED;
     }
   };
@@ -749,7 +641,7 @@ int decode_int4_launch(DecodeInt4Params p, int D, int bs, int sms, cudaStream_t 
       default: return SPD_ERR_UNSUPPORTED;
     }
   };
-  return kHeads == 4 ? by_planes(std::true_type{}) : by_planes(std::false_type{});
+  return dec4_heads(p.dtype, p.Hq / p.Hkv) == 4 ? by_planes(std::true_type{}) : by_planes(std::false_type{});
 }
 
 }  // namespace spd

@@ -27,8 +27,8 @@ int cross_kv_project_launch(const void* enc_out, const void* w_kv, const void* b
                             int T_out, int64_t out_slot_stride, int dtype, int* err, int sms, cudaStream_t st);
 int rope_append_launch(const RopeAppendParams& p, int dtype, bool int4_pool, int sms, cudaStream_t st);
 int gather_int4_launch(const GatherInt4Params& p, int dtype, int sms, cudaStream_t st);
-size_t decode_int4_partial_bytes(int Hq, int Hkv, int D, int dtype, int sms);
-int decode_int4_launch(DecodeInt4Params p, int D, int bs, int sms, cudaStream_t st);
+Int4Split decode_int4_split(int B, int Hq, int Hkv, int D, int dtype, int max_ctx, int sms);
+int decode_int4_launch(const DecodeInt4Params& p, int D, int bs, cudaStream_t st);
 int prompt_attn_launch(PromptParams p, const void* q, const void* k, const void* v, long long q_st, long long q_sh,
                        long long k_st, long long k_sh, long long v_st, long long v_sh, int dtype, int sms,
                        cudaStream_t st);
@@ -492,8 +492,9 @@ size_t spd_paged_decode_attn_int4_workspace_size(int B, int Hq, int Hkv, int D, 
   if (B <= 0 || Hkv <= 0 || Hq <= 0 || Hq % Hkv || !int4_shape_ok(D, block_size) || max_blocks <= 0 ||
       max_ctx > INT32_MAX || sms <= 0)
     return 0;
+  const size_t chunks = (size_t)spd::decode_int4_split(B, Hq, Hkv, D, dtype, (int)max_ctx, sms).chunks;
   return spd::kWsHeaderBytes + spd::round_up((size_t)B * Hq * 4, 256) +
-         spd::round_up(spd::decode_int4_partial_bytes(Hq, Hkv, D, dtype, sms), 256);
+         spd::round_up((size_t)B * Hq * chunks * (D + 4) * 4, 256);
 }
 
 int spd_paged_decode_attn_int4(const void* q, const void* pool, const int32_t* block_tables,
@@ -526,7 +527,10 @@ int spd_paged_decode_attn_int4(const void* q, const void* pool, const int32_t* b
   p.err = reinterpret_cast<int*>(ws);
   p.counters = reinterpret_cast<int*>(ws + spd::kWsHeaderBytes);
   p.partials = reinterpret_cast<float*>(ws + spd::kWsHeaderBytes + spd::round_up((size_t)B * Hq * 4, 256));
-  const int rc = spd::decode_int4_launch(p, D, block_size, sm_count(-1), static_cast<cudaStream_t>(stream));
+  const spd::Int4Split split = spd::decode_int4_split(B, Hq, Hkv, D, dtype, (int)max_ctx, sm_count(-1));
+  p.chunks = split.chunks;
+  p.least = split.least;
+  const int rc = spd::decode_int4_launch(p, D, block_size, static_cast<cudaStream_t>(stream));
   if (rc != SPD_OK)
     return fail(rc, "spd_paged_decode_attn_int4: launch failed: %s", cudaGetErrorString(cudaGetLastError()));
   return ok();

@@ -253,8 +253,6 @@ __device__ __forceinline__ bool mbar_wait_more(uint64_t* bar, uint32_t parity, i
     }
   return true;
 }
-
-// instruction-cache room is worth more than a call there.
 __device__ __forceinline__ bool mbar_wait_suspend(uint64_t* bar, uint32_t parity, int* err,
                                                   unsigned long long limit_ns = SPD_WAIT_NS) {
   return mbar_try_wait_suspend(bar, parity) || mbar_wait_more(bar, parity, err, limit_ns);

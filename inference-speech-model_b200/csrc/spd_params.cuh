@@ -141,6 +141,11 @@ struct PromptParams {  // attention of packed prompts (prompt_attn.cu)
   unsigned long long wait_ns;
 };
 
+// How a 4-bit decode call is split: CTAs per (sequence, head tile) and the fewest tokens for one.
+struct Int4Split {
+  int chunks, least;
+};
+
 struct DecodeInt4Params {  // single-token attention over a 4-bit pool (paged_decode_attn_int4.cu)
   const void* q;
   const unsigned char* pool;
@@ -149,11 +154,12 @@ struct DecodeInt4Params {  // single-token attention over a 4-bit pool (paged_de
   void* out;
   int dtype;
   int B, Hq, Hkv, max_blocks, num_blocks;
-  int whole;          // one CTA per (sequence, head tile)
+  int least;          // tokens a CTA takes at least
+  int chunks;         // CTAs per (sequence, head tile)
   float scale_log2;   // scale * log2(e)
   int* err;           // workspace error word
   int* counters;      // [B * Hkv * head tiles] arrivals, left at zero
-  float* partials;    // two slots per CTA of [heads of a tile][D + 4]
+  float* partials;    // [B * Hq][chunks][D + 4]
   unsigned long long wait_ns;
 };
 
