@@ -15,19 +15,29 @@
 //   head sit in one tile (row = token * pack + head), so K and V are read once for all of
 //   them and short prompts fill the rows.
 // * Warp 0 loads Q, K and V tiles by TMA (3-D maps over [tokens][heads][D], any strides;
-//   128-byte swizzle); warp 1 issues tcgen05.mma: S = Q K^T into TMEM and O += P V with P
-//   read from TMEM (it overwrites S) and V as the MN-major operand, so nothing is transposed
-//   or written back to shared memory.
+//   128-byte swizzle).  One lane of warp 1 issues every tcgen05.mma, four at a time, with nothing
+//   else in its step: S = Q K^T into TMEM and O += P V with P read from TMEM (it overwrites S)
+//   and V as the MN-major operand, so nothing is transposed or written back to shared memory.
 // * Warps 4-7 and 8-11 are the softmax of tiles A and B: one row per thread, so the row
 //   maximum and sum need no shuffles.  While one tile's softmax runs, the tensor cores work on
-//   the other tile.  The running maximum is raised only when a score passes it by 8 (in
-//   log2), so O in TMEM is rescaled rarely; P is at most 2^8 and rounded to the input type
-//   (its 8 or 11 bits are what the tensor core takes), the row sum is taken in fp32 before
-//   the rounding.
-// * Rows of V past a sequence's last key are set to zero in shared memory before they are
-//   multiplied (P is zero there, but 0 * NaN is not), so what another sequence holds never
+//   the other tile; weights are handed over in halves of 64 keys.  The running maximum is raised
+//   only when a score passes it by 8 (in log2), so O in TMEM is rescaled rarely; P is at most
+//   2^8 and rounded to the input type (its 8 or 11 bits are what the tensor core takes), the row
+//   sum is taken in fp32 before the rounding.  A quarter of the exponentials is a polynomial on
+//   the fp32 pipes.
+// * Rows of V past a sequence's last key are set to zero in shared memory by warp 2 before they
+//   are multiplied (P is zero there, but 0 * NaN is not), so what another sequence holds never
 //   reaches this one's result.
-// * Persistent: one CTA per SM walks the (tile, head) items; every wait is bounded.
+// * Persistent: one CTA per SM walks the (tile, head) items; every wait is bounded, and waits
+//   suspend the thread, which leaves the issue slots to the softmax warps.
+//
+// Measured (bf16, 32 query and 8 key/value heads of 128, causal): 8192 tokens 486 us, 1.13 PFLOP/s,
+// 0.69 of the library product's rate in a short run; 4 x 4096 tokens, 16 heads, not causal 1.18.  A
+// step of 128 keys of both tiles takes about 3,250 cycles against 2,050 of products: a tile's chain
+// (scores, their maximum, 128 exponentials a thread, weights, P V, next scores) is 1.5 times as long
+// as the other tile's products can cover.  fp16, 20 heads of 64, 8 x 1500 tokens, not causal: 167 us,
+// 0.55 PFLOP/s, where exponentials alone take 115.  Two threads a row, two issuing lanes (the tiles fall
+// into step), and a second read of S in place of 128 registers were all slower (579, 565 and 525 us).
 #include "spd_tc.cuh"
 
 namespace spd {
@@ -157,6 +167,13 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   }
 }
 
+// the largest of three, NaN if one of them is
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
 // ---- pairs of fp32 in one instruction ----------------------------------------------------
 typedef unsigned long long f32x2;
 __device__ __forceinline__ f32x2 pair(float a, float b) {
@@ -210,7 +227,7 @@ __device__ __forceinline__ float2 exp2_poly(f32x2 x) {
 
 constexpr int kPoly = 2;  // of 8 pairs, to the polynomial
 // Weights of 64 keys: p = 2^(s * c - m) rounded to T and packed, sums added.  EXACT: all on the
-// special-function unit, so that a masked score (-inf) gives an exact zero; otherwise kPoly of
+// special-function unit, so that a masked score (-inf) gives an exact zero and a NaN a NaN; otherwise kPoly of
 // each 8 pairs go to the polynomial (0: 492 us, 2: 484 us, 4: 496 us for 8192 causal tokens, 32 / 8
 // heads of 128; the polynomial's six packed fp32 instructions soon cost more than they free).
 template <typename T, bool EXACT>
@@ -568,8 +585,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int c = 4; c < 64; c += 8)
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            mx4[i] = c + 4 + i < 64 ? fmaxf(fmaxf(mx4[i], __uint_as_float(s[c + i])), __uint_as_float(s[c + 4 + i]))
-                                    : fmaxf(mx4[i], __uint_as_float(s[c + i]));
+            mx4[i] = max3_nan(mx4[i], __uint_as_float(s[c + i]), __uint_as_float(s[c + 4 + i < 64 ? c + 4 + i : c + i]));
         if (!edge) {
           tmem_ld_wait(s + 64);
           tmem_ld_wait(s + 96);
@@ -578,10 +594,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int c = 64; c < BN; c += 8)
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            mx4[i] = fmaxf(fmaxf(mx4[i], __uint_as_float(s[c + i])), __uint_as_float(s[c + 4 + i]));
-        const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * p.scale_log2;
-        const bool raise = mx > m + kLazy;
+            mx4[i] = max3_nan(mx4[i], __uint_as_float(s[c + i]), __uint_as_float(s[c + 4 + i]));
+        const float mx = max3_nan(max3_nan(mx4[0], mx4[1], mx4[2]), mx4[3], mx4[3]) * p.scale_log2;
+        // Also for a NaN and for infinite scores, which only the exact exponentials treat as they are.
+        const bool raise = !(mx < m + kLazy);
+        bool exact = edge;
         if (__any_sync(0xffffffffu, raise)) {
+          exact |= __any_sync(0xffffffffu, !(fabsf(mx) < INFINITY));
           const float mn = fmaxf(m, mx);
           const float f = m == mn ? 1.f : ex2_approx(m - mn);
           m = mn;
@@ -605,7 +624,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           uint32_t pk[32];
-          if (edge) weights64<T, true>(s + 64 * h, c2, nm2, pk, sum);
+          if (exact) weights64<T, true>(s + 64 * h, c2, nm2, pk, sum);
           else weights64<T, false>(s + 64 * h, c2, nm2, pk, sum);
           tmem_st32(s_col + 32 * h, pk);
           tmem_st_wait();

@@ -15,8 +15,16 @@
 //   code  = clamp(rint((x - zero) / scale), 0, 15),        0 where scale is 0
 // computed from the fp32 rotated keys (no rounding to the model's type in between).  A NaN
 // makes its 64 values NaN (through the parameters); an infinity saturates.
-#include <limits>
-
+//
+// What bounds them: HBM for prompts, since each value is read once and written once (a 4-bit row as
+// 4.5 bits per value) and the rotation is a few operations; the latency of a few dependent loads
+// (sequence, table, row) for a decode step.  So a CTA looks up the places of its tokens once, a thread
+// keeps its dimensions for all of them, and for few tokens a CTA takes one.
+// Measured: a step's 64 tokens, 12 heads of 64, fp16: 2.8 us; 16 prompts of 200 to 2,000 tokens, 32/8
+// heads of 128, bf16 (468 MB): 91 us, 5.1 TB/s, 0.79 of a plain copy's rate.  Into 4 bits, 7 prompts
+// of up to 4,001 tokens, 16/8 heads of 128: 73 us for 199 MB, by then bounded by the issue of about ten
+// instructions a value.  16 prefixes of 1,000 to 8,000 tokens out of 4 bits, 8 heads of 128 (390 MB):
+// 76 us, 5.1 TB/s.
 #include "spd_int4.cuh"
 #include "spd_params.cuh"
 

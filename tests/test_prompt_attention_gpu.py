@@ -151,6 +151,37 @@ def test_other_sequences_never_leak():
     assert torch.equal(got[50:127], want[50:127]) and torch.isnan(got[:50]).all()
 
 
+@pytest.mark.parametrize("at", [0, 3, 5, 64, 130, 255])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("D", [64, 128])
+def test_a_bad_key_shows_in_the_rows_that_see_it(at, bad, causal, D):
+    """One NaN or infinite key element: rows that see the key give NaN, the others their result."""
+    q, k, v = make(at, 256, 256, 2, 1, D, torch.bfloat16)
+    q[:, :, 7] = q[:, :, 7].abs() + 0.1  # the infinite score is +inf
+    out, A, slack = reference(q, k, v, [256], [256], causal, 1 / math.sqrt(D))
+    bound = UNIT[q.dtype] * (A + out.abs() * 1.001) + slack
+    k[at, 0, 7] = bad
+    got = ops.prompt_attention(q.to(DEV), k.to(DEV), v.to(DEV), cu([256]).to(DEV), causal=causal)
+    first = at if causal else 0
+    assert torch.isnan(got[first:]).all()
+    assert ((got.cpu().double() - out).abs() <= bound)[:first].all()
+
+
+def test_scores_of_minus_infinity():
+    """Keys whose scores are -inf have no weight; a row that has no other key gives zeros."""
+    q, k, v = make(5, 200, 200, 2, 1, 64, torch.float16)
+    q[:, :, 7] = q[:, :, 7].abs() + 0.1
+    k[:150, 0, 7] = -math.inf
+    got = ops.prompt_attention(q.to(DEV), k.to(DEV), v.to(DEV), cu([200]).to(DEV))
+    assert not got[:150].any()
+    keys = k[150:].clone()
+    want = ops.prompt_attention(q[150:].contiguous().to(DEV), keys.to(DEV), v[150:].contiguous().to(DEV), cu([50]).to(DEV))
+    # two ways to the same sums: the unit of the output and of a weight, twice each
+    bound = 4 * UNIT[torch.float16] * v[150:].abs().max().item()
+    assert (got[150:].float() - want.float()).abs().max().item() <= bound
+
+
 def test_rows_of_no_sequence_are_left_alone():
     q, k, v = (t.to(DEV) for t in make(8, 100, 100, 2, 2, 64, torch.float16))
     out = torch.full_like(q, 7.0)
