@@ -270,7 +270,7 @@ size_t spd_kv_int4_page_bytes(int D, int block_size); /* 0: not supported */
  *   dimensions >= rot pass through.  fp32 arithmetic, one rounding to dtype.
  *   Tokens of skipped sequences, past cu[B], or whose position or block is out of range
  *   (flagged in error_word) are not written; their rows of q_out are zero.
- * Requires D % 8 == 0, rot % 16 == 0, rot <= D, 16-byte aligned pointers, strides and rows. */
+ * Requires D % 8 == 0, D <= 1024, rot % 16 == 0, rot <= D, 16-byte aligned pointers, strides and rows. */
 int spd_rope_kv_append(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k, int64_t k_stride_t,
                        int64_t k_stride_h, const void* v, int64_t v_stride_t, int64_t v_stride_h, void* q_out,
                        const float* cos_table, const float* sin_table, void* k_pool, void* v_pool,

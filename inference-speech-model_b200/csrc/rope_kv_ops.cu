@@ -21,18 +21,23 @@
 // (sequence, table, row) for a decode step.  So a CTA looks up the places of its tokens once, a thread
 // keeps its dimensions for all of them, and for few tokens a CTA takes one.
 // Measured: a step's 64 tokens, 12 heads of 64, fp16: 2.8 us; 16 prompts of 200 to 2,000 tokens, 32/8
-// heads of 128, bf16 (468 MB): 91 us, 5.1 TB/s, 0.79 of a plain copy's rate.  Into 4 bits, 7 prompts
-// of up to 4,001 tokens, 16/8 heads of 128: 73 us for 199 MB, by then bounded by the issue of about ten
-// instructions a value.  16 prefixes of 1,000 to 8,000 tokens out of 4 bits, 8 heads of 128 (390 MB):
-// 76 us, 5.1 TB/s.
+// heads of 128, bf16 (468 MB): 87 us, 5.4 TB/s, 0.82 of a plain copy's rate.  Into 4 bits, 7 prompts
+// of up to 4,001 tokens, 16/8 heads of 128 (199 MB): 55 us, 3.6 TB/s, by then bounded by the latency and
+// issue of the groups' exchanges and parameters.  16 prefixes of 1,000 to 8,000 tokens out of 4 bits,
+// 8 heads of 128 (390 MB): 64 us, 6.1 TB/s.
 #include "spd_int4.cuh"
 #include "spd_params.cuh"
 
 namespace spd {
 namespace rope {
 
-constexpr int kThreads = 256;
-constexpr int kMaxTokens = 16;  // tokens per CTA
+// Threads and most tokens of a CTA.  Small CTAs: rows of q are done before rows that are quantised,
+// and a CTA's room is free as soon as its own rows are done (256 threads: 59 us in place of 55 for the
+// 7 prompts above into 4 bits, 91 in place of 87 for the 16 into 16 bits).  Eight tokens share a
+// look-up (four: 57 and 88 us; two: 64 and 93); where nothing but copying is left, four (the 16
+// prefixes: 64 us, eight 71, sixteen 78).
+constexpr int kThreads = 64, kMaxTokens = 8;
+constexpr int kGatherThreads = 256, kGatherTokens = 4;
 
 // Where a packed token lives: its position and the pool row block * block_size + offset.
 struct Place {
@@ -92,6 +97,16 @@ __device__ __forceinline__ float min_nan(float a, float b) {
 __device__ __forceinline__ float max_nan(float a, float b) {
   float r;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float min_nan(float a, float b, float c) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
 
@@ -178,23 +193,31 @@ __device__ __forceinline__ void turn(float (&lo)[8], float (&hi)[8], const float
 }
 
 // Eight values of one 64-value group to a word of codes, rint((y - z) / s) clamped to 0..15 each.
-// The quotient is taken as a product with 1 / s, which is within 2^-20 of it here; only where that
-// leaves the rounding open (within 2e-5 of a half, 4e-5 of all values) is the division made.  The
-// rounded code is read from the low bits of t + 2^23, whose constant high part is taken off
-// the whole word.
-__device__ __forceinline__ uint32_t encode8(const float (&y)[8], float s, float z, float inv) {
+// One multiply-add per value gives v = 2^16 ((y - z) / s + 1/2) + 2 as a whole number in the low bits of
+// 2^23 + v: byte 2 is the code, the low half says how far it is from the next one.  It is within 1.2
+// of the quotient's own (three roundings of at most 1/2, 1/2 and 0.2 while |z| < 64 s), so a code may
+// be another one only where the low half is at most 4: one value in 13,000, whose word is then made
+// by division.  So is a word where s or z is saturated or s subnormal, or |z| >= 64 s: elsewhere the
+// parameters' own rounding moves no quotient out of 0..15.
+__device__ __forceinline__ uint32_t encode8(const float (&y)[8], float s, float z) {
   if (!(s > 0.f)) return 0u;
-  uint32_t word = 0;
-  float open = 0.f;
+  const float inv = __frcp_rn(s), a = inv * 65536.f, c = fmaf(-z, a, 8388608.f + 32768.f + 2.f);
+  uint32_t u[8];
 #pragma unroll
-  for (int k = 7; k >= 0; --k) {
-    const float t = fminf(fmaxf(__fmul_rn(__fsub_rn(y[k], z), inv), 0.f), 15.f);
-    const float u = __fadd_rn(t, 8388608.f);
-    open = fmaxf(open, fabsf(__fsub_rn(t, __fsub_rn(u, 8388608.f))));
-    word = (word << 4) + __float_as_uint(u);
-  }
-  word -= 0xFB000000u;  // 0x4B000000 * (1 + 16 + ... + 16^7) modulo 2^32
-  if (open > 0.49998f) {
+  for (int k = 0; k < 8; ++k) u[k] = __float_as_uint(fmaf(y[k], a, c));
+  auto least = [](uint32_t p, uint32_t q) {
+    uint32_t r;
+    asm("min.u16x2 %0, %1, %2;" : "=r"(r) : "r"(p), "r"(q));
+    return r;
+  };
+  auto lows = [&](int k) { return __byte_perm(u[k], u[k + 1], 0x5410); };
+  const uint32_t low = least(least(lows(0), lows(2)), least(lows(4), lows(6)));
+  auto codes = [&](int k) {  // of values k, k + 2, k + 4, k + 6
+    return __byte_perm(__byte_perm(u[k], u[k + 2], 0x0062), __byte_perm(u[k + 4], u[k + 6], 0x0062), 0x5410);
+  };
+  uint32_t word = (codes(0) & 0x0F0F0F0Fu) | (codes(1) & 0x0F0F0F0Fu) << 4;
+  const bool sure = s >= 6.103515625e-5f && s < 65504.f && fabsf(z) < 65504.f && fabsf(z * inv) < 64.f;
+  if (!sure || min(low & 0xFFFFu, low >> 16) <= 4u) {
     word = 0;
 #pragma unroll 1
     for (int k = 7; k >= 0; --k) {
@@ -214,7 +237,8 @@ __device__ __forceinline__ uint32_t encode8(const float (&y)[8], float s, float 
 // so every value is loaded once, shares its eight angles, and all that depends on the row is worked
 // out once.  The next tokens' values are loaded while one is worked on.
 template <typename T, bool INT4>
-__global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 4 : 3) rope_append_kernel(const RopeAppendParams p, int tokens, int rpc) {
+__global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 16 : INT4 ? 10 : 12)
+    rope_append_kernel(const RopeAppendParams p, int tokens, int rpc) {
   __shared__ Place place[kMaxTokens];
   const int token0 = blockIdx.x * tokens, n = min(tokens, p.N - token0);
   const int upr = (p.D + 15) / 16;  // units per head row
@@ -232,8 +256,15 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 4 : 3) rope_append_
                  h * (is_q ? p.q_sh : is_k ? p.k_sh : p.v_sh);
   T* dst = reinterpret_cast<T*>(is_q ? p.q_out : is_k ? p.k_pool : p.v_pool) + (long long)h * p.D;
   const long long q_step = (long long)p.Hq * p.D;
+  // planes of 64 dimensions share a scale: does every thread of this warp hold 16 dimensions of the
+  // plane of its own four neighbours?  (Not where a rotation over more than 64 dimensions pairs planes.)
+  const int planes = p.D / int4::kPlane;
+  const bool one_plane =
+      INT4 && __all_sync(0xffffffffu, !live || is_q || (d0 / int4::kPlane == u / 4 && d1 / int4::kPlane == u / 4));
   const float *cs = p.cos + 8 * u, *sn = p.sin + 8 * u;
-  constexpr int kAhead = sizeof(T) == 2 ? 2 : 1;  // tokens loaded ahead (one: 94 us against 91 for 17,000 tokens)
+  // tokens loaded ahead (of 16 bits one: 94 us against 91 for the 16 prompts above; into 4 bits two: 63 us
+  // against 59, for want of registers)
+  constexpr int kAhead = sizeof(T) == 2 && !INT4 ? 2 : 1;
   Raw8<T> lo_raw[kAhead], hi_raw[kAhead];
   auto load = [&](int t, int slot) {
     if (live && t < n) {
@@ -268,49 +299,77 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 4 : 3) rope_append_
     }
     if constexpr (INT4) {
       if (__any_sync(0xffffffffu, live && !is_q && w.block >= 0)) {
-        // least and largest of each plane over the row's 4, 8 or 16 threads; a thread's two chunks
-        // may lie in different planes
-        const int planes = p.D / int4::kPlane, pl0 = d0 / int4::kPlane, pl1 = d1 / int4::kPlane;
-        float mn0 = lo[0], mx0 = lo[0], mn1 = hi[0], mx1 = hi[0];
+        float mn0 = min_nan(lo[0], lo[1]), mx0 = max_nan(lo[0], lo[1]), mn1 = min_nan(hi[0], hi[1]), mx1 = max_nan(hi[0], hi[1]);
 #pragma unroll
-        for (int k = 1; k < 8; ++k) {
-          mn0 = min_nan(mn0, lo[k]);
-          mx0 = max_nan(mx0, lo[k]);
-          mn1 = min_nan(mn1, hi[k]);
-          mx1 = max_nan(mx1, hi[k]);
+        for (int k = 2; k < 8; k += 2) {
+          mn0 = min_nan(mn0, lo[k], lo[k + 1]);
+          mx0 = max_nan(mx0, lo[k], lo[k + 1]);
+          mn1 = min_nan(mn1, hi[k], hi[k + 1]);
+          mx1 = max_nan(mx1, hi[k], hi[k + 1]);
         }
-        float a0 = 0.f, b0 = 0.f, a1 = 0.f, b1 = 0.f;  // (least, largest) of each chunk's plane
-        for (int pl = 0; pl < planes; ++pl) {
-          float mn = INFINITY, mx = -INFINITY;
-          if (pl0 == pl) mn = mn0, mx = mx0;
-          if (pl1 == pl) mn = min_nan(mn, mn1), mx = max_nan(mx, mx1);
-          for (int o = 1; o < upr; o <<= 1) {
+        const bool writes = live && !is_q && w.block >= 0;
+        const int half = int4::half_bytes(planes, p.block_size);
+        unsigned char* page = reinterpret_cast<unsigned char*>(p.k_pool) + ((long long)w.block * p.Hkv + h) * (2 * half) +
+                              (is_k ? 0 : half);
+        // scale and zero of a group from its least and largest value; the rounded ones in s and z
+        auto parameters = [](float mn, float mx, float& s, float& z) {
+          constexpr float kMax = 65504.f;
+          s = __fdiv_rn(__fsub_rn(mx, mn), 15.f);
+          s = s > kMax ? kMax : s;  // a NaN stays
+          z = mn > kMax ? kMax : mn < -kMax ? -kMax : mn;
+          const __half2 h = __halves2half2(__float2half_rn(s), __float2half_rn(z));
+          s = __low2float(h);
+          z = __high2float(h);
+          return h;
+        };
+        auto put = [&](const float (&y)[8], int d, __half2 sz, float s, float z) {
+          const int slot = (d / int4::kPlane) * p.block_size + w.off, in = d % int4::kPlane;
+          *reinterpret_cast<uint32_t*>(page + slot * int4::kRowBytes + in / 2) = encode8(y, s, z);
+          if (in == 0)
+            *reinterpret_cast<__half2*>(page + planes * p.block_size * int4::kRowBytes + slot * int4::kParamBytes) = sz;
+        };
+        float s, z;
+        if (one_plane) {
+          float mn = min_nan(mn0, mn1), mx = max_nan(mx0, mx1);
+#pragma unroll
+          for (int o = 1; o < 4; o <<= 1) {
             mn = min_nan(mn, __shfl_xor_sync(0xffffffffu, mn, o));
             mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, o));
           }
-          if (pl0 == pl) a0 = mn, b0 = mx;
-          if (pl1 == pl) a1 = mn, b1 = mx;
-        }
-        if (live && !is_q && w.block >= 0) {
-          const int half = int4::half_bytes(planes, p.block_size);
-          unsigned char* page = reinterpret_cast<unsigned char*>(p.k_pool) +
-                                ((long long)w.block * p.Hkv + h) * (2 * half) + (is_k ? 0 : half);
-          auto put = [&](const float (&y)[8], int d, float mn, float mx) {
-            constexpr float kMax = 65504.f;
-            float s = __fdiv_rn(__fsub_rn(mx, mn), 15.f);
-            s = s > kMax ? kMax : s;  // a NaN stays
-            const float z = mn > kMax ? kMax : mn < -kMax ? -kMax : mn;
-            const __half sh = __float2half_rn(s), zh = __float2half_rn(z);
-            s = __half2float(sh);
-            const int slot = (d / int4::kPlane) * p.block_size + w.off, in = d % int4::kPlane;
-            *reinterpret_cast<uint32_t*>(page + slot * int4::kRowBytes + in / 2) =
-                encode8(y, s, __half2float(zh), __frcp_rn(s));
-            if (in == 0)
-              *reinterpret_cast<__half2*>(page + planes * p.block_size * int4::kRowBytes + slot * int4::kParamBytes) =
-                  __halves2half2(sh, zh);
-          };
-          put(lo, d0, a0, b0);
-          put(hi, d1, a1, b1);
+          if (writes) {
+            const __half2 sz = parameters(mn, mx, s, z);
+            put(lo, d0, sz, s, z);
+            put(hi, d1, sz, s, z);
+          }
+        } else {
+          const int pl0 = d0 / int4::kPlane, pl1 = d1 / int4::kPlane;
+          float a0 = 0.f, b0 = 0.f, a1 = 0.f, b1 = 0.f;  // (least, largest) of each chunk's plane
+          for (int pl = 0; pl < planes; pl += 2) {        // two planes' exchanges beside each other
+            float mn[2], mx[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              mn[i] = pl0 == pl + i ? mn0 : INFINITY;
+              mx[i] = pl0 == pl + i ? mx0 : -INFINITY;
+              if (pl1 == pl + i) mn[i] = min_nan(mn[i], mn1), mx[i] = max_nan(mx[i], mx1);
+            }
+            for (int o = 1; o < upr; o <<= 1)
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                mn[i] = min_nan(mn[i], __shfl_xor_sync(0xffffffffu, mn[i], o));
+                mx[i] = max_nan(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], o));
+              }
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              if (pl0 == pl + i) a0 = mn[i], b0 = mx[i];
+              if (pl1 == pl + i) a1 = mn[i], b1 = mx[i];
+            }
+          }
+          if (writes) {
+            __half2 sz = parameters(a0, b0, s, z);
+            put(lo, d0, sz, s, z);
+            sz = parameters(a1, b1, s, z);
+            put(hi, d1, sz, s, z);
+          }
         }
       }
     }
@@ -328,9 +387,9 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 4 : 3) rope_append_
 // subnormal (c * 2^-24, or 16c * 2^-24), so its conversion is exact and the powers of two go into
 // the scale: c * scale + zero is one fp32 multiply-add whatever way c came.
 template <typename T>
-__global__ void __launch_bounds__(kThreads) gather_int4_kernel(const GatherInt4Params p, int tokens, int rpc) {
-  __shared__ Place place[kMaxTokens];
-  __shared__ int owner[kMaxTokens];
+__global__ void __launch_bounds__(kGatherThreads) gather_int4_kernel(const GatherInt4Params p, int tokens, int rpc) {
+  __shared__ Place place[kGatherTokens];
+  __shared__ int owner[kGatherTokens];
   const int token0 = blockIdx.x * tokens, n = min(tokens, p.N - token0);
   find_places(token0, n, p.cu_seqlens, p.B, p.starts, p.block_tables, p.max_blocks, p.num_blocks, p.block_size,
               0x7fffffff, p.err, place, owner);
@@ -390,22 +449,22 @@ __global__ void __launch_bounds__(kThreads) gather_int4_kernel(const GatherInt4P
 }  // namespace rope
 
 // Tokens per CTA: one while there are fewer tokens than 16 per SM, so that a step's few tokens
-// spread over the SMs, up to sixteen, so that the look-up of a token's place is shared.
-static int tokens_per_cta(int N, int sms) {
+// spread over the SMs, up to `most`, so that the look-up of a token's place is shared.
+static int tokens_per_cta(int N, int most, int sms) {
   const int t = N / (sms * 16);
-  return t < 1 ? 1 : t > rope::kMaxTokens ? rope::kMaxTokens : t;
+  return t < 1 ? 1 : t > most ? most : t;
 }
 
-// Rows per CTA: as even a split of all rows as fits 256 threads of `upr` units a row.
-static int rows_per_cta(int rows, int upr) {
-  const int most = rope::kThreads / upr, parts = (rows + most - 1) / most;
+// Rows per CTA: as even a split of all rows as fits its threads, of `upr` units a row.
+static int rows_per_cta(int rows, int upr, int threads) {
+  const int most = threads / upr, parts = (rows + most - 1) / most;
   return (rows + parts - 1) / parts;
 }
 
 int rope_append_launch(const RopeAppendParams& p, int dtype, bool int4_pool, int sms, cudaStream_t st) {
   using namespace rope;
-  const int tokens = tokens_per_cta(p.N, sms), upr = (p.D + 15) / 16, rows = (p.q ? p.Hq : 0) + 2 * p.Hkv;
-  const int rpc = rows_per_cta(rows, upr);
+  const int tokens = tokens_per_cta(p.N, kMaxTokens, sms), upr = (p.D + 15) / 16, rows = (p.q ? p.Hq : 0) + 2 * p.Hkv;
+  const int rpc = rows_per_cta(rows, upr, kThreads);
   const dim3 grid((unsigned)((p.N + tokens - 1) / tokens), (unsigned)((rows + rpc - 1) / rpc));
   const dim3 block((unsigned)((rpc * upr + 31) / 32 * 32));
   auto run = [&](auto tag) {
@@ -421,7 +480,7 @@ int rope_append_launch(const RopeAppendParams& p, int dtype, bool int4_pool, int
 
 int gather_int4_launch(const GatherInt4Params& p, int dtype, int sms, cudaStream_t st) {
   using namespace rope;
-  const int tokens = tokens_per_cta(p.N, sms), upr = p.D / 32, rpc = rows_per_cta(2 * p.Hkv, upr);
+  const int tokens = tokens_per_cta(p.N, kGatherTokens, sms), upr = p.D / 32, rpc = rows_per_cta(2 * p.Hkv, upr, kGatherThreads);
   const dim3 grid((unsigned)((p.N + tokens - 1) / tokens), (unsigned)((2 * p.Hkv + rpc - 1) / rpc));
   const dim3 block((unsigned)((rpc * upr + 31) / 32 * 32));
   if (dtype == SPD_F32) gather_int4_kernel<float><<<grid, block, 0, st>>>(p, tokens, rpc);

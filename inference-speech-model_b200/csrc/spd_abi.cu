@@ -97,8 +97,10 @@ int rope_append_check(const char* fn, const spd::RopeAppendParams& p, int dtype)
   if (p.N < 0 || p.B < 0 || p.Hkv <= 0 || (p.q && p.Hq <= 0) || p.D <= 0 || p.max_pos <= 0 || p.block_size <= 0 ||
       p.max_blocks <= 0 || p.num_blocks <= 0 || (!p.cu_seqlens && p.N != p.B))
     return fail(SPD_ERR_INVALID_ARG, "%s: bad sizes N=%d B=%d Hq=%d Hkv=%d D=%d", fn, p.N, p.B, p.Hq, p.Hkv, p.D);
-  if (p.D % 8 || p.rot <= 0 || p.rot % 16 || p.rot > p.D)
-    return fail(SPD_ERR_UNSUPPORTED, "%s: need D %% 8 == 0 and a rotated part that is a multiple of 16 up to D", fn);
+  if (p.D % 8 || p.D > 1024 || p.rot <= 0 || p.rot % 16 || p.rot > p.D)
+    return fail(SPD_ERR_UNSUPPORTED,
+                "%s: need D a multiple of 8 up to 1024 and a rotated part that is a multiple of 16 up to D", fn);
+  if (p.Hkv > 4096 || (p.q && p.Hq > 4096)) return fail(SPD_ERR_UNSUPPORTED, "%s: more than 4096 heads", fn);
   for (long long s : {p.k_st, p.k_sh, p.v_st, p.v_sh, p.q ? p.q_st : 0ll, p.q ? p.q_sh : 0ll})
     if ((s * eb) % 16) return fail(SPD_ERR_INVALID_ARG, "%s: strides must be multiples of 16 bytes", fn);
   for (const void* t : {p.q, p.k, p.v, (const void*)p.q_out, (const void*)p.cos, (const void*)p.sin,
@@ -473,6 +475,7 @@ int spd_kv_gather_int4(const void* pool, const int32_t* block_tables, const int3
     return fail(SPD_ERR_INVALID_ARG, "spd_kv_gather_int4: null tensor pointer");
   if (N < 0 || B <= 0 || Hkv <= 0 || max_blocks <= 0 || num_blocks <= 0)
     return fail(SPD_ERR_INVALID_ARG, "spd_kv_gather_int4: bad sizes");
+  if (Hkv > 4096) return fail(SPD_ERR_UNSUPPORTED, "spd_kv_gather_int4: more than 4096 heads");
   if (!aligned16(pool) || !aligned16(k_out) || !aligned16(v_out))
     return fail(SPD_ERR_INVALID_ARG, "spd_kv_gather_int4: tensors must be 16-byte aligned");
   if (N == 0) return ok();

@@ -111,6 +111,47 @@ def test_append_and_gather_4_bit(case, interleaved, dtype):
     assert ops.read_error_word(err) == 0
 
 
+@pytest.mark.parametrize("D,rot", [(128, 64), (128, 96), (128, 112), (256, 128), (256, 192), (256, 256)])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_rotations_that_pair_groups(D, rot, interleaved):
+    """Halves of a rotation in the same group of 64 dimensions, in two, and across their borders."""
+    c = Case([19, 1, 4], [5, 0, 60], 3, 3, D, rot, 8, torch.float16, interleaved, seed=rot)
+    pool = ops.kv_pool_int4(c.blocks, 3, D, 8)
+    ops.rope_kv_append_int4(c.dq, c.dk, c.dv, *c.args, pool, *c.where, cu_seqlens=c.cu.to(DEV), interleaved=interleaved)
+    kc, kp, vc, vp = R.unpack(pool.cpu(), D, 8)
+    for codes, params, x in ((kc, kp, c.rotated(c.k, torch.float32)), (vc, vp, c.v.float())):
+        want = R.quantise(x)
+        assert torch.equal(codes[c.block, c.row], want[0]) and torch.equal(params[c.block, c.row], want[1])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+def test_codes_of_all_kinds_of_groups(dtype):
+    """Groups far from zero, wide, narrow to scales below fp16's normal numbers, and quotients that lie
+    halfway between two codes: the same codes as the plain form's, bit for bit."""
+    D, bs, g = 64, 32, torch.Generator().manual_seed(2)
+    rows = []
+    for offset in (0.0, -0.3, 3.0, -40.0, 1000.0, -6e4, 9e4):
+        for spread in (1e-7, 1e-4, 1e-2, 1.0, 50.0, 2e4, 1e6):
+            rows += [offset + spread * torch.randn(D, generator=g), offset + spread * torch.rand(D, generator=g)]
+    for scale in (2.0 ** -20, 2.0 ** -14, 2.0 ** -3, 1.0, 512.0):
+        ties = torch.randint(0, 31, (D,), generator=g) / 2  # 0, 1/2, ..., 15
+        ties[:2] = torch.tensor([0.0, 15.0])
+        rows += [scale * ties, scale * (ties - 7), scale * (ties - 900)]
+    x = torch.stack(rows)[:, None]
+    x = x if dtype == torch.float32 else x.clamp(-65504.0, 65504.0).to(dtype)
+    n = x.shape[0]
+    blocks = -(-n // bs)
+    cos, sin = torch.ones(blocks * bs, 8), torch.zeros(blocks * bs, 8)
+    pool = ops.kv_pool_int4(blocks, 1, D, bs)
+    ops.rope_kv_append_int4(None, x.to(DEV), x.to(DEV), cos.to(DEV), sin.to(DEV), pool,
+                            torch.arange(blocks, dtype=torch.int32, device=DEV)[None],
+                            torch.zeros(1, dtype=torch.int32, device=DEV), cu_seqlens=R.cu([n]).to(DEV))
+    want = R.quantise(x.float())
+    for codes, params in (R.unpack(pool.cpu(), D, bs)[:2], R.unpack(pool.cpu(), D, bs)[2:]):
+        assert torch.equal(params.flatten(0, 1)[:n], want[1])
+        assert torch.equal(codes.flatten(0, 1)[:n], want[0])
+
+
 def test_decode_form_without_cu_seqlens_and_without_q():
     c = Case([1] * 7, [0, 15, 16, 3, -1, 99, 40], 8, 2, 64, 64, 16, torch.float16, False, packed=False)
     one, two = (ops.kv_pool_int4(c.blocks, 2, 64, 16) for _ in range(2))
@@ -235,3 +276,16 @@ def test_refusals():
     kp = torch.zeros(4, 16, 1, 64, dtype=torch.float16, device=DEV)
     with pytest.raises(RuntimeError, match="pools must be"):
         ops.rope_kv_append(c.dq, c.dk, c.dv, *c.args, kp, kp.float(), *c.where, cu_seqlens=cu)
+    wide = torch.zeros(3, 1, 1032, dtype=torch.float16, device=DEV)
+    pools = [torch.zeros(c.blocks, 16, 1, 1032, dtype=torch.float16, device=DEV) for _ in range(2)]
+    with pytest.raises(RuntimeError, match="up to 1024"):
+        ops.rope_kv_append(None, wide, wide, *c.args, *pools, *c.where, cu_seqlens=cu)
+
+
+def test_the_widest_heads():
+    c = Case([3, 1], [2, 0], 2, 1, 1024, 1024, 16, torch.bfloat16, False)
+    kp, vp = (torch.zeros(c.blocks, 16, 1, 1024, dtype=torch.bfloat16, device=DEV) for _ in range(2))
+    q = ops.rope_kv_append(c.dq, c.dk, c.dv, *c.args, kp, vp, *c.where, cu_seqlens=c.cu.to(DEV))
+    assert torch.equal(q.cpu(), c.rotated(c.q, torch.float32).bfloat16())
+    assert torch.equal(kp.cpu()[c.block, c.row], c.rotated(c.k, torch.float32).bfloat16())
+    assert torch.equal(vp.cpu()[c.block, c.row], c.v)
