@@ -23,21 +23,25 @@
 //   the other tile; weights are handed over in halves of 64 keys.  The running maximum is raised
 //   only when a score passes it by 8 (in log2), so O in TMEM is rescaled rarely; P is at most
 //   2^8 and rounded to the input type (its 8 or 11 bits are what the tensor core takes), the row
-//   sum is taken in fp32 before the rounding.  A quarter of the exponentials is a polynomial on
+//   sum is taken in fp32 before the rounding.  An eighth of the exponentials is a polynomial on
 //   the fp32 pipes.
 // * Rows of V past a sequence's last key are set to zero in shared memory by warp 2 before they
 //   are multiplied (P is zero there, but 0 * NaN is not), so what another sequence holds never
 //   reaches this one's result.
-// * Persistent: one CTA per SM walks the (tile, head) items; every wait is bounded, and waits
-//   suspend the thread, which leaves the issue slots to the softmax warps.
+// * Persistent: one CTA per SM walks the (tile, head) items, the longest first and forwards and
+//   backwards in turn, so that the CTAs' sums come out alike; warp 3 finds them ahead.  Every wait
+//   is bounded, and waits suspend the thread, which leaves the issue slots to the softmax warps.
 //
-// Measured (bf16, 32 query and 8 key/value heads of 128, causal): 8192 tokens 486 us, 1.13 PFLOP/s,
-// 0.69 of the library product's rate in a short run; 4 x 4096 tokens, 16 heads, not causal 1.18.  A
+// Measured (bf16, 32 query and 8 key/value heads of 128, causal): 8192 tokens 453 us, 1.21 PFLOP/s,
+// 0.74 of the library product's rate in a short run; 4 x 4096 tokens, 16 heads, not causal 1.20.  A
 // step of 128 keys of both tiles takes about 3,250 cycles against 2,050 of products: a tile's chain
 // (scores, their maximum, 128 exponentials a thread, weights, P V, next scores) is 1.5 times as long
 // as the other tile's products can cover.  fp16, 20 heads of 64, 8 x 1500 tokens, not causal: 167 us,
-// 0.55 PFLOP/s, where exponentials alone take 115.  Two threads a row, two issuing lanes (the tiles fall
-// into step), and a second read of S in place of 128 registers were all slower (579, 565 and 525 us).
+// 0.55 PFLOP/s, where exponentials alone take 90.  Slower, all before items were ranked: for the 8192
+// two threads a row 579 us, two issuing lanes (the tiles fall into step) 565 and a second read of S
+// in place of 128 registers 525; two CTAs an SM with steps of 64 keys at D = 64 292 us for 4 x 4096
+// causal tokens, 16 heads, in place of 251 (but 150 for the 8 x 1500).  Unranked items: 485 us for the
+// 8192 and 251 for the 4 x 4096, which takes 225 to 271 now with the clock it finds.
 #include "spd_tc.cuh"
 
 namespace spd {
@@ -47,6 +51,7 @@ using namespace tc;
 constexpr int BM = 128;  // query rows per tile (two tiles per CTA)
 constexpr int BN = 128;  // keys per step
 constexpr int kThreads = 384;
+constexpr int kItems = 2;  // found ahead
 constexpr float kLazy = 8.f;
 
 template <int DP> struct Cfg {
@@ -225,11 +230,12 @@ __device__ __forceinline__ float2 exp2_poly(f32x2 x) {
                      __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(n.y) << 23)));
 }
 
-constexpr int kPoly = 2;  // of 8 pairs, to the polynomial
+constexpr int kPoly = 1;  // of 8 pairs, to the polynomial
 // Weights of 64 keys: p = 2^(s * c - m) rounded to T and packed, sums added.  EXACT: all on the
 // special-function unit, so that a masked score (-inf) gives an exact zero and a NaN a NaN; otherwise kPoly of
-// each 8 pairs go to the polynomial (0: 492 us, 2: 484 us, 4: 496 us for 8192 causal tokens, 32 / 8
-// heads of 128; the polynomial's six packed fp32 instructions soon cost more than they free).
+// each 8 pairs go to the polynomial (0: 493 us, 1: 485, 2: 484, 4: 496 for 8192 causal tokens, 32 / 8
+// heads of 128, and 259, 251 and 251 of 0, 1 and 2 for 4 x 4096, 16 heads of 64, with unranked items: the
+// polynomial's six packed fp32 instructions soon cost more than they free).
 template <typename T, bool EXACT>
 __device__ __forceinline__ void weights64(const uint32_t* s, f32x2 c, f32x2 neg_m, uint32_t* pk, f32x2 (&sum)[2]) {
   constexpr int kDeg = std::is_same<T, __half>::value ? 4 : 3;
@@ -272,23 +278,72 @@ struct Item {
   int tok0;            // first token of the CTA's tiles within the sequence
   int h0, kvh;
   int n[2];            // key steps of tiles A and B
+  int there;           // 0 past the last item
 };
 
-// The it-th item, found by the whole warp from the prefix sums; false past the last one.
-// Tiles of a sequence come last-first (the longest of a causal prompt first), heads fastest.
+// A CTA's n-th item: the CTAs take turns forwards and backwards, so that the one that has the longest of
+// one round has the shortest of the next.
+__device__ __forceinline__ int nth_item(int n) {
+  return n * (int)gridDim.x + (int)((n & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+}
+
+// Sequence s of the packed batch: its query and key rows, clamped to what there is, and its tiles.
+struct Span {
+  int q0, Tq, k0, Tk, tiles;
+  __device__ __forceinline__ Span(const PromptParams& p, int s, int tokens) {
+    q0 = max(0, min(p.Nq, p.cu_q[s]));
+    Tq = max(q0, min(p.Nq, p.cu_q[s + 1])) - q0;
+    k0 = max(0, min(p.Nk, p.cu_k[s]));
+    Tk = max(k0, min(p.Nk, p.cu_k[s + 1])) - k0;
+    tiles = (Tq + tokens - 1) / tokens;
+  }
+  // How many of its tiles (the last ones) take t key steps or more.
+  __device__ __forceinline__ int longer(const PromptParams& p, int t, int tokens) const {
+    if (t <= 0 || tiles == 0) return tiles;
+    const int need = (t - 1) * BN + 1;  // keys
+    if (Tk < need) return 0;
+    if (!p.causal) return tiles;
+    return tiles - max(0, min(tiles - 1, (need - (Tk - Tq) + tokens - 1) / tokens - 1));
+  }
+};
+
+// The it-th item, found by the whole warp from the prefix sums; false past the last one.  Heads come
+// fastest.  With `ranked` the tiles come in the order of their key steps, the longest first: the
+// number of steps that `tile` others have is searched for by halving, counting over the sequences.
+// Otherwise (no CTA has a second item) they come sequence by sequence.
 __device__ __forceinline__ bool find_item(const PromptParams& p, int it, Item& w) {
   const int lane = threadIdx.x & 31;
   const int tokens = 2 * BM / p.pack, groups = p.Hq / p.pack;
   const int tile = it / groups, grp = it % groups;
+  int steps = 0;  // of the tile; the tiles that have more come before
   int before = 0, b = -1, lvl = 0;
-  for (int base = 0; base < p.B; base += 32) {
-    const int s = base + lane;
-    int q0 = 0, q1 = 0;
-    if (s < p.B) {
-      q0 = max(0, min(p.Nq, p.cu_q[s]));
-      q1 = max(q0, min(p.Nq, p.cu_q[s + 1]));
+  if (p.ranked) {
+    int most = 0;
+    for (int base = 0; base < p.B; base += 32)
+      if (base + lane < p.B) most = max(most, Span(p, base + lane, tokens).Tk);
+    int none = (int)(__reduce_max_sync(0xffffffffu, (unsigned)most) + BN - 1) / BN + 1;  // nothing is as long
+    while (none - steps > 1) {
+      const int mid = (steps + none) / 2;
+      int n = 0;
+      for (int base = 0; base < p.B; base += 32)
+        if (base + lane < p.B) n += Span(p, base + lane, tokens).longer(p, mid, tokens);
+      n = __reduce_add_sync(0xffffffffu, n);
+      if (n > tile) {
+        steps = mid;
+      } else {
+        none = mid;
+        before = n;
+      }
     }
-    const int tiles = (q1 - q0 + tokens - 1) / tokens;
+  }
+  for (int base = 0; base < p.B; base += 32) {
+    int tiles = 0, first = 0;
+    if (base + lane < p.B) {
+      const Span s(p, base + lane, tokens);
+      const int n = p.ranked ? s.longer(p, steps, tokens) : s.tiles;
+      first = s.tiles - n;
+      tiles = p.ranked ? n - s.longer(p, steps + 1, tokens) : n;
+    }
     int incl = tiles;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -299,17 +354,17 @@ __device__ __forceinline__ bool find_item(const PromptParams& p, int it, Item& w
     if (hit) {
       const int src = __ffs(hit) - 1;
       b = base + src;
-      const int excl = __shfl_sync(0xffffffffu, incl - tiles, src), n = __shfl_sync(0xffffffffu, tiles, src);
-      lvl = n - 1 - (tile - before - excl);
+      lvl = __shfl_sync(0xffffffffu, first - (incl - tiles), src) + tile - before;
       break;
     }
     before += __shfl_sync(0xffffffffu, incl, 31);
   }
   if (b < 0) return false;
-  w.q0 = max(0, min(p.Nq, p.cu_q[b]));
-  w.Tq = max(w.q0, min(p.Nq, p.cu_q[b + 1])) - w.q0;
-  w.k0 = max(0, min(p.Nk, p.cu_k[b]));
-  w.Tk = max(w.k0, min(p.Nk, p.cu_k[b + 1])) - w.k0;
+  const Span s(p, b, tokens);
+  w.q0 = s.q0;
+  w.Tq = s.Tq;
+  w.k0 = s.k0;
+  w.Tk = s.Tk;
   w.tok0 = lvl * tokens;
   w.h0 = grp * p.pack;
   w.kvh = w.h0 / (p.Hq / p.Hkv);
@@ -330,6 +385,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   using C = Cfg<DP>;
   constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
   extern __shared__ unsigned char smem_raw[];
+  __shared__ Item items[kItems];
+  __shared__ __align__(8) uint64_t item_full[kItems], item_empty[kItems];
   unsigned char* smem = smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023);
   unsigned char* q_tiles = smem;                        // [2]
   unsigned char* kv_tiles = smem + 2 * C::kTileBytes;   // [kStages]
@@ -363,6 +420,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&o_full[x], 1);
       mbar_init(&o_empty[x], 4);
     }
+    for (int i = 0; i < kItems; ++i) {
+      mbar_init(&item_full[i], 1);
+      mbar_init(&item_empty[i], 11);  // the warps of TMA, MMA, V's rows and softmax
+    }
     mbar_init(v_landed, 1);
     mbar_init(v_fixed, 1);
     mbar_init(done, 1);
@@ -373,6 +434,16 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   Item w;
+  // The next item as warp 3 found it, for a whole warp; false past the last one or after a wait that gave up.
+  auto next_item = [&](int it, bool& ok, Item& w) {
+    const int slot = it % kItems;
+    if (ok) ok = __all_sync(0xffffffffu, mbar_wait_suspend(&item_full[slot], (uint32_t)((it / kItems) & 1), p.err, p.wait_ns));
+    if (!ok) return false;
+    w = items[slot];
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&item_empty[slot]);
+    return w.there != 0;
+  };
 
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
@@ -391,7 +462,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                       &kv_full[ring.slot]);
         ring.next(C::kStages);
       };
-      for (int it = blockIdx.x; ok && find_item(p, it, w); it += gridDim.x) {
+      for (int it = 0; next_item(it, ok, w); ++it) {
         if (lane == 0) {
           const int n = max(w.n[0], w.n[1]);
           auto load_q = [&](int x) {
@@ -444,7 +515,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                    idesc_s, c != 0);
         umma_commit(&s_full[x]);
       };
-      for (int it = blockIdx.x; ok && find_item(p, it, w); it += gridDim.x) {
+      for (int it = 0; next_item(it, ok, w); ++it) {
         const int n = max(w.n[0], w.n[1]);
         if (n > 0 && leader) {
           int kslot = ring.slot;
@@ -518,7 +589,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       Ring ring;
       uint32_t ph = 0;
       bool ok = true;
-      for (int it = blockIdx.x; ok && find_item(p, it, w); it += gridDim.x) {
+      for (int it = 0; next_item(it, ok, w); ++it) {
         const int n = max(w.n[0], w.n[1]), valid = w.Tk - (n - 1) * BN;
         if (n == 0) continue;
         ring.skip(2 * n - 1, C::kStages);
@@ -536,6 +607,21 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         ring.skip(1, C::kStages);
       }
+    } else {
+      // ---- this CTA's items, found ahead of their use ---------------------------------------------
+      bool ok = true;
+      for (int it = 0; ok; ++it) {
+        const int slot = it % kItems;
+        w.there = find_item(p, nth_item(it), w);
+        if (it >= kItems)
+          ok = __all_sync(0xffffffffu, mbar_wait_suspend(&item_empty[slot], (uint32_t)((it / kItems - 1) & 1), p.err, p.wait_ns));
+        if (!ok) break;
+        if (lane == 0) {
+          items[slot] = w;
+          mbar_arrive(&item_full[slot]);
+        }
+        if (!w.there) break;
+      }
     }
   } else {
     // ---- softmax and epilogue of tile x: thread = query row = TMEM lane --------------------
@@ -547,13 +633,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int half_tok = BM / p.pack;
     int s_use = 0, o_use = 0;
     bool ok = true;
-    for (int it = blockIdx.x; ok && find_item(p, it, w); it += gridDim.x) {
+    for (int it = 0; next_item(it, ok, w); ++it) {
       const int tok = w.tok0 + x * half_tok + row / p.pack;  // of this row, within the sequence
       const int first = w.tok0 + x * half_tok;
       const int off = w.Tk - w.Tq;
       // keys this row sees, and the fewest any row of the tile sees
       const int limit = p.causal ? min(w.Tk, tok + 1 + off) : w.Tk;
       const int least = p.causal ? min(w.Tk, first + 1 + off) : w.Tk;
+      const bool live = tok < w.Tq;
       float m = -INFINITY, l = 0.f;
       const int n = w.n[x];
       for (int j = 0; j < n; ++j) {
@@ -596,11 +683,12 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int i = 0; i < 4; ++i)
             mx4[i] = max3_nan(mx4[i], __uint_as_float(s[c + i]), __uint_as_float(s[c + 4 + i]));
         const float mx = max3_nan(max3_nan(mx4[0], mx4[1], mx4[2]), mx4[3], mx4[3]) * p.scale_log2;
-        // Also for a NaN and for infinite scores, which only the exact exponentials treat as they are.
-        const bool raise = !(mx < m + kLazy);
+        // Also for a NaN and for infinite scores, which only the exact exponentials treat as they are.  Rows
+        // past the sequence's end have no say: what they hold changes no rounding of the others.
+        const bool raise = live && !(mx < m + kLazy);
         bool exact = edge;
         if (__any_sync(0xffffffffu, raise)) {
-          exact |= __any_sync(0xffffffffu, !(fabsf(mx) < INFINITY));
+          exact |= __any_sync(0xffffffffu, live && !(fabsf(mx) < INFINITY));
           const float mn = fmaxf(m, mx);
           const float f = m == mn ? 1.f : ex2_approx(m - mn);
           m = mn;
@@ -638,7 +726,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!ok) break;
       T* out = reinterpret_cast<T*>(p.out) +
                ((long long)(w.q0 + tok) * p.Hq + w.h0 + row % p.pack) * p.D;
-      const bool live = tok < w.Tq;
       if (n > 0) {
         ok = __all_sync(0xffffffffu, mbar_wait_suspend(&o_full[x], (uint32_t)(o_use & 1), p.err, p.wait_ns));
         ++o_use;
@@ -718,6 +805,7 @@ int prompt_attn_launch(PromptParams p, const void* q, const void* k, const void*
   const int tokens = 2 * BM / p.pack;
   const long long most = ((long long)p.Nq / tokens + p.B) * (p.Hq / p.pack);  // items at most
   const dim3 grid((unsigned)(most < sms ? most : sms));
+  p.ranked = most > sms;
   auto by_d = [&](auto tag) -> int {
     using T = decltype(tag);
     return p.D <= 64 ? launch<T, 64>(tq, tk, tv, p, grid, st) : launch<T, 128>(tq, tk, tv, p, grid, st);

@@ -136,6 +136,7 @@ struct PromptParams {  // attention of packed prompts (prompt_attn.cu)
   const int* cu_k;    // [B + 1]
   int Nq, Nk, B, Hq, Hkv, D, causal;
   int pack;           // query heads of one key/value head that share a tile (a power of two)
+  int ranked;         // items in the order of their length
   float scale_log2;   // scale * log2(e)
   int* err;
   unsigned long long wait_ns;

@@ -235,3 +235,15 @@ def test_refusals():
         ops.prompt_attention(wide, wide, wide, cu([4]).to(DEV))
     assert ops.prompt_attention(q[:0], k[:0], v[:0], cu([0]).to(DEV)).shape == (0, 4, 64)
     assert not ops.prompt_attention(q, k[:0], v[:0], c, cu([0]).to(DEV)).any()
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_neighbours_change_no_rounding(D):
+    """A sequence's rows are the same bits whatever the rows after it in its last tile hold."""
+    lens = [400, 200]
+    q, k, v = make(11, 600, 600, 4, 2, D, torch.bfloat16)
+    args = [k.to(DEV), v.to(DEV), cu(lens).to(DEV)]
+    want = ops.prompt_attention(q.to(DEV), *args)
+    for other in (100.0, float("nan"), float("inf")):
+        q[400:] = other
+        assert torch.equal(ops.prompt_attention(q.to(DEV), *args)[:400], want[:400])
