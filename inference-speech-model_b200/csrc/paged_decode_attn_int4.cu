@@ -600,21 +600,22 @@ static long long dec4_tiles(int Hq, int Hkv, int dtype) {
   return (long long)Hkv * ((G + heads - 1) / heads);
 }
 
-// CTAs for each (sequence, head tile), from the longest contexts that the tables hold.  With up to 2048
+// CTAs for each (sequence, head tile), from the longest contexts that the tables hold.  With up to 4096
 // tokens for each CTA slot of the device all CTAs run at once, in chunks of 1024 tokens (four steps a
 // warp) or more: less makes the join cost more than it saves (one context of 32,000 tokens, 8 key/value
 // heads of 128: 17.5 us in chunks of 1024, 20.6 of 640, 22.0 of 1536; one of 448, 12 heads of 64:
-// 5.3 us in one chunk, 7.1 in two).  Beyond that, chunks of 2048 to 4096 tokens, half a slot's share
-// within these: the SMs' rates differ by up to a third, and CTAs that are dealt out as slots fall free
-// even that out (the 32 contexts above: one equal share per slot 132 us, chunks of 512 tokens 192, 1024
-// 146, 2048 126, 4096 128; the 128 contexts: 97, 102, 80, 70, 66).
+// 5.3 us in one chunk, 7.1 in two; 12 of 8,000 to 16,000, 8 heads of 128: 44.7 us at once, 48.9 in
+// chunks of 2048).  Beyond that, chunks of 2048 to 4096 tokens, half a slot's share within these: the
+// SMs' rates differ by up to a third, and CTAs that are dealt out as slots fall free even that out
+// (the 32 contexts above: one equal share per slot 132 us, chunks of 512 tokens 192, 1024 146, 2048
+// 126, 4096 128; the 128 contexts: 97, 102, 80, 70, 66).
 Int4Split decode_int4_split(int B, int Hq, int Hkv, int D, int dtype, int max_ctx, int sms) {
   using namespace dec4;
   constexpr int kLeast = 1024, kChunk = 2048;
   const int per_sm = D == 64 ? ctas_per_sm<1>() : D == 128 ? ctas_per_sm<2>() : ctas_per_sm<4>();
   const long long slots = (long long)sms * per_sm, pairs = B * dec4_tiles(Hq, Hkv, dtype);
   const long long share = max_ctx * pairs / slots;  // tokens
-  if (share <= kChunk) return {(int)std::max(1ll, std::min(slots / pairs, (max_ctx + kLeast - 1ll) / kLeast)), kLeast};
+  if (share <= 2 * kChunk) return {(int)std::max(1ll, std::min(slots / pairs, (max_ctx + kLeast - 1ll) / kLeast)), kLeast};
   const long long c = std::min(std::max(share / 2, (long long)kChunk), 2ll * kChunk);
   return {(int)((max_ctx + c - 1) / c), kChunk};
 }
