@@ -20,28 +20,32 @@
 //   and V as the MN-major operand, so nothing is transposed or written back to shared memory.
 // * Warps 4-7 and 8-11 are the softmax of tiles A and B: one row per thread, so the row
 //   maximum and sum need no shuffles.  While one tile's softmax runs, the tensor cores work on
-//   the other tile; weights are handed over in halves of 64 keys.  The running maximum is raised
+//   the other tile; weights are handed over 64 keys at a time.  The running maximum is raised
 //   only when a score passes it by 8 (in log2), so O in TMEM is rescaled rarely; P is at most
 //   2^8 and rounded to the input type (its 8 or 11 bits are what the tensor core takes), the row
-//   sum is taken in fp32 before the rounding.  An eighth of the exponentials is a polynomial on
+//   sum is taken in fp32 before the rounding.  A quarter of the exponentials is a polynomial on
 //   the fp32 pipes.
 // * Rows of V past a sequence's last key are set to zero in shared memory by warp 2 before they
 //   are multiplied (P is zero there, but 0 * NaN is not), so what another sequence holds never
 //   reaches this one's result.
-// * Persistent: one CTA per SM walks the (tile, head) items, the longest first and forwards and
-//   backwards in turn, so that the CTAs' sums come out alike; warp 3 finds them ahead.  Every wait
-//   is bounded, and waits suspend the thread, which leaves the issue slots to the softmax warps.
+// * Steps are of 128 keys with one CTA an SM; at D <= 64, where TMEM holds four tiles, of 64 keys
+//   with two CTAs an SM, unless no SM gets a second item.
+// * One CTA is launched for each item (tile pair and head group), ranked by length; a running CTA
+//   takes over the items of CTAs that have not started (warp 3 calls off their launch), so tiles
+//   follow one another in it without a gap and the longest come first.  Every wait is bounded, and
+//   waits suspend the thread, which leaves the issue slots to the softmax warps.
 //
-// Measured (bf16, 32 query and 8 key/value heads of 128, causal): 8192 tokens 453 us, 1.21 PFLOP/s,
-// 0.74 of the library product's rate in a short run; 4 x 4096 tokens, 16 heads, not causal 1.20.  A
+// Measured (bf16, 32 query and 8 key/value heads of 128, causal): 8192 tokens 450 us, 1.22 PFLOP/s,
+// 0.75 of the library product's rate in a short run; 4 x 4096 tokens, 16 heads, not causal 1.16.  A
 // step of 128 keys of both tiles takes about 3,250 cycles against 2,050 of products: a tile's chain
 // (scores, their maximum, 128 exponentials a thread, weights, P V, next scores) is 1.5 times as long
-// as the other tile's products can cover.  fp16, 20 heads of 64, 8 x 1500 tokens, not causal: 167 us,
-// 0.55 PFLOP/s, where exponentials alone take 90.  Slower, all before items were ranked: for the 8192
-// two threads a row 579 us, two issuing lanes (the tiles fall into step) 565 and a second read of S
-// in place of 128 registers 525; two CTAs an SM with steps of 64 keys at D = 64 292 us for 4 x 4096
-// causal tokens, 16 heads, in place of 251 (but 150 for the 8 x 1500).  Unranked items: 485 us for the
-// 8192 and 251 for the 4 x 4096, which takes 225 to 271 now with the clock it finds.
+// as the other tile's products can cover.  fp16, 20 heads of 64, 8 x 1500 tokens, not causal: 143 us,
+// 0.64 PFLOP/s, where exponentials alone take 63 to 84.  64 keys and two CTAs against 128 and one at D = 64:
+// 143 against 166 us there, 202 against 224 for 4 x 4096 causal tokens of 16 heads, but 11.5 against
+// 10.3 for 6 short prompts of 12 heads, one item an SM at most.  Items dealt out in fixed turns instead of taken
+// over: 147 (forwards) and 163 us (forwards and backwards) for the 8 x 1500, 215 and 210 for the 4 x
+// 4096.  Slower at D = 128: two threads a row, two issuing lanes (the tiles fall into step) and a
+// second read of S in place of 128 registers (579, 565 and 525 us when this one took 485).
 #include "spd_tc.cuh"
 
 namespace spd {
@@ -49,21 +53,37 @@ namespace pa {
 using namespace tc;
 
 constexpr int BM = 128;  // query rows per tile (two tiles per CTA)
-constexpr int BN = 128;  // keys per step
 constexpr int kThreads = 384;
-constexpr int kItems = 2;  // found ahead
-constexpr float kLazy = 8.f;
+constexpr int kItems = 2;   // item slots
+// Key steps before an item's end (counted by its loads) that the next one is asked for: late enough that
+// the CTA that is done first takes the longest, early enough to hide the search.  2, 4 and 8 for the 8 x
+// 1500 above: 143, 143, 145 us; for ragged grouped prompts 226, 222, 222; for 16 of up to 700 tokens
+// 27.6, 28.0, 31.
+constexpr int kAhead = 4;
+constexpr float kLazy = 8.f;  // log2 units a score may pass the reference maximum by
 
-template <int DP> struct Cfg {
+// DP: head size, padded to 64 or 128; BN: keys per step.
+template <int DP, int BN> struct Cfg {
+  static constexpr int kCtas = BN == 128 ? 1 : 2;         // CTAs per SM
   static constexpr int kBoxes = DP / 64;                  // 64-column boxes of a row
-  static constexpr int kTileBytes = 128 * DP * 2;         // one Q, K or V tile
-  static constexpr int kBoxBytes = 128 * 128;             // 128 rows of 128 bytes
+  static constexpr int kQBox = 128 * 128;                 // 128 rows of 128 bytes
+  static constexpr int kQBytes = kBoxes * kQBox;          // one Q tile
+  static constexpr int kKvBox = BN * 128;
+  static constexpr int kKvBytes = kBoxes * kKvBox;        // one K or V tile
+  static constexpr int kParts = BN / 64;                  // weights are handed over 64 keys at a time
   static constexpr int kStages = DP == 128 ? 5 : 8;       // K and V tiles in flight
   static constexpr int kBarBytes = 512;
-  static constexpr size_t kSmem = 1024 + (size_t)(2 + kStages) * kTileBytes + kBarBytes;
-  static constexpr uint32_t kTmemCols = 512;
-  static constexpr uint32_t kO = 256;                     // TMEM column of O_A; S_A at 0, S_B at 128
+  static constexpr size_t kSmem = 1024 + 2 * (size_t)kQBytes + (size_t)kStages * kKvBytes + kBarBytes;
+  static constexpr uint32_t kO = 2 * BN;                  // TMEM column of O_A; S_A at 0, S_B at BN
+  static constexpr uint32_t kTmemCols = BN == 128 ? 512 : 256;
+  // registers of the softmax threads and of the others; their sum is within what the launch gives to
+  // all 384 (168 or 80 each, checked at the launch)
+  static constexpr int kSoftmaxRegs = BN == 128 ? 216 : 96, kOtherRegs = BN == 128 ? 72 : 48;
+  static constexpr int kAllRegs = 256 * kSoftmaxRegs + 128 * kOtherRegs;
+  static_assert(kO + 2 * DP <= kTmemCols, "scores and outputs fit in TMEM");
 };
+template <int N> __device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N> __device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 
 __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
   asm volatile(
@@ -113,7 +133,7 @@ __device__ __forceinline__ void umma4_ts(uint32_t d_tmem, uint32_t a, uint64_t b
 }
 
 // MN-major operand with 128-byte swizzle: 8 k-rows of 64 consecutive elements form a 1024-byte
-// atom; atoms follow each other along k (stride 1024) and 64-element blocks every kBoxBytes.
+// atom; atoms follow each other along k (stride 1024) and 64-element blocks every block_bytes.
 __device__ __forceinline__ uint64_t smem_desc_mn(const void* tile, uint32_t block_bytes) {
   const uint64_t addr = smem_addr(tile);
   uint64_t d = 0;
@@ -157,6 +177,13 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
       "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
       "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
       "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -230,17 +257,17 @@ __device__ __forceinline__ float2 exp2_poly(f32x2 x) {
                      __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(n.y) << 23)));
 }
 
-constexpr int kPoly = 1;  // of 8 pairs, to the polynomial
-// Weights of 64 keys: p = 2^(s * c - m) rounded to T and packed, sums added.  EXACT: all on the
+constexpr int kPoly = 2;  // of 8 pairs, to the polynomial
+// Weights of 2 * PAIRS keys: p = 2^(s * c - m) rounded to T and packed, sums added.  EXACT: all on the
 // special-function unit, so that a masked score (-inf) gives an exact zero and a NaN a NaN; otherwise kPoly of
-// each 8 pairs go to the polynomial (0: 493 us, 1: 485, 2: 484, 4: 496 for 8192 causal tokens, 32 / 8
-// heads of 128, and 259, 251 and 251 of 0, 1 and 2 for 4 x 4096, 16 heads of 64, with unranked items: the
+// each 8 pairs go to the polynomial (with items dealt out in fixed turns 0: 493 us, 1: 485, 2: 484, 4:
+// 496 for the 8192 tokens above, and 170, 164 and 163 us of 0, 1 and 2 for the 8 x 1500: the
 // polynomial's six packed fp32 instructions soon cost more than they free).
-template <typename T, bool EXACT>
-__device__ __forceinline__ void weights64(const uint32_t* s, f32x2 c, f32x2 neg_m, uint32_t* pk, f32x2 (&sum)[2]) {
+template <typename T, bool EXACT, int PAIRS>
+__device__ __forceinline__ void weights(const uint32_t* s, f32x2 c, f32x2 neg_m, uint32_t* pk, f32x2 (&sum)[2]) {
   constexpr int kDeg = std::is_same<T, __half>::value ? 4 : 3;
 #pragma unroll
-  for (int k = 0; k < 32; ++k) {
+  for (int k = 0; k < PAIRS; ++k) {
     const f32x2 x = fma2(pair(__uint_as_float(s[2 * k]), __uint_as_float(s[2 * k + 1])), c, neg_m);
     float2 e;
     if (!EXACT && (k * kPoly) % 8 < kPoly) {  // spread evenly
@@ -252,6 +279,26 @@ __device__ __forceinline__ void weights64(const uint32_t* s, f32x2 c, f32x2 neg_
     sum[k & 1] = add2(sum[k & 1], pair(e.x, e.y));
     pk[k] = pack2<T>(e.x, e.y);
   }
+}
+
+// scores of keys at or past `seen` to -inf
+template <int N>
+__device__ __forceinline__ void mask(uint32_t* s, int seen) {
+#pragma unroll
+  for (int c = 0; c < N; ++c)
+    if (c >= seen) s[c] = 0xff800000u;
+}
+// four running maxima over N scores
+template <int N, bool FIRST>
+__device__ __forceinline__ void max4(const uint32_t* s, float (&m)[4]) {
+  if (FIRST)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) m[i] = __uint_as_float(s[i]);
+#pragma unroll
+  for (int c = FIRST ? 4 : 0; c < N; c += 8)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      m[i] = max3_nan(m[i], __uint_as_float(s[c + i]), __uint_as_float(s[c + 4 + i < N ? c + 4 + i : c + i]));
 }
 
 // Position in a ring of stages: the slot, and how often the ring has come round.
@@ -281,10 +328,28 @@ struct Item {
   int there;           // 0 past the last item
 };
 
-// A CTA's n-th item: the CTAs take turns forwards and backwards, so that the one that has the longest of
-// one round has the shortest of the next.
-__device__ __forceinline__ int nth_item(int n) {
-  return n * (int)gridDim.x + (int)((n & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+// Asks for the next CTA that has not started yet: its index arrives in `response`, and its launch is
+// called off.
+__device__ __forceinline__ void ask_for_cta(void* response, uint64_t* bar) {
+  asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(
+                   smem_addr(response)),
+               "r"(smem_addr(bar))
+               : "memory");
+}
+// The index of the CTA that was called off, or -1 if none was left.
+__device__ __forceinline__ int called_off(const void* response) {
+  uint32_t yes, x;
+  asm volatile(
+      "{\n\t.reg .b128 h;\n\t.reg .pred p;\n\t"
+      "ld.shared.b128 h, [%2];\n\t"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, h;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t"
+      "mov.u32 %1, 0;\n\t"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, h;\n\t}"
+      : "=r"(yes), "=r"(x)
+      : "r"(smem_addr(response))
+      : "memory");
+  return yes ? (int)x : -1;
 }
 
 // Sequence s of the packed batch: its query and key rows, clamped to what there is, and its tiles.
@@ -298,6 +363,7 @@ struct Span {
     tiles = (Tq + tokens - 1) / tokens;
   }
   // How many of its tiles (the last ones) take t key steps or more.
+  template <int BN>
   __device__ __forceinline__ int longer(const PromptParams& p, int t, int tokens) const {
     if (t <= 0 || tiles == 0) return tiles;
     const int need = (t - 1) * BN + 1;  // keys
@@ -310,7 +376,8 @@ struct Span {
 // The it-th item, found by the whole warp from the prefix sums; false past the last one.  Heads come
 // fastest.  With `ranked` the tiles come in the order of their key steps, the longest first: the
 // number of steps that `tile` others have is searched for by halving, counting over the sequences.
-// Otherwise (no CTA has a second item) they come sequence by sequence.
+// Otherwise (every item starts at once) they come sequence by sequence.
+template <int BN>
 __device__ __forceinline__ bool find_item(const PromptParams& p, int it, Item& w) {
   const int lane = threadIdx.x & 31;
   const int tokens = 2 * BM / p.pack, groups = p.Hq / p.pack;
@@ -326,7 +393,7 @@ __device__ __forceinline__ bool find_item(const PromptParams& p, int it, Item& w
       const int mid = (steps + none) / 2;
       int n = 0;
       for (int base = 0; base < p.B; base += 32)
-        if (base + lane < p.B) n += Span(p, base + lane, tokens).longer(p, mid, tokens);
+        if (base + lane < p.B) n += Span(p, base + lane, tokens).longer<BN>(p, mid, tokens);
       n = __reduce_add_sync(0xffffffffu, n);
       if (n > tile) {
         steps = mid;
@@ -340,9 +407,9 @@ __device__ __forceinline__ bool find_item(const PromptParams& p, int it, Item& w
     int tiles = 0, first = 0;
     if (base + lane < p.B) {
       const Span s(p, base + lane, tokens);
-      const int n = p.ranked ? s.longer(p, steps, tokens) : s.tiles;
+      const int n = p.ranked ? s.longer<BN>(p, steps, tokens) : s.tiles;
       first = s.tiles - n;
-      tiles = p.ranked ? n - s.longer(p, steps + 1, tokens) : n;
+      tiles = p.ranked ? n - s.longer<BN>(p, steps + 1, tokens) : n;
     }
     int incl = tiles;
 #pragma unroll
@@ -378,26 +445,28 @@ __device__ __forceinline__ bool find_item(const PromptParams& p, int it, Item& w
   return true;
 }
 
-template <typename T, int DP>
-__global__ void __launch_bounds__(kThreads, 1)
+template <typename T, int DP, int BN>
+__global__ void __launch_bounds__(kThreads, Cfg<DP, BN>::kCtas)
     prompt_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                        const __grid_constant__ CUtensorMap tm_v, const PromptParams p) {
-  using C = Cfg<DP>;
+  using C = Cfg<DP, BN>;
   constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
   extern __shared__ unsigned char smem_raw[];
   __shared__ Item items[kItems];
+  __shared__ __align__(16) unsigned char response[16];
+  __shared__ __align__(8) uint64_t item_wanted, asked;
   __shared__ __align__(8) uint64_t item_full[kItems], item_empty[kItems];
   unsigned char* smem = smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023);
   unsigned char* q_tiles = smem;                        // [2]
-  unsigned char* kv_tiles = smem + 2 * C::kTileBytes;   // [kStages]
-  uint64_t* bars = reinterpret_cast<uint64_t*>(kv_tiles + C::kStages * C::kTileBytes);
+  unsigned char* kv_tiles = smem + 2 * C::kQBytes;   // [kStages]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(kv_tiles + C::kStages * C::kKvBytes);
   uint64_t* kv_full = bars;                    // [kStages]
   uint64_t* kv_empty = kv_full + C::kStages;   // [kStages]
   uint64_t* q_full = kv_empty + C::kStages;    // [2]
   uint64_t* q_empty = q_full + 2;              // [2]
   uint64_t* s_full = q_empty + 2;              // [2] scores ready (and all earlier products done)
-  uint64_t* p_full = s_full + 2;               // [2 tiles][2 halves] weights written (and the output rescaled)
-  uint64_t* o_full = p_full + 4;               // [2] output complete
+  uint64_t* p_full = s_full + 2;               // [2 tiles][kParts] weights written (and the output rescaled)
+  uint64_t* o_full = p_full + 2 * C::kParts;               // [2] output complete
   uint64_t* o_empty = o_full + 2;              // [2] output read
   uint64_t* v_landed = o_empty + 2;            // a V tile with rows past the last key is there
   uint64_t* v_fixed = v_landed + 1;            // and those rows are zero
@@ -415,15 +484,16 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&q_full[x], 1);
       mbar_init(&q_empty[x], 1);
       mbar_init(&s_full[x], 1);
-      mbar_init(&p_full[2 * x], 4);  // one arrival per warp
-      mbar_init(&p_full[2 * x + 1], 4);
+      for (int h = 0; h < C::kParts; ++h) mbar_init(&p_full[C::kParts * x + h], 4);  // one arrival per warp
       mbar_init(&o_full[x], 1);
       mbar_init(&o_empty[x], 4);
     }
     for (int i = 0; i < kItems; ++i) {
       mbar_init(&item_full[i], 1);
-      mbar_init(&item_empty[i], 11);  // the warps of TMA, MMA, V's rows and softmax
+      mbar_init(&item_empty[i], 11);
     }
+    mbar_init(&item_wanted, 1);
+    mbar_init(&asked, 1);
     mbar_init(v_landed, 1);
     mbar_init(v_fixed, 1);
     mbar_init(done, 1);
@@ -446,7 +516,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   };
 
   if (warp < 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    regs_down<C::kOtherRegs>();
     if (warp == 0) {
       // ---- TMA: Q tiles, then K and V tiles of each step, through one ring ------------------
       const int half_tok = BM / p.pack;
@@ -456,9 +526,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       auto load_kv = [&](const CUtensorMap* map, int kv_row) {
         if (ring.round) ok = mbar_wait_suspend(&kv_empty[ring.slot], ring.phase() ^ 1u, p.err, p.wait_ns);
         if (!ok) return;
-        mbar_arrive_expect_tx(&kv_full[ring.slot], C::kTileBytes);
+        mbar_arrive_expect_tx(&kv_full[ring.slot], C::kKvBytes);
         for (int c = 0; c < C::kBoxes; ++c)
-          tma_load_3d(kv_tiles + ring.slot * C::kTileBytes + c * C::kBoxBytes, map, 64 * c, w.kvh, kv_row,
+          tma_load_3d(kv_tiles + ring.slot * C::kKvBytes + c * C::kKvBox, map, 64 * c, w.kvh, kv_row,
                       &kv_full[ring.slot]);
         ring.next(C::kStages);
       };
@@ -470,13 +540,15 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (q_use[x] > 0) ok = mbar_wait_suspend(&q_empty[x], (uint32_t)((q_use[x] - 1) & 1), p.err, p.wait_ns);
             if (!ok) return;
             ++q_use[x];
-            mbar_arrive_expect_tx(&q_full[x], C::kTileBytes);
+            mbar_arrive_expect_tx(&q_full[x], C::kQBytes);
             for (int c = 0; c < C::kBoxes; ++c)
-              tma_load_3d(q_tiles + x * C::kTileBytes + c * C::kBoxBytes, &tm_q, 64 * c, w.h0,
+              tma_load_3d(q_tiles + x * C::kQBytes + c * C::kQBox, &tm_q, 64 * c, w.h0,
                           w.q0 + w.tok0 + x * half_tok, &q_full[x]);
           };
           load_q(0);
+          if (n == 0) mbar_arrive(&item_wanted);
           for (int j = 0; j < n && ok; ++j) {
+            if (j == max(0, n - kAhead)) mbar_arrive(&item_wanted);
             load_kv(&tm_k, w.k0 + j * BN);
             if (j == 0) load_q(1);
             if (ok) load_kv(&tm_v, w.k0 + j * BN);
@@ -496,10 +568,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       // ---- MMA issuer: one lane, with nothing but waits and issues in its step -----------------
       constexpr uint32_t idesc_s = instr_desc_f16(kBf16, BM, BN);
       constexpr uint32_t idesc_o = instr_desc_f16(kBf16, BM, DP) | (1u << 16);  // B is MN-major
-      constexpr uint32_t kTile16 = C::kTileBytes >> 4, kBox16 = C::kBoxBytes >> 4;
+      constexpr uint32_t kQ16 = C::kQBytes >> 4, kQBox16 = C::kQBox >> 4, kKv16 = C::kKvBytes >> 4, kKvBox16 = C::kKvBox >> 4;
       // descriptors of the first Q tile, and of the ring's first tile as K and as V
       const uint64_t q_desc = smem_desc_sw128(q_tiles), kv_desc = smem_desc_sw128(kv_tiles),
-                     v_desc = smem_desc_mn(kv_tiles, C::kBoxBytes);
+                     v_desc = smem_desc_mn(kv_tiles, C::kKvBox);
       const bool leader = elect_one();
       const int leader_lane = __ffs(__ballot_sync(0xffffffffu, leader)) - 1;
       uint32_t q_ph[2] = {0, 0}, p_ph[2] = {0, 0}, o_ph[2] = {1, 1}, fix_ph = 0;
@@ -511,8 +583,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       auto scores = [&](int x, int slot) {  // S_x = Q_x K^T
 #pragma unroll
         for (int c = 0; c < C::kBoxes; ++c)
-          umma4_ss(tmem + x * BN, q_desc + (uint64_t)(x * kTile16 + c * kBox16), kv_desc + (uint64_t)(slot * kTile16 + c * kBox16),
-                   idesc_s, c != 0);
+          umma4_ss(tmem + x * BN, q_desc + (uint64_t)(x * kQ16 + c * kQBox16),
+                   kv_desc + (uint64_t)(slot * kKv16 + c * kKvBox16), idesc_s, c != 0);
         umma_commit(&s_full[x]);
       };
       for (int it = 0; next_item(it, ok, w); ++it) {
@@ -547,7 +619,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               wait(v_fixed, fix_ph);
               fix_ph ^= 1;
             }
-            const uint64_t dv = v_desc + (uint64_t)(vslot * kTile16);
+            const uint64_t dv = v_desc + (uint64_t)(vslot * kKv16);
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
               if (j >= w.n[x] || !ok) continue;
@@ -555,16 +627,16 @@ __global__ void __launch_bounds__(kThreads, 1)
                 wait(&o_empty[x], o_ph[x]);  // passes at once the first time
                 o_ph[x] ^= 1;
               }
-              // O_x += P_x V, each half of the keys when its weights are there
-              wait(&p_full[2 * x], p_ph[x]);
-              if (!ok) continue;
-              tc_fence_after();
-              umma4_ts(tmem + C::kO + x * DP, tmem + x * BN, dv, idesc_o, j != 0);
-              wait(&p_full[2 * x + 1], p_ph[x]);
+              // O_x += P_x V, each 64 of the keys when their weights are there
+#pragma unroll
+              for (int h = 0; h < C::kParts; ++h) {
+                wait(&p_full[C::kParts * x + h], p_ph[x]);
+                if (!ok) break;
+                tc_fence_after();
+                umma4_ts(tmem + C::kO + x * DP, tmem + x * BN + 32 * h, dv + h * 4 * 128, idesc_o, j != 0 || h);
+              }
               p_ph[x] ^= 1;
               if (!ok) continue;
-              tc_fence_after();
-              umma4_ts(tmem + C::kO + x * DP, tmem + x * BN + 32, dv + 4 * 128, idesc_o, 1);
               if (j + 1 < w.n[x]) {
                 scores(x, kslot);
                 if (j + 2 == w.n[x]) umma_commit(&q_empty[x]);
@@ -597,10 +669,10 @@ __global__ void __launch_bounds__(kThreads, 1)
           ok = __all_sync(0xffffffffu, mbar_wait_suspend(v_landed, ph, p.err, p.wait_ns));
           if (!ok) break;
           ph ^= 1;
-          unsigned char* vt = kv_tiles + ring.slot * C::kTileBytes;
+          unsigned char* vt = kv_tiles + ring.slot * C::kKvBytes;
           for (int i = lane; i < (BN - valid) * 8; i += 32)
             for (int c = 0; c < C::kBoxes; ++c)
-              *reinterpret_cast<uint4*>(vt + c * C::kBoxBytes + valid * 128 + i * 16) = make_uint4(0, 0, 0, 0);
+              *reinterpret_cast<uint4*>(vt + c * C::kKvBox + valid * 128 + i * 16) = make_uint4(0, 0, 0, 0);
           fence_proxy_async_smem();
           __syncwarp();
           if (lane == 0) mbar_arrive(v_fixed);
@@ -608,11 +680,29 @@ __global__ void __launch_bounds__(kThreads, 1)
         ring.skip(1, C::kStages);
       }
     } else {
-      // ---- this CTA's items, found ahead of their use ---------------------------------------------
+      // ---- this CTA's items, found ahead of their use: its own, then those of CTAs that have not
+      // started, whose launch it calls off
       bool ok = true;
+      int index = (int)blockIdx.x;
       for (int it = 0; ok; ++it) {
         const int slot = it % kItems;
-        w.there = find_item(p, nth_item(it), w);
+        if (it > 0) {
+          ok = __all_sync(0xffffffffu, mbar_wait_suspend(&item_wanted, (uint32_t)((it - 1) & 1), p.err, p.wait_ns));
+          if (!ok) break;
+          if (lane == 0) {
+            mbar_arrive_expect_tx(&asked, 16);
+            ask_for_cta(response, &asked);
+          }
+          ok = __all_sync(0xffffffffu, mbar_wait_suspend(&asked, (uint32_t)((it - 1) & 1), p.err, p.wait_ns));
+          if (!ok) {  // let the answer land before the CTA can exit
+            (void)mbar_wait_suspend(&asked, (uint32_t)((it - 1) & 1), nullptr);
+            break;
+          }
+          index = called_off(response);
+          fence_proxy_async_smem();  // read before the next answer is written
+          __syncwarp();
+        }
+        w.there = index >= 0 && find_item<BN>(p, index, w);
         if (it >= kItems)
           ok = __all_sync(0xffffffffu, mbar_wait_suspend(&item_empty[slot], (uint32_t)((it / kItems - 1) & 1), p.err, p.wait_ns));
         if (!ok) break;
@@ -625,7 +715,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else {
     // ---- softmax and epilogue of tile x: thread = query row = TMEM lane --------------------
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+    regs_up<C::kSoftmaxRegs>();
     const int x = (warp - 4) >> 2;
     const int row = (warp & 3) * 32 + lane;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
@@ -648,40 +738,40 @@ __global__ void __launch_bounds__(kThreads, 1)
         ++s_use;
         if (!ok) break;
         tc_fence_after();
-        uint32_t s[BN];
-        tmem_ld32_nowait(s_col, s);
-        tmem_ld32_nowait(s_col + 32, s + 32);
-        tmem_ld_wait(s);
-        tmem_ld_wait(s + 32);
-        tmem_ld32_nowait(s_col + 64, s + 64);
-        tmem_ld32_nowait(s_col + 96, s + 96);
-        const int base = j * BN;
+        constexpr int kHeld = BN == 128 ? 128 : 32;  // scores held in registers at a time
+        uint32_t s[kHeld];
+        const int base = j * BN, seen = limit - base;
         const bool edge = base + BN > least;  // some row of the tile does not see all of these keys
-        if (edge) {
-          tmem_ld_wait(s + 64);
-          tmem_ld_wait(s + 96);
-          const int seen = limit - base;
-#pragma unroll
-          for (int c = 0; c < BN; ++c)
-            if (c >= seen) s[c] = 0xff800000u;  // -inf
-        }
         float mx4[4];
+        if constexpr (BN == 128) {
+          tmem_ld32_nowait(s_col, s);
+          tmem_ld32_nowait(s_col + 32, s + 32);
+          tmem_ld_wait(s);
+          tmem_ld_wait(s + 32);
+          tmem_ld32_nowait(s_col + 64, s + 64);
+          tmem_ld32_nowait(s_col + 96, s + 96);
+          if (edge) {
+            tmem_ld_wait(s + 64);
+            tmem_ld_wait(s + 96);
+            mask<BN>(s, seen);
+          }
+          max4<64, true>(s, mx4);  // while the other half is on its way
+          if (!edge) {
+            tmem_ld_wait(s + 64);
+            tmem_ld_wait(s + 96);
+          }
+          max4<64, false>(s + 64, mx4);
+        } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) mx4[i] = __uint_as_float(s[i]);
-#pragma unroll
-        for (int c = 4; c < 64; c += 8)
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            mx4[i] = max3_nan(mx4[i], __uint_as_float(s[c + i]), __uint_as_float(s[c + 4 + i < 64 ? c + 4 + i : c + i]));
-        if (!edge) {
-          tmem_ld_wait(s + 64);
-          tmem_ld_wait(s + 96);
+          for (int c = 0; c < BN; c += 32) {
+            tmem_ld32_nowait(s_col + c, s);
+            tmem_ld_wait(s);
+            if (edge) mask<32>(s, seen - c);
+            if (c == 0) max4<32, true>(s, mx4);
+            else max4<32, false>(s, mx4);
+          }
+          tmem_ld32_nowait(s_col, s);
         }
-#pragma unroll
-        for (int c = 64; c < BN; c += 8)
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            mx4[i] = max3_nan(mx4[i], __uint_as_float(s[c + i]), __uint_as_float(s[c + 4 + i]));
         const float mx = max3_nan(max3_nan(mx4[0], mx4[1], mx4[2]), mx4[3], mx4[3]) * p.scale_log2;
         // Also for a NaN and for infinite scores, which only the exact exponentials treat as they are.  Rows
         // past the sequence's end have no say: what they hold changes no rounding of the others.
@@ -708,17 +798,30 @@ __global__ void __launch_bounds__(kThreads, 1)
         const float mm = m == -INFINITY ? 0.f : m;
         const f32x2 c2 = pair(p.scale_log2, p.scale_log2), nm2 = pair(-mm, -mm);
         f32x2 sum[2] = {pair(0.f, 0.f), pair(0.f, 0.f)};
-        // in two halves, each handed to the tensor cores when it is written
+        // 64 keys at a time, handed to the tensor cores when they are written
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          uint32_t pk[32];
-          if (exact) weights64<T, true>(s + 64 * h, c2, nm2, pk, sum);
-          else weights64<T, false>(s + 64 * h, c2, nm2, pk, sum);
-          tmem_st32(s_col + 32 * h, pk);
+        for (int h = 0; h < C::kParts; ++h) {
+          
+          uint32_t pk[kHeld == 128 ? 32 : 16];
+          if constexpr (BN == 128) {
+            if (exact) weights<T, true, 32>(s + 64 * h, c2, nm2, pk, sum);
+            else weights<T, false, 32>(s + 64 * h, c2, nm2, pk, sum);
+            tmem_st32(s_col + 32 * h, pk);
+          } else {
+#pragma unroll
+            for (int c = 0; c < BN; c += 32) {
+              tmem_ld_wait(s);
+              if (edge) mask<32>(s, seen - c);
+              if (exact) weights<T, true, 16>(s, c2, nm2, pk, sum);
+              else weights<T, false, 16>(s, c2, nm2, pk, sum);
+              if (c + 32 < BN) tmem_ld32_nowait(s_col + c + 32, s);
+              tmem_st16(s_col + c / 2, pk);
+            }
+          }
           tmem_st_wait();
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(&p_full[2 * x + h]);
+          if (lane == 0) mbar_arrive(&p_full[C::kParts * x + h]);
         }
         const float2 t2 = unpair(add2(sum[0], sum[1]));
         l += t2.x + t2.y;
@@ -762,6 +865,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp == 1) tmem_dealloc(tmem, C::kTmemCols);
 }
 
+struct PromptTensors {
+  const void *q, *k, *v;
+  long long q_st, q_sh, k_st, k_sh, v_st, v_sh;
+};
+
 // [tokens][heads][D] of 16-bit elements with any token and head strides, box [rows][heads][64].
 static bool make_map3(CUtensorMap* map, const void* base, int D, int heads, int tokens, long long sh, long long st,
                       int box_heads, int box_tokens, bool bf16) {
@@ -776,11 +884,23 @@ static bool make_map3(CUtensorMap* map, const void* base, int D, int heads, int 
              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <typename T, int DP>
-static int launch(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const PromptParams& p, dim3 grid,
-                  cudaStream_t st) {
-  if (!allow_smem<prompt_attn_kernel<T, DP>>(Cfg<DP>::kSmem)) return SPD_ERR_CUDA;
-  prompt_attn_kernel<T, DP><<<grid, kThreads, Cfg<DP>::kSmem, st>>>(tq, tk, tv, p);
+template <typename T, int DP, int BN>
+static int launch(PromptParams p, const PromptTensors& t, long long items, int sms, cudaStream_t st) {
+  using C = Cfg<DP, BN>;
+  constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
+  CUtensorMap tq, tk, tv;
+  if (!make_map3(&tq, t.q, p.D, p.Hq, p.Nq, t.q_sh, t.q_st, p.pack, BM / p.pack, kBf16) ||
+      !make_map3(&tk, t.k, p.D, p.Hkv, p.Nk, t.k_sh, t.k_st, 1, BN, kBf16) ||
+      !make_map3(&tv, t.v, p.D, p.Hkv, p.Nk, t.v_sh, t.v_st, 1, BN, kBf16))
+    return SPD_ERR_CUDA;
+  p.ranked = items > (long long)sms * C::kCtas;
+  if (!allow_smem<prompt_attn_kernel<T, DP, BN>>(C::kSmem)) return SPD_ERR_CUDA;
+  static const bool enough = [] {  // a warpgroup that asks for more registers than the CTA has would wait for good
+    cudaFuncAttributes a{};
+    return cudaFuncGetAttributes(&a, prompt_attn_kernel<T, DP, BN>) == cudaSuccess && a.numRegs * kThreads >= C::kAllRegs;
+  }();
+  if (!enough) return SPD_ERR_CUDA;
+  prompt_attn_kernel<T, DP, BN><<<(unsigned)items, kThreads, C::kSmem, st>>>(tq, tk, tv, p);
   return cudaPeekAtLastError() == cudaSuccess ? SPD_OK : SPD_ERR_CUDA;
 }
 
@@ -797,18 +917,15 @@ int prompt_attn_launch(PromptParams p, const void* q, const void* k, const void*
   const int G = p.Hq / p.Hkv;
   p.pack = G & -G;
   if (p.pack > BM) p.pack = BM;
-  CUtensorMap tq, tk, tv;
-  if (!make_map3(&tq, q, p.D, p.Hq, p.Nq, q_sh, q_st, p.pack, BM / p.pack, bf16) ||
-      !make_map3(&tk, k, p.D, p.Hkv, p.Nk, k_sh, k_st, 1, BN, bf16) ||
-      !make_map3(&tv, v, p.D, p.Hkv, p.Nk, v_sh, v_st, 1, BN, bf16))
-    return SPD_ERR_CUDA;
   const int tokens = 2 * BM / p.pack;
-  const long long most = ((long long)p.Nq / tokens + p.B) * (p.Hq / p.pack);  // items at most
-  const dim3 grid((unsigned)(most < sms ? most : sms));
-  p.ranked = most > sms;
+  const long long items = ((long long)p.Nq / tokens + p.B) * (p.Hq / p.pack);  // at most
+  if (items > 0x7fffffffll) return SPD_ERR_UNSUPPORTED;
+  const PromptTensors t{q, k, v, q_st, q_sh, k_st, k_sh, v_st, v_sh};
   auto by_d = [&](auto tag) -> int {
     using T = decltype(tag);
-    return p.D <= 64 ? launch<T, 64>(tq, tk, tv, p, grid, st) : launch<T, 128>(tq, tk, tv, p, grid, st);
+    if (p.D > 64) return launch<T, 128, 128>(p, t, items, sms, st);
+    // two CTAs an SM with 64 keys a step, unless there is no second item for any SM (both measured above)
+    return items <= sms ? launch<T, 64, 128>(p, t, items, sms, st) : launch<T, 64, 64>(p, t, items, sms, st);
   };
   return bf16 ? by_d(__nv_bfloat16{}) : by_d(__half{});
 }
