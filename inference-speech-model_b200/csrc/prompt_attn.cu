@@ -44,8 +44,11 @@
 // 143 against 166 us there, 202 against 224 for 4 x 4096 causal tokens of 16 heads, but 11.5 against
 // 10.3 for 6 short prompts of 12 heads, one item an SM at most.  Items dealt out in fixed turns instead of taken
 // over: 147 (forwards) and 163 us (forwards and backwards) for the 8 x 1500, 215 and 210 for the 4 x
-// 4096.  Slower at D = 128: two threads a row, two issuing lanes (the tiles fall into step) and a
-// second read of S in place of 128 registers (579, 565 and 525 us when this one took 485).
+// 4096.  Slower at D = 128: steps of 64 keys with two score buffers a tile, so that scores are there
+// before the last weights are used (544 us; products of 64 columns read shared memory 1.5 times as
+// often, and each step's hand-over is paid twice); two threads a row, two issuing lanes (the tiles
+// fall into step) and a second read of S in place of 128 registers (579, 565 and 525 us when this one
+// took 485).
 #include "spd_tc.cuh"
 
 namespace spd {
@@ -466,7 +469,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<DP, BN>::kCtas)
   uint64_t* q_empty = q_full + 2;              // [2]
   uint64_t* s_full = q_empty + 2;              // [2] scores ready (and all earlier products done)
   uint64_t* p_full = s_full + 2;               // [2 tiles][kParts] weights written (and the output rescaled)
-  uint64_t* o_full = p_full + 2 * C::kParts;               // [2] output complete
+  uint64_t* o_full = p_full + 2 * C::kParts;   // [2] output complete
   uint64_t* o_empty = o_full + 2;              // [2] output read
   uint64_t* v_landed = o_empty + 2;            // a V tile with rows past the last key is there
   uint64_t* v_fixed = v_landed + 1;            // and those rows are zero

@@ -468,8 +468,9 @@ def rope_kv_append(
 ) -> Optional[torch.Tensor]:
     """Rotates q and k by position and writes k and v into the paged pools; returns rotated q.
 
-    q [N, Hq, D] (or None), k and v [N, Hkv, D]: N packed tokens, any token and head strides
-    (views of a packed q|k|v projection), D contiguous; pools [num_blocks, block_size, Hkv, D].
+    q [N, Hq, D] (or None), k and v [N, Hkv, D]: N packed tokens, any token and head strides that are
+    multiples of 16 bytes (views of a packed q|k|v projection), D (a multiple of 8 up to 1024)
+    contiguous; pools [num_blocks, block_size, Hkv, D].
     cos, sin fp32 [max positions, rotated / 2]: the first ``rotated`` dimensions of a head turn,
     as halves (i with i + rotated/2) or, ``interleaved``, as neighbours (2i with 2i + 1).
     positions int32 [B]: position of each sequence's first token here (< 0 skips it);
