@@ -88,6 +88,10 @@ int spd_get_last_error(char* buf, size_t size);
 size_t spd_paged_decode_attn_workspace_size(int B, int H, int D, int max_blocks, int device);
 size_t spd_cross_attn_workspace_size(int B, int H, int D, int device);
 
+/* A number of its own for the graph capture that `stream` is part of, 0 outside a capture.  A workspace
+ * that is made during a capture is zeroed by a node of that graph alone: it belongs to that capture. */
+uint64_t spd_stream_capture_id(void* stream);
+
 /* Bound on every wait of the attention kernels (spd_paged_decode_attn, its allocation-free
  * variant, spd_cross_attn) launched by the calling thread from now on; each launch takes
  * the value as a kernel parameter.  A wait that runs out records SPD_DEVERR_TIMEOUT in the

@@ -168,6 +168,16 @@ int spd_set_wait_timeout_ns(uint64_t ns) {
 
 uint64_t spd_get_wait_timeout_ns(void) { return g_wait_ns; }
 
+uint64_t spd_stream_capture_id(void* stream) {
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  if (cudaStreamGetCaptureInfo(static_cast<cudaStream_t>(stream), &status, &id) != cudaSuccess) {
+    (void)cudaGetLastError();
+    return 0;
+  }
+  return status == cudaStreamCaptureStatusNone ? 0 : id + 1;
+}
+
 int spd_selftest_wait_timeout(int32_t* error_word, uint64_t timeout_ns, void* stream) {
   if (!error_word || timeout_ns == 0 || timeout_ns > spd::SPD_WAIT_NS)
     return fail(SPD_ERR_INVALID_ARG, "spd_selftest_wait_timeout: error_word and 0 < timeout_ns <= %llu needed",

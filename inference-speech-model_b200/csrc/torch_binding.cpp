@@ -16,6 +16,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/DynamicTypes.h>
 
+#include <algorithm>
 #include <array>
 #include <sstream>
 #include <stdexcept>
@@ -35,6 +36,7 @@ decltype(&spd_paged_decode_attn_int4_workspace_size) f_decode_size;
 decltype(&spd_prompt_attn) f_prompt;
 decltype(&spd_kv_int4_page_bytes) f_page_bytes;
 decltype(&spd_get_last_error) f_last_error;
+decltype(&spd_stream_capture_id) f_capture_id;
 
 struct Refused : std::runtime_error {
   using std::runtime_error::runtime_error;
@@ -269,15 +271,34 @@ std::pair<at::Tensor, at::Tensor> gather(const char* name, PyObject* const* a, P
   return {k, v};
 }
 
-// Zero-filled workspaces of paged_decode_attention_int4, one per geometry, device and stream, kept
-// for the process.
-at::Tensor decode_workspace(const std::array<int64_t, 9>& key, const at::Tensor& like) {
-  static auto* kept = new std::vector<std::pair<std::array<int64_t, 9>, at::Tensor>>();
+// Zero-filled workspaces of paged_decode_attention_int4, one per geometry, device, stream and graph
+// capture.  Those of calls outside captures are kept for the process.  One that is made during a
+// capture lies in the graph's memory and is zeroed by a node of that graph: it serves that capture's
+// calls and no others, and is let go (back to the graph's memory) once kCaptures later ones have come.
+constexpr size_t kCaptures = 8;
+using WorkspaceKey = std::array<int64_t, 10>;  // ... device, stream, capture
+at::Tensor decode_workspace(const WorkspaceKey& key, const at::Tensor& like) {
+  static auto* kept = new std::vector<std::pair<WorkspaceKey, at::Tensor>>();
   for (const auto& e : *kept)
     if (e.first == key) return e.second;
   const size_t bytes = f_decode_size((int)key[0], (int)key[1], (int)key[2], (int)key[3], (int)key[4], (int)key[5], (int)key[6],
                                      (int)key[7]);
   if (bytes == 0) refuse("paged_decode_attn_int4", "unsupported geometry");
+  if (key[9]) {
+    std::vector<int64_t> captures;  // the latest first
+    for (auto e = kept->rbegin(); e != kept->rend(); ++e)
+      if (e->first[9] && std::find(captures.begin(), captures.end(), e->first[9]) == captures.end())
+        captures.push_back(e->first[9]);
+    if (captures.size() >= kCaptures && std::find(captures.begin(), captures.end(), key[9]) == captures.end()) {
+      captures.resize(kCaptures - 1);
+      kept->erase(std::remove_if(kept->begin(), kept->end(),
+                                 [&](const auto& e) {
+                                   return e.first[9] &&
+                                          std::find(captures.begin(), captures.end(), e.first[9]) == captures.end();
+                                 }),
+                  kept->end());
+    }
+  }
   at::Tensor ws = at::zeros({(int64_t)bytes}, like.options().dtype(at::kByte));
   kept->emplace_back(key, ws);
   return ws;
@@ -312,7 +333,7 @@ at::Tensor decode(const char* name, PyObject* const* a, Py_ssize_t n_args) {
     refuse(name, "workspace must be a contiguous uint8 tensor");
   const at::Tensor ws = ws_given.defined() ? ws_given
                                            : decode_workspace({B, Hq, Hkv, D, bs, max_blocks, code, dev,
-                                                               (int64_t)reinterpret_cast<intptr_t>(st)}, q);
+                                                               (int64_t)reinterpret_cast<intptr_t>(st), (int64_t)f_capture_id(st)}, q);
   check(f_decode(ptr(q), ptr(pool), static_cast<const int32_t*>(ptr(tables)), static_cast<const int32_t*>(ptr(lens)), mut(out),
                  B, Hq, Hkv, D, bs, max_blocks, small_int(name, "num_blocks", pool.size(0)), (float)scale, code, mut(ws),
                  (size_t)ws.numel(), st),
@@ -409,7 +430,8 @@ PyObject* py_setup(PyObject*, PyObject* d) {
   if (get("spd_rope_kv_append", f_rope_append) && get("spd_rope_kv_append_int4", f_rope_append_int4) &&
       get("spd_kv_gather_int4", f_gather) && get("spd_paged_decode_attn_int4", f_decode) &&
       get("spd_paged_decode_attn_int4_workspace_size", f_decode_size) && get("spd_prompt_attn", f_prompt) &&
-      get("spd_kv_int4_page_bytes", f_page_bytes) && get("spd_get_last_error", f_last_error))
+      get("spd_kv_int4_page_bytes", f_page_bytes) && get("spd_get_last_error", f_last_error) &&
+      get("spd_stream_capture_id", f_capture_id))
     Py_RETURN_NONE;
   return nullptr;
 }

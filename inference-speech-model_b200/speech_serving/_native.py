@@ -51,6 +51,7 @@ _SIGNATURES = {
     "spd_linear": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _i64, _i64, _i, _i, _vp, _vp]),
     "spd_set_wait_timeout_ns": (_i, [C.c_uint64]),
     "spd_get_wait_timeout_ns": (C.c_uint64, []),
+    "spd_stream_capture_id": (C.c_uint64, [_vp]),
     "spd_selftest_wait_timeout": (_i, [_vp, C.c_uint64, _vp]),
     "spd_paged_decode_attn_noalloc": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _f, _i, _vp, _vp,
                                            _vp, _vp]),
