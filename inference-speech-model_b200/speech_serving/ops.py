@@ -90,13 +90,25 @@ def cross_attn_workspace(B: int, H: int, D: int, device: torch.device) -> torch.
     return torch.zeros(n, dtype=torch.uint8, device=device)
 
 
+_CAPTURES = 8  # graph captures whose workspaces are held
+
+
 def _cached_workspace(kind: str, B: int, H: int, D: int, device: torch.device, max_blocks: int = 0) -> torch.Tensor:
-    """One zero-initialised workspace per (op, geometry, device, stream).  The counter and
-    partial regions are laid out by geometry, so a workspace is never shared between
-    geometries (stale partials would otherwise land in another call's counters)."""
-    key = (kind, B, H, D, max_blocks, device, torch.cuda.current_stream(device).cuda_stream)
+    """One zero-initialised workspace per (op, geometry, device, stream, graph capture).  The counter
+    and partial regions are laid out by geometry, so a workspace is never shared between
+    geometries (stale partials would otherwise land in another call's counters).  One made during a
+    capture lies in the graph's memory and is zeroed by a node of that graph: it serves that
+    capture's calls alone, and is let go once _CAPTURES later ones have come."""
+    stream = torch.cuda.current_stream(device).cuda_stream
+    capture = N.load().spd_stream_capture_id(stream)
+    key = (kind, B, H, D, max_blocks, device, stream, capture)
     ws = _WORKSPACES.get(key)
     if ws is None:
+        if capture:
+            others = dict.fromkeys(k[-1] for k in _WORKSPACES if k[-1] not in (0, capture))  # the oldest first
+            gone = set(list(others)[: max(0, len(others) - (_CAPTURES - 1))])
+            for k in [k for k in _WORKSPACES if k[-1] in gone]:
+                del _WORKSPACES[k]
         ws = (paged_attn_workspace(B, H, D, max_blocks, device) if kind == "paged"
               else cross_attn_workspace(B, H, D, device))
         _WORKSPACES[key] = ws

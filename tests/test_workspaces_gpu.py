@@ -90,3 +90,33 @@ def test_many_captures_keep_their_results():
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("op", ["paged", "cross"])
+def test_captured_calls_of_the_engine_ops_do_not_share_a_workspace(op):
+    """The same for paged_decode_attention and cross_attention, over more captures than are remembered."""
+    g = torch.Generator(device=DEV).manual_seed(4)
+    B, H, D = 4, 12, 64
+    q = torch.randn(B, H, D, generator=g, device=DEV).half()
+    if op == "paged":
+        pools = [torch.randn(128, 16, H, D, generator=g, device=DEV).half() for _ in range(2)]
+        table = torch.randperm(128, generator=g, device=DEV).to(torch.int32)[: B * 28].view(B, 28)
+        args = (q, *pools, table, torch.tensor([448, 100, 17, 300], dtype=torch.int32, device=DEV))
+        call, make = ops.paged_decode_attention, ops.paged_attn_workspace(B, H, D, 28, torch.device(DEV))
+    else:
+        kv = [torch.randn(B, H, 1500, D, generator=g, device=DEV).half() for _ in range(2)]
+        args = (q, *kv, torch.tensor([1500, 100, 17, 900], dtype=torch.int32, device=DEV))
+        call, make = ops.cross_attention, ops.cross_attn_workspace(B, H, D, torch.device(DEV))
+    want = call(*args, workspace=make)
+    pool, poison = poisoned_pool(256)
+    outs, graphs = [torch.zeros_like(want) for _ in range(10)], [torch.cuda.CUDAGraph() for _ in range(10)]
+    for out, graph in zip(outs, graphs):
+        with torch.cuda.graph(graph, pool=pool):
+            call(*args, out=out)
+    assert len({k[-1] for k in ops._WORKSPACES if k[-1]}) <= 8
+    for i in (9, 0, 4, 9, 1):
+        poison.replay()
+        outs[i].fill_(7.0)
+        graphs[i].replay()
+        torch.cuda.synchronize()
+        assert torch.equal(outs[i], want)
