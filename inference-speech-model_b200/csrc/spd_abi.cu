@@ -539,10 +539,13 @@ int spd_paged_decode_attn_int4(const void* q, const void* pool, const int32_t* b
   unsigned char* ws = static_cast<unsigned char*>(workspace);
   p.err = reinterpret_cast<int*>(ws);
   p.counters = reinterpret_cast<int*>(ws + spd::kWsHeaderBytes);
-  p.partials = reinterpret_cast<float*>(ws + spd::kWsHeaderBytes + spd::round_up((size_t)B * Hq * 4, 256));
   const spd::Int4Split split = spd::decode_int4_split(B, Hq, Hkv, D, dtype, (int)max_ctx, sm_count(-1));
   p.chunks = split.chunks;
   p.least = split.least;
+  // at the end of what the caller gave, so that a workspace with room for the counters and the partial
+  // results of several geometries serves them all
+  const size_t results = spd::round_up((size_t)B * Hq * split.chunks * (D + 4) * 4, 256);
+  p.partials = reinterpret_cast<float*>(ws + (workspace_bytes - results) / 256 * 256);
   const int rc = spd::decode_int4_launch(p, D, block_size, static_cast<cudaStream_t>(stream));
   if (rc != SPD_OK)
     return fail(rc, "spd_paged_decode_attn_int4: launch failed: %s", cudaGetErrorString(cudaGetLastError()));

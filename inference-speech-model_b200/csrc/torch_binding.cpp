@@ -271,36 +271,47 @@ std::pair<at::Tensor, at::Tensor> gather(const char* name, PyObject* const* a, P
   return {k, v};
 }
 
-// Zero-filled workspaces of paged_decode_attention_int4, one per geometry, device, stream and graph
-// capture.  Those of calls outside captures are kept for the process.  One that is made during a
-// capture lies in the graph's memory and is zeroed by a node of that graph: it serves that capture's
-// calls and no others, and is let go (back to the graph's memory) once kCaptures later ones have come.
-constexpr size_t kCaptures = 8;
-using WorkspaceKey = std::array<int64_t, 10>;  // ... device, stream, capture
-at::Tensor decode_workspace(const WorkspaceKey& key, const at::Tensor& like) {
-  static auto* kept = new std::vector<std::pair<WorkspaceKey, at::Tensor>>();
-  for (const auto& e : *kept)
-    if (e.first == key) return e.second;
-  const size_t bytes = f_decode_size((int)key[0], (int)key[1], (int)key[2], (int)key[3], (int)key[4], (int)key[5], (int)key[6],
-                                     (int)key[7]);
-  if (bytes == 0) refuse("paged_decode_attn_int4", "unsupported geometry");
-  if (key[9]) {
-    std::vector<int64_t> captures;  // the latest first
+// Workspaces of calls to paged_decode_attention_int4 that bring none: one per device, stream and graph
+// capture, made anew when a call needs more arrival counters or partial results than it has room for.
+// Counters lie at its start and are left at zero by every call, partial results at its end, so one
+// workspace serves all geometries.  One that is made during a capture lies in the graph's memory and is
+// zeroed by a node of that graph: it serves that capture's calls and no others, and is let go (back to
+// the graph's memory) once kCaptures later ones have come.
+constexpr size_t kCaptures = 8, kHeader = 256;
+struct Workspace {
+  int dev;
+  void* stream;
+  uint64_t capture;  // 0: outside captures
+  size_t counters, partials;  // bytes
+  at::Tensor bytes;
+};
+at::Tensor decode_workspace(int dev, void* stream, size_t counters, size_t need, const at::Tensor& like) {
+  static auto* kept = new std::vector<Workspace>();  // in the order of their captures
+  if (need == 0) refuse("paged_decode_attn_int4", "unsupported geometry");
+  size_t partials = need - kHeader - counters;
+  const uint64_t capture = f_capture_id(stream);
+  for (auto e = kept->begin(); e != kept->end(); ++e)
+    if (e->dev == dev && e->stream == stream && e->capture == capture) {
+      if (e->counters >= counters && e->partials >= partials) return e->bytes;
+      counters = std::max(counters, e->counters);
+      partials = std::max(partials, e->partials);
+      kept->erase(e);
+      break;
+    }
+  if (capture) {
+    size_t others = 0;
+    uint64_t last = capture;
     for (auto e = kept->rbegin(); e != kept->rend(); ++e)
-      if (e->first[9] && std::find(captures.begin(), captures.end(), e->first[9]) == captures.end())
-        captures.push_back(e->first[9]);
-    if (captures.size() >= kCaptures && std::find(captures.begin(), captures.end(), key[9]) == captures.end()) {
-      captures.resize(kCaptures - 1);
-      kept->erase(std::remove_if(kept->begin(), kept->end(),
-                                 [&](const auto& e) {
-                                   return e.first[9] &&
-                                          std::find(captures.begin(), captures.end(), e.first[9]) == captures.end();
-                                 }),
+      if (e->capture && e->capture != capture && e->capture != last) last = e->capture, ++others;
+    if (others >= kCaptures) {
+      const auto oldest = std::find_if(kept->begin(), kept->end(), [&](const Workspace& e) { return e.capture; })->capture;
+      kept->erase(std::remove_if(kept->begin(), kept->end(), [&](const Workspace& e) { return e.capture == oldest; }),
                   kept->end());
     }
   }
-  at::Tensor ws = at::zeros({(int64_t)bytes}, like.options().dtype(at::kByte));
-  kept->emplace_back(key, ws);
+  at::Tensor ws = at::empty({(int64_t)(kHeader + counters + partials)}, like.options().dtype(at::kByte));
+  ws.narrow(0, 0, (int64_t)(kHeader + counters)).zero_();
+  kept->push_back({dev, stream, capture, counters, partials, ws});
   return ws;
 }
 
@@ -331,9 +342,10 @@ at::Tensor decode(const char* name, PyObject* const* a, Py_ssize_t n_args) {
   void* st = stream();
   if (ws_given.defined() && (ws_given.scalar_type() != at::kByte || !ws_given.is_contiguous()))
     refuse(name, "workspace must be a contiguous uint8 tensor");
-  const at::Tensor ws = ws_given.defined() ? ws_given
-                                           : decode_workspace({B, Hq, Hkv, D, bs, max_blocks, code, dev,
-                                                               (int64_t)reinterpret_cast<intptr_t>(st), (int64_t)f_capture_id(st)}, q);
+  const size_t counters = ((size_t)B * Hq * 4 + kHeader - 1) / kHeader * kHeader;  // the library's layout
+  const at::Tensor ws = ws_given.defined()
+                            ? ws_given
+                            : decode_workspace(dev, st, counters, f_decode_size(B, Hq, Hkv, D, bs, max_blocks, code, dev), q);
   check(f_decode(ptr(q), ptr(pool), static_cast<const int32_t*>(ptr(tables)), static_cast<const int32_t*>(ptr(lens)), mut(out),
                  B, Hq, Hkv, D, bs, max_blocks, small_int(name, "num_blocks", pool.size(0)), (float)scale, code, mut(ws),
                  (size_t)ws.numel(), st),

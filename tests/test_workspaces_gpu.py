@@ -92,6 +92,26 @@ def test_many_captures_keep_their_results():
         assert torch.equal(out, want)
 
 
+def test_the_kept_workspace_does_not_grow_with_the_geometries_seen():
+    """Batches and tables of many sizes, back and forth: results stay, and no more memory than the largest needs."""
+    cases = [(B, ctx, D, Hq) for B in (1, 2, 5) for ctx in (100, 1500, 6000, 20000, 33000) for D, Hq in ((64, 8), (128, 4))]
+    args = {c: decode_args(seed=3, ctx=c[1], B=c[0], Hq=c[3], D=c[2]) for c in cases}
+    sizes = {c: ops.decode_int4_workspace(c[0], c[3], 2, c[2], 16, args[c][2].shape[1], torch.float16,
+                                          torch.device(DEV)).numel() for c in cases}
+    want = {c: ops.paged_decode_attention_int4(*args[c], workspace=torch.zeros(sizes[c], dtype=torch.uint8, device=DEV))
+            for c in cases}
+    out = {c: torch.full_like(want[c], 7.0) for c in cases}
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    with torch.cuda.stream(side):
+        for c in cases + cases[::-1] + cases[::3]:
+            ops.paged_decode_attention_int4(*args[c], out=out[c].fill_(7.0))
+            assert torch.equal(out[c], want[c])
+    assert torch.cuda.memory_allocated() - before <= 2 * max(sizes.values()) < sum(sizes.values())
+
+
 @pytest.mark.parametrize("op", ["paged", "cross"])
 def test_captured_calls_of_the_engine_ops_do_not_share_a_workspace(op):
     """The same for paged_decode_attention and cross_attention, over more captures than are remembered."""
