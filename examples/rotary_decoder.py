@@ -79,6 +79,7 @@ class RotaryDecoder:
             self.blocks = BlockManager(cfg.layers, cfg.kv_heads, cfg.head_dim, cfg.block_size, cfg.num_blocks, cfg.dtype,
                                        device)
         self.errors = torch.zeros(1, dtype=torch.int32, device=device)
+        self.workspace = None  # of the last decode() call's attention
         self.tables: List[List[int]] = []
         self.lengths: List[int] = []
 
@@ -101,9 +102,18 @@ class RotaryDecoder:
             self.blocks.free_blocks(t)
         self.tables, self.lengths = [], []
 
+    def _decode_workspace(self, columns: int) -> torch.Tensor:
+        c, n, device = self.cfg, len(self.tables), torch.device(self.device)
+        if c.bits == 4:
+            return ops.decode_int4_workspace(n, c.heads, c.kv_heads, c.head_dim, c.block_size, columns, c.dtype, device)
+        return ops.paged_attn_workspace(n, c.heads, c.head_dim, columns, device)
+
     def check_errors(self) -> None:
-        if ops.read_error_word(self.errors):
-            raise RuntimeError(f"a kernel refused a length or a block id: {ops.read_error_word(self.errors):#x}")
+        word = ops.read_error_word(self.errors)
+        if self.workspace is not None:
+            word |= ops.read_error_word(self.workspace)  # where paged_decode_attention leaves its flags
+        if word:
+            raise RuntimeError(f"a kernel refused a length or a block id, or gave up waiting: {word:#x}")
 
     # ---- the network ------------------------------------------------------------------------
     def _qkv(self, layer, x):
@@ -170,15 +180,17 @@ class RotaryDecoder:
         return self._logits(x)
 
     # ---- decode -----------------------------------------------------------------------------
-    def _step(self, tokens, positions, context, tables):
+    def _step(self, tokens, positions, context, tables, workspace):
         x = self.embed[tokens]
         for i, layer in enumerate(self.layers):
             q, k, v = self._qkv(layer, x)
             q = self._append(i, q, k, v, tables, positions, None)
             if self.cfg.bits == 4:
-                attended = ops.paged_decode_attention_int4(q, self.pools[i], tables, context)
+                attended = ops.paged_decode_attention_int4(q, self.pools[i], tables, context, workspace=workspace,
+                                                           error_word=self.errors)
             else:
-                attended = ops.paged_decode_attention(q, self.blocks.key_pool[i], self.blocks.value_pool[i], tables, context)
+                attended = ops.paged_decode_attention(q, self.blocks.key_pool[i], self.blocks.value_pool[i], tables, context,
+                                                      workspace=workspace)
             x = self._rest(layer, x, attended)
         return self._logits(x)
 
@@ -189,20 +201,21 @@ class RotaryDecoder:
             self._reserve(r, n + steps)
         tables, positions = self._device_tables(), self._ints(self.lengths)
         context = positions + 1
+        workspace = self.workspace = self._decode_workspace(tables.shape[1])
         tokens = ops.argmax_rows(logits)
         out = torch.empty(steps, len(self.tables), dtype=torch.long, device=self.device)
 
         def step():
-            ops.argmax_rows(self._step(tokens, positions, context, tables), out=tokens)
+            ops.argmax_rows(self._step(tokens, positions, context, tables, workspace), out=tokens)
             positions.add_(1)
             context.add_(1)
 
         if steps > 1:
-            # once before the capture, for the libraries' workspaces: the same token is written again later
+            # once before the capture, for torch's own workspaces: the same token is written again later
             side = torch.cuda.Stream()
             side.wait_stream(torch.cuda.current_stream())
             with torch.cuda.stream(side):
-                self._step(tokens, positions, context, tables)
+                self._step(tokens, positions, context, tables, workspace)
                 graph = torch.cuda.CUDAGraph()
                 with torch.cuda.graph(graph, stream=side):
                     step()

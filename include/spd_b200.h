@@ -311,6 +311,12 @@ int spd_paged_decode_attn_int4(const void* q, const void* pool, const int32_t* b
                                const int32_t* context_lens, void* out, int B, int Hq, int Hkv, int D, int block_size,
                                int max_blocks, int num_blocks, float scale, int dtype, void* workspace,
                                size_t workspace_bytes, void* stream);
+/* The same with an int32 device word of the caller's (or NULL: the workspace's own) that receives the
+ * SPD_DEVERR_* flags, OR-ed in. */
+int spd_paged_decode_attn_int4_err(const void* q, const void* pool, const int32_t* block_tables,
+                                   const int32_t* context_lens, void* out, int B, int Hq, int Hkv, int D, int block_size,
+                                   int max_blocks, int num_blocks, float scale, int dtype, void* workspace,
+                                   size_t workspace_bytes, int32_t* error_word, void* stream);
 
 /* Attention of whole packed prompts on the tensor cores (dtype F16 or BF16):
  *   q [Nq][Hq][D], k and v [Nk][Hkv][D] with token and head strides in elements, D contiguous;

@@ -514,6 +514,14 @@ int spd_paged_decode_attn_int4(const void* q, const void* pool, const int32_t* b
                                const int32_t* context_lens, void* out, int B, int Hq, int Hkv, int D, int block_size,
                                int max_blocks, int num_blocks, float scale, int dtype, void* workspace,
                                size_t workspace_bytes, void* stream) {
+  return spd_paged_decode_attn_int4_err(q, pool, block_tables, context_lens, out, B, Hq, Hkv, D, block_size, max_blocks,
+                                        num_blocks, scale, dtype, workspace, workspace_bytes, nullptr, stream);
+}
+
+int spd_paged_decode_attn_int4_err(const void* q, const void* pool, const int32_t* block_tables,
+                                   const int32_t* context_lens, void* out, int B, int Hq, int Hkv, int D, int block_size,
+                                   int max_blocks, int num_blocks, float scale, int dtype, void* workspace,
+                                   size_t workspace_bytes, int32_t* error_word, void* stream) {
   if (!elem_bytes(dtype)) return fail(SPD_ERR_UNSUPPORTED, "spd_paged_decode_attn_int4: dtype %d not supported", dtype);
   if (!q || !pool || !block_tables || !context_lens || !out)
     return fail(SPD_ERR_INVALID_ARG, "spd_paged_decode_attn_int4: null tensor pointer");
@@ -537,7 +545,7 @@ int spd_paged_decode_attn_int4(const void* q, const void* pool, const int32_t* b
   p.scale_log2 = scale * 1.4426950408889634f;
   p.wait_ns = g_wait_ns;
   unsigned char* ws = static_cast<unsigned char*>(workspace);
-  p.err = reinterpret_cast<int*>(ws);
+  p.err = error_word ? error_word : reinterpret_cast<int*>(ws);
   p.counters = reinterpret_cast<int*>(ws + spd::kWsHeaderBytes);
   const spd::Int4Split split = spd::decode_int4_split(B, Hq, Hkv, D, dtype, (int)max_ctx, sm_count(-1));
   p.chunks = split.chunks;

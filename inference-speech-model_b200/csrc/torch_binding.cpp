@@ -31,7 +31,7 @@ namespace {
 decltype(&spd_rope_kv_append) f_rope_append;
 decltype(&spd_rope_kv_append_int4) f_rope_append_int4;
 decltype(&spd_kv_gather_int4) f_gather;
-decltype(&spd_paged_decode_attn_int4) f_decode;
+decltype(&spd_paged_decode_attn_int4_err) f_decode;
 decltype(&spd_paged_decode_attn_int4_workspace_size) f_decode_size;
 decltype(&spd_prompt_attn) f_prompt;
 decltype(&spd_kv_int4_page_bytes) f_page_bytes;
@@ -315,13 +315,13 @@ at::Tensor decode_workspace(int dev, void* stream, size_t counters, size_t need,
   return ws;
 }
 
-// (q, pool, block_tables, context_lens, scale, out, workspace)
+// (q, pool, block_tables, context_lens, scale, out, workspace, error_word)
 at::Tensor decode(const char* name, PyObject* const* a, Py_ssize_t n_args) {
-  count(name, n_args, 7);
+  count(name, n_args, 8);
   const at::Tensor &q = tensor(name, "q", a[0]), &pool = tensor(name, "pool", a[1]), &tables = tensor(name, "block_tables", a[2]),
                    &lens = tensor(name, "context_lens", a[3]), &given = tensor(name, "out", a[5], true),
-                   &ws_given = tensor(name, "workspace", a[6], true);
-  const int dev = current_device(name, {&q, &pool, &tables, &lens, &given, &ws_given});
+                   &ws_given = tensor(name, "workspace", a[6], true), &err = tensor(name, "error_word", a[7], true);
+  const int dev = current_device(name, {&q, &pool, &tables, &lens, &given, &ws_given, &err});
   if (q.dim() != 3 || !q.is_contiguous()) refuse(name, "q must be a contiguous [B, Hq, D] tensor");
   const int B = small_int(name, "B", q.size(0)), Hq = small_int(name, "Hq", q.size(1)), D = small_int(name, "D", q.size(2));
   const int Hkv = pool.dim() == 3 ? small_int(name, "Hkv", pool.size(1)) : -1;
@@ -331,6 +331,7 @@ at::Tensor decode(const char* name, PyObject* const* a, Py_ssize_t n_args) {
   int32_vector(name, "context_lens", lens, B);
   if (given.defined() && (given.sizes() != q.sizes() || given.scalar_type() != q.scalar_type() || !given.is_contiguous()))
     refuse(name, "out must be a contiguous ", shape_of(q), " tensor of q's dtype");
+  error_word(name, err);
   const int code = dtype_code(name, q.scalar_type());
   const double scale = PyFloat_AsDouble(a[4]);
   if (PyErr_Occurred()) {
@@ -348,7 +349,7 @@ at::Tensor decode(const char* name, PyObject* const* a, Py_ssize_t n_args) {
                             : decode_workspace(dev, st, counters, f_decode_size(B, Hq, Hkv, D, bs, max_blocks, code, dev), q);
   check(f_decode(ptr(q), ptr(pool), static_cast<const int32_t*>(ptr(tables)), static_cast<const int32_t*>(ptr(lens)), mut(out),
                  B, Hq, Hkv, D, bs, max_blocks, small_int(name, "num_blocks", pool.size(0)), (float)scale, code, mut(ws),
-                 (size_t)ws.numel(), st),
+                 (size_t)ws.numel(), static_cast<int32_t*>(mut(err)), st),
         name);
   return out;
 }
@@ -440,7 +441,7 @@ PyObject* py_setup(PyObject*, PyObject* d) {
     return p != nullptr;
   };
   if (get("spd_rope_kv_append", f_rope_append) && get("spd_rope_kv_append_int4", f_rope_append_int4) &&
-      get("spd_kv_gather_int4", f_gather) && get("spd_paged_decode_attn_int4", f_decode) &&
+      get("spd_kv_gather_int4", f_gather) && get("spd_paged_decode_attn_int4_err", f_decode) &&
       get("spd_paged_decode_attn_int4_workspace_size", f_decode_size) && get("spd_prompt_attn", f_prompt) &&
       get("spd_kv_int4_page_bytes", f_page_bytes) && get("spd_get_last_error", f_last_error) &&
       get("spd_stream_capture_id", f_capture_id))

@@ -63,6 +63,7 @@ _SIGNATURES = {
     "spd_kv_gather_int4": (_i, [_vp] * 6 + [_i] * 8 + [_vp, _vp]),
     "spd_paged_decode_attn_int4_workspace_size": (_sz, [_i] * 8),
     "spd_paged_decode_attn_int4": (_i, [_vp] * 5 + [_i] * 7 + [_f, _i, _vp, _sz, _vp]),
+    "spd_paged_decode_attn_int4_err": (_i, [_vp] * 5 + [_i] * 7 + [_f, _i, _vp, _sz, _vp, _vp]),
     "spd_prompt_attn": (_i, [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _vp] + [_i] * 7
                         + [_f, _i, _vp, _vp]),
 }

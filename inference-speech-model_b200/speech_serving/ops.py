@@ -538,14 +538,18 @@ def paged_decode_attention_int4(
     scale: Optional[float] = None,
     out: Optional[torch.Tensor] = None,
     workspace: Optional[torch.Tensor] = None,
+    error_word: Optional[torch.Tensor] = None,
 ) -> torch.Tensor:
     """Single-token attention over a 4-bit pool with grouped heads.
 
     q [B, Hq, D]; pool from ``kv_pool_int4`` with Hkv heads (Hq a multiple of it; query head h
     reads head h // (Hq // Hkv)); block_tables int32 [B, max_blocks]; context_lens int32 [B]
-    tokens attended (<= 0 gives zeros).  Returns out [B, Hq, D]."""
+    tokens attended (<= 0 gives zeros).  Device flags (a block id or length out of range, a wait that
+    ran out) go to ``error_word`` (int32), else to the first word of ``workspace``; a call that
+    brings neither cannot be asked for them.  Returns out [B, Hq, D]."""
     return N.binding().paged_decode_attention_int4(q, pool, block_tables, context_lens,
-                                                   q.shape[-1] ** -0.5 if scale is None else scale, out, workspace)
+                                                   q.shape[-1] ** -0.5 if scale is None else scale, out, workspace,
+                                                   error_word)
 
 
 def prompt_attention(
