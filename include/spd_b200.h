@@ -10,7 +10,8 @@
  *     so every call can be captured into a CUDA graph;
  *   - validates arguments on the host (SPD_ERR_INVALID_ARG / SPD_ERR_UNSUPPORTED);
  *     out-of-range block ids or lengths found on the device are clamped to in-bounds
- *     addresses and recorded in a device error word (see SPD_DEVERR_*), never trapped.
+ *     addresses or left out (each entry says which) and recorded in a device error word (see
+ *     SPD_DEVERR_*), never trapped.
  *
  * Pool layout (decoder paged KV cache and encoder paged pool), one tensor per layer and
  * per K/V:  pool[num_blocks][block_size][H][D], element type given by `dtype`.
@@ -302,7 +303,8 @@ int spd_kv_gather_int4(const void* pool, const int32_t* block_tables, const int3
 
 /* Single-token attention over a 4-bit pool with grouped heads: query head h attends key/value
  * head h / (Hq / Hkv).
- *   q, out [B][Hq][D]; context_lens int32 [B] tokens attended (<= 0: zeros).
+ *   q, out [B][Hq][D]; context_lens int32 [B] tokens attended (<= 0: zeros; clamped to the table).
+ *   Tokens of a block whose id is out of range are left out.
  * fp32 softmax and sums, output rounded to dtype.  The workspace follows the rules above
  * (zero-filled once; one geometry, one stream at a time).  B <= 4096, Hq a multiple of Hkv. */
 size_t spd_paged_decode_attn_int4_workspace_size(int B, int Hq, int Hkv, int D, int block_size, int max_blocks,
