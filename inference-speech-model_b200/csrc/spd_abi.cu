@@ -88,14 +88,17 @@ bool int4_shape_ok(int D, int block_size) {
   return (D == 64 || D == 128 || D == 256) && (block_size == 8 || block_size == 16 || block_size == 32);
 }
 
-// The shared checks of the two rotating appends; `p` is filled but for the pools.
+// The shared checks of the two rotating appends; `p` is filled but for the pools.  Without tokens the
+// tensors have no elements and, as torch gives them, no address; without sequences neither have theirs.
 int rope_append_check(const char* fn, const spd::RopeAppendParams& p, int dtype) {
   const int eb = elem_bytes(dtype);
   if (!eb) return fail(SPD_ERR_UNSUPPORTED, "%s: dtype %d not supported", fn, dtype);
-  if (!p.k || !p.v || !p.cos || !p.sin || !p.k_pool || !p.block_tables || !p.positions || (p.q && !p.q_out))
+  if (p.N && (!p.k || !p.v || !p.cos || !p.sin || !p.k_pool || (p.q && !p.q_out) ||
+              (p.B && (!p.block_tables || !p.positions))))
     return fail(SPD_ERR_INVALID_ARG, "%s: null tensor pointer", fn);
-  if (p.N < 0 || p.B < 0 || p.Hkv <= 0 || (p.q && p.Hq <= 0) || p.D <= 0 || p.max_pos <= 0 || p.block_size <= 0 ||
-      p.max_blocks <= 0 || p.num_blocks <= 0 || (!p.cu_seqlens && p.N != p.B))
+  if (p.N < 0 || p.B < 0 || p.Hkv <= 0 || (p.q && p.Hq <= 0) || p.D <= 0 || p.max_pos < 0 || p.block_size <= 0 ||
+      p.max_blocks < 0 || p.num_blocks < 0 || (!p.cu_seqlens && p.N != p.B) ||
+      (p.N && (p.max_pos == 0 || p.num_blocks == 0 || (p.B && p.max_blocks == 0))))
     return fail(SPD_ERR_INVALID_ARG, "%s: bad sizes N=%d B=%d Hq=%d Hkv=%d D=%d", fn, p.N, p.B, p.Hq, p.Hkv, p.D);
   if (p.D % 8 || p.D > 1024 || p.rot <= 0 || p.rot % 16 || p.rot > p.D)
     return fail(SPD_ERR_UNSUPPORTED,
@@ -444,8 +447,8 @@ int spd_rope_kv_append(const void* q, int64_t q_stride_t, int64_t q_stride_h, co
                                 D, rot, interleaved, max_pos, block_size, max_blocks, num_blocks, error_word};
   const int rc0 = rope_append_check("spd_rope_kv_append", p, dtype);
   if (rc0 != SPD_OK) return rc0;
-  if (!v_pool) return fail(SPD_ERR_INVALID_ARG, "spd_rope_kv_append: null tensor pointer");
   if (N == 0) return ok();
+  if (!v_pool) return fail(SPD_ERR_INVALID_ARG, "spd_rope_kv_append: null tensor pointer");
   const int sms = sm_count(-1);
   if (sms <= 0) return fail(SPD_ERR_CUDA, "spd_rope_kv_append: no CUDA device");
   const int rc = spd::rope_append_launch(p, dtype, false, sms, static_cast<cudaStream_t>(stream));
@@ -481,14 +484,15 @@ int spd_kv_gather_int4(const void* pool, const int32_t* block_tables, const int3
   if (!elem_bytes(dtype)) return fail(SPD_ERR_UNSUPPORTED, "spd_kv_gather_int4: dtype %d not supported", dtype);
   if (!int4_shape_ok(D, block_size))
     return fail(SPD_ERR_UNSUPPORTED, "spd_kv_gather_int4: head_dim %d / block_size %d not supported", D, block_size);
+  if (N < 0 || B < 0 || Hkv <= 0 || max_blocks < 0 || num_blocks < 0)
+    return fail(SPD_ERR_INVALID_ARG, "spd_kv_gather_int4: bad sizes");
+  if (N == 0 || B == 0) return ok();  // no rows; tensors without elements have no address
+  if (max_blocks == 0 || num_blocks == 0) return fail(SPD_ERR_INVALID_ARG, "spd_kv_gather_int4: bad sizes");
   if (!pool || !block_tables || !cu_seqlens || !k_out || !v_out)
     return fail(SPD_ERR_INVALID_ARG, "spd_kv_gather_int4: null tensor pointer");
-  if (N < 0 || B <= 0 || Hkv <= 0 || max_blocks <= 0 || num_blocks <= 0)
-    return fail(SPD_ERR_INVALID_ARG, "spd_kv_gather_int4: bad sizes");
   if (Hkv > 4096) return fail(SPD_ERR_UNSUPPORTED, "spd_kv_gather_int4: more than 4096 heads");
   if (!aligned16(pool) || !aligned16(k_out) || !aligned16(v_out))
     return fail(SPD_ERR_INVALID_ARG, "spd_kv_gather_int4: tensors must be 16-byte aligned");
-  if (N == 0) return ok();
   const spd::GatherInt4Params p{static_cast<const unsigned char*>(pool), block_tables, cu_seqlens, starts, k_out, v_out, N,
                                 B, Hkv, D, block_size, max_blocks, num_blocks, error_word};
   const int sms = sm_count(-1);
