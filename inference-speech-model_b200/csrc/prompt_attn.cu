@@ -51,6 +51,8 @@
 // took 485).
 #include "spd_tc.cuh"
 
+#include <algorithm>
+
 namespace spd {
 namespace pa {
 using namespace tc;
@@ -868,6 +870,16 @@ __global__ void __launch_bounds__(kThreads, Cfg<DP, BN>::kCtas)
   if (warp == 1) tmem_dealloc(tmem, C::kTmemCols);
 }
 
+// Without a key anywhere: zeros in the rows that belong to a sequence.
+__global__ void no_keys_kernel(const PromptParams p) {
+  const int first = max(0, min(p.Nq, p.cu_q[0])), last = max(first, min(p.Nq, p.cu_q[p.B]));
+  const long long row = (long long)p.Hq * p.D / 8;  // in 16 bytes
+  uint4* out = reinterpret_cast<uint4*>(p.out);
+  for (long long i = first * row + (long long)blockIdx.x * blockDim.x + threadIdx.x; i < last * row;
+       i += (long long)gridDim.x * blockDim.x)
+    out[i] = make_uint4(0, 0, 0, 0);
+}
+
 struct PromptTensors {
   const void *q, *k, *v;
   long long q_st, q_sh, k_st, k_sh, v_st, v_sh;
@@ -914,8 +926,11 @@ int prompt_attn_launch(PromptParams p, const void* q, const void* k, const void*
                        cudaStream_t st) {
   using namespace pa;
   const bool bf16 = dtype == SPD_BF16;
-  if (p.Nk == 0)  // no key anywhere: every row is empty
-    return cudaMemsetAsync(p.out, 0, (size_t)p.Nq * p.Hq * p.D * 2, st) == cudaSuccess ? SPD_OK : SPD_ERR_CUDA;
+  if (p.Nk == 0) {
+    const long long blocks = ((long long)p.Nq * p.Hq * p.D / 8 + 255) / 256;
+    no_keys_kernel<<<(unsigned)std::min(blocks, 8ll * sms), 256, 0, st>>>(p);
+    return cudaPeekAtLastError() == cudaSuccess ? SPD_OK : SPD_ERR_CUDA;
+  }
   // heads of one group in a tile: the largest power of two that divides G (up to 128)
   const int G = p.Hq / p.Hkv;
   p.pack = G & -G;
