@@ -94,8 +94,10 @@ size_t spd_cross_attn_workspace_size(int B, int H, int D, int device);
 uint64_t spd_stream_capture_id(void* stream);
 
 /* Bound on every wait of the attention kernels (spd_paged_decode_attn, its allocation-free
- * variant, spd_cross_attn) launched by the calling thread from now on; each launch takes
- * the value as a kernel parameter.  A wait that runs out records SPD_DEVERR_TIMEOUT in the
+ * variant, spd_cross_attn, spd_paged_decode_attn_int4, spd_prompt_attn) launched by the calling
+ * thread from now on; each launch takes the value as a kernel parameter.  The last two suspend
+ * waiting warps and may hold on for 10 us more; in spd_prompt_attn some warps wait for all keys of
+ * one pair of tiles (about 1.7 us for 128 of them), so a bound below that stops the call.  A wait that runs out records SPD_DEVERR_TIMEOUT in the
  * error word, the launch stops its work (outputs are then undefined), waits for its own
  * copies in flight and returns; the context stays usable.  0 restores the default of 2 s
  * (SPD_DEFAULT_WAIT_NS).  No counterpart in the reference, whose kernels never wait. */

@@ -561,7 +561,9 @@ __global__ void __launch_bounds__(kThreads, Cfg<DP, BN>::kCtas)
         }
         ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
       }
-      if (!ok && lane == 0) {  // let the copies in flight land before the CTA can exit
+      // Let the copies in flight land before the CTA can exit, whichever warp gave up: after its last load
+      // this one waits for nothing that tells it that another has.  (At once otherwise.)
+      if (lane == 0) {
         for (int k = 0; k < C::kStages; ++k) {
           ring.back(C::kStages);
           if (ring.round >= 0) (void)mbar_wait_suspend(&kv_full[ring.slot], ring.phase(), nullptr);
@@ -608,7 +610,9 @@ __global__ void __launch_bounds__(kThreads, Cfg<DP, BN>::kCtas)
               scores(x, kslot);
               if (w.n[x] == 1) umma_commit(&q_empty[x]);
             }
-          umma_commit(&kv_empty[kslot]);
+          // A tile is given back only if its products were issued: after a wait that gave up its copy may still
+          // be in flight, and the loader must not arm its barrier again.
+          if (ok) umma_commit(&kv_empty[kslot]);
           for (int j = 0; j < n && ok; ++j) {
             const int vslot = ring.slot;
             wait(&kv_full[vslot], ring.phase());
@@ -649,8 +653,10 @@ __global__ void __launch_bounds__(kThreads, Cfg<DP, BN>::kCtas)
                 umma_commit(&o_full[x]);
               }
             }
-            umma_commit(&kv_empty[vslot]);
-            if (j + 1 < n) umma_commit(&kv_empty[kslot]);
+            if (ok) {
+              umma_commit(&kv_empty[vslot]);
+              if (j + 1 < n) umma_commit(&kv_empty[kslot]);
+            }
           }
         }
         __syncwarp();

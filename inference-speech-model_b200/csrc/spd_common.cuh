@@ -229,8 +229,9 @@ __device__ __forceinline__ bool mbar_wait_bounded(uint64_t* bar, uint32_t parity
 }
 
 // As mbar_wait_bounded, for kernels whose other warps compute while this one waits: each try may
-// suspend the thread for up to kSuspendNs (it wakes when the phase completes), so that a waiting
-// warp takes next to no issue slots.  The clock is read after every try.
+// suspend the thread for up to kSuspendNs (it wakes when the phase completes; a B200 ends a try after
+// 4 us all the same), so that a waiting warp takes next to no issue slots.  The clock is read after
+// every try.
 constexpr uint32_t kSuspendNs = 100000;
 __device__ __forceinline__ bool mbar_try_wait_suspend(uint64_t* bar, uint32_t parity) {
   uint32_t done;
