@@ -266,7 +266,7 @@ size_t spd_kv_int4_page_bytes(int D, int block_size); /* 0: not supported */
 /* Rotates q and k by position and writes k and v into paged 16/32-bit pools.
  *   q  [N][Hq][D] or NULL, k and v [N][Hkv][D]: N packed tokens, token and head strides in
  *      elements, D contiguous (views of a packed q|k|v tensor)
- *   q_out [N][Hq][D] contiguous; must not overlap q
+ *   q_out [N][Hq][D] contiguous; must not overlap q, k or v
  *   cos_table, sin_table fp32 [max_pos][rot / 2]
  *   cu_seqlens int32 [B + 1]: sequence b owns tokens [cu[b], cu[b + 1]); NULL: N == B and
  *      token b belongs to sequence b (a decode step)
@@ -324,7 +324,7 @@ int spd_paged_decode_attn_int4_err(const void* q, const void* pool, const int32_
 
 /* Attention of whole packed prompts on the tensor cores (dtype F16 or BF16):
  *   q [Nq][Hq][D], k and v [Nk][Hkv][D] with token and head strides in elements, D contiguous;
- *   out [Nq][Hq][D] contiguous.  Sequence b owns queries [cu_q[b], cu_q[b + 1]) and keys
+ *   out [Nq][Hq][D] contiguous, apart from k and v (q itself may be the output).  Sequence b owns queries [cu_q[b], cu_q[b + 1]) and keys
  *   [cu_k[b], cu_k[b + 1]); with causal != 0 its query i sees keys j <= i + Tk - Tq (the
  *   keys of a cached prefix come first).  A query that sees no key gives zeros.  Rows of out
  *   that belong to no sequence are untouched.

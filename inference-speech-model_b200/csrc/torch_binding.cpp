@@ -126,6 +126,11 @@ bool overlap(const at::Tensor& a, const at::Tensor& b) {
   return x.first < y.second && y.first < x.second;
 }
 
+// `out` (contiguous, of q's shape) over some of q, but not over each of its elements in its place
+bool partly_over(const at::Tensor& q, const at::Tensor& out) {
+  return overlap(q, out) && !(q.const_data_ptr() == out.const_data_ptr() && q.is_contiguous());
+}
+
 void error_word(const char* name, const at::Tensor& t) {
   if (t.defined() && (t.scalar_type() != at::kInt || t.numel() < 1)) refuse(name, "error_word must be an int32 tensor");
 }
@@ -199,8 +204,9 @@ at::Tensor rope_append(const char* name, bool int4, PyObject* const* a, Py_ssize
     Hq = small_int(name, "Hq", q.size(1));
     qs = token_strides(name, "q", q);
     if (!given.defined()) out = at::empty(q.sizes(), q.options());
-    else if (given.sizes() != q.sizes() || given.scalar_type() != q.scalar_type() || !given.is_contiguous() || overlap(q, given))
-      refuse(name, "q_out must be a contiguous ", shape_of(q), " tensor of q's dtype apart from q");
+    else if (given.sizes() != q.sizes() || given.scalar_type() != q.scalar_type() || !given.is_contiguous() ||
+             overlap(q, given) || overlap(k, given) || overlap(v, given))
+      refuse(name, "q_out must be a contiguous ", shape_of(q), " tensor of q's dtype apart from q, k and v");
     else out = given;
   } else if (given.defined()) {
     refuse(name, "q_out without q");
@@ -263,6 +269,7 @@ std::pair<at::Tensor, at::Tensor> gather(const char* name, PyObject* const* a, P
   } else {
     k = output(k_given);
     v = output(v_given);
+    if (overlap(k, v)) refuse(name, "k_out and v_out overlap");
   }
   check(f_gather(ptr(pool), static_cast<const int32_t*>(ptr(tables)), static_cast<const int32_t*>(ptr(cu)),
                  static_cast<const int32_t*>(ptr(starts)), mut(k), mut(v), N, small_int(name, "B", B), Hkv, D, bs, max_blocks,
@@ -331,6 +338,7 @@ at::Tensor decode(const char* name, PyObject* const* a, Py_ssize_t n_args) {
   int32_vector(name, "context_lens", lens, B);
   if (given.defined() && (given.sizes() != q.sizes() || given.scalar_type() != q.scalar_type() || !given.is_contiguous()))
     refuse(name, "out must be a contiguous ", shape_of(q), " tensor of q's dtype");
+  if (given.defined() && partly_over(q, given)) refuse(name, "out must be apart from q, or q itself");
   error_word(name, err);
   const int code = dtype_code(name, q.scalar_type());
   const double scale = PyFloat_AsDouble(a[4]);
@@ -373,6 +381,9 @@ at::Tensor prompt(const char* name, PyObject* const* a, Py_ssize_t n_args) {
   int32_vector(name, "cu_seqlens_k", cu_k, B + 1);
   if (given.defined() && (given.sizes() != q.sizes() || given.scalar_type() != q.scalar_type() || !given.is_contiguous()))
     refuse(name, "out must be a contiguous ", shape_of(q), " tensor of q's dtype");
+  // in place of q itself a CTA writes only rows that no other reads
+  if (given.defined() && (overlap(k, given) || overlap(v, given) || partly_over(q, given)))
+    refuse(name, "out must be apart from k and v, and from q unless it is q itself");
   error_word(name, err);
   const double scale = PyFloat_AsDouble(a[6]);
   if (PyErr_Occurred()) {

@@ -569,6 +569,8 @@ def prompt_attention(
     strides, D contiguous; cu_seqlens_q / cu_seqlens_k int32 [B + 1] (keys default to the
     queries' lengths).  With ``causal`` query i of a sequence sees the keys j <= i + Tk - Tq, so
     keys of a cached prefix come first; a query that sees no key gives zeros.  Rows that belong
-    to no sequence are left as they are in ``out``.  Returns out [Nq, Hq, D]."""
+    to no sequence are left as they are in ``out``, which may be q itself but lies apart from k
+    and v.  A wait that runs out is flagged in ``error_word`` (int32); without one it goes unreported.
+    Returns out [Nq, Hq, D]."""
     return N.binding().prompt_attention(q, k, v, cu_seqlens_q, cu_seqlens_k, causal,
                                         q.shape[-1] ** -0.5 if scale is None else scale, out, error_word)
