@@ -81,7 +81,7 @@ int spd_get_last_error(char* buf, size_t size);
 
 /* Number of bytes of workspace the attention kernels need.  The workspace holds a
  * 256-byte header (device error word at offset 0, work counters), arrival counters and
- * fp32 split-KV partial results.  It must be zero-filled once before first use; the
+ * fp32 split-KV partial results.  It starts on a 16-byte boundary and must be zero-filled once before first use; the
  * kernels leave every counter back at zero, so it can be reused by later calls with the
  * same geometry on the same stream.  A workspace used with another geometry must be
  * zero-filled again first; calls that overlap on the GPU must use separate workspaces.

@@ -228,6 +228,7 @@ int spd_paged_decode_attn(const void* q, void* k_pool, void* v_pool, const int32
   const int rc0 = spd::paged_decode_attn_check(q, k_pool, v_pool, block_tables, context_lens, out, B, H, D,
                                                block_size, max_blocks, num_blocks, dtype, k_new, v_new);
   if (rc0 != SPD_OK) return rc0;
+  if (!aligned16(workspace)) return fail(SPD_ERR_INVALID_ARG, "spd_paged_decode_attn: workspace must be 16-byte aligned");
   const size_t need = spd_paged_decode_attn_workspace_size(B, H, D, max_blocks, -1);
   if (!workspace || workspace_bytes < need)
     return fail(SPD_ERR_WORKSPACE, "spd_paged_decode_attn: workspace %zu bytes, need %zu", workspace_bytes, need);
@@ -267,6 +268,7 @@ int spd_cross_attn(const void* q, const void* k, const void* v, const int32_t* v
   if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out) || (kv_batch_stride * eb) % 16 ||
       (kv_head_stride * eb) % 16)
     return fail(SPD_ERR_INVALID_ARG, "spd_cross_attn: pointers and strides must be 16-byte aligned");
+  if (!aligned16(workspace)) return fail(SPD_ERR_INVALID_ARG, "spd_cross_attn: workspace must be 16-byte aligned");
   const size_t need = spd_cross_attn_workspace_size(B, H, D, -1);
   if (!workspace || workspace_bytes < need)
     return fail(SPD_ERR_WORKSPACE, "spd_cross_attn: workspace %zu bytes, need %zu", workspace_bytes, need);
@@ -537,8 +539,8 @@ int spd_paged_decode_attn_int4_err(const void* q, const void* pool, const int32_
       max_ctx > INT32_MAX)
     return fail(SPD_ERR_INVALID_ARG, "spd_paged_decode_attn_int4: bad sizes B=%d Hq=%d Hkv=%d max_blocks=%d", B, Hq, Hkv,
                 max_blocks);
-  if (!aligned16(q) || !aligned16(pool) || !aligned16(out))
-    return fail(SPD_ERR_INVALID_ARG, "spd_paged_decode_attn_int4: tensors must be 16-byte aligned");
+  if (!aligned16(q) || !aligned16(pool) || !aligned16(out) || !aligned16(workspace))
+    return fail(SPD_ERR_INVALID_ARG, "spd_paged_decode_attn_int4: tensors and the workspace must be 16-byte aligned");
   const size_t need = spd_paged_decode_attn_int4_workspace_size(B, Hq, Hkv, D, block_size, max_blocks, dtype, -1);
   if (!workspace || workspace_bytes < need || need == 0)
     return fail(SPD_ERR_WORKSPACE, "spd_paged_decode_attn_int4: workspace %zu bytes, need %zu", workspace_bytes, need);
