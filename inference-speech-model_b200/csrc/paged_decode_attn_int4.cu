@@ -155,7 +155,8 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<P>()) decode_int4_kernel
     return;
   }
   // the sequence's own chunks: as many as there are CTAs for it, but of `least` tokens or more
-  const int size = max(p.least, ((ctx + p.chunks - 1) / p.chunks + kStep - 1) / kStep * kStep);
+  // (unsigned: contexts reach 2^31 - 1)
+  const int size = max(p.least, (int)((((unsigned)ctx + p.chunks - 1) / p.chunks + kStep - 1) / kStep * kStep));
   const long long first = (long long)chunk * size;
   if (first >= ctx) return;
   const int t0 = (int)first;
