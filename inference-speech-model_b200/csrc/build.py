@@ -54,15 +54,20 @@ def _stale(obj: Path, deps: list[Path]) -> bool:
 
 
 def build_binding(force: bool = False) -> Path:
-    """Compiles torch_binding.cpp (no kernels) into ``../lib/spd_torch.so``."""
+    """Compiles torch_binding.cpp (no kernels) into ``../lib/spd_torch.so``, again when it, the C header or the
+    installed torch or Python is another than it was built for."""
     import sysconfig
 
     import torch
 
-    src = HERE / "torch_binding.cpp"
-    if not force and not _stale(BINDING, [src, REPO / "include" / "spd_b200.h"]):
+    src, built_for = HERE / "torch_binding.cpp", OBJ_DIR / "spd_torch.for"
+    present = f"torch {torch.__version__}, Python {sys.version}"
+    if (not force and not _stale(BINDING, [src, REPO / "include" / "spd_b200.h"]) and built_for.exists()
+            and built_for.read_text() == present):
         return BINDING
-    BINDING.parent.mkdir(parents=True, exist_ok=True)
+    for d in (BINDING.parent, OBJ_DIR):
+        d.mkdir(parents=True, exist_ok=True)
+    BINDING.unlink(missing_ok=True)  # one that no longer fits must not be loaded if this fails
     root = Path(torch.__file__).resolve().parent
     cuda = Path(nvcc()).resolve().parent.parent
     cmd = [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden",
@@ -75,6 +80,7 @@ def build_binding(force: bool = False) -> Path:
     if r.returncode != 0:
         sys.stderr.write(r.stdout + r.stderr)
         raise RuntimeError("g++ failed for: torch_binding.cpp")
+    built_for.write_text(present)
     return BINDING
 
 
@@ -104,8 +110,6 @@ def build(verbose: bool = False, force: bool = False, trace: bool = False) -> Pa
                 sys.stderr.write(r.stdout + r.stderr)
             if r.returncode != 0:
                 failed.append(src.name)
-    if binding is not None:
-        binding.result()
     if failed:
         raise RuntimeError(f"nvcc failed for: {', '.join(failed)}")
     objs = [obj_dir / (s.stem + ".o") for s in sources]
@@ -115,6 +119,8 @@ def build(verbose: bool = False, force: bool = False, trace: bool = False) -> Pa
         if r.returncode != 0:
             sys.stderr.write(r.stdout + r.stderr)
             raise RuntimeError(f"linking {lib.name} failed")
+    if binding is not None:
+        binding.result()  # raises if it failed; the operators that do without it have their library all the same
     return lib
 
 

@@ -112,8 +112,12 @@ def binding():
             "`python inference-speech-model_b200/csrc/build.py` (there is no other path)"
         )
     loader = importlib.machinery.ExtensionFileLoader("spd_torch", str(BINDING_PATH))
-    module = importlib.util.module_from_spec(importlib.util.spec_from_loader("spd_torch", loader))
-    loader.exec_module(module)
+    try:
+        module = importlib.util.module_from_spec(importlib.util.spec_from_loader("spd_torch", loader))
+        loader.exec_module(module)
+    except ImportError as e:  # built for another torch or Python
+        raise RuntimeError(f"{BINDING_PATH} does not load ({e}); build it again with "
+                           "`python inference-speech-model_b200/csrc/build.py`") from e
     module.setup({name: C.cast(getattr(lib, name), C.c_void_p).value for name in _SIGNATURES})
     _binding = module
     return module
