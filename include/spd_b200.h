@@ -328,9 +328,8 @@ int spd_paged_decode_attn_int4_err(const void* q, const void* pool, const int32_
  *   [cu_k[b], cu_k[b + 1]); with causal != 0 its query i sees keys j <= i + Tk - Tq (the
  *   keys of a cached prefix come first).  A query that sees no key gives zeros.  Rows of out
  *   that belong to no sequence are untouched.
- * fp32 scores, softmax statistics and accumulation; the weights are rounded to dtype.  Other
- * sequences' values never reach a result, but within a sequence a non-finite v may turn
- * earlier queries of the same 128-key step non-finite.
+ * fp32 scores, softmax statistics and accumulation; the weights are rounded to dtype.  A key that a
+ * query does not see never reaches its result, whatever it and its value hold.
  * Requires D % 8 == 0, D <= 128, scale > 0, Hq a multiple of Hkv, 16-byte aligned pointers and
  * strides.  error_word: optional int32 device word receiving SPD_DEVERR_TIMEOUT. */
 int spd_prompt_attn(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k, int64_t k_stride_t,

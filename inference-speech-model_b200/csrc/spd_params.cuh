@@ -132,6 +132,8 @@ struct GatherInt4Params {  // tokens of a 4-bit pool back as packed k, v (rope_k
 
 struct PromptParams {  // attention of packed prompts (prompt_attn.cu)
   void* out;          // [Nq][Hq][D]
+  const void* v;      // [Nk][Hkv][D], by token and head strides (elements)
+  long long v_st, v_sh;
   const int* cu_q;    // [B + 1]
   const int* cu_k;    // [B + 1]
   int Nq, Nk, B, Hq, Hkv, D, causal;
