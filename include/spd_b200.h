@@ -1,8 +1,9 @@
 /*
  * spd_b200.h — C ABI of the B200 (sm_100a) speech-decode hot path.
  *
- * One shared library (libspd_b200.so) exports the five decode-path operations of the
- * Whisper-class serving engine plus error/workspace helpers.  Every entry point:
+ * One shared library (libspd_b200.so) exports the decode-path operations of the Whisper-class
+ * serving engine, those of decoders with rotary positions, grouped heads and a 4-bit cache, and
+ * error/workspace helpers.  Every entry point:
  *   - takes plain device pointers, sizes and a cudaStream_t passed as `void*`
  *     (NULL = legacy default stream); no torch types cross this boundary;
  *   - returns an int status (SPD_OK == 0); on failure spd_get_last_error() gives text;
@@ -288,7 +289,8 @@ int spd_rope_kv_append(const void* q, int64_t q_stride_t, int64_t q_stride_h, co
 /* The same into a 4-bit pool.  Each token's 64 consecutive dimensions of a head share
  *   scale = fp16((max - min) / 15), zero = fp16(min), saturated to the fp16 range;
  *   code = clamp(rint((x - zero) / scale), 0, 15), 0 where scale is 0,
- * of the fp32 rotated keys and of v.  A NaN makes its 64 values NaN. */
+ * of the fp32 rotated keys and of v.  A NaN makes its 64 values NaN, and so do 64 equal infinities,
+ * whose max - min is one. */
 int spd_rope_kv_append_int4(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k, int64_t k_stride_t,
                             int64_t k_stride_h, const void* v, int64_t v_stride_t, int64_t v_stride_h, void* q_out,
                             const float* cos_table, const float* sin_table, void* pool, const int32_t* block_tables,

@@ -18,8 +18,9 @@
 //   single-token shapes, and tcgen05 (128 rows, operands through shared memory) would have
 //   to write the unpacked codes back to shared memory first.
 // * fp16 holds the query scaled by a power of two to below 2^11, and the weights p * scale_t
-//   scaled by a running power of two to below 2^15: neither overflows, and what underflows
-//   is below 2^-20 of the largest.  With up to four heads per tile (and for fp32 queries)
+//   scaled by a running power of two to below 2^15: neither overflows, and the last bit of
+//   what falls below fp16's normal numbers is 2^-30 of a weight of 1 at the largest value scale
+//   met so far.  With up to four heads per tile (and for fp32 queries)
 //   each head takes two columns, the value and its rounding remainder, so q and p keep 22
 //   bits; with more, q keeps 11 bits (exact for fp16 and bf16 queries) and p 11.
 //

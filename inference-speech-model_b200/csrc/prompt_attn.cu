@@ -29,9 +29,9 @@
 //   sequence's last key to zero in shared memory before they are multiplied, and, among keys that some
 //   rows of the CTA do not see, every element that is not finite; rows that do see such a key add it
 //   at the end.  What another sequence or a later key holds never reaches a result.  The tile is
-//   handed to warp 2 a step ahead, so that its look (one multiply-add a pair) is mostly over in time.
-//   Without the look the 8192 tokens below take 0.7 % less, ragged grouped prompts 2.4 % (a third of
-//   their steps), the 8 x 1500 0.8 % (none of its steps: the code alone).
+//   handed to warp 2 a step ahead, so that its look (one multiply-add a pair) is mostly over in time
+//   (graphs of the calls below with it and without: short prompts 10.6 and 10.2 us, the 8 x 1500, where
+//   it looks at nothing, 145.0 and 142.8, ragged grouped prompts the same).
 // * Steps are of 128 keys with one CTA an SM; at D <= 64, where TMEM holds four tiles, of 64 keys
 //   with two CTAs an SM, unless no SM gets a second item.
 // * One CTA is launched for each item (tile pair and head group), ranked by length; a running CTA
@@ -504,6 +504,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<DP, BN>::kCtas)
   __shared__ Item items[kItems];
   __shared__ __align__(16) unsigned char response[16];
   __shared__ __align__(8) uint64_t item_wanted, asked;
+  __shared__ int gave_up;    // a wait has run out
+  __shared__ int left[4];    // the loader's place in its ring, and how often it loaded each Q tile, at its end
   __shared__ int odd_v;      // warp 2 has set elements of V to zero that are not finite
   __shared__ int stored[8];  // then: items whose rows each softmax warp has stored
   __shared__ __align__(8) uint64_t item_full[kItems], item_empty[kItems];
@@ -527,7 +529,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<DP, BN>::kCtas)
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (warp == 1) tmem_alloc(tmem_slot, C::kTmemCols);
   if (tid == 0) {
-    odd_v = 0;
+    gave_up = odd_v = 0;
     for (int i = 0; i < 8; ++i) stored[i] = 0;
     for (int s = 0; s < C::kStages; ++s) {
       mbar_init(&kv_full[s], 1);
@@ -609,16 +611,13 @@ __global__ void __launch_bounds__(kThreads, Cfg<DP, BN>::kCtas)
         }
         ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
       }
-      // Let the copies in flight land before the CTA can exit, whichever warp gave up: after its last load
-      // this one waits for nothing that tells it that another has.  (At once otherwise.)
       if (lane == 0) {
-        for (int k = 0; k < C::kStages; ++k) {
-          ring.back(C::kStages);
-          if (ring.round >= 0) (void)mbar_wait_suspend(&kv_full[ring.slot], ring.phase(), nullptr);
-        }
-        for (int x = 0; x < 2; ++x)
-          if (q_use[x]) (void)mbar_wait_suspend(&q_full[x], (uint32_t)((q_use[x] - 1) & 1), nullptr);
+        left[0] = ring.slot;
+        left[1] = ring.round;
+        left[2] = q_use[0];
+        left[3] = q_use[1];
       }
+      if (!ok) gave_up = 1;
     } else if (warp == 1) {
       // ---- MMA issuer: one lane, with nothing but waits and issues in its step -----------------
       constexpr uint32_t idesc_s = instr_desc_f16(kBf16, BM, BN);
@@ -713,6 +712,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<DP, BN>::kCtas)
         __syncwarp();
         ok = __shfl_sync(0xffffffffu, (int)ok, leader_lane) != 0;
       }
+      if (!ok) gave_up = 1;
       if (leader) umma_commit(done);
       __syncwarp();
       (void)mbar_wait_suspend(done, 0, p.err);
@@ -802,6 +802,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<DP, BN>::kCtas)
           __syncwarp();
         }
       }
+      if (!ok) gave_up = 1;
     } else {
       // ---- this CTA's items, found ahead of their use: its own, then those of CTAs that have not
       // started, whose launch it calls off
@@ -835,6 +836,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<DP, BN>::kCtas)
         }
         if (!w.there) break;
       }
+      if (!ok) gave_up = 1;
     }
   } else {
     // ---- softmax and epilogue of tile x: thread = query row = TMEM lane --------------------
@@ -978,7 +980,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<DP, BN>::kCtas)
         __syncwarp();
         if (lane == 0) {
           mbar_arrive(&o_empty[x]);
-          if (*(volatile int*)&odd_v)  // set before this item's products were issued, if by it
+          if (p.causal && *(volatile int*)&odd_v)  // set before this item's products were issued, if by it
             asm volatile("st.release.cta.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&stored[warp - 4])), "r"(it + 1)
                          : "memory");
         }
@@ -986,9 +988,23 @@ __global__ void __launch_bounds__(kThreads, Cfg<DP, BN>::kCtas)
         for (int c = 0; c < p.D; c += 8) *reinterpret_cast<uint4*>(out + c) = make_uint4(0, 0, 0, 0);
       }
     }
+    if (!ok) gave_up = 1;
   }
   tc_fence_before();
   __syncthreads();
+  if (gave_up) {
+    // Some warp gave up, perhaps on a copy that is still in flight: all land before the CTA exits.
+    if (tid == 0) {
+      Ring ring{left[0], left[1]};
+      for (int k = 0; k < C::kStages; ++k) {
+        ring.back(C::kStages);
+        if (ring.round >= 0) (void)mbar_wait_suspend(&kv_full[ring.slot], ring.phase(), nullptr);
+      }
+      for (int x = 0; x < 2; ++x)
+        if (left[2 + x]) (void)mbar_wait_suspend(&q_full[x], (uint32_t)((left[2 + x] - 1) & 1), nullptr);
+    }
+    __syncthreads();
+  }
   tc_fence_after();
   if (warp == 1) tmem_dealloc(tmem, C::kTmemCols);
 }

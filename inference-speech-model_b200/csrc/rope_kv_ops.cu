@@ -14,7 +14,8 @@
 //   scale = fp16((max - min) / 15),  zero = fp16(min)      (saturated to the fp16 range)
 //   code  = clamp(rint((x - zero) / scale), 0, 15),        0 where scale is 0
 // computed from the fp32 rotated keys (no rounding to the model's type in between).  A NaN
-// makes its 64 values NaN (through the parameters); an infinity saturates.
+// makes its 64 values NaN (through the parameters), as 64 equal infinities do (max - min is one);
+// an infinity among others saturates.
 //
 // What bounds them: HBM for prompts, since each value is read once and written once (a 4-bit row as
 // 4.5 bits per value) and the rotation is a few operations; the latency of a few dependent loads

@@ -1,8 +1,8 @@
 """Torch-tensor front end of the decode-path kernels (C ABI in include/spd_b200.h).
 
-Each function checks shapes, dtypes, devices and strides, then calls the extension
-through ctypes on ``torch.cuda.current_stream()`` (the capture stream inside
-``torch.cuda.graph``).  Nothing here synchronises or reads device values, so every op
+Each function checks shapes, dtypes, devices and strides, then calls the extension on
+``torch.cuda.current_stream()`` (the capture stream inside ``torch.cuda.graph``): the
+engine's ops through ctypes, the last five below through the torch binding.  Nothing here synchronises or reads device values, so every op
 can be captured in a CUDA graph.  CPU tensors raise ``RuntimeError``: the product path
 has no CPU implementation.
 
