@@ -30,10 +30,13 @@
 // is raised only when a score passes it by 8 (p <= 2^8).  The warps are joined in shared memory, the
 // chunks of a (sequence, head tile) by the last CTA to arrive, which adds them in their order: the
 // result does not depend on who that is.
-// Measured: 32 contexts of 1,000 to 32,000 tokens, 32/8 heads of 128, bf16 (582 MB of pool): 126 us,
-// 4.6 TB/s, 0.70 of a plain copy's rate.  Copies alone take 108 us in this form, the arithmetic alone
-// 125: the two share the SM's issue slots.  128 contexts of up to 3,900, 12 heads of 64: 66 us; one
-// of 32,000: 17.5 us; one of 448: 5.3 us, most of it the latency of table, page and join.
+// Measured in replayed graphs: 32 contexts of 1,000 to 32,000 tokens, 32/8 heads of 128, bf16 (582 MB of
+// pool): 129 us, 4.5 TB/s, 0.69 of a plain copy's rate (a lone call 140); copies alone took 108 us, the
+// arithmetic alone 125.  No pipe and no issue slots are full (48 % of either): at three warps a scheduler,
+// which is what registers allow, the arithmetic waits for its own fixed latencies and its loads.
+// 128 contexts of up to 3,900, 12 heads of 64: 66 us; one of 32,000: 17.5 us; one of 448: 5.1 us, most
+// of it the latency of table, page and join.  (Comparisons below are of the forms of their time, before
+// pages could be left out.)
 #include "spd_int4.cuh"
 #include "spd_params.cuh"
 

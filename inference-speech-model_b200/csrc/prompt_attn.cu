@@ -24,7 +24,8 @@
 //   only when a score passes it by 8 (in log2), so O in TMEM is rescaled rarely; P is at most
 //   2^8 and rounded to the input type (its 8 or 11 bits are what the tensor core takes), the row
 //   sum is taken in fp32 before the rounding.  A quarter of the exponentials is a polynomial on
-//   the fp32 pipes.
+//   the fp32 pipes.  (Both the lazy maximum and the polynomial are published techniques of
+//   attention kernels on this architecture.)
 // * Where a key does not count its weight is zero, but 0 * NaN is not.  So warp 2 sets rows of V past a
 //   sequence's last key to zero in shared memory before they are multiplied, and, among keys that some
 //   rows of the CTA do not see, every element that is not finite; rows that do see such a key add it
@@ -39,13 +40,15 @@
 //   follow one another in it without a gap and the longest come first.  Every wait is bounded, and
 //   waits suspend the thread, which leaves the issue slots to the softmax warps.
 //
-// Measured (bf16, 32 query and 8 key/value heads of 128, causal): 8192 tokens 450 us, 1.22 PFLOP/s,
-// 0.75 of the library product's rate in a short run; 4 x 4096 tokens, 16 heads, not causal 1.16.  A
+// Measured in replayed graphs (bf16, 32 query and 8 key/value heads of 128, causal): 8192 tokens 450 us in
+// the first 60 ms of replays, at 1,965 MHz, 1.22 PFLOP/s and 0.75 of the library product's rate in a
+// short run; 507 us from then on, under the power cap at 1.6 to 1.7 GHz; a lone call 523 us.  A
 // step of 128 keys of both tiles takes about 3,250 cycles against 2,050 of products: a tile's chain
 // (scores, their maximum, 128 exponentials a thread, weights, P V, next scores) is 1.5 times as long
-// as the other tile's products can cover.  fp16, 20 heads of 64, 8 x 1500 tokens, not causal: 143 us,
-// 0.64 PFLOP/s, where exponentials alone take 63 to 84.  64 keys and two CTAs against 128 and one at D = 64:
-// 143 against 166 us there, 202 against 224 for 4 x 4096 causal tokens of 16 heads, but 11.5 against
+// as the other tile's products can cover.  fp16, 20 heads of 64, 8 x 1500 tokens, not causal: 145 us,
+// 0.64 PFLOP/s, where exponentials alone take 63 to 84.  The figures below compared forms when each was
+// chosen, in short runs; the later one's present time may be another.  64 keys and two CTAs against 128 and
+// one at D = 64: 143 against 166 us there, 202 against 224 for 4 x 4096 causal tokens of 16 heads, but 11.5 against
 // 10.3 for 6 short prompts of 12 heads, one item an SM at most.  Items dealt out in fixed turns instead of taken
 // over: 147 (forwards) and 163 us (forwards and backwards) for the 8 x 1500, 215 and 210 for the 4 x
 // 4096.  Slower at D = 128: steps of 64 keys with two score buffers a tile, so that scores are there
@@ -282,9 +285,9 @@ __device__ __forceinline__ float2 exp2_poly(f32x2 x) {
 constexpr int kPoly = 2;  // of 8 pairs, to the polynomial
 // Weights of 2 * PAIRS keys: p = 2^(s * c - m) rounded to T and packed, sums added.  EXACT: all on the
 // special-function unit, so that a masked score (-inf) gives an exact zero and a NaN a NaN; otherwise kPoly of
-// each 8 pairs go to the polynomial (with items dealt out in fixed turns 0: 493 us, 1: 485, 2: 484, 4:
-// 496 for the 8192 tokens above, and 170, 164 and 163 us of 0, 1 and 2 for the 8 x 1500: the
-// polynomial's six packed fp32 instructions soon cost more than they free).
+// each 8 pairs go to the polynomial (0: 151 us, 1: 146, 2: 145, 4: 162 for the 8 x 1500 above, and 516,
+// 518, 519 and 532 in long runs of the 8192 tokens, 493, 485, 484 and 496 of an earlier form in short
+// ones: the polynomial's six packed fp32 instructions soon cost more than they free).
 template <typename T, bool EXACT, int PAIRS>
 __device__ __forceinline__ void weights(const uint32_t* s, f32x2 c, f32x2 neg_m, uint32_t* pk, f32x2 (&sum)[2]) {
   constexpr int kDeg = std::is_same<T, __half>::value ? 4 : 3;

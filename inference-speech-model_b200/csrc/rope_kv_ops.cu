@@ -21,11 +21,12 @@
 // 4.5 bits per value) and the rotation is a few operations; the latency of a few dependent loads
 // (sequence, table, row) for a decode step.  So a CTA looks up the places of its tokens once, a thread
 // keeps its dimensions for all of them, and for few tokens a CTA takes one.
-// Measured: a step's 64 tokens, 12 heads of 64, fp16: 2.8 us; 16 prompts of 200 to 2,000 tokens, 32/8
-// heads of 128, bf16 (468 MB): 87 us, 5.4 TB/s, 0.82 of a plain copy's rate.  Into 4 bits, 7 prompts
-// of up to 4,001 tokens, 16/8 heads of 128 (199 MB): 55 us, 3.6 TB/s, by then bounded by the latency and
-// issue of the groups' exchanges and parameters.  16 prefixes of 1,000 to 8,000 tokens out of 4 bits,
-// 8 heads of 128 (390 MB): 64 us, 6.1 TB/s.
+// Measured in replayed graphs (a lone call in brackets): a step's 64 tokens, 12 heads of 64, fp16: 2.8 us
+// (5.7); 16 prompts of 200 to 2,000 tokens, 32/8 heads of 128, bf16 (468 MB): 87 us (94), 5.4 TB/s, 0.82
+// of a plain copy's rate.  Into 4 bits, 7 prompts of up to 4,001 tokens, 16/8 heads of 128 (199 MB): 55 us,
+// 3.6 TB/s: the groups' exchanges and parameters are a chain that 28 warps an SM do not cover (66 % of the
+// issue slots, no pipe full).  16 prefixes of 1,000 to 8,000 tokens out of 4 bits, 8 heads of 128
+// (390 MB): 63 us (69), 6.1 TB/s.
 #include "spd_int4.cuh"
 #include "spd_params.cuh"
 
