@@ -786,22 +786,26 @@ __global__ void __launch_bounds__(kThreads, Cfg<DP, BN>::kCtas)
             }
           }
           if (!ok) break;
-          const int last = min(w.Tq, w.tok0 + 2 * BM / p.pack), off = w.Tk - w.Tq;
+          // A lane takes every 32nd dimension; along the rows the keys seen only grow.
+          const int last = min(w.Tq, w.tok0 + 2 * BM / p.pack), cleared = min(w.Tk, n * BN);
 #pragma unroll 1
-          for (int key = all; key < min(w.Tk, n * BN); ++key)
+          for (int d = lane; d < p.D; d += 32) {
+            const T* v = reinterpret_cast<const T*>(p.v) + w.k0 * p.v_st + w.kvh * p.v_sh + d;
+            float sum = 0.f;
+            int key = all;
 #pragma unroll 1
-            for (int d = lane; d < p.D; d += 32) {
-              const float f = Elem<T>::to_f(
-                  reinterpret_cast<const T*>(p.v)[(w.k0 + key) * p.v_st + w.kvh * p.v_sh + d]);
-              if (fabsf(f) < INFINITY) continue;
+            for (int t = w.tok0; t < last; ++t) {
 #pragma unroll 1
-              for (int t = max(w.tok0, key - off); t < last; ++t)
+              for (; key < min(cleared, t + 1 + w.Tk - w.Tq); ++key) {
+                const float f = Elem<T>::to_f(v[key * p.v_st]);
+                if (!(fabsf(f) < INFINITY)) sum += f;
+              }
+              if (sum == 0.f) continue;
+              T* o = reinterpret_cast<T*>(p.out) + ((long long)(w.q0 + t) * p.Hq + w.h0) * p.D + d;
 #pragma unroll 1
-                for (int h = w.h0; h < w.h0 + p.pack; ++h) {
-                  T* o = reinterpret_cast<T*>(p.out) + ((long long)(w.q0 + t) * p.Hq + h) * p.D + d;
-                  *o = Elem<T>::from_f(Elem<T>::to_f(*o) + f);
-                }
+              for (int h = 0; h < p.pack; ++h, o += p.D) *o = Elem<T>::from_f(Elem<T>::to_f(*o) + sum);
             }
+          }
           __syncwarp();
         }
       }

@@ -89,3 +89,23 @@ def test_and_where_a_cta_takes_several_items(heads, D):
     check_bad_values(lens, lens, heads, heads, D, torch.float16, at, 7, rows=((790, 1303), (790, 1303)))
     got = check_bad_values(lens, lens, heads, heads, D, torch.float16, at, 8, rows=((1303, 1603), (1303, 1603)))
     assert torch.isfinite(got).all()
+
+
+@pytest.mark.parametrize("value", [NAN, INF], ids=str)
+def test_nothing_but_bad_values_costs_no_multiple(value):
+    """A batch whose v holds nothing finite (a model that has diverged): the repairs are a few milliseconds."""
+    lens = [2000, 700, 3000]
+    n = sum(lens)
+    q, k, v = (t.to(DEV) for t in make(9, n, n, 16, 4, 128, torch.bfloat16))
+    word = torch.zeros(1, dtype=torch.int32, device=DEV)
+    bad = torch.full_like(v, value)
+    c = cu(lens).to(DEV)
+    ops.prompt_attention(q, k, bad, c)
+    start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    start.record()
+    got = ops.prompt_attention(q, k, bad, c, error_word=word)
+    end.record()
+    end.synchronize()
+    assert ops.read_error_word(word) == 0 and not torch.isfinite(got).any()
+    print(f"{start.elapsed_time(end):.2f} ms")
+    assert start.elapsed_time(end) < 100
