@@ -31,8 +31,8 @@
 //   rows of the CTA do not see, every element that is not finite; rows that do see such a key add it
 //   at the end.  What another sequence or a later key holds never reaches a result.  The tile is
 //   handed to warp 2 a step ahead, so that its look (one multiply-add a pair) is mostly over in time
-//   (graphs of the calls below with it and without: short prompts 10.6 and 10.2 us, the 8 x 1500, where
-//   it looks at nothing, 145.0 and 142.8, ragged grouped prompts the same).
+//   (graphs of the calls below with it and without: short prompts 10.4 and 10.2 us, the 8 x 1500, where
+//   it looks at nothing, 147 and 143, ragged grouped prompts the same).
 // * Steps are of 128 keys with one CTA an SM; at D <= 64, where TMEM holds four tiles, of 64 keys
 //   with two CTAs an SM, unless no SM gets a second item.
 // * One CTA is launched for each item (tile pair and head group), ranked by length; a running CTA
@@ -45,8 +45,8 @@
 // short run; 507 us from then on, under the power cap at 1.6 to 1.7 GHz; a lone call 523 us.  A
 // step of 128 keys of both tiles takes about 3,250 cycles against 2,050 of products: a tile's chain
 // (scores, their maximum, 128 exponentials a thread, weights, P V, next scores) is 1.5 times as long
-// as the other tile's products can cover.  fp16, 20 heads of 64, 8 x 1500 tokens, not causal: 145 us,
-// 0.64 PFLOP/s, where exponentials alone take 63 to 84.  The figures below compared forms when each was
+// as the other tile's products can cover.  fp16, 20 heads of 64, 8 x 1500 tokens, not causal: 147 us,
+// 0.63 PFLOP/s, where exponentials alone take 63 to 84.  The figures below compared forms when each was
 // chosen, in short runs; the later one's present time may be another.  64 keys and two CTAs against 128 and
 // one at D = 64: 143 against 166 us there, 202 against 224 for 4 x 4096 causal tokens of 16 heads, but 11.5 against
 // 10.3 for 6 short prompts of 12 heads, one item an SM at most.  Items dealt out in fixed turns instead of taken
@@ -285,7 +285,7 @@ __device__ __forceinline__ float2 exp2_poly(f32x2 x) {
 constexpr int kPoly = 2;  // of 8 pairs, to the polynomial
 // Weights of 2 * PAIRS keys: p = 2^(s * c - m) rounded to T and packed, sums added.  EXACT: all on the
 // special-function unit, so that a masked score (-inf) gives an exact zero and a NaN a NaN; otherwise kPoly of
-// each 8 pairs go to the polynomial (0: 151 us, 1: 146, 2: 145, 4: 162 for the 8 x 1500 above, and 516,
+// each 8 pairs go to the polynomial (0: 151 us, 1: 146, 2: 145, 4: 162 for the 8 x 1500 when last swept, and 516,
 // 518, 519 and 532 in long runs of the 8192 tokens, 493, 485, 484 and 496 of an earlier form in short
 // ones: the polynomial's six packed fp32 instructions soon cost more than they free).
 template <typename T, bool EXACT, int PAIRS>
