@@ -339,6 +339,50 @@ int spd_prompt_attn(const void* q, int64_t q_stride_t, int64_t q_stride_h, const
                     const int32_t* cu_q, const int32_t* cu_k, int Nq, int Nk, int B, int Hq, int Hkv, int D, int causal,
                     float scale, int dtype, int32_t* error_word, void* stream);
 
+/* ---- several candidates of one request ---------------------------------------------------
+ * Operators for sequences (samples, beams) that share a prompt or an encoder's output.  No counterpart in the
+ * reference, which decodes one greedy sequence a request. */
+
+/* Single-token attention with grouped heads over a paged 16-bit pool (dtype F16 or BF16), for sequences that share
+ * a prefix with their group: sequence b of group g attends the group's prefix, then its own tokens.
+ *   q [B][Hq][D] with token and head strides in elements, D contiguous; out [B][Hq][D] contiguous (q itself may
+ *      be the output); query head h reads key/value head h / (Hq / Hkv)
+ *   k_pool, v_pool [num_blocks][block_size][Hkv][D]
+ *   cu_groups int32 [G + 1]: group g owns sequences [cu[g], cu[g + 1]); a sequence of no group has no prefix
+ *   prefix_tables int32 [G][max_prefix_blocks], prefix_lens int32 [G]: the groups' prefixes; G == 0 or
+ *      max_prefix_blocks == 0: none
+ *   block_tables int32 [B][max_blocks], context_lens int32 [B]: the sequences' own tokens (<= 0: none)
+ *   A sequence without any key gives zeros.  Lengths beyond their table are cut to it (flagged); tokens of a block
+ *   whose id is out of range are left out (flagged).
+ * fp32 scores, softmax statistics and accumulation; weights of prefix keys are rounded to dtype.
+ * Requires D % 8 == 0, D <= 128, block_size 8, 16, 32, 64 or 128, Hq / Hkv <= 128, B <= 65536, scale > 0, 16-byte aligned
+ * pointers and strides.  The workspace's first header and counter bytes are zero-filled once; every call leaves the
+ * counters at zero.  It serves one stream at a time. */
+size_t spd_shared_prefix_attn_workspace_size(int B, int G, int Hq, int Hkv, int D, int block_size,
+                                             int max_prefix_blocks, int max_blocks, int device);
+int spd_shared_prefix_attn(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k_pool, const void* v_pool,
+                           const int32_t* prefix_tables, const int32_t* prefix_lens, const int32_t* cu_groups,
+                           const int32_t* block_tables, const int32_t* context_lens, void* out, int B, int G, int Hq,
+                           int Hkv, int D, int block_size, int max_prefix_blocks, int max_blocks, int num_blocks,
+                           float scale, int dtype, void* workspace, size_t workspace_bytes, int32_t* error_word,
+                           void* stream);
+
+/* Attention of any number of queries a request over the keys and values of the request's slot (dtype F16 or BF16),
+ * without a causal mask: query i of request b attends positions t < valid_lens[b] of slot slot_ids[b].
+ *   q [N][Hq][D] packed, token and head strides in elements; out [N][Hq][D] contiguous (q itself may be the output)
+ *   k, v: element (slot, h, t, d) at slot * kv_stride_slot + h * kv_stride_h + t * kv_stride_t + d; S slots, T positions
+ *   cu_seqlens int32 [B + 1]: request b owns queries [cu[b], cu[b + 1]); NULL: N == B, one query a request
+ *   slot_ids int32 [B], or NULL: slot b.  Two requests may share a slot.
+ *   A query without any key gives zeros; rows of out that belong to no request are untouched.  A length beyond T is
+ *   cut to it (flagged), a slot id out of range leaves its request without keys (flagged).
+ * Requires D % 8 == 0, D <= 128, Hq / Hkv <= 128, scale > 0, 16-byte aligned pointers and strides. */
+size_t spd_cross_attn_packed_workspace_size(int N, int Hq, int Hkv, int D, int device);
+int spd_cross_attn_packed(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k, const void* v,
+                          int64_t kv_stride_slot, int64_t kv_stride_h, int64_t kv_stride_t, const int32_t* valid_lens,
+                          const int32_t* cu_seqlens, const int32_t* slot_ids, void* out, int N, int B, int S, int T, int Hq,
+                          int Hkv, int D, float scale, int dtype, void* workspace, size_t workspace_bytes,
+                          int32_t* error_word, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

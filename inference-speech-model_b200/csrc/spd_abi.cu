@@ -32,6 +32,11 @@ int decode_int4_launch(const DecodeInt4Params& p, int D, int bs, cudaStream_t st
 int prompt_attn_launch(PromptParams p, const void* q, const void* k, const void* v, long long q_st, long long q_sh,
                        long long k_st, long long k_sh, long long v_st, long long v_sh, int dtype, int sms,
                        cudaStream_t st);
+int span_piece_rows(int N, int Gq);
+int span_attn_launch(SpanParams p, const SpanTensors& t, int dtype, int sms, cudaStream_t st);
+int own_attn_tiles(int Hq, int Hkv);
+Int4Split own_attn_split(int B, int Hq, int Hkv, int max_ctx, int sms);
+int own_attn_launch(const OwnParams& p, int dtype, cudaStream_t st);
 }  // namespace spd
 
 namespace {
@@ -110,6 +115,33 @@ int rope_append_check(const char* fn, const spd::RopeAppendParams& p, int dtype)
                         (const void*)p.k_pool, (const void*)p.v_pool})
     if (!aligned16(t)) return fail(SPD_ERR_INVALID_ARG, "%s: tensors must be 16-byte aligned", fn);
   return SPD_OK;
+}
+
+// log2 of a block size of the span kernels (a power of two, 8 to 128), or -1
+int block_log2(int block_size) {
+  for (int l = 3; l <= 7; ++l)
+    if (block_size == 1 << l) return l;
+  return -1;
+}
+
+// The workspace of shared-prefix decode attention: counters behind the header, results at the end.
+struct PrefixSpace {
+  size_t counters, partials, whole, pieces, desc;  // bytes
+  spd::Int4Split split;
+  size_t results() const { return partials + whole + pieces + desc; }
+};
+PrefixSpace prefix_space(int B, int G, int Hq, int Hkv, int D, int max_ctx, int sms) {
+  PrefixSpace s{};
+  const size_t row = (size_t)(D + 4) * 4;
+  s.split = spd::own_attn_split(B, Hq, Hkv, max_ctx, sms);
+  s.counters = spd::round_up((size_t)B * spd::own_attn_tiles(Hq, Hkv) * 4, 256);
+  s.partials = s.split.chunks > 1 ? spd::round_up((size_t)B * Hq * s.split.chunks * row, 256) : 0;
+  if (G > 0) {
+    s.whole = spd::round_up((size_t)B * Hq * row, 256);
+    s.pieces = spd::round_up(2 * (size_t)sms * spd::span_piece_rows(B, Hq / Hkv) * row, 256);
+    s.desc = spd::round_up((size_t)B * Hkv * sizeof(int2), 256);
+  }
+  return s;
 }
 
 bool head_dim_ok(int D) { return D == 16 || D == 32 || D == 64 || D == 128; }
@@ -595,6 +627,142 @@ int spd_prompt_attn(const void* q, int64_t q_stride_t, int64_t q_stride_h, const
   const int rc = spd::prompt_attn_launch(p, q, k, v, q_stride_t, q_stride_h, k_stride_t, k_stride_h, v_stride_t,
                                          v_stride_h, dtype, sms, static_cast<cudaStream_t>(stream));
   if (rc != SPD_OK) return fail(rc, "spd_prompt_attn: launch failed: %s", cudaGetErrorString(cudaGetLastError()));
+  return ok();
+}
+
+size_t spd_shared_prefix_attn_workspace_size(int B, int G, int Hq, int Hkv, int D, int block_size,
+                                             int max_prefix_blocks, int max_blocks, int device) {
+  const int sms = sm_count(device), bl = block_log2(block_size);
+  if (B <= 0 || G < 0 || Hkv <= 0 || Hq <= 0 || Hq % Hkv || Hq / Hkv > 128 || D <= 0 || D % 8 || D > 128 || bl < 0 ||
+      max_blocks < 0 || max_prefix_blocks < 0 || (long long)max_blocks << bl > INT32_MAX || sms <= 0)
+    return 0;
+  const PrefixSpace s = prefix_space(B, max_prefix_blocks ? G : 0, Hq, Hkv, D, max_blocks << bl, sms);
+  return spd::kWsHeaderBytes + s.counters + s.results();
+}
+
+int spd_shared_prefix_attn(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k_pool, const void* v_pool,
+                           const int32_t* prefix_tables, const int32_t* prefix_lens, const int32_t* cu_groups,
+                           const int32_t* block_tables, const int32_t* context_lens, void* out, int B, int G, int Hq,
+                           int Hkv, int D, int block_size, int max_prefix_blocks, int max_blocks, int num_blocks,
+                           float scale, int dtype, void* workspace, size_t workspace_bytes, int32_t* error_word,
+                           void* stream) {
+  if (dtype != SPD_F16 && dtype != SPD_BF16)
+    return fail(SPD_ERR_UNSUPPORTED, "spd_shared_prefix_attn: dtype %d not supported (F16/BF16 only)", dtype);
+  const int bl = block_log2(block_size);
+  if (B < 0 || G < 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || D <= 0 || max_prefix_blocks < 0 || max_blocks < 0 || num_blocks < 0)
+    return fail(SPD_ERR_INVALID_ARG, "spd_shared_prefix_attn: bad sizes B=%d G=%d Hq=%d Hkv=%d D=%d", B, G, Hq, Hkv, D);
+  if (D % 8 || D > 128 || bl < 0 || Hq / Hkv > 128 || Hq > 4096 || B > 65536)
+    return fail(SPD_ERR_UNSUPPORTED,
+                "spd_shared_prefix_attn: need D a multiple of 8 up to 128, block_size 8 to 128 (a power of two), up to 128 "
+                "query heads a key/value head, up to 65536 sequences");
+  if ((long long)max_blocks << bl > INT32_MAX || (long long)max_prefix_blocks << bl > INT32_MAX)
+    return fail(SPD_ERR_UNSUPPORTED, "spd_shared_prefix_attn: tables reach past 2^31 tokens");
+  if (!(scale > 0.f) || scale > 1e30f) return fail(SPD_ERR_INVALID_ARG, "spd_shared_prefix_attn: scale must be positive");
+  if (B == 0) return ok();
+  if (max_prefix_blocks == 0) G = 0;
+  if (!q || !k_pool || !v_pool || !context_lens || !out || (max_blocks && !block_tables) || num_blocks == 0 ||
+      (G && (!prefix_tables || !prefix_lens || !cu_groups)))
+    return fail(SPD_ERR_INVALID_ARG, "spd_shared_prefix_attn: null tensor pointer or empty pool");
+  if (q_stride_t < 0 || q_stride_h < 0 || (q_stride_t * 2) % 16 || (q_stride_h * 2) % 16)
+    return fail(SPD_ERR_INVALID_ARG, "spd_shared_prefix_attn: strides must be multiples of 16 bytes");
+  if (!aligned16(q) || !aligned16(k_pool) || !aligned16(v_pool) || !aligned16(out) || !aligned16(workspace))
+    return fail(SPD_ERR_INVALID_ARG, "spd_shared_prefix_attn: tensors and the workspace must be 16-byte aligned");
+  const int sms = sm_count(-1);
+  if (sms <= 0) return fail(SPD_ERR_CUDA, "spd_shared_prefix_attn: no CUDA device");
+  const PrefixSpace space = prefix_space(B, G, Hq, Hkv, D, max_blocks << bl, sms);
+  const size_t need = spd::kWsHeaderBytes + space.counters + space.results();
+  if (!workspace || workspace_bytes < need)
+    return fail(SPD_ERR_WORKSPACE, "spd_shared_prefix_attn: workspace %zu bytes, need %zu", workspace_bytes, need);
+  unsigned char* ws = static_cast<unsigned char*>(workspace);
+  // results at the end of what the caller gave, so that a workspace with room for the counters and the results of
+  // several geometries serves them all
+  unsigned char* at = ws + (workspace_bytes - space.results()) / 256 * 256;
+  auto take = [&](size_t bytes) {
+    unsigned char* here = at;
+    at += bytes;
+    return bytes ? here : nullptr;
+  };
+  spd::OwnParams o{};
+  o.q = q; o.k_pool = k_pool; o.v_pool = v_pool; o.block_tables = block_tables; o.context_lens = context_lens; o.out = out;
+  o.q_st = q_stride_t; o.q_sh = q_stride_h;
+  o.B = B; o.Hq = Hq; o.Hkv = Hkv; o.D = D; o.max_blocks = max_blocks; o.num_blocks = num_blocks; o.bs_log2 = bl;
+  o.chunks = space.split.chunks; o.least = space.split.least;
+  o.scale_log2 = scale * 1.4426950408889634f;
+  o.counters = reinterpret_cast<int*>(ws + spd::kWsHeaderBytes);
+  o.partials = reinterpret_cast<float*>(take(space.partials));
+  o.G = G; o.cu_groups = cu_groups; o.prefix_lens = prefix_lens;
+  o.err = error_word ? error_word : reinterpret_cast<int*>(ws);
+  float* whole = reinterpret_cast<float*>(take(space.whole));
+  float* pieces = reinterpret_cast<float*>(take(space.pieces));
+  int2* desc = reinterpret_cast<int2*>(take(space.desc));
+  o.whole = whole; o.pieces = pieces; o.row_desc = desc;
+  o.piece_rows = spd::span_piece_rows(B, Hq / Hkv);
+  int rc = SPD_OK;
+  if (G) {
+    spd::SpanParams p{};
+    p.lens = prefix_lens; p.cu = cu_groups; p.tables = prefix_tables;
+    p.paged = 1; p.max_keys = max_prefix_blocks << bl; p.max_blocks = max_prefix_blocks; p.blocks = num_blocks; p.bs_log2 = bl;
+    p.N = B; p.G = G; p.Hq = Hq; p.Hkv = Hkv; p.D = D;
+    p.scale_log2 = o.scale_log2;
+    p.whole = whole; p.row_desc = desc; p.pieces = pieces;
+    p.err = o.err; p.wait_ns = g_wait_ns;
+    const spd::SpanTensors t{q, k_pool, v_pool, q_stride_t, q_stride_h, 0, 0, 0};
+    rc = spd::span_attn_launch(p, t, dtype, sms, static_cast<cudaStream_t>(stream));
+  }
+  if (rc == SPD_OK) rc = spd::own_attn_launch(o, dtype, static_cast<cudaStream_t>(stream));
+  if (rc != SPD_OK) return fail(rc, "spd_shared_prefix_attn: launch failed: %s", cudaGetErrorString(cudaGetLastError()));
+  return ok();
+}
+
+size_t spd_cross_attn_packed_workspace_size(int N, int Hq, int Hkv, int D, int device) {
+  const int sms = sm_count(device);
+  if (N <= 0 || Hkv <= 0 || Hq <= 0 || Hq % Hkv || Hq / Hkv > 128 || D <= 0 || D % 8 || D > 128 || sms <= 0) return 0;
+  return spd::kWsHeaderBytes + spd::round_up((size_t)sms * sizeof(::int4), 256) +
+         spd::round_up(2 * (size_t)sms * spd::span_piece_rows(N, Hq / Hkv) * (D + 4) * 4, 256);
+}
+
+int spd_cross_attn_packed(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k, const void* v,
+                          int64_t kv_stride_slot, int64_t kv_stride_h, int64_t kv_stride_t, const int32_t* valid_lens,
+                          const int32_t* cu_seqlens, const int32_t* slot_ids, void* out, int N, int B, int S, int T, int Hq,
+                          int Hkv, int D, float scale, int dtype, void* workspace, size_t workspace_bytes,
+                          int32_t* error_word, void* stream) {
+  if (dtype != SPD_F16 && dtype != SPD_BF16)
+    return fail(SPD_ERR_UNSUPPORTED, "spd_cross_attn_packed: dtype %d not supported (F16/BF16 only)", dtype);
+  if (N < 0 || B < 0 || S < 0 || T < 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || D <= 0 || (!cu_seqlens && N != B) ||
+      (!slot_ids && B > S))
+    return fail(SPD_ERR_INVALID_ARG, "spd_cross_attn_packed: bad sizes N=%d B=%d S=%d T=%d Hq=%d Hkv=%d D=%d", N, B, S, T, Hq,
+                Hkv, D);
+  if (D % 8 || D > 128 || Hq / Hkv > 128 || Hq > 4096)
+    return fail(SPD_ERR_UNSUPPORTED,
+                "spd_cross_attn_packed: need D a multiple of 8 up to 128 and up to 128 query heads a key/value head");
+  if (!(scale > 0.f) || scale > 1e30f) return fail(SPD_ERR_INVALID_ARG, "spd_cross_attn_packed: scale must be positive");
+  if (N == 0 || B == 0) return ok();
+  if (!q || !k || !v || !valid_lens || !out || S == 0 || T == 0)
+    return fail(SPD_ERR_INVALID_ARG, "spd_cross_attn_packed: null tensor pointer or no keys");
+  for (int64_t s : {q_stride_t, q_stride_h, kv_stride_slot, kv_stride_h, kv_stride_t})
+    if (s < 0 || (s * 2) % 16) return fail(SPD_ERR_INVALID_ARG, "spd_cross_attn_packed: strides must be multiples of 16 bytes");
+  if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out) || !aligned16(workspace))
+    return fail(SPD_ERR_INVALID_ARG, "spd_cross_attn_packed: tensors and the workspace must be 16-byte aligned");
+  const int sms = sm_count(-1);
+  if (sms <= 0) return fail(SPD_ERR_CUDA, "spd_cross_attn_packed: no CUDA device");
+  const size_t need = spd_cross_attn_packed_workspace_size(N, Hq, Hkv, D, -1);
+  if (!workspace || workspace_bytes < need)
+    return fail(SPD_ERR_WORKSPACE, "spd_cross_attn_packed: workspace %zu bytes, need %zu", workspace_bytes, need);
+  unsigned char* ws = static_cast<unsigned char*>(workspace);
+  unsigned char* at = ws + (workspace_bytes - (need - spd::kWsHeaderBytes)) / 256 * 256;  // as above
+  spd::SpanParams p{};
+  p.lens = valid_lens; p.cu = cu_seqlens; p.slots = slot_ids;
+  p.max_keys = T; p.blocks = S;
+  p.N = N; p.G = B; p.Hq = Hq; p.Hkv = Hkv; p.D = D;
+  p.scale_log2 = scale * 1.4426950408889634f;
+  p.out = out;
+  p.cta_desc = reinterpret_cast<::int4*>(at);
+  p.pieces = reinterpret_cast<float*>(at + spd::round_up((size_t)sms * sizeof(::int4), 256));
+  p.err = error_word ? error_word : reinterpret_cast<int*>(ws);
+  p.wait_ns = g_wait_ns;
+  const spd::SpanTensors t{q, k, v, q_stride_t, q_stride_h, kv_stride_t, kv_stride_h, kv_stride_slot};
+  const int rc = spd::span_attn_launch(p, t, dtype, sms, static_cast<cudaStream_t>(stream));
+  if (rc != SPD_OK) return fail(rc, "spd_cross_attn_packed: launch failed: %s", cudaGetErrorString(cudaGetLastError()));
   return ok();
 }
 

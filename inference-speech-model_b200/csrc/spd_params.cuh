@@ -21,6 +21,23 @@ inline bool allow_smem(size_t bytes) {
   return true;
 }
 
+// Launches kfn(args) with programmatic dependent launch: its CTAs may start as soon as those of the kernel
+// before it on the stream have signalled, and wait (griddepcontrol.wait) for that kernel's results.
+template <typename K, typename... Args>
+inline int launch_dependent(K kfn, dim3 grid, dim3 block, size_t smem, cudaStream_t st, const Args&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kfn, args...) == cudaSuccess ? SPD_OK : SPD_ERR_CUDA;
+}
+
 struct PagedParams {
   const void* q;
   void* k_pool;
@@ -164,6 +181,57 @@ struct DecodeInt4Params {  // single-token attention over a 4-bit pool (paged_de
   int* counters;      // [B * Hkv * head tiles] arrivals, left at zero
   float* partials;    // [B * Hq][chunks][D + 4]
   unsigned long long wait_ns;
+};
+
+struct SpanParams {  // attention of groups of queries, each over the keys of its own span (span_attn.cu)
+  const int* lens;    // [G] keys of each span
+  const int* cu;      // [G + 1] queries of each group, or null: query g
+  const int* tables;  // [G][max_blocks] of paged spans
+  const int* slots;   // [G] planes of unpaged spans, or null: plane g
+  int paged, max_keys;            // most keys a span can have
+  int max_blocks, blocks;         // table columns; blocks of the pool (or planes)
+  int bs_log2;                    // block size
+  int N, G, Hq, Hkv, D;
+  int per_tile;       // queries a tile: its rows are queries x the heads of one key/value head
+  int q_rows;         // rows of a Q box
+  float scale_log2;   // scale * log2(e)
+  void* out;          // [N][Hq][D]; null: results stay partial
+  float* whole;       // [N * Hq][D + 4] partial results of items in one piece (out null)
+  int2* row_desc;     // [N * Hkv] where the pieces of a query's heads lie (out null)
+  float* pieces;      // [2 * grid][rows][D + 4]
+  ::int4* cta_desc;     // [grid] items that begin in a CTA and end in a later one (out given)
+  int piece_rows;     // rows a piece has room for
+  int* err;
+  unsigned long long wait_ns;
+};
+
+struct SpanTensors {  // what a span call reads by TMA; strides in elements
+  const void *q, *k, *v;
+  long long q_st, q_sh;         // token and head
+  long long kv_st, kv_sh, kv_sb;  // row, head and plane of unpaged keys and values
+};
+
+struct OwnParams {  // a sequence's own keys, joined with its prefix's results (own_attn.cu)
+  const void* q;
+  const void* k_pool;
+  const void* v_pool;
+  const int* block_tables;
+  const int* context_lens;
+  void* out;              // [B][Hq][D]
+  long long q_st, q_sh;   // token and head strides of q (elements)
+  int B, Hq, Hkv, D, max_blocks, num_blocks, bs_log2;
+  int chunks, least;      // CTAs per (sequence, head tile), and the fewest tokens for one
+  float scale_log2;
+  int* counters;          // [B * Hkv * head tiles] arrivals, left at zero
+  float* partials;        // [B * Hq][chunks][D + 4]
+  int G;                  // groups that may have a prefix (0: none, and no kernel before this one)
+  const int* cu_groups;
+  const int* prefix_lens;
+  const float* whole;
+  const int2* row_desc;
+  const float* pieces;
+  int piece_rows;
+  int* err;
 };
 
 }  // namespace spd

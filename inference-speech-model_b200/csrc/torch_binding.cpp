@@ -1,11 +1,12 @@
 // torch_binding.cpp — CPython module that takes torch tensors straight to the C ABI for the
 // operators a decode step calls once per layer (rope_kv_append, rope_kv_append_int4,
-// kv_gather_int4, paged_decode_attention_int4, prompt_attention).
+// kv_gather_int4, paged_decode_attention_int4, prompt_attention, shared_prefix_decode_attention,
+// cross_attention_packed).
 //
 // Their kernels take a few microseconds, while checking some fifteen tensors from Python and
 // converting thirty arguments through ctypes took 8 to 11 (append of a 64-request step: 14.7 us
 // a call, of which the launch 3.1).  Here the same checks read the tensors directly.  The module
-// holds no kernel and no state but the workspaces of paged_decode_attention_int4: setup()
+// holds no kernel and no state but the workspaces of calls that bring none: setup()
 // is given the addresses of the C ABI's functions, so it serves whichever libspd_b200.so the
 // process has loaded.  Every refusal is a Python RuntimeError; no C++ exception leaves it.
 #include <Python.h>
@@ -37,6 +38,10 @@ decltype(&spd_prompt_attn) f_prompt;
 decltype(&spd_kv_int4_page_bytes) f_page_bytes;
 decltype(&spd_get_last_error) f_last_error;
 decltype(&spd_stream_capture_id) f_capture_id;
+decltype(&spd_shared_prefix_attn) f_prefix;
+decltype(&spd_shared_prefix_attn_workspace_size) f_prefix_size;
+decltype(&spd_cross_attn_packed) f_cross;
+decltype(&spd_cross_attn_packed_workspace_size) f_cross_size;
 
 struct Refused : std::runtime_error {
   using std::runtime_error::runtime_error;
@@ -278,8 +283,8 @@ std::pair<at::Tensor, at::Tensor> gather(const char* name, PyObject* const* a, P
   return {k, v};
 }
 
-// Workspaces of calls to paged_decode_attention_int4 that bring none: one per device, stream and graph
-// capture, made anew when a call needs more arrival counters or partial results than it has room for.
+// Workspaces of calls that bring none: one per device, stream and graph
+// capture, for all operators, made anew when a call needs more arrival counters or partial results than it has room for.
 // Counters lie at its start and are left at zero by every call, partial results at its end, so one
 // workspace serves all geometries.  One that is made during a capture lies in the graph's memory and is
 // zeroed by a node of that graph: it serves that capture's calls and no others, and is let go (back to
@@ -292,9 +297,9 @@ struct Workspace {
   size_t counters, partials;  // bytes
   at::Tensor bytes;
 };
-at::Tensor decode_workspace(int dev, void* stream, size_t counters, size_t need, const at::Tensor& like) {
+at::Tensor kept_workspace(const char* name, int dev, void* stream, size_t counters, size_t need, const at::Tensor& like) {
   static auto* kept = new std::vector<Workspace>();  // in the order of their captures
-  if (need == 0) refuse("paged_decode_attn_int4", "unsupported geometry");
+  if (need == 0) refuse(name, "unsupported geometry");
   size_t partials = need - kHeader - counters;
   const uint64_t capture = f_capture_id(stream);
   for (auto e = kept->begin(); e != kept->end(); ++e)
@@ -354,7 +359,7 @@ at::Tensor decode(const char* name, PyObject* const* a, Py_ssize_t n_args) {
   const size_t counters = ((size_t)B * Hq * 4 + kHeader - 1) / kHeader * kHeader;  // the library's layout
   const at::Tensor ws = ws_given.defined()
                             ? ws_given
-                            : decode_workspace(dev, st, counters, f_decode_size(B, Hq, Hkv, D, bs, max_blocks, code, dev), q);
+                            : kept_workspace(name, dev, st, counters, f_decode_size(B, Hq, Hkv, D, bs, max_blocks, code, dev), q);
   check(f_decode(ptr(q), ptr(pool), static_cast<const int32_t*>(ptr(tables)), static_cast<const int32_t*>(ptr(lens)), mut(out),
                  B, Hq, Hkv, D, bs, max_blocks, small_int(name, "num_blocks", pool.size(0)), (float)scale, code, mut(ws),
                  (size_t)ws.numel(), static_cast<int32_t*>(mut(err)), st),
@@ -401,6 +406,130 @@ at::Tensor prompt(const char* name, PyObject* const* a, Py_ssize_t n_args) {
   return out;
 }
 
+double number(const char* name, const char* what, PyObject* o) {
+  const double v = PyFloat_AsDouble(o);
+  if (PyErr_Occurred()) {
+    PyErr_Clear();
+    refuse(name, what, " must be a number");
+  }
+  return v;
+}
+
+void workspace_bytes(const char* name, const at::Tensor& ws) {
+  if (ws.defined() && (ws.scalar_type() != at::kByte || !ws.is_contiguous()))
+    refuse(name, "workspace must be a contiguous uint8 tensor");
+}
+
+const int32_t* ints(const at::Tensor& t) { return static_cast<const int32_t*>(ptr(t)); }
+
+// (q, k_pool, v_pool, prefix_tables, prefix_lens, cu_groups, block_tables, context_lens, scale, out, workspace, error_word)
+at::Tensor prefix(const char* name, PyObject* const* a, Py_ssize_t n_args) {
+  count(name, n_args, 12);
+  const at::Tensor &q = tensor(name, "q", a[0]), &k = tensor(name, "k_pool", a[1]), &v = tensor(name, "v_pool", a[2]),
+                   &ptab = tensor(name, "prefix_tables", a[3], true), &plens = tensor(name, "prefix_lens", a[4], true),
+                   &cu = tensor(name, "cu_groups", a[5], true), &tables = tensor(name, "block_tables", a[6]),
+                   &lens = tensor(name, "context_lens", a[7]), &given = tensor(name, "out", a[9], true),
+                   &ws_given = tensor(name, "workspace", a[10], true), &err = tensor(name, "error_word", a[11], true);
+  const int dev = current_device(name, {&q, &k, &v, &ptab, &plens, &cu, &tables, &lens, &given, &ws_given, &err});
+  if (q.dim() != 3 || k.dim() != 4 || v.sizes() != k.sizes() || k.size(3) != q.size(2))
+    refuse(name, "q [B, Hq, D] and pools [num_blocks, block_size, Hkv, D] expected");
+  if (k.scalar_type() != q.scalar_type() || v.scalar_type() != q.scalar_type()) refuse(name, "q and the pools must share a dtype");
+  if (!k.is_contiguous() || !v.is_contiguous()) refuse(name, "pools must be contiguous");
+  const int B = small_int(name, "B", q.size(0)), Hq = small_int(name, "Hq", q.size(1)), D = small_int(name, "D", q.size(2)),
+            bs = small_int(name, "block_size", k.size(1)), Hkv = small_int(name, "Hkv", k.size(2)),
+            blocks = small_int(name, "num_blocks", k.size(0));
+  if (Hkv == 0 || Hq % Hkv) refuse(name, Hq, " query heads do not divide over ", Hkv, " key/value heads");
+  const int max_blocks = table_columns(name, tables, B);
+  int32_vector(name, "context_lens", lens, B);
+  if (ptab.defined() != plens.defined() || ptab.defined() != cu.defined())
+    refuse(name, "prefix_tables, prefix_lens and cu_groups come together");
+  int G = 0, max_prefix = 0;
+  if (ptab.defined()) {
+    if (ptab.dim() != 2 || ptab.scalar_type() != at::kInt || !ptab.is_contiguous())
+      refuse(name, "prefix_tables must be contiguous int32 [G, max_prefix_blocks]");
+    G = small_int(name, "G", ptab.size(0));
+    max_prefix = small_int(name, "max_prefix_blocks", ptab.size(1));
+    int32_vector(name, "prefix_lens", plens, G);
+    int32_vector(name, "cu_groups", cu, (int64_t)G + 1);
+  }
+  if (given.defined() && (given.sizes() != q.sizes() || given.scalar_type() != q.scalar_type() || !given.is_contiguous()))
+    refuse(name, "out must be a contiguous ", shape_of(q), " tensor of q's dtype");
+  if (given.defined() && (overlap(k, given) || overlap(v, given) || partly_over(q, given)))
+    refuse(name, "out must be apart from the pools, and from q unless it is q itself");
+  error_word(name, err);
+  workspace_bytes(name, ws_given);
+  const int code = dtype_code(name, q.scalar_type());
+  const double scale = number(name, "scale", a[8]);
+  const auto qs = token_strides(name, "q", q);
+  at::Tensor out = given.defined() ? given : at::empty(q.sizes(), q.options());
+  if (B == 0) return out;
+  void* st = stream();
+  at::Tensor ws = ws_given;
+  if (!ws.defined()) {
+    const size_t need = f_prefix_size(B, G, Hq, Hkv, D, bs, max_prefix, max_blocks, dev);
+    const size_t counters = ((size_t)B * Hq * 4 + kHeader - 1) / kHeader * kHeader;  // as much as the library's, or more
+    ws = kept_workspace(name, dev, st, counters, need ? need + counters : 0, q);
+  }
+  check(f_prefix(ptr(q), qs.first, qs.second, ptr(k), ptr(v), ints(ptab), ints(plens), ints(cu), ints(tables), ints(lens),
+                 mut(out), B, G, Hq, Hkv, D, bs, max_prefix, max_blocks, blocks, (float)scale, code, mut(ws),
+                 (size_t)ws.numel(), static_cast<int32_t*>(mut(err)), st),
+        name);
+  return out;
+}
+
+// (q, k, v, valid_lens, cu_seqlens, slot_ids, scale, out, workspace, error_word)
+at::Tensor cross(const char* name, PyObject* const* a, Py_ssize_t n_args) {
+  count(name, n_args, 10);
+  const at::Tensor &q = tensor(name, "q", a[0]), &k = tensor(name, "k", a[1]), &v = tensor(name, "v", a[2]),
+                   &lens = tensor(name, "valid_lens", a[3]), &cu = tensor(name, "cu_seqlens", a[4], true),
+                   &slots = tensor(name, "slot_ids", a[5], true), &given = tensor(name, "out", a[7], true),
+                   &ws_given = tensor(name, "workspace", a[8], true), &err = tensor(name, "error_word", a[9], true);
+  const int dev = current_device(name, {&q, &k, &v, &lens, &cu, &slots, &given, &ws_given, &err});
+  if (q.dim() != 3 || k.dim() != 4 || v.sizes() != k.sizes() || k.size(3) != q.size(2))
+    refuse(name, "q [N, Hq, D] and k, v [S, Hkv, T, D] expected");
+  if (k.scalar_type() != q.scalar_type() || v.scalar_type() != q.scalar_type()) refuse(name, "q, k and v must share a dtype");
+  const int N = small_int(name, "N", q.size(0)), Hq = small_int(name, "Hq", q.size(1)), D = small_int(name, "D", q.size(2)),
+            S = small_int(name, "S", k.size(0)), Hkv = small_int(name, "Hkv", k.size(1)), T = small_int(name, "T", k.size(2));
+  if (Hkv == 0 || Hq % Hkv) refuse(name, Hq, " query heads do not divide over ", Hkv, " key/value heads");
+  if (lens.dim() != 1) refuse(name, "valid_lens must be a contiguous int32 [B] tensor");
+  const int B = small_int(name, "B", lens.size(0));
+  int32_vector(name, "valid_lens", lens, B);
+  if (cu.defined()) int32_vector(name, "cu_seqlens", cu, (int64_t)B + 1);
+  else if (N != B) refuse(name, "without cu_seqlens one query per request is expected (", N, " queries, ", B, " requests)");
+  if (slots.defined()) int32_vector(name, "slot_ids", slots, B);
+  else if (B > S) refuse(name, "more requests than slots and no slot_ids");
+  // strides of dimensions of one entry, which nothing steps over, are taken as dense
+  int64_t st_[2][3];
+  for (int i = 0; i < 2; ++i) {
+    const at::Tensor& x = i ? v : k;
+    if (x.stride(3) != 1 && D > 1) refuse(name, "k and v need a contiguous last dimension");
+    st_[i][2] = T == 1 ? D : x.stride(2);
+    st_[i][1] = Hkv == 1 ? st_[i][2] * T : x.stride(1);
+    st_[i][0] = S == 1 ? st_[i][1] * Hkv : x.stride(0);
+  }
+  for (int i = 0; i < 3; ++i)
+    if (st_[0][i] != st_[1][i]) refuse(name, "k and v need identical strides");
+  if (given.defined() && (given.sizes() != q.sizes() || given.scalar_type() != q.scalar_type() || !given.is_contiguous()))
+    refuse(name, "out must be a contiguous ", shape_of(q), " tensor of q's dtype");
+  if (given.defined() && (overlap(k, given) || overlap(v, given) || partly_over(q, given)))
+    refuse(name, "out must be apart from k and v, and from q unless it is q itself");
+  error_word(name, err);
+  workspace_bytes(name, ws_given);
+  const int code = dtype_code(name, q.scalar_type());
+  const double scale = number(name, "scale", a[6]);
+  const auto qs = token_strides(name, "q", q);
+  at::Tensor out = given.defined() ? given : at::empty(q.sizes(), q.options());
+  if (N == 0 || B == 0) return out;
+  void* st = stream();
+  at::Tensor ws = ws_given;
+  if (!ws.defined()) ws = kept_workspace(name, dev, st, 0, f_cross_size(N, Hq, Hkv, D, dev), q);
+  check(f_cross(ptr(q), qs.first, qs.second, ptr(k), ptr(v), st_[0][0], st_[0][1], st_[0][2], ints(lens), ints(cu), ints(slots),
+                mut(out), N, B, S, T, Hq, Hkv, D, (float)scale, code, mut(ws), (size_t)ws.numel(),
+                static_cast<int32_t*>(mut(err)), st),
+        name);
+  return out;
+}
+
 // Runs `body` with every C++ exception turned into a Python RuntimeError.
 template <typename F>
 PyObject* guarded(const F& body) {
@@ -441,6 +570,12 @@ PyObject* py_decode(PyObject*, PyObject* const* a, Py_ssize_t n) {
 PyObject* py_prompt(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&] { return wrap(prompt("prompt_attn", a, n)); });
 }
+PyObject* py_prefix(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&] { return wrap(prefix("shared_prefix_attn", a, n)); });
+}
+PyObject* py_cross(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&] { return wrap(cross("cross_attn_packed", a, n)); });
+}
 
 // setup({name: address}) of the C ABI's functions
 PyObject* py_setup(PyObject*, PyObject* d) {
@@ -455,7 +590,9 @@ PyObject* py_setup(PyObject*, PyObject* d) {
       get("spd_kv_gather_int4", f_gather) && get("spd_paged_decode_attn_int4_err", f_decode) &&
       get("spd_paged_decode_attn_int4_workspace_size", f_decode_size) && get("spd_prompt_attn", f_prompt) &&
       get("spd_kv_int4_page_bytes", f_page_bytes) && get("spd_get_last_error", f_last_error) &&
-      get("spd_stream_capture_id", f_capture_id))
+      get("spd_stream_capture_id", f_capture_id) && get("spd_shared_prefix_attn", f_prefix) &&
+      get("spd_shared_prefix_attn_workspace_size", f_prefix_size) && get("spd_cross_attn_packed", f_cross) &&
+      get("spd_cross_attn_packed_workspace_size", f_cross_size))
     Py_RETURN_NONE;
   return nullptr;
 }
@@ -467,6 +604,8 @@ PyMethodDef methods[] = {
     {"kv_gather_int4", reinterpret_cast<PyCFunction>(py_gather), METH_FASTCALL, nullptr},
     {"paged_decode_attention_int4", reinterpret_cast<PyCFunction>(py_decode), METH_FASTCALL, nullptr},
     {"prompt_attention", reinterpret_cast<PyCFunction>(py_prompt), METH_FASTCALL, nullptr},
+    {"shared_prefix_decode_attention", reinterpret_cast<PyCFunction>(py_prefix), METH_FASTCALL, nullptr},
+    {"cross_attention_packed", reinterpret_cast<PyCFunction>(py_cross), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "spd_torch", "torch tensors to the C ABI of libspd_b200.so", -1, methods};

@@ -2,8 +2,8 @@
 
 Each function checks shapes, dtypes, devices and strides, then calls the extension on
 ``torch.cuda.current_stream()`` (the capture stream inside ``torch.cuda.graph``): the
-engine's ops through ctypes, the last five below through the torch binding.  Nothing here synchronises or reads device values, so every op
-can be captured in a CUDA graph.  CPU tensors raise ``RuntimeError``: the product path
+engine's ops through ctypes, those without a counterpart in the reference through the torch binding.  Nothing
+here synchronises or reads device values, so every op can be captured in a CUDA graph.  CPU tensors raise ``RuntimeError``: the product path
 has no CPU implementation.
 
 Ops and the reference code they replace:
@@ -24,6 +24,10 @@ key/value heads and a 4-bit cache:
   kv_gather_int4                        cached tokens of a 4-bit pool as packed k and v
   paged_decode_attention_int4           single-token attention over a 4-bit pool
   prompt_attention                      attention of whole packed prompts
+
+and for several candidates (samples, beams) of one request:
+  shared_prefix_decode_attention        single-token attention over a shared prefix and own tokens
+  cross_attention_packed                any number of queries a request over the request's slot
 """
 from __future__ import annotations
 
@@ -574,3 +578,77 @@ def prompt_attention(
     Returns out [Nq, Hq, D]."""
     return N.binding().prompt_attention(q, k, v, cu_seqlens_q, cu_seqlens_k, causal,
                                         q.shape[-1] ** -0.5 if scale is None else scale, out, error_word)
+
+
+# ----------------------------------------------------------------------------- several candidates of one request
+def shared_prefix_workspace(B: int, G: int, Hq: int, Hkv: int, D: int, block_size: int, max_prefix_blocks: int, max_blocks: int,
+                            device: torch.device) -> torch.Tensor:
+    """Zero-filled workspace for ``shared_prefix_decode_attention`` (reusable on one stream)."""
+    idx = device.index if device.index is not None else torch.cuda.current_device()
+    n = N.load().spd_shared_prefix_attn_workspace_size(B, G, Hq, Hkv, D, block_size, max_prefix_blocks, max_blocks, idx)
+    if n == 0:
+        raise RuntimeError(f"shared_prefix_workspace: unsupported geometry B={B} Hq={Hq} Hkv={Hkv} D={D} block_size={block_size}")
+    return torch.zeros(n, dtype=torch.uint8, device=device)
+
+
+def cross_attn_packed_workspace(N_queries: int, Hq: int, Hkv: int, D: int, device: torch.device) -> torch.Tensor:
+    """Zero-filled workspace for ``cross_attention_packed`` (reusable on one stream)."""
+    idx = device.index if device.index is not None else torch.cuda.current_device()
+    n = N.load().spd_cross_attn_packed_workspace_size(N_queries, Hq, Hkv, D, idx)
+    if n == 0:
+        raise RuntimeError(f"cross_attn_packed_workspace: unsupported geometry N={N_queries} Hq={Hq} Hkv={Hkv} D={D}")
+    return torch.zeros(n, dtype=torch.uint8, device=device)
+
+
+def shared_prefix_decode_attention(
+    q: torch.Tensor,
+    k_pool: torch.Tensor,
+    v_pool: torch.Tensor,
+    prefix_tables: Optional[torch.Tensor],
+    prefix_lens: Optional[torch.Tensor],
+    cu_groups: Optional[torch.Tensor],
+    block_tables: torch.Tensor,
+    context_lens: torch.Tensor,
+    scale: Optional[float] = None,
+    out: Optional[torch.Tensor] = None,
+    workspace: Optional[torch.Tensor] = None,
+    error_word: Optional[torch.Tensor] = None,
+) -> torch.Tensor:
+    """Single-token attention with grouped heads over a paged 16-bit pool, for sequences that share prefixes:
+    each group's prefix is read once for all its sequences.
+
+    q [B, Hq, D] (fp16 / bf16, D a multiple of 8 up to 128, any token and head strides that are multiples of 16
+    bytes); k_pool / v_pool [num_blocks, block_size, Hkv, D] as ``rope_kv_append`` writes them (Hq a multiple of
+    Hkv, block_size 8 to 128, a power of two).  Group g is the sequences [cu_groups[g], cu_groups[g + 1])
+    (int32 [G + 1]); each attends the first prefix_lens[g] tokens of prefix_tables[g] (int32 [G], [G, columns]), then
+    its own context_lens[b] tokens of block_tables[b] (int32 [B], [B, columns]; <= 0: none).  A sequence of no group has
+    no prefix, and without the three prefix arguments (None) none has.  A sequence without any key gives
+    zeros.  ``out`` may be q itself.  Device flags (a block id or length out of range, a wait that ran out)
+    go to ``error_word`` (int32), else to the first word of ``workspace``.  Returns out [B, Hq, D]."""
+    return N.binding().shared_prefix_decode_attention(q, k_pool, v_pool, prefix_tables, prefix_lens, cu_groups, block_tables,
+                                                      context_lens, q.shape[-1] ** -0.5 if scale is None else scale, out,
+                                                      workspace, error_word)
+
+
+def cross_attention_packed(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    valid_lens: torch.Tensor,
+    cu_seqlens: Optional[torch.Tensor] = None,
+    slot_ids: Optional[torch.Tensor] = None,
+    scale: Optional[float] = None,
+    out: Optional[torch.Tensor] = None,
+    workspace: Optional[torch.Tensor] = None,
+    error_word: Optional[torch.Tensor] = None,
+) -> torch.Tensor:
+    """Attention of any number of queries a request (beams, prompt tokens) over encoder keys and values, which are
+    read once for all of them (fp16 / bf16, D a multiple of 8 up to 128, Hq a multiple of Hkv).
+
+    q [N, Hq, D] packed: request b owns rows [cu_seqlens[b], cu_seqlens[b + 1]) (int32 [B + 1]; None: one query a
+    request); k, v [S, Hkv, T, D] with any slot, head and row strides that are multiples of 16 bytes (the same for
+    both); request b attends positions t < valid_lens[b] (int32 [B]) of slot slot_ids[b] (int32 [B]; None: slot
+    b).  A query without any key gives zeros; rows that belong to no request are left as they are in ``out``,
+    which may be q itself.  Flags as in ``shared_prefix_decode_attention``.  Returns out [N, Hq, D]."""
+    return N.binding().cross_attention_packed(q, k, v, valid_lens, cu_seqlens, slot_ids,
+                                              q.shape[-1] ** -0.5 if scale is None else scale, out, workspace, error_word)
