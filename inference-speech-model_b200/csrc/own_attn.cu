@@ -300,6 +300,9 @@ __global__ void __launch_bounds__(kThreads, 2) own_attn_kernel(const OwnParams p
       if (hit) group = first + __ffs(hit) - 1;
     }
     if (group >= 0 && p.prefix_lens[group] > 0) found = __ldcg(p.row_desc + (long long)b * p.Hkv + kvh);
+    // What a prefix's kernel that gave up waiting did not write is not followed.
+    const int row0 = (int)((unsigned)found.y >> 16), count = found.y & 0xffff;
+    if (found.x < -1 || found.x + count > p.span_ctas || row0 + Gq > p.piece_rows || (found.x < 0 && count > 1)) found.y = 0;
     if (lane == 0) desc = found;
   }
   __syncthreads();

@@ -697,6 +697,7 @@ int spd_shared_prefix_attn(const void* q, int64_t q_stride_t, int64_t q_stride_h
   int2* desc = reinterpret_cast<int2*>(take(space.desc));
   o.whole = whole; o.pieces = pieces; o.row_desc = desc;
   o.piece_rows = spd::span_piece_rows(B, Hq / Hkv);
+  o.span_ctas = sms;
   int rc = SPD_OK;
   if (G) {
     spd::SpanParams p{};

@@ -230,7 +230,7 @@ struct OwnParams {  // a sequence's own keys, joined with its prefix's results (
   const float* whole;
   const int2* row_desc;
   const float* pieces;
-  int piece_rows;
+  int piece_rows, span_ctas;  // rows of a piece, and CTAs that left pieces
   int* err;
 };
 
