@@ -24,7 +24,7 @@ using tc::pack2;
 
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
-constexpr int kStages = 3;
+constexpr int kStages = 2;
 constexpr int kStageBytes = 8192;  // keys and values of a step
 
 template <int DP> struct Cfg {
@@ -71,13 +71,12 @@ struct Sum {
 
 // SPLIT: rows 8 to 15 hold the rounding remainders of the weights of rows 0 to 7.
 template <typename T, int DP, bool SPLIT>
-__global__ void __launch_bounds__(kThreads, 2) own_attn_kernel(const OwnParams p) {
+__global__ void __launch_bounds__(kThreads, 3) own_attn_kernel(const OwnParams p) {
   using C = Cfg<DP>;
   constexpr int kKeys = C::kKeys, kHeads = SPLIT ? 8 : 16, kTiles = DP / 8;
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ uint32_t there[kWarps][kStages];  // tokens of a step that count, a bit each
   __shared__ float stat_m[kWarps][16], stat_l[kWarps][16];
-  __shared__ int2 desc;
   __shared__ int last_flag;
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -147,8 +146,17 @@ __global__ void __launch_bounds__(kThreads, 2) own_attn_kernel(const OwnParams p
     cp_commit();
   };
   look_up();
+
+  // ---- the group whose prefix this sequence shares
+  int group = -1;
 #pragma unroll 1
-  for (int i = 0; i < kStages - 1; ++i) fetch();
+  for (int first = 0; first < p.G && group < 0; first += 32) {
+    const int i = first + lane;
+    const bool in = i < p.G && p.cu_groups[i] <= b && b < p.cu_groups[i + 1];
+    const uint32_t hit = __ballot_sync(0xffffffffu, in);
+    if (hit) group = first + __ffs(hit) - 1;
+  }
+  if (group >= 0 && p.prefix_lens[group] <= 0) group = -1;
 
   // ---- query fragments: rows g and g + 8, pairs of dimensions 2t and 2t + 8 of each 16 ----------
   uint32_t qa[DP / 16][4];
@@ -170,8 +178,9 @@ __global__ void __launch_bounds__(kThreads, 2) own_attn_kernel(const OwnParams p
 
   int used = 0;
 #pragma unroll 1
-  for (int i = warp; i < steps; i += kWarps) {
+  for (int i = warp - (kStages - 1) * kWarps; i < steps; i += kWarps) {
     fetch();
+    if (i < 0) continue;  // the first copies
     cp_wait<kStages - 1>();
     __syncwarp();
     const int st = used % kStages;
@@ -288,88 +297,72 @@ __global__ void __launch_bounds__(kThreads, 2) own_attn_kernel(const OwnParams p
       stat_l[warp][g + 8] = l[1];
     }
   }
-  // ---- the group's prefix: where its pieces lie --------------------------------------------------
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (warp == 0) {
-    int2 found = make_int2(0, 0);
-    int group = -1;
-    for (int first = 0; first < p.G && group < 0; first += 32) {
-      const int i = first + lane;
-      const bool in = i < p.G && p.cu_groups[i] <= b && b < p.cu_groups[i + 1];
-      const uint32_t hit = __ballot_sync(0xffffffffu, in);
-      if (hit) group = first + __ffs(hit) - 1;
-    }
-    if (group >= 0 && p.prefix_lens[group] > 0) found = __ldcg(p.row_desc + (long long)b * p.Hkv + kvh);
-    // What a prefix's kernel that gave up waiting did not write is not followed.
-    const int row0 = (int)((unsigned)found.y >> 16), count = found.y & 0xffff;
-    if (found.x < -1 || found.x + count > p.span_ctas || row0 + Gq > p.piece_rows || (found.x < 0 && count > 1)) found.y = 0;
-    if (lane == 0) desc = found;
-  }
   __syncthreads();
-  const int pieces = desc.y & 0xffff, piece_row = (int)((unsigned)desc.y >> 16), first_cta = desc.x;
   const int quads = p.D / 4;
-  auto prefix = [&](int h, int i) {
-    const int in_group = tile * kHeads + h;
-    return first_cta < 0 ? p.whole + (head0 + h) * step
-                         : p.pieces + ((long long)(2 * (first_cta + i) + (i == 0)) * p.piece_rows + piece_row + in_group) * step;
-  };
-  auto add_prefix = [&](Sum& s, int h, int d) {
-#pragma unroll 4
-    for (int i = 0; i < pieces; ++i) {
-      const float* row = prefix(h, i);
-      const float2 st = __ldcg(reinterpret_cast<const float2*>(row + p.D));
-      s.add(__ldcg(reinterpret_cast<const float4*>(row + d)), st.x, st.y);
-    }
-  };
-  auto store = [&](int h, int d, const Sum& s) {
-    const float r = s.l != 0.f ? 1.f / s.l : 0.f;  // no weight at all: zeros
-    T* out = reinterpret_cast<T*>(p.out) + (head0 + h) * p.D + d;
-    *reinterpret_cast<uint2*>(out) = make_uint2(pack2<T>(s.a.x * r, s.a.y * r), pack2<T>(s.a.z * r, s.a.w * r));
-  };
-#pragma unroll 1
-  for (int e = tid; e < heads * quads; e += kThreads) {
-    const int h = e / quads, d = e % quads * 4;
-    Sum s;
+  auto of_warps = [&](Sum& s, int h, int d) {
 #pragma unroll
     for (int w = 0; w < kWarps; ++w)
       if (w < steps)
         s.add(*reinterpret_cast<const float4*>(reinterpret_cast<const float*>(smem + (size_t)w * kStages * kStageBytes) + h * DP + d),
               stat_m[w][h], stat_l[w][h]);
-    if (parts == 1) {
-      add_prefix(s, h, d);
-      store(h, d, s);
-    } else {
+  };
+  // the n partial results of a row
+  auto of_memory = [&](Sum& s, const float* row, long long next, int n, int d) {
+#pragma unroll 4
+    for (int c = 0; c < n; ++c, row += next) {
+      const float2 st = __ldcg(reinterpret_cast<const float2*>(row + p.D));
+      s.add(__ldcg(reinterpret_cast<const float4*>(row + d)), st.x, st.y);
+    }
+  };
+  if (parts > 1) {
+    // ---- the chunks of a sequence are joined by the last CTA of this (sequence, head tile) to arrive ----
+#pragma unroll 1
+    for (int e = tid; e < heads * quads; e += kThreads) {
+      const int h = e / quads, d = e % quads * 4;
+      Sum s;
+      of_warps(s, h, d);
       float* row = p.partials + ((head0 + h) * p.chunks + chunk) * step;
       *reinterpret_cast<float4*>(row + d) = s.a;
       if (d == 0) *reinterpret_cast<float2*>(row + p.D) = make_float2(s.m, s.l);
     }
+    __threadfence();
+    __syncthreads();
+    if (tid == 0) {
+      int* counter = p.counters + (long long)b * Y + y;
+      last_flag = atomicAdd(counter, 1) == parts - 1;
+      if (last_flag) *counter = 0;
+    }
+    __syncthreads();
   }
-  if (parts == 1) return;
-
-  // ---- join the chunks: the last CTA of this (sequence, head tile) to arrive ----------------------
-  __threadfence();
-  __syncthreads();
-  if (tid == 0) {
-    int* counter = p.counters + (long long)b * Y + y;
-    last_flag = atomicAdd(counter, 1) == parts - 1;
-    if (last_flag) *counter = 0;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (parts > 1) {
+    if (!last_flag) return;
+    __threadfence();
   }
-  __syncthreads();
-  if (!last_flag) return;
-  __threadfence();
+  // ---- and with the group's prefix ---------------------------------------------------------------
+  int2 desc = make_int2(0, 0);
+  if (group >= 0) {
+    desc = __ldcg(p.row_desc + (long long)b * p.Hkv + kvh);
+    // What a prefix's kernel that gave up waiting did not write is not followed.
+    const int row0 = (int)((unsigned)desc.y >> 16), count = desc.y & 0xffff;
+    if (desc.x < -1 || desc.x + count > p.span_ctas || row0 + Gq > p.piece_rows || (desc.x < 0 && count > 1)) desc.y = 0;
+  }
+  const int pieces = desc.y & 0xffff, first_cta = desc.x;
+  const long long piece = (long long)p.piece_rows * step;
 #pragma unroll 1
   for (int e = tid; e < heads * quads; e += kThreads) {
     const int h = e / quads, d = e % quads * 4;
-    const float* rows = p.partials + (head0 + h) * p.chunks * step;
     Sum s;
-#pragma unroll 4
-    for (int c = 0; c < parts; ++c) {
-      const float* row = rows + (long long)c * step;
-      const float2 st = __ldcg(reinterpret_cast<const float2*>(row + p.D));
-      s.add(__ldcg(reinterpret_cast<const float4*>(row + d)), st.x, st.y);
-    }
-    add_prefix(s, h, d);
-    store(h, d, s);
+    if (parts == 1) of_warps(s, h, d);
+    else of_memory(s, p.partials + (head0 + h) * p.chunks * step, step, parts, d);
+    // the first piece lies in the second place of its CTA, the others in the first place of theirs
+    const long long row = (long long)((unsigned)desc.y >> 16) + tile * kHeads + h;
+    const float* at = first_cta < 0 ? p.whole + (head0 + h) * step : p.pieces + (2 * first_cta + 1) * piece + row * step;
+    of_memory(s, at, 0, min(pieces, 1), d);
+    of_memory(s, at + piece, 2 * piece, pieces - 1, d);
+    const float r = s.l != 0.f ? 1.f / s.l : 0.f;  // no weight at all: zeros
+    T* out = reinterpret_cast<T*>(p.out) + (head0 + h) * p.D + d;
+    *reinterpret_cast<uint2*>(out) = make_uint2(pack2<T>(s.a.x * r, s.a.y * r), pack2<T>(s.a.z * r, s.a.w * r));
   }
 }
 
@@ -397,7 +390,7 @@ int own_attn_tiles(int Hq, int Hkv) {
 // slots fall free.
 Int4Split own_attn_split(int B, int Hq, int Hkv, int max_ctx, int sms) {
   constexpr int kLeast = 512, kChunk = 1024;
-  const long long slots = 2ll * sms, pairs = (long long)B * own_attn_tiles(Hq, Hkv);
+  const long long slots = 3ll * sms, pairs = (long long)B * own_attn_tiles(Hq, Hkv);
   const long long share = max_ctx * pairs / slots;
   if (share <= 2 * kChunk) return {(int)std::max(1ll, std::min(slots / pairs, (max_ctx + kLeast - 1ll) / kLeast)), kLeast};
   const long long c = std::min(std::max(share / 2, (long long)kChunk), 4ll * kChunk);

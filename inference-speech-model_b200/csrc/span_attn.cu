@@ -286,7 +286,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       // them, K tiles in ring 0 and V tiles in ring 1.  Warp 0 deals the pieces besides, two ahead.
       const int x = warp == 0 ? 0 : 1;
       const uint64_t policy = l2_policy_evict_first();  // (the code, the pieces and the tables stay in L2)
-      const int page = lane / C::kBoxes, box = lane % C::kBoxes;  // of this lane's copy in a paged step
       const int bl7 = p.bs_log2 + 7;  // log2 of a page's bytes in one box
       unsigned char* const ring = kv_tiles + x * C::kStages * C::kTile;
       int used = 0, hole_at = 0;
@@ -360,10 +359,10 @@ __global__ void __launch_bounds__(kThreads, 1)
           break;
         }
         const Steps st(w, x);
-        const int* table = PAGED ? p.tables + (long long)w.group * p.max_blocks + page : nullptr;
+        const int* table = PAGED ? p.tables + (long long)w.group * p.max_blocks + lane : nullptr;
         const int plane = PAGED ? 0 : p.slots ? p.slots[w.group] : w.group;
-        auto look_up = [&](int t) {  // this lane's block of step t, a step ahead of its use
-          return PAGED && t < st.n && page < pages_of(p, w.len - (w.j0 + t) * BN)
+        auto look_up = [&](int t) {  // the block of page `lane` of step t, a step ahead of its use
+          return PAGED && t < st.n && lane < pages_of(p, w.len - (w.j0 + t) * BN)
                      ? __ldg(table + (w.j0 + t) * (BN >> p.bs_log2)) : 0;
         };
         int id = look_up(st.first);
@@ -383,16 +382,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int t = st.first; t < st.n && ok; t += st.by) {
           const int id_next = look_up(t + st.by);
           uint32_t bytes = C::kTile, gone = 0;  // gone: pages whose block id is out of range, a bit each
-          bool fine = lane < C::kBoxes;
-          if constexpr (PAGED) {  // (pages of 8 tokens with two boxes each fill the warp exactly)
-            const int pages = pages_of(p, w.len - (w.j0 + t) * BN);
-            fine = page < pages && id >= 0 && id < p.blocks;
-            const uint32_t bad = __ballot_sync(0xffffffffu, page < pages && !fine);
-            if (bad) {
-              if (page < pages && !fine) set_error(p.err, SPD_DEVERR_BLOCK_ID);
-#pragma unroll 1
-              for (int q = 0; q < 32 / C::kBoxes; ++q) gone |= (bad >> (q * C::kBoxes) & 1u) << q;
-            }
+          int pages = 1;
+          if constexpr (PAGED) {
+            pages = pages_of(p, w.len - (w.j0 + t) * BN);
+            const bool bad = lane < pages && (id < 0 || id >= p.blocks);
+            gone = __ballot_sync(0xffffffffu, bad);
+            if (bad) set_error(p.err, SPD_DEVERR_BLOCK_ID);
             bytes = (uint32_t)((pages - __popc(gone)) * C::kBoxes) << bl7;
             // known before K is armed, to all that wait for it
             if (lane == 0 && !(w.pair && x)) holes[(hole_at + t) % kHoles] = gone;
@@ -401,15 +396,25 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int kind = w.pair ? x : 0; kind <= (w.pair ? x : 1); ++kind) {
             const int slot = used % C::kStages;
             if (used >= C::kStages && !wait(&kv_empty[x][slot], (uint32_t)(used / C::kStages - 1))) break;
-            unsigned char* tile = ring + slot * C::kTile + box * C::kBox;
+            unsigned char* tile = ring + slot * C::kTile;
+            const CUtensorMap* map = kind ? &tm_v : &tm_k;
             if (lane == 0) mbar_arrive_expect_tx(&kv_full[x][slot], bytes);
             ++used;
             __syncwarp();
-            if (fine) {
-              const CUtensorMap* map = kind ? &tm_v : &tm_k;
-              if constexpr (PAGED) tma_load_4d(tile + (page << bl7), map, 64 * box, w.kvh, 0, id, &kv_full[x][slot], policy);
-              else tma_load_4d(tile, map, 64 * box, (w.j0 + t) * BN, w.kvh, plane, &kv_full[x][slot], policy);
+            // One lane issues, page after page: lanes with a page each would have their operands made uniform one by one
+            // (2,600 cycles a tile of 8 pages).
+#pragma unroll 1
+            for (int page = 0; page < pages; ++page) {
+              const int block = PAGED ? __shfl_sync(0xffffffffu, id, page) : plane;
+              if ((gone >> page & 1u) || lane) continue;
+#pragma unroll
+              for (int box = 0; box < C::kBoxes; ++box) {
+                unsigned char* to = tile + box * C::kBox + (PAGED ? page << bl7 : 0);
+                if constexpr (PAGED) tma_load_4d(to, map, 64 * box, w.kvh, 0, block, &kv_full[x][slot], policy);
+                else tma_load_4d(to, map, 64 * box, (w.j0 + t) * BN, w.kvh, block, &kv_full[x][slot], policy);
+              }
             }
+            __syncwarp();
           }
           id = id_next;
           if (x == 0 && more && dealt < it + 3) deal();  // two ahead, between copies
@@ -471,7 +476,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           // need is waited for before.
           const bool begin = t < st.first, more = t + st.by < st.n;
           const int k_slot = k_at % C::kStages, v_slot = v_at % C::kStages;
-          if (more && !wait(&kv_full[k_ring][k_slot], (uint32_t)(k_at / C::kStages))) break;
+          // (with few tiles to a ring the next K is loaded late, and the product does not wait for it)
+          const bool early = C::kStages > 2 || w.pair;
+          if ((early || begin) && more && !wait(&kv_full[k_ring][k_slot], (uint32_t)(k_at / C::kStages))) break;
           if (begin) {
             v_at -= st.by;
           } else {
@@ -509,9 +516,13 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (!ok) break;
             p_odd ^= 1;
           }
+          if (!early && !begin) {
+            if (leader) give_back(&kv_empty[v_ring][v_slot]);
+            if (more && !wait(&kv_full[k_ring][k_slot], (uint32_t)(k_at / C::kStages))) break;
+          }
           if (leader) {
             if (more) {  // S = Q K^T
-              if (begin) tc_fence_after();
+              if (begin || !early) tc_fence_after();
 #pragma unroll
               for (int c = 0; c < C::kBoxes; ++c)
                 umma4_ss(tmem + x * BN, q_desc + (uint64_t)(q * kTile16 + c * kBox16),
@@ -526,7 +537,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               umma_commit(&o_full[x]);
             }
             if (!begin) {
-              give_back(&kv_empty[v_ring][v_slot]);
+              if (early) give_back(&kv_empty[v_ring][v_slot]);
               if (w.pair && !x) mbar_arrive(&turn[turns % C::kStages]);
             }
           }
