@@ -383,6 +383,22 @@ int spd_cross_attn_packed(const void* q, int64_t q_stride_t, int64_t q_stride_h,
                           int Hkv, int D, float scale, int dtype, void* workspace, size_t workspace_bytes,
                           int32_t* error_word, void* stream);
 
+/* A token a row, beside spd_argmax_rows: x [rows][ld], of which the first cols columns (up to 2^19) take part; skip_mask
+ * uint8 [cols] or NULL, columns that count as -inf.  temperature, top_k, top_p, min_p: [rows] device arrays, or NULL for the
+ * *_all value in every row.  uniforms fp32 [rows], each in [0, 1).  With a row's largest value m and temperature t:
+ *   t <= 0 (or NaN), or m not finite: the first largest column (a NaN wins), as spd_argmax_rows picks it;
+ *   otherwise, with w = exp((x - m) / t) and the columns sorted by x, the largest first, equal ones by their place:
+ *   top_k > 0 leaves the first top_k; of these top_p < 1 leaves those before which less than top_p of their weight lies
+ *   (at least one); of these min_p > 0 leaves those with x >= m + t log(min_p) (at least one).
+ *   The token is the first column, by its place, at which the weight of what is left so far passes uniforms[r] times
+ *   all of it.
+ * Decisions are those of fp64 arithmetic; ties and order never depend on scheduling.  out int64 [rows]; logprobs fp32
+ * [rows] or NULL: log softmax(x) of the token over the columns that are not skipped (temperature 1, nothing cut). */
+int spd_sample_rows(const void* x, int rows, int cols, int64_t ld, const uint8_t* skip_mask, const float* uniforms,
+                    const float* temperature, float temperature_all, const int32_t* top_k, int top_k_all,
+                    const float* top_p, float top_p_all, const float* min_p, float min_p_all, int64_t* out,
+                    float* logprobs, int dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -19,6 +19,7 @@ int kv_append_launch(const AppendParams& p, int sms, cudaStream_t st);
 int block_gather_launch(const GatherParams& p, int sms, cudaStream_t st);
 int add_layernorm_launch(const AddLnParams& p, int dtype, cudaStream_t st);
 int argmax_rows_launch(const ArgmaxParams& p, int dtype, cudaStream_t st);
+int sample_rows_launch(const SampleParams& p, int dtype, int sms, cudaStream_t st);
 int linear_small_m_launch(const void* x, const void* w, const void* bias, void* y, int M, int N, int K,
                           long long group_cols, long long group_stride, int act, int dtype, int* err, int sms,
                           cudaStream_t st);
@@ -764,6 +765,31 @@ int spd_cross_attn_packed(const void* q, int64_t q_stride_t, int64_t q_stride_h,
   const spd::SpanTensors t{q, k, v, q_stride_t, q_stride_h, kv_stride_t, kv_stride_h, kv_stride_slot};
   const int rc = spd::span_attn_launch(p, t, dtype, sms, static_cast<cudaStream_t>(stream));
   if (rc != SPD_OK) return fail(rc, "spd_cross_attn_packed: launch failed: %s", cudaGetErrorString(cudaGetLastError()));
+  return ok();
+}
+
+int spd_sample_rows(const void* x, int rows, int cols, int64_t ld, const uint8_t* skip_mask, const float* uniforms,
+                    const float* temperature, float temperature_all, const int32_t* top_k, int top_k_all,
+                    const float* top_p, float top_p_all, const float* min_p, float min_p_all, int64_t* out,
+                    float* logprobs, int dtype, void* stream) {
+  const int eb = elem_bytes(dtype);
+  if (!eb) return fail(SPD_ERR_UNSUPPORTED, "spd_sample_rows: dtype %d not supported", dtype);
+  if (rows < 0 || cols <= 0 || ld < cols) return fail(SPD_ERR_INVALID_ARG, "spd_sample_rows: bad sizes rows=%d cols=%d", rows, cols);
+  if (rows == 0) return ok();
+  if (!x || !uniforms || !out) return fail(SPD_ERR_INVALID_ARG, "spd_sample_rows: null pointer");
+  if (cols > (1 << 19)) return fail(SPD_ERR_UNSUPPORTED, "spd_sample_rows: more than 2^19 columns");
+  const int sms = sm_count(-1);
+  if (sms <= 0) return fail(SPD_ERR_CUDA, "spd_sample_rows: no CUDA device");
+  spd::SampleParams p{};
+  p.x = x; p.skip = skip_mask; p.uniforms = uniforms;
+  p.temperature = temperature; p.top_k = top_k; p.top_p = top_p; p.min_p = min_p;
+  p.temperature_all = temperature_all; p.top_k_all = top_k_all; p.top_p_all = top_p_all; p.min_p_all = min_p_all;
+  p.out = reinterpret_cast<long long*>(out); p.logprobs = logprobs;
+  p.rows = rows; p.cols = cols; p.ld = ld;
+  p.vec = aligned16(x) && (ld * eb) % 16 == 0;
+  p.skip_vec = (reinterpret_cast<uintptr_t>(skip_mask) & 7u) == 0;
+  const int rc = spd::sample_rows_launch(p, dtype, sms, static_cast<cudaStream_t>(stream));
+  if (rc != SPD_OK) return fail(rc, "spd_sample_rows: launch failed: %s", cudaGetErrorString(cudaGetLastError()));
   return ok();
 }
 

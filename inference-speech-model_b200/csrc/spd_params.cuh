@@ -108,6 +108,24 @@ struct ArgmaxParams {  // greedy token pick over rows (decoder_layer_ops.cu)
   int vec;           // rows start 16-byte aligned: 16-byte loads
 };
 
+struct SampleParams {  // a token a row by temperature, top-k, top-p, min-p (sample_rows.cu)
+  const void* x;
+  const unsigned char* skip;  // [cols] or null: columns that count as -inf
+  const float* uniforms;      // [rows]
+  const float* temperature;   // [rows], or null: the same for all; so the next three
+  const int* top_k;
+  const float* top_p;
+  const float* min_p;
+  float temperature_all;
+  int top_k_all;
+  float top_p_all, min_p_all;
+  long long* out;   // int64 [rows]
+  float* logprobs;  // [rows] or null
+  int rows, cols;
+  long long ld;     // elements between rows
+  int vec, skip_vec;  // rows allow loads of 16 bytes, the mask loads of 8
+};
+
 struct GatherParams {
   const unsigned char* pool;
   const int* block_tables;

@@ -1,7 +1,7 @@
 // torch_binding.cpp — CPython module that takes torch tensors straight to the C ABI for the
 // operators a decode step calls once per layer (rope_kv_append, rope_kv_append_int4,
 // kv_gather_int4, paged_decode_attention_int4, prompt_attention, shared_prefix_decode_attention,
-// cross_attention_packed).
+// cross_attention_packed, sample_rows).
 //
 // Their kernels take a few microseconds, while checking some fifteen tensors from Python and
 // converting thirty arguments through ctypes took 8 to 11 (append of a 64-request step: 14.7 us
@@ -40,6 +40,7 @@ decltype(&spd_get_last_error) f_last_error;
 decltype(&spd_stream_capture_id) f_capture_id;
 decltype(&spd_shared_prefix_attn) f_prefix;
 decltype(&spd_shared_prefix_attn_workspace_size) f_prefix_size;
+decltype(&spd_sample_rows) f_sample;
 decltype(&spd_cross_attn_packed) f_cross;
 decltype(&spd_cross_attn_packed_workspace_size) f_cross_size;
 
@@ -530,6 +531,70 @@ at::Tensor cross(const char* name, PyObject* const* a, Py_ssize_t n_args) {
   return out;
 }
 
+// A setting of sample_rows: a number for all rows, or a tensor with one for each.
+struct Setting {
+  const void* rows = nullptr;
+  double all = 0.0;
+};
+Setting setting(const char* name, const char* what, PyObject* o, int64_t rows, at::ScalarType type) {
+  Setting s;
+  if (!THPVariable_Check(o)) {
+    s.all = number(name, what, o);
+    return s;
+  }
+  const at::Tensor& t = THPVariable_Unpack(o);
+  if (t.scalar_type() != type || t.dim() != 1 || t.size(0) != rows || !t.is_contiguous())
+    refuse(name, what, " must be a number or a contiguous ", c10::toString(type), " [", rows, "] tensor");
+  s.rows = ptr(t);
+  return s;
+}
+
+// (x, uniforms, temperature, top_k, top_p, min_p, cols, skip, out, logprobs)
+at::Tensor sample(const char* name, PyObject* const* a, Py_ssize_t n_args) {
+  count(name, n_args, 10);
+  const at::Tensor &x = tensor(name, "x", a[0]), &u = tensor(name, "uniforms", a[1]), &skip = tensor(name, "skip", a[7], true),
+                   &given = tensor(name, "out", a[8], true), &logs = tensor(name, "logprobs", a[9], true);
+  std::vector<const at::Tensor*> all{&x, &u, &skip, &given, &logs};
+  for (int i = 2; i < 6; ++i)
+    if (THPVariable_Check(a[i])) all.push_back(&THPVariable_Unpack(a[i]));
+  for (const at::Tensor* t : all) current_device(name, {t});
+  if (x.dim() != 2 || (x.stride(1) != 1 && x.size(1) > 1)) refuse(name, "x must be [rows, ld] with unit column stride");
+  const int rows = small_int(name, "rows", x.size(0));
+  int64_t cols = x.size(1);
+  if (a[6] != Py_None) {
+    cols = PyLong_AsLongLong(a[6]);
+    if (PyErr_Occurred()) {
+      PyErr_Clear();
+      refuse(name, "cols must be an integer");
+    }
+  }
+  if (cols <= 0 || cols > x.size(1)) refuse(name, "cols ", cols, " outside [1, ", x.size(1), "]");
+  if (u.scalar_type() != at::kFloat || u.dim() != 1 || u.size(0) != rows || !u.is_contiguous())
+    refuse(name, "uniforms must be a contiguous float32 [", rows, "] tensor");
+  if (skip.defined() && (skip.scalar_type() != at::kBool || skip.numel() < cols || !skip.is_contiguous()))
+    refuse(name, "skip must be a contiguous bool mask of at least cols entries");
+  const Setting t = setting(name, "temperature", a[2], rows, at::kFloat), k = setting(name, "top_k", a[3], rows, at::kInt),
+                tp = setting(name, "top_p", a[4], rows, at::kFloat), mp = setting(name, "min_p", a[5], rows, at::kFloat);
+  if (!(k.all >= INT32_MIN && k.all <= INT32_MAX) || k.all != (double)(int)k.all) refuse(name, "top_k must be a whole number");
+  if (given.defined() && (given.scalar_type() != at::kLong || given.dim() != 1 || given.size(0) != rows || !given.is_contiguous()))
+    refuse(name, "out must be a contiguous int64 [", rows, "] tensor");
+  if (logs.defined() && (logs.scalar_type() != at::kFloat || logs.dim() != 1 || logs.size(0) != rows || !logs.is_contiguous()))
+    refuse(name, "logprobs must be a contiguous float32 [", rows, "] tensor");
+  const int code = dtype_code(name, x.scalar_type());
+  const at::Tensor out = given.defined() ? given : at::empty({rows}, x.options().dtype(at::kLong));
+  for (const at::Tensor* w : {&out, &logs})
+    for (const at::Tensor* o : all)
+      if (w->defined() && o->defined() && !w->is_same(*o) && overlap(*w, *o)) refuse(name, "out and logprobs must be apart from all else");
+  const int64_t ld = rows > 1 ? x.stride(0) : x.size(1);
+  if (ld < cols) refuse(name, "rows of x overlap");
+  check(f_sample(ptr(x), rows, (int)cols, ld, static_cast<const uint8_t*>(ptr(skip)), static_cast<const float*>(ptr(u)),
+                 static_cast<const float*>(t.rows), (float)t.all, static_cast<const int32_t*>(k.rows), (int)k.all,
+                 static_cast<const float*>(tp.rows), (float)tp.all, static_cast<const float*>(mp.rows), (float)mp.all,
+                 static_cast<int64_t*>(mut(out)), static_cast<float*>(mut(logs)), code, stream()),
+        name);
+  return out;
+}
+
 // Runs `body` with every C++ exception turned into a Python RuntimeError.
 template <typename F>
 PyObject* guarded(const F& body) {
@@ -573,6 +638,9 @@ PyObject* py_prompt(PyObject*, PyObject* const* a, Py_ssize_t n) {
 PyObject* py_prefix(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&] { return wrap(prefix("shared_prefix_attn", a, n)); });
 }
+PyObject* py_sample(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&] { return wrap(sample("sample_rows", a, n)); });
+}
 PyObject* py_cross(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&] { return wrap(cross("cross_attn_packed", a, n)); });
 }
@@ -591,7 +659,7 @@ PyObject* py_setup(PyObject*, PyObject* d) {
       get("spd_paged_decode_attn_int4_workspace_size", f_decode_size) && get("spd_prompt_attn", f_prompt) &&
       get("spd_kv_int4_page_bytes", f_page_bytes) && get("spd_get_last_error", f_last_error) &&
       get("spd_stream_capture_id", f_capture_id) && get("spd_shared_prefix_attn", f_prefix) &&
-      get("spd_shared_prefix_attn_workspace_size", f_prefix_size) && get("spd_cross_attn_packed", f_cross) &&
+      get("spd_shared_prefix_attn_workspace_size", f_prefix_size) && get("spd_cross_attn_packed", f_cross) && get("spd_sample_rows", f_sample) &&
       get("spd_cross_attn_packed_workspace_size", f_cross_size))
     Py_RETURN_NONE;
   return nullptr;
@@ -605,6 +673,7 @@ PyMethodDef methods[] = {
     {"paged_decode_attention_int4", reinterpret_cast<PyCFunction>(py_decode), METH_FASTCALL, nullptr},
     {"prompt_attention", reinterpret_cast<PyCFunction>(py_prompt), METH_FASTCALL, nullptr},
     {"shared_prefix_decode_attention", reinterpret_cast<PyCFunction>(py_prefix), METH_FASTCALL, nullptr},
+    {"sample_rows", reinterpret_cast<PyCFunction>(py_sample), METH_FASTCALL, nullptr},
     {"cross_attention_packed", reinterpret_cast<PyCFunction>(py_cross), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 

@@ -68,6 +68,7 @@ _SIGNATURES = {
                         + [_f, _i, _vp, _vp]),
     "spd_shared_prefix_attn_workspace_size": (_sz, [_i] * 9),
     "spd_shared_prefix_attn": (_i, [_vp, _i64, _i64] + [_vp] * 8 + [_i] * 9 + [_f, _i, _vp, _sz, _vp, _vp]),
+    "spd_sample_rows": (_i, [_vp, _i, _i, _i64, _vp, _vp, _vp, _f, _vp, _i, _vp, _f, _vp, _f, _vp, _vp, _i, _vp]),
     "spd_cross_attn_packed_workspace_size": (_sz, [_i] * 5),
     "spd_cross_attn_packed": (_i, [_vp, _i64, _i64, _vp, _vp, _i64, _i64, _i64] + [_vp] * 4 + [_i] * 7
                               + [_f, _i, _vp, _sz, _vp, _vp]),

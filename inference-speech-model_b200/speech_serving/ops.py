@@ -28,11 +28,12 @@ key/value heads and a 4-bit cache:
 and for several candidates (samples, beams) of one request:
   shared_prefix_decode_attention        single-token attention over a shared prefix and own tokens
   cross_attention_packed                any number of queries a request over the request's slot
+  sample_rows                           a token a row from a given random number, beside argmax_rows
 """
 from __future__ import annotations
 
 import math
-from typing import Dict, Optional, Tuple
+from typing import Dict, Optional, Tuple, Union
 
 import torch
 
@@ -652,3 +653,32 @@ def cross_attention_packed(
     which may be q itself.  Flags as in ``shared_prefix_decode_attention``.  Returns out [N, Hq, D]."""
     return N.binding().cross_attention_packed(q, k, v, valid_lens, cu_seqlens, slot_ids,
                                               q.shape[-1] ** -0.5 if scale is None else scale, out, workspace, error_word)
+
+
+def sample_rows(
+    x: torch.Tensor,
+    uniforms: torch.Tensor,
+    temperature: Union[float, torch.Tensor] = 1.0,
+    top_k: Union[int, torch.Tensor] = 0,
+    top_p: Union[float, torch.Tensor] = 1.0,
+    min_p: Union[float, torch.Tensor] = 0.0,
+    cols: Optional[int] = None,
+    skip: Optional[torch.Tensor] = None,
+    out: Optional[torch.Tensor] = None,
+    logprobs: Optional[torch.Tensor] = None,
+) -> torch.Tensor:
+    """Draws a token from the first ``cols`` columns of each row of ``x`` [rows, ld] (fp32 / fp16 / bf16, unit column
+    stride) with the row's random number uniforms[r] (float32 [rows], in [0, 1)); ``skip``, a bool [cols] mask or
+    None, marks columns that count as -inf.
+
+    temperature, top_k, top_p and min_p are numbers, or tensors with one for each row (float32, top_k int32).  With the
+    row's largest value m and w = exp((x - m) / temperature): top_k > 0 leaves the top_k largest (equal ones by their
+    place); of these, in that order, top_p < 1 leaves those before which less than top_p of their weight lies; of
+    these min_p > 0 leaves those with x >= m + temperature log(min_p); each leaves at least one.  The token is the
+    first column, by its place, at which the weight of what is left so far passes uniforms[r] times all of it, as
+    fp64 arithmetic decides.  A temperature <= 0 picks the first largest column, and so does a row whose largest value
+    is not finite (a NaN wins), as ``argmax_rows`` does.
+
+    Returns int64 [rows].  ``logprobs`` (float32 [rows]), if given, receives the tokens' log-probabilities under
+    softmax(x) over the columns not skipped (temperature 1, nothing cut)."""
+    return N.binding().sample_rows(x, uniforms, temperature, top_k, top_p, min_p, cols, skip, out, logprobs)
