@@ -5,16 +5,21 @@
 //   its place, at which the weight left so far passes u times all of it.
 //
 // What bounds it: a row is read once from memory, 2 or 4 bytes a column, and again from L1 or L2 by each later pass; the
-// work is a few dozen instructions a column.  Nothing is sorted:
-// * A cluster of up to 8 CTAs shares a row.  A cut (the k-th largest, or the value at which the weight reaches p)
-//   is found by histograms: 1,024 bins over the distance from m, then over the order-preserving integers of the values in
-//   the bin that holds the cut, until a bin holds one value.  Equal values that the cut divides count by their place.
+// passes' instructions, some 50 a column in all, are what takes the time.  Nothing is sorted:
+// * A cluster of up to 4 CTAs shares a row.  A cut (the k-th largest, or the value at which the weight reaches p) is
+//   found by histograms.  The first counts columns by their distance from m (one atomic a column).  For the k-th largest
+//   the cut lies in one of its bins.  For p each bin's weight is known to within 1 %, so the cut
+//   lies in a few; the next pass adds up the weights above, in and below these, and only the columns in them, a hundredth of
+//   the whole, enter a histogram of weights.  Later passes look at the order-preserving integers of the values in the bin
+//   that holds the cut, until a bin holds one value.  Equal values that the cut divides count by their place.
 // * Every sum of weights is an integer (units of 2^-44 of the largest weight), so no order of atomics or threads changes a
 //   result, and cumulative sums are exact in their weights.
-// * Weights are computed twice as precisely as fp32 needs where it matters: the exponent's argument in fp64, then the
-//   hardware's 2^f (2^-22).  A decision that an error of 2^-20 of the whole could turn is
-//   taken again with weights in fp64 (a few rows in a hundred where a hundred thousand columns are alike, else next to
-//   none), so that the token is the one that fp64 arithmetic gives.
+// * Weights are the hardware's 2^f (2^-22) of an argument that keeps the rounding of x - m.  A decision that an error of
+//   2^-20 of the whole could turn is taken again with weights in fp64 (one row in ten where a hundred thousand columns
+//   weigh alike, else next to none), so that the token is the one that fp64 arithmetic gives.
+// * A CTA's columns lie in its shared memory, and what is known of the row beside them: passes are functions that are
+//   called, so that none holds another's registers.  (In one function the state went to local memory, whose traffic
+//   was twice that of the columns: 87 us for the 64 rows of 51,865 columns below.)
 #include "spd_params.cuh"
 
 #include <cooperative_groups.h>
@@ -28,14 +33,16 @@ typedef unsigned long long u64;
 
 constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
-constexpr int kBins = 1024;
+constexpr int kFirst = 4096;      // bins of the first histogram (counts)
+constexpr int kBins = 512;        // of the later ones (counts and weights)
 constexpr int kMaxChunks = 1024;  // of a CTA's columns
+constexpr int kCtas = 8;          // of a cluster, at most
 constexpr int kScale = 44;        // a weight of 1 is 2^44: sums of 2^19 columns fit in 64 bits
 
 // a value's place among all values: the larger, the larger (values of 16 bits leave low bits unused)
 template <typename T> constexpr int unused_bits() { return sizeof(T) == 4 ? 0 : std::is_same<T, __half>::value ? 13 : 16; }
 template <typename T> __device__ __forceinline__ unsigned place_of(float x) {
-  const unsigned b = __float_as_uint(x);
+  const unsigned b = __float_as_uint(x + 0.f);  // (-0 is 0)
   return (b & 0x80000000u ? ~b : b | 0x80000000u) >> unused_bits<T>();
 }
 template <typename T> __device__ __forceinline__ float value_of(unsigned place) {  // of a place that some value has
@@ -43,23 +50,12 @@ template <typename T> __device__ __forceinline__ float value_of(unsigned place) 
   return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~(k | ((1u << unused_bits<T>()) - 1u)));
 }
 
-struct Best {
-  float v;
-  int i;
-};
-// a beats b: NaN over numbers, larger value, then the lower index
-__device__ __forceinline__ bool better(Best a, Best b) {
-  const bool an = a.v != a.v, bn = b.v != b.v;
-  if (an || bn) return an && (!bn || a.i < b.i);
-  return a.v > b.v || (a.v == b.v && a.i < b.i);
-}
-
 // What CTAs of a cluster tell one another: written before, read after a cluster barrier.
 struct Told {
-  Best best;
-  int count;
-  u64 sum;
-  float z;
+  float mx, z;
+  int count, first, last;
+  u64 sum, inside, below;
+  float least, most;
 };
 // The bin that holds a cut, and what lies above it.
 struct Cut {
@@ -69,86 +65,67 @@ struct Cut {
   int open;  // the decision could be another with exact weights
 };
 
-// The E columns that a thread loads at a time, taken one by one (`next`): the code that looks at a column exists once
-// a pass, not E times (unrolled, the kernel had 380 KB).
-template <typename T> struct Columns {
-  static constexpr int E = 16 / sizeof(T);
-  u64 a, b, skip;
-  __device__ __forceinline__ float next() {
-    float v;
-    if constexpr (sizeof(T) == 4) {
-      v = __uint_as_float((unsigned)a);
-      a = a >> 32 | b << 32;
-      b >>= 32;
-    } else {
-      const unsigned short h = (unsigned short)a;
-      v = Elem<T>::to_f(*reinterpret_cast<const T*>(&h));
-      a = a >> 16 | b << 48;
-      b >>= 16;
-    }
-    if (skip & 0xff) v = -INFINITY;
-    skip >>= 8;
-    return v + 0.f;  // no -0
-  }
+// What a pass over the row does with its columns.
+enum Pass { kMax, kSeek, kCount, kWeigh, kRefine, kSum, kDone };
+
+// What is known of the row: the same in all CTAs of its cluster but for the first line.
+struct State {
+  int rank, first_column, vectors, chunk, chunks;
+  int ctas, k;
+  float t, top_p, min_p;
+  double u;
+  Pass pass;
+  int token;
+  bool by_count, exact, z_due;
+  float m, xmin, hi, lo;  // the largest value, the least that min-p leaves, log2(e) / t in two parts
+  float xt, xt0, xt_k;    // what is left: values above xt, and the first `ties` columns that have it;
+  int ties, ties0, ties_k;  // as the cut under way found it; as top-k left it
+  // the cut under way: bins [first, last] of the first histogram, places [from, to] among them, `shift` bits of a bin's
+  int k_left, first, last, shift;
+  unsigned from, to;
+  float inv;
+  u64 whole, above;
+  double target;
 };
-// A row's columns of one CTA, in chunks of a warp (32 * E columns at a time).
-template <typename T> struct Row {
-  static constexpr int E = 16 / sizeof(T);
-  const T* x;
-  const unsigned char* mask;
-  int lo, hi, chunk, chunks;
-  bool vec, mask_vec;  // loads of 16 bytes, of E mask bytes
-  // columns c .. c + E - 1; those past the end count as suppressed
-  __device__ __forceinline__ Columns<T> load(int c) const {
-    Columns<T> v{0, 0, 0};
-    const bool whole = c + E <= hi;
-    if (vec && whole) {
-      const ulonglong2 w = *reinterpret_cast<const ulonglong2*>(x + c);
-      v.a = w.x;
-      v.b = w.y;
-    } else {
-#pragma unroll 1
-      for (int k = E - 1; k >= 0; --k) {
-        unsigned bits = 0;
-        if (c + k < hi) {
-          if constexpr (sizeof(T) == 4) bits = *reinterpret_cast<const unsigned*>(x + c + k);
-          else bits = *reinterpret_cast<const unsigned short*>(x + c + k);
-        } else {
-          v.skip |= 0xffull << (8 * k);
-        }
-        constexpr int kBits = 8 * sizeof(T);
-        v.b = v.b << kBits | v.a >> (64 - kBits);
-        v.a = v.a << kBits | bits;
-      }
-    }
-    if (mask) {
-      if (mask_vec && whole) {
-        if constexpr (E == 4) v.skip = *reinterpret_cast<const unsigned*>(mask + c);
-        else v.skip = *reinterpret_cast<const u64*>(mask + c);
-      } else {
-#pragma unroll 1
-        for (int k = 0; k < E && c + k < hi; ++k)
-          if (mask[c + k]) v.skip |= 0xffull << (8 * k);
-      }
-    }
-    return v;
-  }
+// A CTA's columns follow it: vectors of 16 bytes that lie on 16-byte boundaries of the row (so the first may begin before
+// it), in chunks of a warp, 32 vectors at a time.  Suppressed columns, and those that there are not, hold -inf.
+struct Shared {
+  State st;
+  Cut cut;
+  Told told[4];
+  float z[kWarps], floats[3][kWarps];
+  int counts[3][kWarps], chunk_ties[kMaxChunks];
+  u64 sums[3][kWarps], chunk_sum[kMaxChunks];
+  unsigned first_count[kFirst], count[kBins], low[kBins], high[kBins];
 };
+constexpr size_t kSharedBytes = (sizeof(Shared) + 127) / 128 * 128;
+constexpr size_t kMostBytes = 226 * 1024, kGoodBytes = 112 * 1024;  // of a CTA's shared memory
+extern __shared__ __align__(128) unsigned char shared_bytes[];
+__device__ __forceinline__ Shared& shared() { return *reinterpret_cast<Shared*>(shared_bytes); }
 
 // The weight of a value, in units of 2^-44.
 __device__ __noinline__ u64 exact_weight(double below, double t) {
   return (u64)(exp(below / t) * (double)(1ull << kScale) + 0.5);
 }
-struct Weight {
-  double m, per, t;  // the largest value, log2(e) / t, t
+template <typename T> struct Weight {
+  float m, hi, lo;  // the largest value, and log2(e) / t in two parts
+  double t;
   bool exact;
+  __device__ __forceinline__ explicit Weight(const State& st) : m(st.m), hi(st.hi), lo(st.lo), t(st.t), exact(st.exact) {}
   __device__ __forceinline__ u64 operator()(float x) const {
-    const double below = (double)x - m;  // <= 0
-    if (exact) return exact_weight(below, t);
-    const double y = fmax(below * per, -100.0);
-    const int n = __double2int_rn(y);
-    const unsigned b = __float_as_uint(ex2_approx((float)(y - (double)n)));  // in [2^-1/2, 2^1/2]
-    const int shift = kScale - 23 + n + (int)(b >> 23) - 127;
+    if (exact) return exact_weight((double)x - (double)m, t);
+    const float d = x - m;  // <= 0
+    const float n = fmaxf(rintf(d * hi), -100.f);
+    // d * log2(e) / t - n, with what the subtraction rounded off (16-bit values: next to nothing)
+    float f = fmaf(d, hi, -n);
+    float rest = d * lo;
+    if constexpr (sizeof(T) == 4) {
+      const float b = d - x, a = d - b;
+      rest = fmaf((x - a) - (m + b), hi, rest);
+    }
+    f = fminf(f + rest, 1.f);
+    const unsigned b = __float_as_uint(ex2_approx(f));
+    const int shift = kScale - 23 + (int)n + (int)(b >> 23) - 127;
     const u64 bits = (b & 0x7fffffu) | 0x800000u;
     return shift >= 0 ? bits << shift : shift > -25 ? bits >> -shift : 0;
   }
@@ -171,445 +148,711 @@ template <typename V> __device__ __forceinline__ V warp_inclusive(V v) {
   return v;
 }
 
-// What a pass over the row does with its columns.
-enum Pass { kMax, kBin, kSum, kLog };
+// What lies before this thread's v in the CTA, and the whole of it (slots: one a warp).
+template <typename V> __device__ __forceinline__ V before_thread(V v, V* slots, V& whole) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const V incl = warp_inclusive(v);
+  if (lane == 31) slots[warp] = incl;
+  __syncthreads();
+  const V of_warps = warp_inclusive(lane < kWarps ? slots[lane] : V(0));
+  whole = __shfl_sync(0xffffffffu, of_warps, 31);
+  const V before = __shfl_sync(0xffffffffu, of_warps, max(warp - 1, 0));
+  return (warp ? before : V(0)) + incl - v;
+}
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const SampleParams p) {
-  cg::cluster_group cluster = cg::this_cluster();
-  __shared__ unsigned count[kBins], low[kBins], high[kBins];
-  __shared__ u64 chunk_sum[kMaxChunks];
-  __shared__ int chunk_ties[kMaxChunks];
-  __shared__ Told told[4];
-  __shared__ Cut cut_here;
-  __shared__ Best bests[kWarps];
-  __shared__ float zs[kWarps];
-  __shared__ u64 sums[kWarps];
-  __shared__ int counts[kWarps];
+// All CTAs of the cluster, and what they wrote before.
+__device__ __forceinline__ void together(int ctas) {
+  if (ctas > 1) cg::this_cluster().sync();
+  else __syncthreads();
+}
+// The shared memory of CTA i.
+__device__ __forceinline__ Shared& of_cta(int i) { return *cg::this_cluster().map_shared_rank(&shared(), i); }
 
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
-  const long long r = (long long)blockIdx.x / C;
-  constexpr int E = Row<T>::E, kUnit = 32 * E;
-  Row<T> row;
-  row.x = reinterpret_cast<const T*>(p.x) + r * p.ld;
-  row.mask = p.skip;
-  row.vec = p.vec;
-  row.mask_vec = p.skip_vec;
-  {
-    const int per = ((p.cols + C - 1) / C + kUnit - 1) / kUnit * kUnit;  // columns of a CTA
-    row.lo = (int)min((long long)p.cols, (long long)rank * per);
-    row.hi = (int)min((long long)p.cols, (long long)row.lo + per);
-    row.chunk = ((per / kUnit + kMaxChunks - 1) / kMaxChunks) * kUnit;
-    row.chunks = (row.hi - row.lo + row.chunk - 1) / row.chunk;
+// f(column, value) for the columns of this CTA, and g(chunk) after each chunk
+template <typename T, typename F, typename G> __device__ __forceinline__ void each(F&& f, G&& g) {
+  constexpr int E = 16 / sizeof(T);
+  const State& st = shared().st;
+  const uint4* at = reinterpret_cast<const uint4*>(shared_bytes + kSharedBytes);
+  const int lane = threadIdx.x & 31, vectors = st.vectors, chunk = st.chunk, chunks = st.chunks, first = st.first_column;
+#pragma unroll 1
+  for (int ch = threadIdx.x >> 5; ch < chunks; ch += kWarps) {
+    const int end = min(vectors, (ch + 1) * chunk);
+#pragma unroll 1
+    for (int j = ch * chunk + lane; j < end; j += 32) {
+      const uint4 w = at[j];
+      const T* e = reinterpret_cast<const T*>(&w);
+#pragma unroll
+      for (int k = 0; k < E; ++k) f(first + E * j + k, Elem<T>::to_f(e[k]));
+    }
+    __syncwarp();
+    g(ch);
   }
-  const float t = p.temperature ? p.temperature[r] : p.temperature_all;
-  const int k = p.top_k ? p.top_k[r] : p.top_k_all;
-  const float top_p = p.top_p ? p.top_p[r] : p.top_p_all;
-  const float min_p = p.min_p ? p.min_p[r] : p.min_p_all;
-
-  int token = -1;  // known to every thread once it is
-  Best best{-INFINITY, 0x7fffffff};
-  float m = 0.f, z = 0.f;  // the largest value; sum of exp(x - m)
-  bool z_due = p.logprobs != nullptr;
-  float xmin = -INFINITY;  // min-p
-  float xt = -INFINITY;    // what is left: values above xt, and the first `ties` columns that have it
-  int ties = 0x7fffffff;
-  Weight weight{0.0, 0.0, 1.0, false};
-  // a cut under way
-  bool by_count = false;
-  float xt0 = xt, xt_k = xt, inv = 0.f;
-  int ties0 = ties, ties_k = ties, k_left = 0, bin1 = -1, shift = 0;
-  unsigned from = 0, to = 0;
-  u64 whole = 0, above = 0;
-  double target = 0.0;
-
-  auto bin_of = [&](float v) { return (int)fminf((m - v) * inv, (float)(kBins - 1)); };
-  // this value's bin in the present histogram, or -1
-  auto place_in = [&](float v) {
-    const int bin = bin_of(v);
-    if (bin1 < 0) return bin;
-    const unsigned place = place_of<T>(v);
-    return bin == bin1 && place >= from && place <= to ? (int)((to - place) >> shift) : -1;
-  };
-  auto put = [&](int bin, unsigned n, u64 w) {
-    atomicAdd(&count[bin], n);
-    if (w) {
-      const unsigned l = (unsigned)w, old = atomicAdd(&low[bin], l), h = (unsigned)(w >> 32) + (old + l < old);
-      if (h) atomicAdd(&high[bin], h);
-    }
-  };
-  auto begin_cut = [&](bool count_them) {
-    by_count = count_them;
-    xt0 = xt;
-    ties0 = ties;
-    k_left = k;
-    bin1 = -1;
-    whole = above = 0;
-    inv = (float)(kBins - 1) / (by_count ? 32.f : 40.f * t);
-  };
-
-  Pass pass = kMax;
-#pragma unroll 1
-  while (true) {
-    // ---- one pass over the row ----------------------------------------------------------------------
-    if (pass == kBin) {
-#pragma unroll 1
-      for (int i = tid; i < kBins; i += kThreads) count[i] = low[i] = high[i] = 0;
-      __syncthreads();
-      if (!by_count && xt0 > -INFINITY && rank == 0 && tid == 0) {  // columns that have xt0 itself, by their number
-        const int bin = place_in(xt0);
-        if (bin >= 0) put(bin, (unsigned)ties0, weight(xt0) * (u64)ties0);
-      }
-    }
-    u64 mine = 0;
-    int mine_ties = 0;
-#pragma unroll 1
-    for (int ch = warp; ch < row.chunks; ch += kWarps) {
-      u64 s = 0;
-      int n = 0;
-      const int end = min(row.hi, row.lo + (ch + 1) * row.chunk);
-#pragma unroll 1
-      for (int c = row.lo + ch * row.chunk + lane * E; c < end; c += kUnit) {
-        Columns<T> v4 = row.load(c);
-#pragma unroll 1
-        for (int e = 0; e < E; ++e) {
-          const float v = v4.next();
-          if (pass == kMax) {
-            const Best b{v, c + e};
-            if (c + e < row.hi && better(b, best)) best = b;
-            continue;
-          }
-          if (z_due) z += ex2_approx((v - m) * 1.4426950408889634f);
-          if (pass == kBin) {
-            const int bin = v > xt0 ? place_in(v) : -1;
-            if (bin >= 0) put(bin, 1, by_count ? 0 : weight(v));
-          } else if (pass == kSum && v >= xmin) {
-            if (v > xt) s += weight(v);
-            n += v == xt && xt > -INFINITY;
-          }
-        }
-      }
-      if (pass == kSum) {
-        s = warp_total(s);
-        n = warp_total(n);
-        if (lane == 0) chunk_sum[ch] = s, chunk_ties[ch] = n;
-        mine += s;
-        mine_ties += n;
-      }
-    }
-    if (pass != kMax) z_due = false;
-
-    // ---- and what follows from it -------------------------------------------------------------------
-    if (pass == kMax) {
-      auto best_of_warp = [&]() {
-#pragma unroll 1
-        for (int o = 16; o > 0; o >>= 1) {
-          const Best b{__shfl_xor_sync(0xffffffffu, best.v, o), __shfl_xor_sync(0xffffffffu, best.i, o)};
-          if (better(b, best)) best = b;
-        }
-      };
-      best_of_warp();
-      if (lane == 0) bests[warp] = best;
-      __syncthreads();
-      best = lane < kWarps ? bests[lane] : Best{-INFINITY, 0x7fffffff};
-      best_of_warp();
-      if (tid == 0) told[0].best = best;
-      cluster.sync();
-#pragma unroll 1
-      for (int i = 0; i < C; ++i) {
-        const Best b = cluster.map_shared_rank(told, i)[0].best;
-        if (better(b, best)) best = b;
-      }
-      m = best.v;
-      weight = Weight{(double)m, 1.4426950408889634 / (double)t, (double)t, false};
-      if (!(fabsf(m) < INFINITY) || !(t > 0.f)) token = best.i;
-      if (min_p > 0.f && token < 0) {
-        xmin = __double2float_ru((double)m + (double)t * log((double)min_p));
-        if (!(xmin <= m)) token = best.i;
-      }
-      if (token >= 0) {
-        pass = kLog;
-        if (!z_due) break;
-      } else if (k > 0 && k < p.cols) {
-        begin_cut(true);
-        pass = kBin;
-      } else if (top_p < 1.f) {
-        begin_cut(false);
-        pass = kBin;
-      } else {
-        pass = kSum;
-      }
-    } else if (pass == kBin) {
-      // The first bin, of the histograms of all CTAs added, at which the counts reach k_left or the sums the target.
-      cluster.sync();
-      const int per = kBins / C;  // bins of a rank: 1024 (two a thread), 512, 256 or 128
-      const int bins = per > kThreads ? 2 : tid < per ? 1 : 0, first = rank * per + (per > kThreads ? 2 * tid : tid);
-      int n = 0, n0 = 0;
-      u64 s = 0, s0 = 0;
-#pragma unroll 1
-      for (int j = 0; j < bins; ++j) {
-        n0 = n;
-        s0 = s;
-#pragma unroll 1
-        for (int i = 0; i < C; ++i) {
-          n += (int)cluster.map_shared_rank(count, i)[first + j];
-          s += (u64)cluster.map_shared_rank(low, i)[first + j] + ((u64)cluster.map_shared_rank(high, i)[first + j] << 32);
-        }
-      }
-      int incl = warp_inclusive(n);
-      u64 incl_s = warp_inclusive(s);
-      if (lane == 31) counts[warp] = incl, sums[warp] = incl_s;
-      __syncthreads();
-      int all = 0;
-      u64 all_s = 0;
-#pragma unroll 1
-      for (int i = 0; i < kWarps; ++i) {
-        if (i == warp) incl += all, incl_s += all_s;
-        all += counts[i];
-        all_s += sums[i];
-      }
-      if (tid == 0) {
-        told[1].count = all;
-        told[1].sum = all_s;
-        cut_here.bin = -1;
-      }
-      cluster.sync();  // every CTA's totals are there, and no cut found before is read any more
-      int before = 0;
-      u64 before_s = 0;
-      all = 0;
-      all_s = 0;
-#pragma unroll 1
-      for (int i = 0; i < C; ++i) {
-        if (i == rank) before = all, before_s = all_s;
-        const Told& o = cluster.map_shared_rank(told, i)[1];
-        all += o.count;
-        all_s += o.sum;
-      }
-      if (bin1 < 0 && !by_count) {
-        whole = all_s;
-        target = (double)top_p * (double)whole;
-      }
-      int at = before + incl - n;  // above this thread's bins, of this histogram
-      u64 at_s = before_s + incl_s - s;
-#pragma unroll 1
-      for (int j = 0; j < bins; ++j) {
-        const int to_n = before + incl - (j + 1 < bins ? n - n0 : 0);
-        const u64 to_s = before_s + incl_s - (j + 1 < bins ? s - s0 : 0);
-        if (to_n > at) {
-          const double a = (double)(above + at_s), b = (double)(above + to_s);
-          const bool last = to_n == all;  // the cut lies here at the latest
-          const bool starts = by_count ? at < k_left : at == 0 || a < target, ends = by_count ? to_n >= k_left : b >= target || last;
-          if (starts && ends) {
-            const double g = weight.guard(whole);
-            const int open = !by_count && ((at > 0 && fabs(a - target) <= g) || (!last && fabs(b - target) <= g));
-            const Cut f{first + j, at, to_n - at, at_s, to_s - at_s, open};
-#pragma unroll 1
-            for (int i = 0; i < C; ++i) cluster.map_shared_rank(&cut_here, i)[0] = f;
-          }
-        }
-        at = to_n;
-        at_s = to_s;
-      }
-      cluster.sync();
-      const Cut f = cut_here;
-      bool cut_done = f.bin < 0;  // fewer than k: all of it
-      bool open = !cut_done && f.open && !weight.exact;
-      if (!cut_done) {
-        if (bin1 < 0) {  // the first histogram, over distances: the places of the values in the bin lie in [from, to]
-          bin1 = f.bin;
-          const double slack = 1.0 + 0x1p-21;
-          const float top = bin1 ? fminf(m, __double2float_ru((double)m - bin1 / slack / (double)inv)) : m;
-          const float bottom = bin1 == kBins - 1 ? -INFINITY : __double2float_rd((double)m - (bin1 + 1) * slack / (double)inv);
-          to = place_of<T>(top);
-          from = place_of<T>(fmaxf(bottom, -3.402823466e38f));
-          if (unused_bits<T>()) ++to, from -= from > 0;  // (a bound may lie between two values of 16 bits)
-        } else {
-          // (of one value, the columns that are left are counted below)
-          if (shift == 0 && f.inside > 1) open = false;
-          to -= (unsigned)f.bin << shift;
-          from = shift ? max(from, to - ((1u << shift) - 1u)) : to;
-        }
-        k_left -= f.above;
-        above += f.sum_above;
-        if (from == to && !open) {  // one value: how many of the columns that have it
-          xt = value_of<T>(to);
-          if (by_count) {
-            ties = k_left;
-          } else {
-            const u64 w = weight(xt);
-            const double need = w ? (target - (double)above) / (double)w : 1.0, g = w ? weight.guard(whole) / (double)w : 0.0;
-            const double left = fmin(fmax(ceil(need), 1.0), (double)f.inside);
-            open = !weight.exact && ((left > 1.0 && fabs(need - (left - 1.0)) <= g) || (left < f.inside && fabs(need - left) <= g));
-            ties = (int)left;
-          }
-          cut_done = true;
-        } else {
-          shift = 0;
-          while ((to - from) >> shift >= (unsigned)kBins) ++shift;
-        }
-      }
-      if (open) {  // again with exact weights, from this cut's start (decided alike by every thread of the cluster)
-        weight.exact = true;
-        xt = xt_k;
-        ties = ties_k;
-        begin_cut(false);
-      } else if (cut_done) {
-        if (by_count) {
-          xt_k = xt;
-          ties_k = ties;
-        }
-        if (by_count && top_p < 1.f) begin_cut(false);
-        else pass = kSum;
-      }
-    } else if (pass == kSum) {
-      // The CTA, the chunk and the column at which the sum passes u times the whole.
-      if (lane == 0) sums[warp] = mine, counts[warp] = mine_ties;
-      __syncthreads();
-      if (tid == 0) {
-        u64 s = 0;
-        int n = 0;
-#pragma unroll 1
-        for (int i = 0; i < kWarps; ++i) s += sums[i], n += counts[i];
-        told[2].sum = s;
-        told[2].count = n;
-        cut_here.bin = -1;
-      }
-      cluster.sync();
-      const u64 w_tie = xt > -INFINITY ? weight(xt) : 0;
-      u64 before = 0, here = 0;
-      int ties_before = 0, seen = 0;
-      whole = 0;
-#pragma unroll 1
-      for (int i = 0; i < C; ++i) {
-        const Told& o = cluster.map_shared_rank(told, i)[2];
-        const int n = max(0, min(o.count, ties - seen));
-        const u64 s = o.sum + w_tie * (u64)n;
-        if (i == rank) before = whole, here = s, ties_before = seen;
-        whole += s;
-        seen += o.count;
-      }
-      const double u = fmax((double)p.uniforms[r], 0.0);  // (a NaN counts as 0)
-      const double goal = u < 1.0 ? u * (double)whole : (double)whole - 0.5, guard = weight.guard(whole);
-      if (warp == 0 && here > 0 && (before == 0 || (double)before <= goal) && (double)(before + here) > goal) {
-        u64 at = before;
-        int had = ties_before, found = -1;
-#pragma unroll 1
-        for (int ch0 = 0; ch0 < row.chunks && found < 0; ch0 += 32) {  // 32 chunks at a time
-          const int ch = ch0 + lane, n = ch < row.chunks ? chunk_ties[ch] : 0;
-          const int n_incl = warp_inclusive(n), kept = max(0, min(n, ties - (had + n_incl - n)));
-          const u64 s = (ch < row.chunks ? chunk_sum[ch] : 0) + w_tie * (u64)kept, incl = warp_inclusive(s);
-          const unsigned hit = __ballot_sync(0xffffffffu, (double)(at + incl) > goal);
-          const int src = hit ? __ffs(hit) - 1 : 31;
-          at += __shfl_sync(0xffffffffu, hit ? incl - s : incl, src);
-          had += __shfl_sync(0xffffffffu, hit ? n_incl - n : n_incl, src);
-          if (hit) found = ch0 + src;
-        }
-        int column = -1, open = 0;
-        const int end = min(row.hi, row.lo + (found + 1) * row.chunk);
-#pragma unroll 1
-        for (int c0 = row.lo + found * row.chunk; found >= 0 && c0 < end && column < 0; c0 += kUnit) {
-          const int c = c0 + lane * E;
-          const Columns<T> v4 = c < end ? row.load(c) : Columns<T>{0, 0, ~0ull};
-          int n = 0;
-          Columns<T> v = v4;
-#pragma unroll 1
-          for (int e = 0; e < E; ++e) {
-            const float x = v.next();
-            n += x == xt && x >= xmin && xt > -INFINITY;
-          }
-          const int n_incl = warp_inclusive(n);
-          // the sum of this thread's columns, then the column: the second time over from the sum before them
-          u64 incl = 0, s = 0;
-          unsigned hit = 0;
-          int src = 0;
-#pragma unroll 1
-          for (int round = 0; round < 2; ++round) {
-            int rank_tie = had + n_incl - n;
-            u64 sum = round ? at + incl - s : 0;
-            v = v4;
-#pragma unroll 1
-            for (int e = 0; e < E; ++e) {
-              const float x = v.next();
-              u64 w = 0;
-              if (x >= xmin && x > xt) w = weight(x);
-              else if (x >= xmin && x == xt && xt > -INFINITY && rank_tie++ < ties) w = w_tie;
-              if (round && lane == src && column < 0 && w && (double)(sum + w) > goal) {
-                column = c + e;
-                open = (sum > 0 && fabs((double)sum - goal) <= guard) || (sum + w < whole && fabs((double)(sum + w) - goal) <= guard);
-              }
-              sum += w;
-            }
-            if (round == 0) {
-              s = sum;
-              incl = warp_inclusive(s);
-              hit = __ballot_sync(0xffffffffu, (double)(at + incl) > goal);
-              if (!hit) break;
-              src = __ffs(hit) - 1;
-            }
-          }
-          if (hit) {
-            column = __shfl_sync(0xffffffffu, column, src);
-            open = __shfl_sync(0xffffffffu, open, src);
-          }
-          at += __shfl_sync(0xffffffffu, incl, 31);
-          had += __shfl_sync(0xffffffffu, n_incl, 31);
-        }
-        if (lane == 0 && column >= 0) {
-          const Cut f{column, 0, 0, 0, 0, open && !weight.exact};
-#pragma unroll 1
-          for (int i = 0; i < C; ++i) cluster.map_shared_rank(&cut_here, i)[0] = f;
-        }
-      }
-      cluster.sync();
-      if (cut_here.bin >= 0 && cut_here.open) {
-        weight.exact = true;
-        if (top_p < 1.f) {
-          xt = xt_k;
-          ties = ties_k;
-          begin_cut(false);
-          pass = kBin;
-        }
-        cluster.sync();  // (read by all before it is written again)
-      } else {
-        token = cut_here.bin >= 0 ? cut_here.bin : best.i;
-        break;
-      }
-    } else {
-      break;
-    }
+}
+struct Nothing {
+  __device__ __forceinline__ void operator()(int) const {}
+};
+// The sum of exp(x - m), added up by the first pass that looks at the values again.
+struct Z {
+  float m, z = 0.f;
+  bool due;
+  __device__ __forceinline__ explicit Z(const State& st) : m(st.m), due(st.z_due) {}
+  __device__ __forceinline__ void add(float v) {
+    if (due) z += ex2_approx((v - m) * 1.4426950408889634f);
   }
-
-  // ---- the token and its log-probability ------------------------------------------------------------
-  if (p.logprobs) {
+  __device__ __forceinline__ void keep() {
+    if (!due) return;
     z = warp_sum(z);
-    if (lane == 0) zs[warp] = z;
+    if ((threadIdx.x & 31) == 0) shared().z[threadIdx.x >> 5] = z;
+  }
+};
+__device__ __forceinline__ int bin_of(float v, float m, float inv) { return (int)fminf((m - v) * inv, (float)(kFirst - 1)); }
+__device__ __forceinline__ void put(int bin, unsigned n, u64 w) {
+  Shared& sh = shared();
+  atomicAdd(&sh.count[bin], n);
+  if (w) {
+    const unsigned l = (unsigned)w, old = atomicAdd(&sh.low[bin], l), h = (unsigned)(w >> 32) + (old + l < old);
+    if (h) atomicAdd(&sh.high[bin], h);
+  }
+}
+__device__ __forceinline__ void clear_bins() {
+  Shared& sh = shared();
+  for (int i = threadIdx.x; i < kBins; i += kThreads) sh.count[i] = sh.low[i] = sh.high[i] = 0;
+  __syncthreads();
+}
+__device__ __forceinline__ int sub_of(unsigned place, const State& st) {
+  return place >= st.from && place <= st.to ? (int)((st.to - place) >> st.shift) : -1;
+}
+
+// ---- passes ----------------------------------------------------------------------------------------
+template <typename T> __device__ __noinline__ void pass_max() {
+  float m = -INFINITY;
+  each<T>([&](int, float v) { asm("max.NaN.f32 %0, %0, %1;" : "+f"(m) : "f"(v)); }, Nothing{});
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const float w = __shfl_xor_sync(0xffffffffu, m, o);
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(m) : "f"(w));
+  }
+  if ((threadIdx.x & 31) == 0) shared().floats[0][threadIdx.x >> 5] = m;
+}
+// the first column that has the largest value, or the first NaN
+template <typename T> __device__ __noinline__ void pass_seek() {
+  Z z(shared().st);
+  const float m = z.m;
+  int at = 0x7fffffff;
+  each<T>([&](int c, float v) {
+    z.add(v);
+    if (v == m || v != v) at = min(at, max(c, 0));  // (a row without a finite value: its first column)
+  }, Nothing{});
+  z.keep();
+  at = (int)__reduce_min_sync(0xffffffffu, (unsigned)at);
+  if ((threadIdx.x & 31) == 0) shared().counts[0][threadIdx.x >> 5] = at;
+}
+// columns by their distance from the largest
+template <typename T> __device__ __noinline__ void pass_count() {
+  Shared& sh = shared();
+  const float m = sh.st.m, inv = sh.st.inv, xt0 = sh.st.xt0;
+  for (int i = threadIdx.x; i < kFirst; i += kThreads) sh.first_count[i] = 0;
+  __syncthreads();
+  if (!sh.st.by_count && xt0 > -INFINITY && sh.st.rank == 0 && threadIdx.x == 0)  // columns that have xt0 itself, by their number
+    sh.first_count[bin_of(xt0, m, inv)] = (unsigned)sh.st.ties0;
+  __syncthreads();
+  each<T>([&](int, float v) {
+    if (v > xt0) atomicAdd(&shared().first_count[bin_of(v, m, inv)], 1u);
+  }, Nothing{});
+}
+// weights: above the cut's bins (chunk by chunk, too), in them (by their place) and below
+template <typename T> __device__ __noinline__ void pass_weigh() {
+  Shared& sh = shared();
+  const State& st = sh.st;
+  const Weight<T> weight(st);
+  const bool cut = st.top_p < 1.f;
+  const float m = st.m, inv = st.inv, xt0 = st.xt0, xmin = st.xmin;
+  const int first = cut ? st.first : kFirst, last = st.last, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (cut) clear_bins();
+  u64 above = 0, inside = 0, below = 0, mine = 0;
+  if (cut && xt0 > -INFINITY && st.rank == 0 && threadIdx.x == 0) {  // columns that have xt0 itself, by their number
+    const int bin = bin_of(xt0, m, inv);
+    const u64 w = weight(xt0) * (u64)st.ties0;
+    if (bin < first) {
+      above = w;
+    } else if (bin > last) {
+      below = w;
+    } else {
+      inside = w;
+      put(sub_of(place_of<T>(xt0), st), (unsigned)st.ties0, w);
+    }
+  }
+  Z z(st);
+  each<T>([&](int, float v) {
+    z.add(v);
+    if (!(v > xt0)) return;
+    const u64 w = weight(v);
+    const int bin = cut ? bin_of(v, m, inv) : 0;
+    if (bin < first) {
+      above += w;
+      if (v >= xmin) mine += w;
+    } else if (bin > last) {
+      below += w;
+    } else {
+      inside += w;
+      const int sub = sub_of(place_of<T>(v), shared().st);
+      if (sub >= 0) put(sub, 1, w);
+    }
+  }, [&](int ch) {
+    mine = warp_total(mine);
+    if (lane == 0) shared().chunk_sum[ch] = mine;
+    mine = 0;
+  });
+  z.keep();
+  above = warp_total(above), inside = warp_total(inside), below = warp_total(below);
+  if (lane == 0) sh.sums[0][warp] = above, sh.sums[1][warp] = inside, sh.sums[2][warp] = below;
+}
+template <typename T> __device__ __noinline__ void pass_refine() {
+  Shared& sh = shared();
+  const State& st = sh.st;
+  const Weight<T> weight(st);
+  const float m = st.m, inv = st.inv, xt0 = st.xt0;
+  const bool by_count = st.by_count;
+  const int first = st.first, last = st.last, shift = st.shift;
+  const unsigned from = st.from, to = st.to;
+  clear_bins();
+  auto look = [&](float v, unsigned n) {
+    const unsigned place = place_of<T>(v);
+    if (place < from || place > to) return;
+    const int bin = bin_of(v, m, inv);
+    if (bin >= first && bin <= last) put((int)((to - place) >> shift), n, by_count ? 0 : weight(v) * (u64)n);
+  };
+  if (!by_count && xt0 > -INFINITY && st.rank == 0 && threadIdx.x == 0) look(xt0, (unsigned)st.ties0);
+  each<T>([&](int, float v) {
+    if (v > xt0) look(v, 1);
+  }, Nothing{});
+}
+// the chunks' sums completed by what is left of the cut's bins, and the columns that have xt itself
+template <typename T> __device__ __noinline__ void pass_sum() {
+  Shared& sh = shared();
+  const State& st = sh.st;
+  const Weight<T> weight(st);
+  const float m = st.m, inv = st.inv, xt = st.xt, xmin = st.xmin;
+  const int first = st.first, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  u64 mine = 0, all = 0;
+  int n = 0, all_n = 0;
+  each<T>([&](int, float v) {
+    if (!(v >= xt && v >= xmin && v > -INFINITY)) return;
+    if (v == xt) ++n;
+    else if (first < kFirst && bin_of(v, m, inv) >= first) mine += weight(v);
+  }, [&](int ch) {
+    mine = warp_total(mine);
+    n = (int)__reduce_add_sync(0xffffffffu, (unsigned)n);
+    mine += shared().chunk_sum[ch];
+    __syncwarp();
+    if (lane == 0) shared().chunk_sum[ch] = mine, shared().chunk_ties[ch] = n;
+    all += mine, all_n += n;
+    mine = 0, n = 0;
+  });
+  if (lane == 0) sh.sums[0][warp] = all, sh.counts[0][warp] = all_n;
+}
+
+// ---- what follows from them (thread 0 writes the state; every CTA of the cluster comes to the same) ---
+__device__ __forceinline__ void begin_cut(State& st, bool by_count) {
+  st.by_count = by_count;
+  st.xt0 = st.xt;
+  st.ties0 = st.ties;
+  st.k_left = st.k;
+  st.inv = (float)(kFirst - 1) / (by_count ? 32.f : 40.f * st.t);
+  st.pass = kCount;
+}
+__device__ __forceinline__ void again_exactly(State& st) {
+  st.exact = true;
+  st.xt = st.xt_k;
+  st.ties = st.ties_k;
+  begin_cut(st, false);
+  if (!(st.top_p < 1.f)) st.pass = kWeigh, st.first = kFirst;
+}
+__device__ __forceinline__ double guard(const State& st, u64 whole) { return st.exact ? 0.0 : (double)whole * 0x1p-20; }
+// the largest value, and what comes first
+__device__ __noinline__ void after_max() {
+  Shared& sh = shared();
+  State& st = sh.st;
+  const int lane = threadIdx.x & 31;
+  __syncthreads();
+  float m = sh.floats[0][lane % kWarps];
+  auto of_warp = [&]() {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      const float w = __shfl_xor_sync(0xffffffffu, m, o);
+      asm("max.NaN.f32 %0, %0, %1;" : "+f"(m) : "f"(w));
+    }
+  };
+  of_warp();
+  if (st.ctas > 1) {
+    if (threadIdx.x == 0) sh.told[0].mx = m;
+    together(st.ctas);
+    m = lane < st.ctas ? of_cta(lane).told[0].mx : -INFINITY;
+    of_warp();
+  }
+  if (threadIdx.x) return;
+  const double per = 1.4426950408889634 / (double)st.t;
+  st.m = m;
+  st.hi = (float)per;
+  st.lo = (float)(per - st.hi);
+  bool pick_first = !(fabsf(m) < INFINITY) || !(st.t > 0.f);
+  if (st.min_p > 0.f && !pick_first) {
+    st.xmin = __double2float_ru((double)m + (double)st.t * log((double)st.min_p));
+    pick_first = !(st.xmin <= m);
+  }
+  if (pick_first) st.pass = kSeek;
+  else if (st.k > 0) begin_cut(st, true);
+  else if (st.top_p < 1.f) begin_cut(st, false);
+  else st.pass = kWeigh, st.first = kFirst;
+}
+__device__ __noinline__ void after_seek() {
+  Shared& sh = shared();
+  const int lane = threadIdx.x & 31;
+  __syncthreads();
+  int at = (int)__reduce_min_sync(0xffffffffu, (unsigned)sh.counts[0][lane % kWarps]);
+  if (threadIdx.x == 0) sh.told[1].count = at;
+  together(sh.st.ctas);
+  at = (int)__reduce_min_sync(0xffffffffu, lane < sh.st.ctas ? (unsigned)of_cta(lane).told[1].count : 0x7fffffffu);
+  if (threadIdx.x == 0) sh.st.token = at, sh.st.pass = kDone;
+}
+// The bins of the first histogram that hold the cut.
+template <typename T> __device__ __noinline__ void after_count() {
+  Shared& sh = shared();
+  State& st = sh.st;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, C = st.ctas, rank = st.rank, k_left = st.k_left;
+  const bool by_count = st.by_count;
+  together(C);
+  // A thread has 8, 4, 2 or 1 bins of the rank's share of them.  Weights of a bin: between these.
+  const int per = kFirst / kThreads / C, at0 = (rank * kThreads + tid) * per;
+  const float step = (float)(1.4426950408889634 / ((double)st.inv * st.t));
+  auto most_of = [&](int bin) { return bin ? ex2_approx(-bin * step) * (1.f + 2e-5f) : 1.f; };
+  auto least_of = [&](int bin) { return bin + 1 < kFirst ? most_of(bin + 1) * (1.f - 6e-5f) : 0.f; };
+  int n[8], all_n = 0;
+  float least = 0.f, most = 0.f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    n[j] = 0;
+    if (j < per) {
+      unsigned c[kCtas];
+#pragma unroll
+      for (int i = 0; i < kCtas; ++i) c[i] = i < C ? of_cta(i).first_count[at0 + j] : 0;
+#pragma unroll
+      for (int i = 0; i < kCtas; ++i) n[j] += (int)c[i];
+      all_n += n[j];
+      most += n[j] * most_of(at0 + j);
+      least += n[j] * least_of(at0 + j);
+    }
+  }
+  int all;
+  float all_least, all_most;
+  int above_n = before_thread(all_n, sh.counts[0], all);
+  float a_least = before_thread(least, sh.floats[0], all_least), a_most = before_thread(most, sh.floats[1], all_most);
+  if (C > 1) {
+    if (tid == 0) sh.told[1].count = all, sh.told[1].least = all_least, sh.told[1].most = all_most;
+    together(C);
+    const Told& o = of_cta(min(lane, C - 1)).told[1];
+    const int o_n = lane < C ? o.count : 0;
+    const float o_least = lane < C ? o.least : 0.f, o_most = lane < C ? o.most : 0.f;
+    above_n += warp_total(lane < rank ? o_n : 0), a_least += warp_total(lane < rank ? o_least : 0.f);
+    a_most += warp_total(lane < rank ? o_most : 0.f);
+    all = warp_total(o_n), all_least = warp_total(o_least), all_most = warp_total(o_most);
+  }
+  // The bins before the cut's: how many there are in all.  (Sums of fp32 here are off by less than 1e-5 of the whole.)
+  const float off = 2e-5f * all_most, t_least = st.top_p * all_least - off, t_most = st.top_p * all_most + off;
+  int not_yet = 0, below_cut = 0, n_before = 0;  // n_before: columns above the cut's bin, if it is this thread's
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    if (j >= per) break;
+    if (by_count) {
+      if (above_n + n[j] < k_left) ++not_yet;
+      else if (above_n < k_left) n_before = above_n;
+    } else {
+      below_cut += a_least < t_most || above_n == 0;  // may begin below the target
+      a_most += n[j] * most_of(at0 + j);
+      a_least += n[j] * least_of(at0 + j);
+      not_yet += a_most < t_least || above_n + n[j] == 0;  // surely ends below it
+    }
+    above_n += n[j];
+  }
+  not_yet = (int)__reduce_add_sync(0xffffffffu, (unsigned)not_yet);
+  below_cut = (int)__reduce_add_sync(0xffffffffu, (unsigned)below_cut);
+  n_before = (int)__reduce_max_sync(0xffffffffu, (unsigned)n_before);
+  if (lane == 0) sh.counts[0][warp] = not_yet, sh.counts[1][warp] = below_cut, sh.counts[2][warp] = n_before;
+  __syncthreads();
+  if (warp) return;
+  int first = (int)__reduce_add_sync(0xffffffffu, lane < kWarps ? (unsigned)sh.counts[0][lane] : 0u);
+  int last = (int)__reduce_add_sync(0xffffffffu, lane < kWarps ? (unsigned)sh.counts[1][lane] : 0u);
+  int n_above = (int)__reduce_max_sync(0xffffffffu, (unsigned)sh.counts[2][lane % kWarps]);
+  if (lane == 0) sh.told[2].first = first, sh.told[2].last = last, sh.told[2].count = n_above, sh.told[2].mx = (float)(by_count && all < k_left);
+}
+template <typename T> __device__ __noinline__ void after_count_together() {
+  Shared& sh = shared();
+  State& st = sh.st;
+  together(st.ctas);
+  if (threadIdx.x) return;
+  int first = 0, last = 0, n_above = 0;
+#pragma unroll
+  for (int i = 0; i < kCtas; ++i)
+    if (i < st.ctas) {
+      const Told& o = of_cta(i).told[2];
+      first += o.first, last += o.last, n_above = max(n_above, o.count);
+    }
+  if (sh.told[2].mx != 0.f) {  // fewer than k: all of it
+    if (st.top_p < 1.f) begin_cut(st, false);
+    else st.by_count = false, st.pass = kWeigh, st.first = kFirst;
+    return;
+  }
+  if (st.by_count) {
+    last = first;
+    st.k_left -= n_above;
+  } else {
+    first = min(first, kFirst - 1);
+    last = max(first, min(last, kFirst) - 1);
+  }
+  // the places of the values in these bins
+  const double slack = 1.0 + 0x1p-21, m = st.m, inv = st.inv;
+  const float upper = first ? fminf(st.m, __double2float_ru(m - first / slack / inv)) : st.m;
+  const float lower = last == kFirst - 1 ? -INFINITY : __double2float_rd(m - (last + 1) * slack / inv);
+  unsigned to = place_of<T>(upper), from = place_of<T>(fmaxf(lower, -3.402823466e38f));
+  if (unused_bits<T>()) ++to, from -= from > 0;  // (a bound may lie between two values of 16 bits)
+  int shift = 0;
+  while ((to - from) >> shift >= (unsigned)kBins) ++shift;
+  st.first = first, st.last = last, st.to = to, st.from = from, st.shift = shift;
+  st.above = 0;
+  st.pass = st.by_count ? kRefine : kWeigh;
+}
+// The first bin, of the histograms of all CTAs added, at which the counts reach k_left or the sums the target.
+__device__ __noinline__ void find_bin() {
+  Shared& sh = shared();
+  const State& st = sh.st;
+  const int tid = threadIdx.x, lane = tid & 31, C = st.ctas, rank = st.rank, k_left = st.k_left;
+  const bool by_count = st.by_count, weighed = st.pass == kWeigh;
+  if (weighed) {
     __syncthreads();
-    if (tid == 0) {
-      float s = 0.f;
-#pragma unroll 1
-      for (int i = 0; i < kWarps; ++i) s += zs[i];
-      told[3].z = s;
-    }
-    cluster.sync();
+    const u64 above = warp_total(lane < kWarps ? sh.sums[0][lane] : 0), inside = warp_total(lane < kWarps ? sh.sums[1][lane] : 0),
+              below = warp_total(lane < kWarps ? sh.sums[2][lane] : 0);
+    if (tid == 0) sh.told[0].sum = above, sh.told[0].inside = inside, sh.told[0].below = below;
   }
-  if (rank == 0 && tid == 0) {
-    p.out[r] = token;
-    if (p.logprobs) {
-      float s = 0.f;
+  if (tid == 0) sh.cut.bin = -1;  // (the last one was read before this pass)
+  together(C);
+  const int per = kBins / C, at0 = rank * per + tid;  // a thread a bin of the rank's share
+  int n = 0;
+  u64 s = 0;
+  if (tid < per) {
+    unsigned a[kCtas], b[kCtas], c[kCtas];
+#pragma unroll
+    for (int i = 0; i < kCtas; ++i)
+      if (i < C) a[i] = of_cta(i).count[at0], b[i] = of_cta(i).low[at0], c[i] = of_cta(i).high[at0];
+#pragma unroll
+    for (int i = 0; i < kCtas; ++i)
+      if (i < C) n += (int)a[i], s += ((u64)c[i] << 32) + b[i];
+  }
+  u64 whole = st.whole, above = st.above;
+  double target = st.target;
+  if (weighed) {
+    const Told& o = of_cta(min(lane, C - 1)).told[0];
+    above = warp_total(lane < C ? o.sum : 0);
+    whole = above + warp_total(lane < C ? o.inside + o.below : 0);
+    target = (double)st.top_p * (double)whole;
+  }
+  int all;
+  u64 all_s;
+  int at = before_thread(n, sh.counts[0], all);
+  u64 at_s = before_thread(s, sh.sums[0], all_s);
+  if (C > 1) {
+    if (tid == 0) sh.told[1].count = all, sh.told[1].sum = all_s;
+    together(C);
+    const Told& o = of_cta(min(lane, C - 1)).told[1];
+    const int o_n = lane < C ? o.count : 0;
+    const u64 o_s = lane < C ? o.sum : 0;
+    at += warp_total(lane < rank ? o_n : 0), at_s += warp_total(lane < rank ? o_s : 0);
+    all = warp_total(o_n);
+  }
+  if (n > 0) {
+    const int to_n = at + n;
+    const u64 to_s = at_s + s;
+    const double a = (double)(above + at_s), b = (double)(above + to_s);
+    const bool final = to_n == all;  // the cut lies here at the latest
+    const bool starts = by_count ? at < k_left : at == 0 || a < target, ends = by_count ? to_n >= k_left : b >= target || final;
+    if (starts && ends) {
+      const double g = guard(st, whole);
+      const int open = !by_count && ((above + at_s > 0 && fabs(a - target) <= g) || (to_s + above < whole && fabs(b - target) <= g));
+      const Cut f{at0, at, n, at_s, s, open};
 #pragma unroll 1
-      for (int i = 0; i < C; ++i) s += cluster.map_shared_rank(told, i)[3].z;
-      const bool skipped = p.skip && p.skip[token];
-      const float x = skipped ? -INFINITY : Elem<T>::to_f(row.x[token]);
-      p.logprobs[r] = x - m - logf(s);
+      for (int i = 0; i < C; ++i) of_cta(i).cut = f;
     }
   }
-  cluster.sync();  // no CTA leaves while another reads what it told
+  __syncthreads();  // (the state is read above)
+  if (tid == 0 && weighed) sh.st.whole = whole, sh.st.above = above, sh.st.target = target;
+}
+template <typename T> __device__ __noinline__ void after_bin() {
+  Shared& sh = shared();
+  State& st = sh.st;
+  together(st.ctas);
+  if (threadIdx.x) return;
+  const Cut f = sh.cut;
+  bool open = f.open && !st.exact && !(st.shift == 0 && f.inside > 1);  // (one value: its columns are counted below)
+  const unsigned to = st.to - ((unsigned)f.bin << st.shift), from = st.shift ? max(st.from, to - ((1u << st.shift) - 1u)) : to;
+  st.to = to, st.from = from;
+  st.k_left -= f.above;
+  st.above += f.sum_above;
+  if (!open && from == to) {  // one value: how many of the columns that have it
+    st.xt = value_of<T>(to);
+    if (st.by_count) {
+      st.ties = st.k_left;
+      st.xt_k = st.xt0 = st.xt;
+      st.ties_k = st.ties0 = st.ties;
+      if (st.top_p < 1.f) begin_cut(st, false);
+      else st.by_count = false, st.pass = kWeigh, st.first = kFirst;
+      return;
+    }
+    const u64 w = Weight<T>(st)(st.xt);
+    const double need = w ? (st.target - (double)st.above) / (double)w : 1.0, g = w ? guard(st, st.whole) / (double)w : 0.0;
+    const double left = fmin(fmax(ceil(need), 1.0), (double)f.inside);
+    open = !st.exact && ((left > 1.0 && fabs(need - (left - 1.0)) <= g) || (left < f.inside && fabs(need - left) <= g));
+    st.ties = (int)left;
+    if (!open) {
+      st.pass = kSum;
+      return;
+    }
+  }
+  if (open) {  // again with exact weights, from this cut's start
+    again_exactly(st);
+  } else {
+    int shift = 0;
+    while ((to - from) >> shift >= (unsigned)kBins) ++shift;
+    st.shift = shift;
+    st.pass = kRefine;
+  }
+}
+// The CTA, the chunk and the column at which the sum passes u times the whole.
+template <typename T> __device__ __noinline__ void draw() {
+  Shared& sh = shared();
+  State& st = sh.st;
+  constexpr int E = 16 / sizeof(T);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, C = st.ctas, rank = st.rank, ties = st.ties;
+  const float xt = st.xt, xmin = st.xmin;
+  const Weight<T> weight(st);
+  __syncthreads();
+  const u64 mine = warp_total(lane < kWarps ? sh.sums[0][lane] : 0);
+  const int mine_n = warp_total(lane < kWarps ? sh.counts[0][lane] : 0);
+  if (tid == 0) sh.told[3].sum = mine, sh.told[3].count = mine_n, sh.cut.bin = -1;
+  together(C);
+  if (warp == 0) {
+    const u64 w_tie = xt > -INFINITY ? weight(xt) : 0;
+    const Told& o = of_cta(min(lane, C - 1)).told[3];
+    const int o_n = lane < C ? o.count : 0, o_before = warp_inclusive(o_n) - o_n;
+    const u64 o_s = lane < C ? o.sum + w_tie * (u64)max(0, min(o_n, ties - o_before)) : 0, o_incl = warp_inclusive(o_s);
+    const u64 whole = __shfl_sync(0xffffffffu, o_incl, 31), before = __shfl_sync(0xffffffffu, o_incl - o_s, rank),
+              here = __shfl_sync(0xffffffffu, o_s, rank);
+    const int ties_before = __shfl_sync(0xffffffffu, o_before, rank);
+    const double u = st.u, goal = u < 1.0 ? u * (double)whole : (double)whole - 0.5, g = guard(st, whole);
+    if (here > 0 && (before == 0 || (double)before <= goal) && (double)(before + here) > goal) {
+      u64 at = before;
+      int had = ties_before, found = -1;
+#pragma unroll 1
+      for (int ch0 = 0; ch0 < st.chunks && found < 0; ch0 += 32) {  // 32 chunks at a time
+        const int ch = ch0 + lane, n = ch < st.chunks ? sh.chunk_ties[ch] : 0;
+        const int n_incl = warp_inclusive(n), kept = max(0, min(n, ties - (had + n_incl - n)));
+        const u64 s = (ch < st.chunks ? sh.chunk_sum[ch] : 0) + w_tie * (u64)kept, incl = warp_inclusive(s);
+        const unsigned hit = __ballot_sync(0xffffffffu, (double)(at + incl) > goal);
+        const int src = hit ? __ffs(hit) - 1 : 31;
+        at += __shfl_sync(0xffffffffu, hit ? incl - s : incl, src);
+        had += __shfl_sync(0xffffffffu, hit ? n_incl - n : n_incl, src);
+        if (hit) found = ch0 + src;
+      }
+      int column = -1, open = 0;
+      const int end = min(st.vectors, (found + 1) * st.chunk);
+#pragma unroll 1
+      for (int j0 = found * st.chunk; found >= 0 && j0 < end && column < 0; j0 += 32) {
+        const int j = j0 + lane;
+        const uint4 bits = reinterpret_cast<const uint4*>(shared_bytes + kSharedBytes)[min(j, end - 1)];
+        const T* e = reinterpret_cast<const T*>(&bits);
+        auto value = [&](int k) { return j < end ? Elem<T>::to_f(e[k]) : -INFINITY; };
+        auto is_tie = [&](float x) { return x == xt && x >= xmin && x > -INFINITY; };
+        int n = 0;
+#pragma unroll
+        for (int k = 0; k < E; ++k) n += is_tie(value(k));
+        const int n_incl = warp_inclusive(n);
+        // this thread's sum, and then, from what lies before it, the column
+        u64 sum = 0, incl = 0;
+        int src = -1;
+#pragma unroll 1
+        for (int round = 0; round < 2; ++round) {
+          int rank_tie = had + n_incl - n;
+#pragma unroll
+          for (int k = 0; k < E; ++k) {
+            const float x = value(k);
+            u64 w = 0;
+            if (x >= xmin && x > xt) w = weight(x);
+            else if (is_tie(x) && rank_tie++ < ties) w = w_tie;
+            if (lane == src && column < 0 && w && (double)(sum + w) > goal) {
+              column = st.first_column + E * j + k;
+              open = (sum > 0 && fabs((double)sum - goal) <= g) || (sum + w < whole && fabs((double)(sum + w) - goal) <= g);
+            }
+            sum += w;
+          }
+          if (round) break;
+          incl = warp_inclusive(sum);
+          const unsigned hit = __ballot_sync(0xffffffffu, (double)(at + incl) > goal);
+          if (!hit) break;
+          src = __ffs(hit) - 1;
+          sum = at + incl - sum;
+        }
+        if (src >= 0) {
+          column = __shfl_sync(0xffffffffu, column, src);
+          open = __shfl_sync(0xffffffffu, open, src);
+        }
+        at += __shfl_sync(0xffffffffu, incl, 31);
+        had += __shfl_sync(0xffffffffu, n_incl, 31);
+      }
+      if (lane == 0 && column >= 0) {
+        const Cut f{column, 0, 0, 0, 0, open && !st.exact};
+#pragma unroll 1
+        for (int i = 0; i < C; ++i) of_cta(i).cut = f;
+      }
+    }
+  }
+  together(C);
+  if (tid) return;
+  if (sh.cut.bin >= 0 && sh.cut.open) {
+    again_exactly(st);
+  } else {
+    st.token = max(sh.cut.bin, 0);  // (a column is always found: the largest has weight)
+    st.pass = kDone;
+  }
+}
+
+// Copies this CTA's part of the row to shared memory, and clears what does not take part.
+template <typename T> __device__ __forceinline__ void load_row(const SampleParams& p, const T* x) {
+  constexpr int E = 16 / sizeof(T);
+  State& st = shared().st;
+  const int tid = threadIdx.x, C = (int)cg::this_cluster().num_blocks(), rank = (int)cg::this_cluster().block_rank();
+  const int shift = (int)(reinterpret_cast<uintptr_t>(x) % 16 / sizeof(T));  // columns between the boundary and the row
+  const int all = (p.cols + shift + E - 1) / E, per = ((all + C - 1) / C + 31) / 32 * 32, lo = min(all, rank * per);
+  const int vectors = min(all, lo + per) - lo, first_column = E * lo - shift;
+  uint4* columns = reinterpret_cast<uint4*>(shared_bytes + kSharedBytes);
+  // (whole vectors: the row's ends share theirs with columns that are not its own)
+  const uint4* from = reinterpret_cast<const uint4*>(x - shift) + lo;
+#pragma unroll 4
+  for (int j = tid; j < vectors; j += kThreads)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_addr(columns + j)), "l"(from + j) : "memory");
+  if (tid == 0) {
+    st.rank = rank, st.ctas = C;
+    st.first_column = first_column, st.vectors = vectors;
+    st.chunk = (per / 32 / kMaxChunks + 1) * 32;
+    st.chunks = (vectors + st.chunk - 1) / st.chunk;
+  }
+  asm volatile("cp.async.wait_all;" ::: "memory");
+  __syncthreads();
+  T* own = reinterpret_cast<T*>(columns);
+  const T none = Elem<T>::from_f(-INFINITY);
+  if (tid < 2 * E) {
+    const int i = tid < E ? tid : E * vectors - 2 * E + tid;
+    if (i >= 0 && i < E * vectors && (first_column + i < 0 || first_column + i >= p.cols)) own[i] = none;
+  }
+  if (p.skip) {
+    const int begin = max(0, first_column), end = min(p.cols, first_column + E * vectors);
+    // 16 columns a thread where the mask allows it
+    const int head = max(0, min(end - begin, (int)((16 - (reinterpret_cast<uintptr_t>(p.skip + begin) & 15)) & 15)));
+    const int wide = max(0, end - begin - head) / 16;
+#pragma unroll 1
+    for (int j = tid; j < wide; j += kThreads) {
+      const int c = begin + head + 16 * j;
+      const uint4 w = *reinterpret_cast<const uint4*>(p.skip + c);
+      if (w.x | w.y | w.z | w.w)
+#pragma unroll 1
+        for (int i = 0; i < 16; ++i)
+          if (p.skip[c + i]) own[c + i - first_column] = none;
+    }
+#pragma unroll 1
+    for (int i = tid; i < end - begin - 16 * wide; i += kThreads) {
+      const int c = begin + (i < head ? i : 16 * wide + i);
+      if (p.skip[c]) own[c - first_column] = none;
+    }
+  }
 }
 
 template <typename T>
-static int launch(const SampleParams& p, int cluster, cudaStream_t st) {
+__global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const SampleParams p) {
+  Shared& sh = shared();
+  State& st = sh.st;
+  const int tid = threadIdx.x, lane = tid & 31;
+  const long long r = (long long)blockIdx.x / cg::this_cluster().num_blocks();
+  const T* x = reinterpret_cast<const T*>(p.x) + r * p.ld;
+  if (tid == 0) {
+    const int k = p.top_k ? p.top_k[r] : p.top_k_all;
+    st.t = p.temperature ? p.temperature[r] : p.temperature_all;
+    st.k = k < p.cols ? k : 0;
+    st.top_p = p.top_p ? p.top_p[r] : p.top_p_all;
+    st.min_p = p.min_p ? p.min_p[r] : p.min_p_all;
+    st.u = fmax((double)p.uniforms[r], 0.0);  // (a NaN counts as 0)
+    st.z_due = p.logprobs != nullptr;
+    st.by_count = st.exact = false;
+    st.xmin = st.xt = st.xt0 = st.xt_k = -INFINITY;
+    st.ties = st.ties0 = st.ties_k = 0x7fffffff;
+    st.first = kFirst, st.last = -1, st.token = 0;
+    st.pass = kMax;
+  }
+  load_row<T>(p, x);
+  __syncthreads();
+#pragma unroll 1
+  for (Pass pass = kMax; pass != kDone;) {
+    if (pass == kMax) {
+      pass_max<T>();
+      after_max();
+    } else if (pass == kSeek) {
+      pass_seek<T>();
+      after_seek();
+    } else if (pass == kCount) {
+      pass_count<T>();
+      after_count<T>();
+      after_count_together<T>();
+    } else if (pass == kSum) {
+      pass_sum<T>();
+      draw<T>();
+    } else {
+      const bool weigh = pass == kWeigh;
+      if (weigh) pass_weigh<T>();
+      else pass_refine<T>();
+      if (weigh && !(st.top_p < 1.f)) {
+        __syncthreads();
+        if (tid == 0) st.pass = kSum;
+      } else {
+        find_bin();
+        after_bin<T>();
+      }
+    }
+    __syncthreads();
+    if (tid == 0 && (pass == kSeek || pass == kWeigh)) st.z_due = false;
+    pass = st.pass;
+  }
+
+  // ---- the token and its log-probability ------------------------------------------------------------
+  float z = 0.f;
+  if (p.logprobs) {
+    z = warp_sum(lane < kWarps ? sh.z[lane] : 0.f);
+    if (tid == 0) sh.told[2].z = z;
+  }
+  together(st.ctas);
+  if (st.rank == 0 && tid == 0) {
+    p.out[r] = st.token;
+    if (p.logprobs) {
+      z = 0.f;
+#pragma unroll 1
+      for (int i = 0; i < st.ctas; ++i) z += of_cta(i).told[2].z;
+      const float v = p.skip && p.skip[st.token] ? -INFINITY : Elem<T>::to_f(x[st.token]);
+      p.logprobs[r] = v - st.m - logf(z);
+    }
+  }
+  together(st.ctas);  // no CTA leaves while another reads what it told
+}
+
+template <typename T>
+static int launch(const SampleParams& p, int cluster, size_t bytes, cudaStream_t st) {
+  if (!allow_smem<sample_rows_kernel<T>>(kMostBytes)) return SPD_ERR_CUDA;
   cudaLaunchConfig_t cfg = {};
+  cfg.dynamicSmemBytes = bytes;
   cfg.gridDim = dim3((unsigned)(p.rows * cluster));
   cfg.blockDim = dim3(kThreads);
   cfg.stream = st;
@@ -624,15 +867,22 @@ static int launch(const SampleParams& p, int cluster, cudaStream_t st) {
 
 }  // namespace pick
 
-// CTAs that share a row: as many as let all rows run at once (four CTAs an SM), with 4,096 columns each or more.
+// CTAs that share a row: as many as it takes for each one's part to leave room for a second CTA on its SM (or for the part to
+// fit at all), and as let all rows run at once with 8,192 columns each or more.
 int sample_rows_launch(const SampleParams& p, int dtype, int sms, cudaStream_t st) {
-  int cluster = 8;
-  while (cluster > 1 && ((long long)p.rows * cluster > 4ll * sms || p.cols < 4096 * cluster)) cluster /= 2;
-  if ((long long)p.rows * cluster > 0x7fffffffll) return SPD_ERR_UNSUPPORTED;
+  const int e = dtype == SPD_F32 ? 4 : 8;
+  auto bytes = [&](int cluster) {  // of a CTA's shared memory (a vector more than the columns fill, for a row off the boundary)
+    const long long vectors = ((long long)p.cols + e - 1) / e + 1;
+    return pick::kSharedBytes + (size_t)(((vectors + cluster - 1) / cluster + 31) / 32 * 32 * 16);
+  };
+  int cluster = 1;
+  while (cluster < pick::kCtas && (bytes(cluster) > pick::kGoodBytes || ((long long)p.rows * cluster < sms && p.cols >= 16384 * cluster)))
+    cluster *= 2;
+  if (bytes(cluster) > pick::kMostBytes || (long long)p.rows * cluster > 0x7fffffffll) return SPD_ERR_UNSUPPORTED;
   switch (dtype) {
-    case SPD_F32: return pick::launch<float>(p, cluster, st);
-    case SPD_F16: return pick::launch<__half>(p, cluster, st);
-    case SPD_BF16: return pick::launch<__nv_bfloat16>(p, cluster, st);
+    case SPD_F32: return pick::launch<float>(p, cluster, bytes(cluster), st);
+    case SPD_F16: return pick::launch<__half>(p, cluster, bytes(cluster), st);
+    case SPD_BF16: return pick::launch<__nv_bfloat16>(p, cluster, bytes(cluster), st);
     default: return SPD_ERR_UNSUPPORTED;
   }
 }

@@ -777,6 +777,7 @@ int spd_sample_rows(const void* x, int rows, int cols, int64_t ld, const uint8_t
   if (rows < 0 || cols <= 0 || ld < cols) return fail(SPD_ERR_INVALID_ARG, "spd_sample_rows: bad sizes rows=%d cols=%d", rows, cols);
   if (rows == 0) return ok();
   if (!x || !uniforms || !out) return fail(SPD_ERR_INVALID_ARG, "spd_sample_rows: null pointer");
+  if (reinterpret_cast<uintptr_t>(x) % eb) return fail(SPD_ERR_INVALID_ARG, "spd_sample_rows: x off its elements' boundary");
   if (cols > (1 << 19)) return fail(SPD_ERR_UNSUPPORTED, "spd_sample_rows: more than 2^19 columns");
   const int sms = sm_count(-1);
   if (sms <= 0) return fail(SPD_ERR_CUDA, "spd_sample_rows: no CUDA device");
@@ -786,8 +787,6 @@ int spd_sample_rows(const void* x, int rows, int cols, int64_t ld, const uint8_t
   p.temperature_all = temperature_all; p.top_k_all = top_k_all; p.top_p_all = top_p_all; p.min_p_all = min_p_all;
   p.out = reinterpret_cast<long long*>(out); p.logprobs = logprobs;
   p.rows = rows; p.cols = cols; p.ld = ld;
-  p.vec = aligned16(x) && (ld * eb) % 16 == 0;
-  p.skip_vec = (reinterpret_cast<uintptr_t>(skip_mask) & 7u) == 0;
   const int rc = spd::sample_rows_launch(p, dtype, sms, static_cast<cudaStream_t>(stream));
   if (rc != SPD_OK) return fail(rc, "spd_sample_rows: launch failed: %s", cudaGetErrorString(cudaGetLastError()));
   return ok();

@@ -123,7 +123,6 @@ struct SampleParams {  // a token a row by temperature, top-k, top-p, min-p (sam
   float* logprobs;  // [rows] or null
   int rows, cols;
   long long ld;     // elements between rows
-  int vec, skip_vec;  // rows allow loads of 16 bytes, the mask loads of 8
 };
 
 struct GatherParams {
