@@ -14,9 +14,9 @@
 //   that holds the cut, until a bin holds one value.  Equal values that the cut divides count by their place.
 // * Every sum of weights is an integer (units of 2^-44 of the largest weight), so no order of atomics or threads changes a
 //   result, and cumulative sums are exact in their weights.
-// * Weights are the hardware's 2^f (2^-22) of an argument that keeps the rounding of x - m.  A decision that an error of
-//   2^-20 of the whole could turn is taken again with weights in fp64 (one row in ten where a hundred thousand columns
-//   weigh alike, else next to none), so that the token is the one that fp64 arithmetic gives.
+// * Weights are fp32 polynomials of an argument that keeps the rounding of x - m, good to 2^-23.8.  A decision that an error
+//   of 2^-22.4 of the whole could turn is taken again with weights in fp64 (one row in twenty where two hundred
+//   thousand columns weigh alike, else next to none), so that the token is the one that fp64 arithmetic gives.
 // * A CTA's columns lie in its shared memory, and what is known of the row beside them: passes are functions that are
 //   called, so that none holds another's registers.  (In one function the state went to local memory, whose traffic
 //   was twice that of the columns: 87 us for the 64 rows of 51,865 columns below.)
@@ -103,9 +103,27 @@ constexpr size_t kMostBytes = 226 * 1024, kGoodBytes = 112 * 1024;  // of a CTA'
 extern __shared__ __align__(128) unsigned char shared_bytes[];
 __device__ __forceinline__ Shared& shared() { return *reinterpret_cast<Shared*>(shared_bytes); }
 
-// The weight of a value, in units of 2^-44.
-__device__ __noinline__ u64 exact_weight(double below, double t) {
-  return (u64)(exp(below / t) * (double)(1ull << kScale) + 0.5);
+// The weight of a value, in units of 2^-44: 2^y with y = (x - m) log2(e) / t = n + f, |f| <= 1/2.
+// In fp64: the Taylor series of 2^f to the 12th power (2e-16).
+__device__ __noinline__ u64 exact_weight(double y) {
+  const double n = fmax(rint(y), -100.0), f = fmax(y - n, -1.0) * 0.69314718055994530942;
+  double q = 1.0 / 479001600.0;
+  q = fma(q, f, 1.0 / 39916800.0);
+  q = fma(q, f, 1.0 / 3628800.0);
+  q = fma(q, f, 1.0 / 362880.0);
+  q = fma(q, f, 1.0 / 40320.0);
+  q = fma(q, f, 1.0 / 5040.0);
+  q = fma(q, f, 1.0 / 720.0);
+  q = fma(q, f, 1.0 / 120.0);
+  q = fma(q, f, 1.0 / 24.0);
+  q = fma(q, f, 1.0 / 6.0);
+  q = fma(q, f, 0.5);
+  q = fma(q, f, 1.0);
+  q = fma(q, f, 1.0);
+  // in units of 2^-60, rounded, and then to their place
+  const u64 bits = (u64)__double2ll_rn(q * 0x1p60);
+  const int down = 60 - kScale - (int)n;
+  return down < 63 ? (bits + (1ull << (down - 1))) >> down : 0;
 }
 template <typename T> struct Weight {
   float m, hi, lo;  // the largest value, and log2(e) / t in two parts
@@ -113,24 +131,28 @@ template <typename T> struct Weight {
   bool exact;
   __device__ __forceinline__ explicit Weight(const State& st) : m(st.m), hi(st.hi), lo(st.lo), t(st.t), exact(st.exact) {}
   __device__ __forceinline__ u64 operator()(float x) const {
-    if (exact) return exact_weight((double)x - (double)m, t);
+    if (exact) return exact_weight(((double)x - (double)m) / t * 1.4426950408889634074);
     const float d = x - m;  // <= 0
     const float n = fmaxf(rintf(d * hi), -100.f);
-    // d * log2(e) / t - n, with what the subtraction rounded off (16-bit values: next to nothing)
-    float f = fmaf(d, hi, -n);
-    float rest = d * lo;
+    // f keeps what the subtraction rounded off (16-bit values: next to nothing)
+    float f = fmaf(d, hi, -n), rest = d * lo;
     if constexpr (sizeof(T) == 4) {
       const float b = d - x, a = d - b;
       rest = fmaf((x - a) - (m + b), hi, rest);
     }
-    f = fminf(f + rest, 1.f);
-    const unsigned b = __float_as_uint(ex2_approx(f));
-    const int shift = kScale - 23 + (int)n + (int)(b >> 23) - 127;
-    const u64 bits = (b & 0x7fffffu) | 0x800000u;
-    return shift >= 0 ? bits << shift : shift > -25 ? bits >> -shift : 0;
+    f = fmaxf(f + rest, -1.f);
+    // 2^f = 1 + f q(f), q a polynomial fitted to (2^f - 1) / f on [-1/2, 1/2] (2e-10), in units of 2^-28: off by less than
+    // 2^-24.3 of itself with its roundings, 2^-23.8 with those of f
+    float q = fmaf(1.530370172986295e-05f, f, 0.00015461447765119374f);
+    q = fmaf(q, f, 0.0013333478709682822f);
+    q = fmaf(q, f, 0.009618056938052177f);
+    q = fmaf(q, f, 0.05550410971045494f);
+    q = fmaf(q, f, 0.24022650718688965f);
+    q = fmaf(q, f, 0.6931471824645996f);
+    const unsigned bits = (1u << 28) + (unsigned)__float2int_rn(f * q * 0x1p28f);
+    const int shift = kScale - 28 + (int)n;
+    return shift >= 0 ? (u64)bits << shift : shift > -29 ? bits >> -shift : 0;
   }
-  // How far a sum may be off, seen against the whole of it.
-  __device__ __forceinline__ double guard(u64 whole) const { return exact ? 0.0 : (double)whole * 0x1p-20; }
 };
 
 template <typename V> __device__ __forceinline__ V warp_total(V v) {
@@ -368,7 +390,8 @@ __device__ __forceinline__ void again_exactly(State& st) {
   begin_cut(st, false);
   if (!(st.top_p < 1.f)) st.pass = kWeigh, st.first = kFirst;
 }
-__device__ __forceinline__ double guard(const State& st, u64 whole) { return st.exact ? 0.0 : (double)whole * 0x1p-20; }
+// How far a sum and a target of it may be off: twice 2^-23.8 of the target.
+__device__ __forceinline__ double guard(const State& st, u64 whole) { return st.exact ? 0.0 : (double)whole * 0x1.78p-23; }
 // the largest value, and what comes first
 __device__ __noinline__ void after_max() {
   Shared& sh = shared();
