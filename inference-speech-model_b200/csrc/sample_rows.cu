@@ -4,14 +4,17 @@
 //   than p of their weight lies, min-p the ones with x >= m + t log(min_p); the token is the first column, by
 //   its place, at which the weight left so far passes u times all of it.
 //
-// What bounds it: a row is read once from memory, 2 or 4 bytes a column, and again from L1 or L2 by each later pass; the
-// passes' instructions, some 50 a column in all, are what takes the time.  Nothing is sorted:
-// * A cluster of up to 4 CTAs shares a row.  A cut (the k-th largest, or the value at which the weight reaches p) is
+// What bounds it: a row is read once from memory, 2 or 4 bytes a column, and again from shared memory by each later pass;
+// the passes' instructions, some 50 a column in all, are what takes the time, and for one row the clusters' barriers
+// between them.  Nothing is sorted:
+// * A cluster of up to 8 CTAs shares a row.  A cut (the k-th largest, or the value at which the weight reaches p) is
 //   found by histograms.  The first counts columns by their distance from m (one atomic a column).  For the k-th largest
-//   the cut lies in one of its bins.  For p each bin's weight is known to within 1 %, so the cut
-//   lies in a few; the next pass adds up the weights above, in and below these, and only the columns in them, a hundredth of
-//   the whole, enter a histogram of weights.  Later passes look at the order-preserving integers of the values in the bin
-//   that holds the cut, until a bin holds one value.  Equal values that the cut divides count by their place.
+//   the cut lies in one of its bins.  For p each bin's weight is known to within 2 %, and nearly always to within a
+//   thousandth, so the cut lies in a few; the next pass adds up the weights above, in and below these, and only the
+//   columns in them enter a histogram of weights.  (If the thousandth did not hold, which the sums show, the bins are
+//   taken anew from what is certain.  At once from that, a cut far down a flat row had a tenth of the columns to put in
+//   their bins.)  Later passes look at the order-preserving integers of the values in the bin that holds the cut, until a
+//   bin holds one value.  Equal values that the cut divides count by their place.
 // * Every sum of weights is an integer (units of 2^-44 of the largest weight), so no order of atomics or threads changes a
 //   result, and cumulative sums are exact in their weights.
 // * Weights are fp32 polynomials of an argument that keeps the rounding of x - m, good to 2^-23.8.  A decision that an error
@@ -33,9 +36,9 @@ typedef unsigned long long u64;
 
 constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
-constexpr int kFirst = 4096;      // bins of the first histogram (counts)
+constexpr int kFirst = 2048;      // bins of the first histogram (counts)
 constexpr int kBins = 512;        // of the later ones (counts and weights)
-constexpr int kMaxChunks = 1024;  // of a CTA's columns
+constexpr int kMaxChunks = 256;   // of a CTA's columns
 constexpr int kCtas = 8;          // of a cluster, at most
 constexpr int kScale = 44;        // a weight of 1 is 2^44: sums of 2^19 columns fit in 64 bits
 
@@ -77,6 +80,7 @@ struct State {
   Pass pass;
   int token;
   bool by_count, exact, z_due;
+  bool sure, missed;      // the cut's bins are taken from certain bounds; they were not, and did not hold it
   float m, xmin, hi, lo;  // the largest value, the least that min-p leaves, log2(e) / t in two parts
   float xt, xt0, xt_k;    // what is left: values above xt, and the first `ties` columns that have it;
   int ties, ties0, ties_k;  // as the cut under way found it; as top-k left it
@@ -94,9 +98,16 @@ struct Shared {
   Cut cut;
   Told told[4];
   float z[kWarps], floats[3][kWarps];
-  int counts[3][kWarps], chunk_ties[kMaxChunks];
-  u64 sums[3][kWarps], chunk_sum[kMaxChunks];
-  unsigned first_count[kFirst], count[kBins], low[kBins], high[kBins];
+  int counts[3][kWarps];
+  u64 sums[3][kWarps];
+  union {  // the first histogram, or the later ones and the chunks' sums, which come after it
+    unsigned first_count[kFirst];
+    struct {
+      u64 chunk_sum[kMaxChunks];
+      int chunk_ties[kMaxChunks];
+      unsigned count[kBins], low[kBins], high[kBins];
+    };
+  };
 };
 constexpr size_t kSharedBytes = (sizeof(Shared) + 127) / 128 * 128;
 constexpr size_t kMostBytes = 226 * 1024, kGoodBytes = 112 * 1024;  // of a CTA's shared memory
@@ -445,15 +456,22 @@ template <typename T> __device__ __noinline__ void after_count() {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, C = st.ctas, rank = st.rank, k_left = st.k_left;
   const bool by_count = st.by_count;
   together(C);
-  // A thread has 8, 4, 2 or 1 bins of the rank's share of them.  Weights of a bin: between these.
-  const int per = kFirst / kThreads / C, at0 = (rank * kThreads + tid) * per;
+  // A thread has 4, 2 or 1 bins of the rank's share of them (or, of eight CTAs, every other thread one).  Weights of a bin:
+  // between these.
+  const int share = kFirst / C, per = tid * max(1, share / kThreads) < share ? max(1, share / kThreads) : 0;
+  const int at0 = rank * share + tid * per;
   const float step = (float)(1.4426950408889634 / ((double)st.inv * st.t));
   auto most_of = [&](int bin) { return bin ? ex2_approx(-bin * step) * (1.f + 2e-5f) : 1.f; };
-  auto least_of = [&](int bin) { return bin + 1 < kFirst ? most_of(bin + 1) * (1.f - 6e-5f) : 0.f; };
-  int n[8], all_n = 0;
+  const bool sure = st.sure;
+  const float half = ex2_approx(-0.5f * step);  // the middle of a bin against its upper end
+  auto most_at = [&](int bin) { return sure || bin + 1 == kFirst ? most_of(bin) : most_of(bin) * half * 1.001f; };
+  auto least_at = [&](int bin) {
+    return bin + 1 == kFirst ? 0.f : sure ? most_of(bin + 1) * (1.f - 6e-5f) : most_of(bin) * half * 0.999f;
+  };
+  int n[4], all_n = 0;
   float least = 0.f, most = 0.f;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
+  for (int j = 0; j < 4; ++j) {
     n[j] = 0;
     if (j < per) {
       unsigned c[kCtas];
@@ -462,8 +480,8 @@ template <typename T> __device__ __noinline__ void after_count() {
 #pragma unroll
       for (int i = 0; i < kCtas; ++i) n[j] += (int)c[i];
       all_n += n[j];
-      most += n[j] * most_of(at0 + j);
-      least += n[j] * least_of(at0 + j);
+      most += n[j] * most_at(at0 + j);
+      least += n[j] * least_at(at0 + j);
     }
   }
   int all;
@@ -484,15 +502,15 @@ template <typename T> __device__ __noinline__ void after_count() {
   const float off = 2e-5f * all_most, t_least = st.top_p * all_least - off, t_most = st.top_p * all_most + off;
   int not_yet = 0, below_cut = 0, n_before = 0;  // n_before: columns above the cut's bin, if it is this thread's
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
+  for (int j = 0; j < 4; ++j) {
     if (j >= per) break;
     if (by_count) {
       if (above_n + n[j] < k_left) ++not_yet;
       else if (above_n < k_left) n_before = above_n;
     } else {
       below_cut += a_least < t_most || above_n == 0;  // may begin below the target
-      a_most += n[j] * most_of(at0 + j);
-      a_least += n[j] * least_of(at0 + j);
+      a_most += n[j] * most_at(at0 + j);
+      a_least += n[j] * least_at(at0 + j);
       not_yet += a_most < t_least || above_n + n[j] == 0;  // surely ends below it
     }
     above_n += n[j];
@@ -506,7 +524,9 @@ template <typename T> __device__ __noinline__ void after_count() {
   int first = (int)__reduce_add_sync(0xffffffffu, lane < kWarps ? (unsigned)sh.counts[0][lane] : 0u);
   int last = (int)__reduce_add_sync(0xffffffffu, lane < kWarps ? (unsigned)sh.counts[1][lane] : 0u);
   int n_above = (int)__reduce_max_sync(0xffffffffu, (unsigned)sh.counts[2][lane % kWarps]);
-  if (lane == 0) sh.told[2].first = first, sh.told[2].last = last, sh.told[2].count = n_above, sh.told[2].mx = (float)(by_count && all < k_left);
+  if (lane) return;
+  sh.told[2].first = first, sh.told[2].last = last, sh.told[2].count = n_above;
+  sh.told[2].mx = (float)(by_count && all < k_left);
 }
 template <typename T> __device__ __noinline__ void after_count_together() {
   Shared& sh = shared();
@@ -552,9 +572,9 @@ __device__ __noinline__ void find_bin() {
   const bool by_count = st.by_count, weighed = st.pass == kWeigh;
   if (weighed) {
     __syncthreads();
-    const u64 above = warp_total(lane < kWarps ? sh.sums[0][lane] : 0), inside = warp_total(lane < kWarps ? sh.sums[1][lane] : 0),
-              below = warp_total(lane < kWarps ? sh.sums[2][lane] : 0);
-    if (tid == 0) sh.told[0].sum = above, sh.told[0].inside = inside, sh.told[0].below = below;
+    const u64 a = warp_total(lane < kWarps ? sh.sums[0][lane] : 0), b = warp_total(lane < kWarps ? sh.sums[1][lane] : 0),
+              c = warp_total(lane < kWarps ? sh.sums[2][lane] : 0);
+    if (tid == 0) sh.told[0].sum = a, sh.told[0].inside = b, sh.told[0].below = c;
   }
   if (tid == 0) sh.cut.bin = -1;  // (the last one was read before this pass)
   together(C);
@@ -570,12 +590,13 @@ __device__ __noinline__ void find_bin() {
     for (int i = 0; i < kCtas; ++i)
       if (i < C) n += (int)a[i], s += ((u64)c[i] << 32) + b[i];
   }
-  u64 whole = st.whole, above = st.above;
+  u64 whole = st.whole, above = st.above, inside = 0;
   double target = st.target;
   if (weighed) {
     const Told& o = of_cta(min(lane, C - 1)).told[0];
     above = warp_total(lane < C ? o.sum : 0);
-    whole = above + warp_total(lane < C ? o.inside + o.below : 0);
+    inside = warp_total(lane < C ? o.inside : 0);
+    whole = above + inside + warp_total(lane < C ? o.below : 0);
     target = (double)st.top_p * (double)whole;
   }
   int all;
@@ -599,14 +620,19 @@ __device__ __noinline__ void find_bin() {
     const bool starts = by_count ? at < k_left : at == 0 || a < target, ends = by_count ? to_n >= k_left : b >= target || final;
     if (starts && ends) {
       const double g = guard(st, whole);
-      const int open = !by_count && ((above + at_s > 0 && fabs(a - target) <= g) || (to_s + above < whole && fabs(b - target) <= g));
+      const int open = !by_count && ((above + at_s > 0 && fabs(a - target) <= g) ||
+                                     (to_s + above < whole && fabs(b - target) <= g));
       const Cut f{at0, at, n, at_s, s, open};
 #pragma unroll 1
       for (int i = 0; i < C; ++i) of_cta(i).cut = f;
     }
   }
   __syncthreads();  // (the state is read above)
-  if (tid == 0 && weighed) sh.st.whole = whole, sh.st.above = above, sh.st.target = target;
+  if (tid == 0 && weighed) {
+    sh.st.whole = whole, sh.st.above = above, sh.st.target = target;
+    sh.st.missed = !st.sure && ((above > 0 && (double)above >= target) ||
+                                (inside < whole - above && (double)(above + inside) < target));
+  }
 }
 template <typename T> __device__ __noinline__ void after_bin() {
   Shared& sh = shared();
@@ -614,6 +640,12 @@ template <typename T> __device__ __noinline__ void after_bin() {
   together(st.ctas);
   if (threadIdx.x) return;
   const Cut f = sh.cut;
+  if (st.missed) {
+    st.missed = false;
+    st.sure = true;
+    begin_cut(st, false);
+    return;
+  }
   bool open = f.open && !st.exact && !(st.shift == 0 && f.inside > 1);  // (one value: its columns are counted below)
   const unsigned to = st.to - ((unsigned)f.bin << st.shift), from = st.shift ? max(st.from, to - ((1u << st.shift) - 1u)) : to;
   st.to = to, st.from = from;
@@ -669,7 +701,7 @@ template <typename T> __device__ __noinline__ void draw() {
     const u64 whole = __shfl_sync(0xffffffffu, o_incl, 31), before = __shfl_sync(0xffffffffu, o_incl - o_s, rank),
               here = __shfl_sync(0xffffffffu, o_s, rank);
     const int ties_before = __shfl_sync(0xffffffffu, o_before, rank);
-    const double u = st.u, goal = u < 1.0 ? u * (double)whole : (double)whole - 0.5, g = guard(st, whole);
+    const double goal = st.u * (double)whole, g = guard(st, whole);
     if (here > 0 && (before == 0 || (double)before <= goal) && (double)(before + here) > goal) {
       u64 at = before;
       int had = ties_before, found = -1;
@@ -805,13 +837,14 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const SamplePa
   const T* x = reinterpret_cast<const T*>(p.x) + r * p.ld;
   if (tid == 0) {
     const int k = p.top_k ? p.top_k[r] : p.top_k_all;
-    st.t = p.temperature ? p.temperature[r] : p.temperature_all;
+    const float t = p.temperature ? p.temperature[r] : p.temperature_all;
+    st.t = t > 0.f ? fmaxf(t, 0x1p-100f) : t;  // (below that its inverse would not be finite)
     st.k = k < p.cols ? k : 0;
     st.top_p = p.top_p ? p.top_p[r] : p.top_p_all;
     st.min_p = p.min_p ? p.min_p[r] : p.min_p_all;
-    st.u = fmax((double)p.uniforms[r], 0.0);  // (a NaN counts as 0)
+    st.u = fmin(fmax((double)p.uniforms[r], 0.0), 1.0 - 0x1p-52);  // (a NaN counts as 0, 1 as a little less)
     st.z_due = p.logprobs != nullptr;
-    st.by_count = st.exact = false;
+    st.by_count = st.exact = st.sure = st.missed = false;
     st.xmin = st.xt = st.xt0 = st.xt_k = -INFINITY;
     st.ties = st.ties0 = st.ties_k = 0x7fffffff;
     st.first = kFirst, st.last = -1, st.token = 0;
@@ -891,7 +924,7 @@ static int launch(const SampleParams& p, int cluster, size_t bytes, cudaStream_t
 }  // namespace pick
 
 // CTAs that share a row: as many as it takes for each one's part to leave room for a second CTA on its SM (or for the part to
-// fit at all), and as let all rows run at once with 8,192 columns each or more.
+// fit at all), and as let all rows run at once with 2,048 columns each or more.
 int sample_rows_launch(const SampleParams& p, int dtype, int sms, cudaStream_t st) {
   const int e = dtype == SPD_F32 ? 4 : 8;
   auto bytes = [&](int cluster) {  // of a CTA's shared memory (a vector more than the columns fill, for a row off the boundary)
@@ -899,7 +932,8 @@ int sample_rows_launch(const SampleParams& p, int dtype, int sms, cudaStream_t s
     return pick::kSharedBytes + (size_t)(((vectors + cluster - 1) / cluster + 31) / 32 * 32 * 16);
   };
   int cluster = 1;
-  while (cluster < pick::kCtas && (bytes(cluster) > pick::kGoodBytes || ((long long)p.rows * cluster < sms && p.cols >= 16384 * cluster)))
+  while (cluster < pick::kCtas && (bytes(cluster) > pick::kGoodBytes ||
+                                   ((long long)p.rows * cluster < sms && p.cols >= 4096 * cluster)))
     cluster *= 2;
   if (bytes(cluster) > pick::kMostBytes || (long long)p.rows * cluster > 0x7fffffffll) return SPD_ERR_UNSUPPORTED;
   switch (dtype) {
