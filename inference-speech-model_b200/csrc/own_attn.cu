@@ -303,8 +303,7 @@ __global__ void __launch_bounds__(kThreads, 3) own_attn_kernel(const OwnParams p
 #pragma unroll
     for (int w = 0; w < kWarps; ++w)
       if (w < steps)
-        s.add(*reinterpret_cast<const float4*>(reinterpret_cast<const float*>(smem + (size_t)w * kStages * kStageBytes) + h * DP + d),
-              stat_m[w][h], stat_l[w][h]);
+        s.add(reinterpret_cast<const float4*>(smem + (size_t)w * kStages * kStageBytes)[(h * DP + d) / 4], stat_m[w][h], stat_l[w][h]);
   };
   // the n partial results of a row
   auto of_memory = [&](Sum& s, const float* row, long long next, int n, int d) {
@@ -345,7 +344,7 @@ __global__ void __launch_bounds__(kThreads, 3) own_attn_kernel(const OwnParams p
     desc = __ldcg(p.row_desc + (long long)b * p.Hkv + kvh);
     // What a prefix's kernel that gave up waiting did not write is not followed.
     const int row0 = (int)((unsigned)desc.y >> 16), count = desc.y & 0xffff;
-    if (desc.x < -1 || desc.x + count > p.span_ctas || row0 + Gq > p.piece_rows || (desc.x < 0 && count > 1)) desc.y = 0;
+    if (desc.x < -1 || desc.x > p.span_ctas - count || row0 + Gq > p.piece_rows || (desc.x < 0 && count > 1)) desc.y = 0;
   }
   const int pieces = desc.y & 0xffff, first_cta = desc.x;
   const long long piece = (long long)p.piece_rows * step;

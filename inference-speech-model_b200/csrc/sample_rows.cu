@@ -923,6 +923,12 @@ static int launch(const SampleParams& p, int cluster, size_t bytes, cudaStream_t
 
 }  // namespace pick
 
+// Columns that fit in the shared memory of a cluster, whatever the row's place.
+int sample_rows_most_cols(int dtype) {
+  const int e = dtype == SPD_F32 ? 4 : 8, vectors = (int)(pick::kMostBytes - pick::kSharedBytes) / 512 * 32 * pick::kCtas;
+  return std::min(1 << 19, (vectors - 1) * e);  // (2^19: sums of weights fit in 64 bits)
+}
+
 // CTAs that share a row: as many as it takes for each one's part to leave room for a second CTA on its SM (or for the part to
 // fit at all), and as let all rows run at once with 2,048 columns each or more.
 int sample_rows_launch(const SampleParams& p, int dtype, int sms, cudaStream_t st) {
@@ -935,7 +941,7 @@ int sample_rows_launch(const SampleParams& p, int dtype, int sms, cudaStream_t s
   while (cluster < pick::kCtas && (bytes(cluster) > pick::kGoodBytes ||
                                    ((long long)p.rows * cluster < sms && p.cols >= 4096 * cluster)))
     cluster *= 2;
-  if (bytes(cluster) > pick::kMostBytes || (long long)p.rows * cluster > 0x7fffffffll) return SPD_ERR_UNSUPPORTED;
+  if ((long long)p.rows * cluster > 0x7fffffffll) return SPD_ERR_UNSUPPORTED;
   switch (dtype) {
     case SPD_F32: return pick::launch<float>(p, cluster, bytes(cluster), st);
     case SPD_F16: return pick::launch<__half>(p, cluster, bytes(cluster), st);

@@ -35,8 +35,8 @@ namespace span {
 using namespace tc;
 
 // Code size counts here: roles side by side miss the instruction cache, and each miss waits in L2 behind the
-// K/V stream.  (134 KB of code took 101 us for the 32 x 5 beams where XXX does.)  So waits are one
-// small loop each, the error word is set once at the end, and divisions of 64 bits are calls.
+// K/V stream.  So waits are one small loop each, and the error word is set once at the end.  (32 x 5 beams over 1,500
+// positions took 101 us with 134 KB of code; with this and four threads a row for few rows 51.)
 
 // Waits for phase `parity` of `bar`, suspended, for `limit_ns` at most; false if it ran out.
 __device__ __forceinline__ bool wait_on(uint64_t* bar, uint32_t parity, unsigned long long limit_ns) {
@@ -191,6 +191,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ __align__(8) uint64_t p_full[2][2];  // weights written, 64 keys each (and the output rescaled)
   __shared__ __align__(8) uint64_t o_full[2], o_empty[2];  // output complete, output read
   __shared__ __align__(8) uint64_t turn[C::kStages];       // of two tiles' steps: the first stream's products are issued
+  __shared__ __align__(8) uint64_t meet;          // both issuing warps are here
   __shared__ __align__(8) uint64_t done;          // every MMA has completed
   __shared__ uint32_t tmem_slot;
   unsigned char* smem = smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023);
@@ -225,17 +226,27 @@ __global__ void __launch_bounds__(kThreads, 1)
     init(41, 1, &other_empty, 4);
     init(42, 1, &done, 2);
     init(43, C::kStages, turn, 1);
+    init(43 + C::kStages, 1, &meet, 2);
     if (i >= 0 && i < 64) fence_barrier_init();
   }
   // Warp 0 finds its share meanwhile.
   int total = 0, lo = 0, hi = 0, share = 1, g = 0, base = 0;
   if (warp == 0) {
     auto cost_of = [&](int i) { return i < p.G ? Group(p, i).cost() * p.Hkv : 0; };
-    int mine = cost_of(lane);  // of group `lane` (the host refuses calls whose sum could reach 2^31)
-    total = mine;
+    // The host refuses calls whose sum could reach 2^31 with each query in one group.  If groups overlap and it does, no
+    // work is done.
+    int mine = cost_of(lane);  // of group `lane`
+    unsigned sum = (unsigned)mine;
+    bool over = false;
 #pragma unroll 1
-    for (int i = lane + 32; i < p.G; i += 32) total += cost_of(i);
-    total = (int)__reduce_add_sync(0xffffffffu, (unsigned)total);
+    for (int i = lane + 32; i < p.G; i += 32) {
+      sum += (unsigned)cost_of(i);
+      over |= sum >> 31;
+      sum &= 0x7fffffffu;
+    }
+    over = __any_sync(0xffffffffu, over) || __reduce_add_sync(0xffffffffu, sum >> 8) >= (1u << 23) - 32;
+    total = over ? 0 : (int)__reduce_add_sync(0xffffffffu, sum);
+    if (over && blockIdx.x == 0) set_error(p.err, SPD_DEVERR_LENGTH);
     const int shares = max(1, min((int)gridDim.x, total / kMinShare));
     share = max(1, (total + shares - 1) / shares);  // more than a step if there are two: every CTA between has one
     lo = (int)min((long long)total, (long long)blockIdx.x * share);
@@ -263,9 +274,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
-  bool ok = true;  // of the whole warp
+  bool ok = true;  // of the whole warp: no wait has run out
   auto wait = [&](uint64_t* bar, uint32_t phase) {
-    ok = __all_sync(0xffffffffu, wait_on(bar, phase & 1u, p.wait_ns));
+    if (ok) ok = __all_sync(0xffffffffu, wait_on(bar, phase & 1u, p.wait_ns));
     return ok;
   };
   Piece w;
@@ -448,7 +459,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       uint32_t q_odd = 0, p_odd = 0, o_odd = 1;  // phases (q: a bit each)
       int hole_at = 0, u0 = 0, u1 = 0;           // tiles of the two rings before this item
       bool single_before = false;
-      int turns = 0;  // steps of two tiles
+      int turns = 0, meets = 0;  // steps of two tiles; times that the two warps have met
       // A tile is given back only if its products were issued: after a wait that gave up its copy may still be in
       // flight, and the loader must not arm its barrier again.
       auto give_back = [&](uint64_t* bar) {
@@ -461,7 +472,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int q = w.pair ? x : w.q_slot;
         // Each barrier's phases must be seen one by one.  Q: of both tiles, whoever uses them.  Rings: the one that
         // only the other stream used is known to have landed once that stream's warp is here.
-        if (w.pair && single_before) asm volatile("bar.sync 1, 64;" ::: "memory");
+        if (w.pair && single_before) {
+          if (lane == 0) mbar_arrive(&meet);
+          if (!wait(&meet, (uint32_t)meets++)) break;
+        }
         single_before = !w.pair;
 #pragma unroll 1
         for (int r = w.pair ? 0 : q; r <= (w.pair ? 1 : q) && ok; ++r) {

@@ -19,7 +19,9 @@ int kv_append_launch(const AppendParams& p, int sms, cudaStream_t st);
 int block_gather_launch(const GatherParams& p, int sms, cudaStream_t st);
 int add_layernorm_launch(const AddLnParams& p, int dtype, cudaStream_t st);
 int argmax_rows_launch(const ArgmaxParams& p, int dtype, cudaStream_t st);
+int sample_rows_most_cols(int dtype);
 int sample_rows_launch(const SampleParams& p, int dtype, int sms, cudaStream_t st);
+bool span_fits(int N, int G, int Hq, int Hkv, int max_keys);
 int linear_small_m_launch(const void* x, const void* w, const void* bias, void* y, int M, int N, int K,
                           long long group_cols, long long group_stride, int act, int dtype, int* err, int sms,
                           cudaStream_t st);
@@ -668,6 +670,8 @@ int spd_shared_prefix_attn(const void* q, int64_t q_stride_t, int64_t q_stride_h
     return fail(SPD_ERR_INVALID_ARG, "spd_shared_prefix_attn: strides must be multiples of 16 bytes");
   if (!aligned16(q) || !aligned16(k_pool) || !aligned16(v_pool) || !aligned16(out) || !aligned16(workspace))
     return fail(SPD_ERR_INVALID_ARG, "spd_shared_prefix_attn: tensors and the workspace must be 16-byte aligned");
+  if (G && !spd::span_fits(B, G, Hq, Hkv, max_prefix_blocks << bl))
+    return fail(SPD_ERR_UNSUPPORTED, "spd_shared_prefix_attn: too many groups, heads and prefix blocks for one call");
   const int sms = sm_count(-1);
   if (sms <= 0) return fail(SPD_ERR_CUDA, "spd_shared_prefix_attn: no CUDA device");
   const PrefixSpace space = prefix_space(B, G, Hq, Hkv, D, max_blocks << bl, sms);
@@ -745,6 +749,8 @@ int spd_cross_attn_packed(const void* q, int64_t q_stride_t, int64_t q_stride_h,
     if (s < 0 || (s * 2) % 16) return fail(SPD_ERR_INVALID_ARG, "spd_cross_attn_packed: strides must be multiples of 16 bytes");
   if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out) || !aligned16(workspace))
     return fail(SPD_ERR_INVALID_ARG, "spd_cross_attn_packed: tensors and the workspace must be 16-byte aligned");
+  if (!spd::span_fits(N, B, Hq, Hkv, T))
+    return fail(SPD_ERR_UNSUPPORTED, "spd_cross_attn_packed: too many requests, queries, heads and positions for one call");
   const int sms = sm_count(-1);
   if (sms <= 0) return fail(SPD_ERR_CUDA, "spd_cross_attn_packed: no CUDA device");
   const size_t need = spd_cross_attn_packed_workspace_size(N, Hq, Hkv, D, -1);
@@ -778,7 +784,9 @@ int spd_sample_rows(const void* x, int rows, int cols, int64_t ld, const uint8_t
   if (rows == 0) return ok();
   if (!x || !uniforms || !out) return fail(SPD_ERR_INVALID_ARG, "spd_sample_rows: null pointer");
   if (reinterpret_cast<uintptr_t>(x) % eb) return fail(SPD_ERR_INVALID_ARG, "spd_sample_rows: x off its elements' boundary");
-  if (cols > (1 << 19)) return fail(SPD_ERR_UNSUPPORTED, "spd_sample_rows: more than 2^19 columns");
+  if (cols > spd::sample_rows_most_cols(dtype))
+    return fail(SPD_ERR_UNSUPPORTED, "spd_sample_rows: %d columns, at most %d of this dtype", cols,
+                spd::sample_rows_most_cols(dtype));
   const int sms = sm_count(-1);
   if (sms <= 0) return fail(SPD_ERR_CUDA, "spd_sample_rows: no CUDA device");
   spd::SampleParams p{};

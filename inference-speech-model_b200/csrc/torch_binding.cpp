@@ -582,9 +582,9 @@ at::Tensor sample(const char* name, PyObject* const* a, Py_ssize_t n_args) {
     refuse(name, "logprobs must be a contiguous float32 [", rows, "] tensor");
   const int code = dtype_code(name, x.scalar_type());
   const at::Tensor out = given.defined() ? given : at::empty({rows}, x.options().dtype(at::kLong));
-  for (const at::Tensor* w : {&out, &logs})
-    for (const at::Tensor* o : all)
-      if (w->defined() && o->defined() && !w->is_same(*o) && overlap(*w, *o)) refuse(name, "out and logprobs must be apart from all else");
+  for (size_t i = 0; i < all.size(); ++i)  // (3: out itself, 4: logprobs; one tensor may stand in two places)
+    if (all[i]->defined() && ((i != 3 && overlap(out, *all[i])) || (i != 4 && logs.defined() && overlap(logs, *all[i]))))
+      refuse(name, "out and logprobs must be apart from all else");
   const int64_t ld = rows > 1 ? x.stride(0) : x.size(1);
   if (ld < cols) refuse(name, "rows of x overlap");
   check(f_sample(ptr(x), rows, (int)cols, ld, static_cast<const uint8_t*>(ptr(skip)), static_cast<const float*>(ptr(u)),
@@ -659,7 +659,8 @@ PyObject* py_setup(PyObject*, PyObject* d) {
       get("spd_paged_decode_attn_int4_workspace_size", f_decode_size) && get("spd_prompt_attn", f_prompt) &&
       get("spd_kv_int4_page_bytes", f_page_bytes) && get("spd_get_last_error", f_last_error) &&
       get("spd_stream_capture_id", f_capture_id) && get("spd_shared_prefix_attn", f_prefix) &&
-      get("spd_shared_prefix_attn_workspace_size", f_prefix_size) && get("spd_cross_attn_packed", f_cross) && get("spd_sample_rows", f_sample) &&
+      get("spd_shared_prefix_attn_workspace_size", f_prefix_size) && get("spd_cross_attn_packed", f_cross) &&
+      get("spd_sample_rows", f_sample) &&
       get("spd_cross_attn_packed_workspace_size", f_cross_size))
     Py_RETURN_NONE;
   return nullptr;
