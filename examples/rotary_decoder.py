@@ -50,10 +50,12 @@ class Config:
 class RotaryDecoder:
     """Weights, cache and the packed batch of requests of one decoder."""
 
+    grouped_16_bit = False  # whether a 16-bit cache may have fewer key/value heads (paged_decode_attention has as many)
+
     def __init__(self, cfg: Config, device: str = "cuda"):
         if cfg.bits not in (4, 16):
             raise ValueError(f"cache of {cfg.bits} bits: 4 or 16")
-        if cfg.bits == 16 and cfg.heads != cfg.kv_heads:
+        if cfg.bits == 16 and cfg.heads != cfg.kv_heads and not self.grouped_16_bit:
             raise ValueError("a 16-bit cache needs as many key/value heads as query heads")
         self.cfg, self.device = cfg, device
         g = torch.Generator().manual_seed(cfg.seed)
