@@ -38,6 +38,7 @@ constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
 constexpr int kFirst = 2048;      // bins of the first histogram (counts)
 constexpr int kBins = 512;        // of the later ones (counts and weights)
+constexpr int kList = 2 * kThreads;  // columns that one CTA can put in order
 constexpr int kMaxChunks = 256;   // of a CTA's columns
 constexpr int kCtas = 8;          // of a cluster, at most
 constexpr int kScale = 44;        // a weight of 1 is 2^44: sums of 2^19 columns fit in 64 bits
@@ -69,7 +70,7 @@ struct Cut {
 };
 
 // What a pass over the row does with its columns.
-enum Pass { kMax, kSeek, kCount, kWeigh, kRefine, kSum, kDone };
+enum Pass { kMax, kSeek, kCount, kWeigh, kRefine, kSum, kGather, kDone };
 
 // What is known of the row: the same in all CTAs of its cluster but for the first line.
 struct State {
@@ -98,10 +99,12 @@ struct Shared {
   Cut cut;
   Told told[4];
   float z[kWarps], floats[3][kWarps];
-  int counts[3][kWarps];
+  int counts[4][kWarps];
+  int listed;  // columns in `list`
   u64 sums[3][kWarps];
-  union {  // the first histogram, or the later ones and the chunks' sums, which come after it
+  union {  // the first histogram, and what comes after it: the later ones and the chunks' sums, or the columns that are left
     unsigned first_count[kFirst];
+    u64 list[kList];  // place << 32 | ~column
     struct {
       u64 chunk_sum[kMaxChunks];
       int chunk_ties[kMaxChunks];
@@ -285,6 +288,7 @@ template <typename T> __device__ __noinline__ void pass_count() {
   Shared& sh = shared();
   const float m = sh.st.m, inv = sh.st.inv, xt0 = sh.st.xt0;
   for (int i = threadIdx.x; i < kFirst; i += kThreads) sh.first_count[i] = 0;
+  if (threadIdx.x == 0) sh.listed = 0;
   __syncthreads();
   if (!sh.st.by_count && xt0 > -INFINITY && sh.st.rank == 0 && threadIdx.x == 0)  // columns that have xt0 itself, by their number
     sh.first_count[bin_of(xt0, m, inv)] = (unsigned)sh.st.ties0;
@@ -359,6 +363,28 @@ template <typename T> __device__ __noinline__ void pass_refine() {
   each<T>([&](int, float v) {
     if (v > xt0) look(v, 1);
   }, Nothing{});
+}
+// the columns that are left, or above and in the bins of the cut: they fit in one CTA's list
+template <typename T> __device__ __noinline__ void pass_gather() {
+  Shared& sh = shared();
+  const State& st = sh.st;
+  const Weight<T> weight(st);
+  const bool by_count = st.by_count;
+  const float m = st.m, inv = st.inv;
+  const int last = st.last;
+  u64 all = 0;
+  Z z(st);
+  each<T>([&](int c, float v) {
+    z.add(v);
+    if (!(v > -INFINITY)) return;
+    if (!by_count) all += weight(v);
+    if (bin_of(v, m, inv) > last) return;
+    const int at = atomicAdd(&shared().listed, 1);
+    if (at < kList) shared().list[at] = (u64)place_of<T>(v) << 32 | (unsigned)~c;
+  }, Nothing{});
+  z.keep();
+  all = warp_total(all);
+  if ((threadIdx.x & 31) == 0) sh.sums[0][threadIdx.x >> 5] = all;
 }
 // the chunks' sums completed by what is left of the cut's bins, and the columns that have xt itself
 template <typename T> __device__ __noinline__ void pass_sum() {
@@ -501,14 +527,18 @@ template <typename T> __device__ __noinline__ void after_count() {
   // The bins before the cut's: how many there are in all.  (Sums of fp32 here are off by less than 1e-5 of the whole.)
   const float off = 2e-5f * all_most, t_least = st.top_p * all_least - off, t_most = st.top_p * all_most + off;
   int not_yet = 0, below_cut = 0, n_before = 0;  // n_before: columns above the cut's bin, if it is this thread's
+  int n_left = 0;                                // and those above and in the cut's bins
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     if (j >= per) break;
     if (by_count) {
       if (above_n + n[j] < k_left) ++not_yet;
       else if (above_n < k_left) n_before = above_n;
+      if (above_n < k_left) n_left += n[j];
     } else {
-      below_cut += a_least < t_most || above_n == 0;  // may begin below the target
+      const bool may = a_least < t_most || above_n == 0;  // begin below the target
+      below_cut += may;
+      if (may) n_left += n[j];
       a_most += n[j] * most_at(at0 + j);
       a_least += n[j] * least_at(at0 + j);
       not_yet += a_most < t_least || above_n + n[j] == 0;  // surely ends below it
@@ -518,13 +548,16 @@ template <typename T> __device__ __noinline__ void after_count() {
   not_yet = (int)__reduce_add_sync(0xffffffffu, (unsigned)not_yet);
   below_cut = (int)__reduce_add_sync(0xffffffffu, (unsigned)below_cut);
   n_before = (int)__reduce_max_sync(0xffffffffu, (unsigned)n_before);
-  if (lane == 0) sh.counts[0][warp] = not_yet, sh.counts[1][warp] = below_cut, sh.counts[2][warp] = n_before;
+  n_left = (int)__reduce_add_sync(0xffffffffu, (unsigned)n_left);
+  if (lane == 0) sh.counts[0][warp] = not_yet, sh.counts[1][warp] = below_cut, sh.counts[2][warp] = n_before, sh.counts[3][warp] = n_left;
   __syncthreads();
   if (warp) return;
   int first = (int)__reduce_add_sync(0xffffffffu, lane < kWarps ? (unsigned)sh.counts[0][lane] : 0u);
   int last = (int)__reduce_add_sync(0xffffffffu, lane < kWarps ? (unsigned)sh.counts[1][lane] : 0u);
   int n_above = (int)__reduce_max_sync(0xffffffffu, (unsigned)sh.counts[2][lane % kWarps]);
+  n_left = (int)__reduce_add_sync(0xffffffffu, lane < kWarps ? (unsigned)sh.counts[3][lane] : 0u);
   if (lane) return;
+  sh.told[2].inside = (u64)n_left;
   sh.told[2].first = first, sh.told[2].last = last, sh.told[2].count = n_above;
   sh.told[2].mx = (float)(by_count && all < k_left);
 }
@@ -533,12 +566,12 @@ template <typename T> __device__ __noinline__ void after_count_together() {
   State& st = sh.st;
   together(st.ctas);
   if (threadIdx.x) return;
-  int first = 0, last = 0, n_above = 0;
+  int first = 0, last = 0, n_above = 0, n_left = 0;
 #pragma unroll
   for (int i = 0; i < kCtas; ++i)
     if (i < st.ctas) {
       const Told& o = of_cta(i).told[2];
-      first += o.first, last += o.last, n_above = max(n_above, o.count);
+      first += o.first, last += o.last, n_above = max(n_above, o.count), n_left += (int)o.inside;
     }
   if (sh.told[2].mx != 0.f) {  // fewer than k: all of it
     if (st.top_p < 1.f) begin_cut(st, false);
@@ -551,6 +584,11 @@ template <typename T> __device__ __noinline__ void after_count_together() {
   } else {
     first = min(first, kFirst - 1);
     last = max(first, min(last, kFirst) - 1);
+  }
+  if (n_left <= kList && st.xt0 == -INFINITY && !st.exact) {
+    st.last = last;
+    st.pass = kGather;
+    return;
   }
   // the places of the values in these bins
   const double slack = 1.0 + 0x1p-21, m = st.m, inv = st.inv;
@@ -678,6 +716,118 @@ template <typename T> __device__ __noinline__ void after_bin() {
     while ((to - from) >> shift >= (unsigned)kBins) ++shift;
     st.shift = shift;
     st.pass = kRefine;
+  }
+}
+// Elements 2 tid and 2 tid + 1 (a, b) of n2 (a power of two, up to kList), put in falling order by exchanges.
+__device__ __noinline__ void sort_falling(u64& a, u64& b, int n2) {
+  const int tid = threadIdx.x;
+  u64* const list = shared().list;
+#pragma unroll 1
+  for (int size = 2; size <= n2; size <<= 1) {
+    const bool falling = !(2 * tid & size);
+#pragma unroll 1
+    for (int stride = size >> 1; stride > 1; stride >>= 1) {
+      u64 c, d;
+      if (stride < 64) {
+        c = __shfl_xor_sync(0xffffffffu, a, stride >> 1), d = __shfl_xor_sync(0xffffffffu, b, stride >> 1);
+      } else {
+        __syncthreads();
+        list[2 * tid] = a, list[2 * tid + 1] = b;
+        __syncthreads();
+        c = list[(2 * tid) ^ stride], d = list[(2 * tid + 1) ^ stride];
+      }
+      const bool larger = !(2 * tid & stride) == falling;
+      a = larger == (a < c) ? c : a;
+      b = larger == (b < d) ? d : b;
+    }
+    if ((a < b) == falling) {
+      const u64 c = a;
+      a = b, b = c;
+    }
+  }
+}
+// The first CTA puts the gathered columns in order, finds the cuts by the sums before each, puts what is left in the order of
+// its places, and draws.  Of top-k's columns weights are taken in fp64 at once; top-p alone has its whole from
+// all columns, in fp32 as elsewhere.
+template <typename T> __device__ __noinline__ void finish() {
+  Shared& sh = shared();
+  State& st = sh.st;
+  const int tid = threadIdx.x, lane = tid & 31, C = st.ctas;
+  const bool by_count = st.by_count;
+  __syncthreads();
+  const u64 mine = warp_total(lane < kWarps ? sh.sums[0][lane] : 0);
+  if (tid == 0) sh.told[3].sum = mine, sh.told[3].count = min(sh.listed, kList);
+  together(C);
+  if (st.rank == 0) {
+    const Told& o = of_cta(min(lane, C - 1)).told[3];
+    const int upto = warp_inclusive(lane < C ? o.count : 0), n = min(kList, __shfl_sync(0xffffffffu, upto, 31));
+    u64 whole = warp_total(lane < C ? o.sum : 0);
+    u64 e[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      int from = 0, cta = 0;
+#pragma unroll 1
+      for (int i = 0; i + 1 < C; ++i) {
+        const int end = __shfl_sync(0xffffffffu, upto, i);
+        if (2 * tid + j >= end) from = end, cta = i + 1;
+      }
+      e[j] = 2 * tid + j < n ? of_cta(cta).list[2 * tid + j - from] : 0;
+    }
+    int n2 = 2;
+    while (n2 < n) n2 <<= 1;
+    sort_falling(e[0], e[1], n2);
+    Weight<T> weight(st);
+    weight.exact |= by_count;
+    const int k = by_count ? st.k : n;
+    float x[2];
+    u64 w[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      x[j] = value_of<T>((unsigned)(e[j] >> 32));
+      w[j] = 2 * tid + j < k ? weight(x[j]) : 0;
+    }
+    u64 all;
+    const u64 before = before_thread(w[0] + w[1], sh.sums[1], all);
+    if (by_count) whole = all;
+    const double target = st.top_p < 1.f ? (double)st.top_p * (double)whole : INFINITY, g = by_count ? 0.0 : guard(st, whole);
+    const bool beyond = !by_count && all < whole && (double)all < target, missed = beyond && !st.sure;
+    bool open = beyond || (!by_count && all < whole && fabs((double)all - target) <= g);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int i = 2 * tid + j;
+      const double b = (double)(before + (j ? w[0] : 0));
+      if (i > 0 && i < k) open |= !by_count && fabs(b - target) <= g;
+      const bool keep = i < k && x[j] >= st.xmin && (i == 0 || b < target);
+      e[j] = keep ? e[j] << 32 | e[j] >> 32 : 0;
+    }
+    open = __syncthreads_or(open);
+    sort_falling(e[0], e[1], n2);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) w[j] = e[j] ? weight(value_of<T>((unsigned)e[j])) : 0;
+    u64 at = before_thread(w[0] + w[1], sh.sums[2], all);
+    const double goal = st.u * (double)all;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const u64 to = at + w[j];
+      if (w[j] && (double)to > goal && (at == 0 || (double)at <= goal)) {
+        open |= !by_count && ((at > 0 && fabs((double)at - goal) <= g) || (to < all && fabs((double)to - goal) <= g));
+        const Cut f{(int)~(unsigned)(e[j] >> 32), missed, 0, 0, 0, open};
+#pragma unroll 1
+        for (int i = 0; i < C; ++i) of_cta(i).cut = f;
+      }
+      at = to;
+    }
+  }
+  together(C);
+  if (tid) return;
+  if (sh.cut.above) {
+    st.sure = true;
+    begin_cut(st, false);
+  } else if (sh.cut.open) {
+    again_exactly(st);
+  } else {
+    st.token = sh.cut.bin;
+    st.pass = kDone;
   }
 }
 // The CTA, the chunk and the column at which the sum passes u times the whole.
@@ -864,6 +1014,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const SamplePa
       pass_count<T>();
       after_count<T>();
       after_count_together<T>();
+    } else if (pass == kGather) {
+      pass_gather<T>();
+      finish<T>();
     } else if (pass == kSum) {
       pass_sum<T>();
       draw<T>();
@@ -880,7 +1033,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const SamplePa
       }
     }
     __syncthreads();
-    if (tid == 0 && (pass == kSeek || pass == kWeigh)) st.z_due = false;
+    if (tid == 0 && (pass == kSeek || pass == kWeigh || pass == kGather)) st.z_due = false;
     pass = st.pass;
   }
 
