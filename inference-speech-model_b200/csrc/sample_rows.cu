@@ -38,7 +38,7 @@ constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
 constexpr int kFirst = 2048;      // bins of the first histogram (counts)
 constexpr int kBins = 512;        // of the later ones (counts and weights)
-constexpr int kList = 2 * kThreads;  // columns that one CTA can put in order
+constexpr int kList = kThreads;   // columns that one CTA puts in order
 constexpr int kMaxChunks = 256;   // of a CTA's columns
 constexpr int kCtas = 8;          // of a cluster, at most
 constexpr int kScale = 44;        // a weight of 1 is 2^44: sums of 2^19 columns fit in 64 bits
@@ -104,7 +104,7 @@ struct Shared {
   u64 sums[3][kWarps];
   union {  // the first histogram, and what comes after it: the later ones and the chunks' sums, or the columns that are left
     unsigned first_count[kFirst];
-    u64 list[kList];  // place << 32 | ~column
+    u64 list[2][kList];  // place << 32 | ~column; and in their order
     struct {
       u64 chunk_sum[kMaxChunks];
       int chunk_ties[kMaxChunks];
@@ -380,7 +380,7 @@ template <typename T> __device__ __noinline__ void pass_gather() {
     if (!by_count) all += weight(v);
     if (bin_of(v, m, inv) > last) return;
     const int at = atomicAdd(&shared().listed, 1);
-    if (at < kList) shared().list[at] = (u64)place_of<T>(v) << 32 | (unsigned)~c;
+    if (at < kList) shared().list[0][at] = (u64)place_of<T>(v) << 32 | (unsigned)~c;
   }, Nothing{});
   z.keep();
   all = warp_total(all);
@@ -718,33 +718,27 @@ template <typename T> __device__ __noinline__ void after_bin() {
     st.pass = kRefine;
   }
 }
-// Elements 2 tid and 2 tid + 1 (a, b) of n2 (a power of two, up to kList), put in falling order by exchanges.
-__device__ __noinline__ void sort_falling(u64& a, u64& b, int n2) {
+// The tid-th largest of the n elements that threads have, element tid each; all differ.  A thread finds a part of one
+// element's rank, which is what a sorting network's many short steps lose to (340 cycles each; 114 elements 9,400).
+__device__ __noinline__ u64 nth_largest(u64 element, int n) {
   const int tid = threadIdx.x;
-  u64* const list = shared().list;
-#pragma unroll 1
-  for (int size = 2; size <= n2; size <<= 1) {
-    const bool falling = !(2 * tid & size);
-#pragma unroll 1
-    for (int stride = size >> 1; stride > 1; stride >>= 1) {
-      u64 c, d;
-      if (stride < 64) {
-        c = __shfl_xor_sync(0xffffffffu, a, stride >> 1), d = __shfl_xor_sync(0xffffffffu, b, stride >> 1);
-      } else {
-        __syncthreads();
-        list[2 * tid] = a, list[2 * tid + 1] = b;
-        __syncthreads();
-        c = list[(2 * tid) ^ stride], d = list[(2 * tid + 1) ^ stride];
-      }
-      const bool larger = !(2 * tid & stride) == falling;
-      a = larger == (a < c) ? c : a;
-      b = larger == (b < d) ? d : b;
-    }
-    if ((a < b) == falling) {
-      const u64 c = a;
-      a = b, b = c;
-    }
+  u64 (&list)[2][kList] = shared().list;
+  int parts = 1;  // of the list, a thread each
+  while (parts < 32 && 2 * parts * n <= kThreads) parts *= 2;
+  __syncthreads();
+  if (tid < n) list[0][tid] = element;
+  __syncthreads();
+  const int i = tid / parts, part = tid % parts;
+  int rank = 0;
+  if (tid / 32 * 32 < n * parts) {
+    const u64 mine = list[0][min(i, n - 1)];
+#pragma unroll 4
+    for (int j = part; j < n; j += parts) rank += list[0][j] > mine;
+    for (int o = 1; o < parts; o *= 2) rank += __shfl_xor_sync(0xffffffffu, rank, o);
+    if (i < n && part == 0) list[1][rank] = mine;
   }
+  __syncthreads();
+  return tid < n ? list[1][tid] : 0;
 }
 // The first CTA puts the gathered columns in order, finds the cuts by the sums before each, puts what is left in the order of
 // its places, and draws.  Of top-k's columns weights are taken in fp64 at once; top-p alone has its whole from
@@ -762,60 +756,36 @@ template <typename T> __device__ __noinline__ void finish() {
     const Told& o = of_cta(min(lane, C - 1)).told[3];
     const int upto = warp_inclusive(lane < C ? o.count : 0), n = min(kList, __shfl_sync(0xffffffffu, upto, 31));
     u64 whole = warp_total(lane < C ? o.sum : 0);
-    u64 e[2];
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      int from = 0, cta = 0;
+    int from = 0, cta = 0;  // whose list holds element tid
 #pragma unroll 1
-      for (int i = 0; i + 1 < C; ++i) {
-        const int end = __shfl_sync(0xffffffffu, upto, i);
-        if (2 * tid + j >= end) from = end, cta = i + 1;
-      }
-      e[j] = 2 * tid + j < n ? of_cta(cta).list[2 * tid + j - from] : 0;
+    for (int i = 0; i + 1 < C; ++i) {
+      const int end = __shfl_sync(0xffffffffu, upto, i);
+      if (tid >= end) from = end, cta = i + 1;
     }
-    int n2 = 2;
-    while (n2 < n) n2 <<= 1;
-    sort_falling(e[0], e[1], n2);
+    u64 e = nth_largest(tid < n ? of_cta(cta).list[0][tid - from] : 0, n);
     Weight<T> weight(st);
     weight.exact |= by_count;
     const int k = by_count ? st.k : n;
-    float x[2];
-    u64 w[2];
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      x[j] = value_of<T>((unsigned)(e[j] >> 32));
-      w[j] = 2 * tid + j < k ? weight(x[j]) : 0;
-    }
-    u64 all;
-    const u64 before = before_thread(w[0] + w[1], sh.sums[1], all);
+    const float x = value_of<T>((unsigned)(e >> 32));
+    u64 w = tid < k ? weight(x) : 0, all;
+    const u64 before = before_thread(w, sh.sums[1], all);
     if (by_count) whole = all;
     const double target = st.top_p < 1.f ? (double)st.top_p * (double)whole : INFINITY, g = by_count ? 0.0 : guard(st, whole);
     const bool beyond = !by_count && all < whole && (double)all < target, missed = beyond && !st.sure;
     bool open = beyond || (!by_count && all < whole && fabs((double)all - target) <= g);
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const int i = 2 * tid + j;
-      const double b = (double)(before + (j ? w[0] : 0));
-      if (i > 0 && i < k) open |= !by_count && fabs(b - target) <= g;
-      const bool keep = i < k && x[j] >= st.xmin && (i == 0 || b < target);
-      e[j] = keep ? e[j] << 32 | e[j] >> 32 : 0;
-    }
+    if (tid > 0 && tid < k) open |= !by_count && fabs((double)before - target) <= g;
+    const bool keep = tid < k && x >= st.xmin && (tid == 0 || (double)before < target);
     open = __syncthreads_or(open);
-    sort_falling(e[0], e[1], n2);
-#pragma unroll
-    for (int j = 0; j < 2; ++j) w[j] = e[j] ? weight(value_of<T>((unsigned)e[j])) : 0;
-    u64 at = before_thread(w[0] + w[1], sh.sums[2], all);
+    const int kept = __syncthreads_count(keep);  // the first ones
+    e = nth_largest(e << 32 | e >> 32, kept);    // by their places
+    w = e ? weight(value_of<T>((unsigned)e)) : 0;
+    const u64 at = before_thread(w, sh.sums[2], all), to = at + w;
     const double goal = st.u * (double)all;
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const u64 to = at + w[j];
-      if (w[j] && (double)to > goal && (at == 0 || (double)at <= goal)) {
-        open |= !by_count && ((at > 0 && fabs((double)at - goal) <= g) || (to < all && fabs((double)to - goal) <= g));
-        const Cut f{(int)~(unsigned)(e[j] >> 32), missed, 0, 0, 0, open};
+    if (w && (double)to > goal && (at == 0 || (double)at <= goal)) {
+      open |= !by_count && ((at > 0 && fabs((double)at - goal) <= g) || (to < all && fabs((double)to - goal) <= g));
+      const Cut f{(int)~(unsigned)(e >> 32), missed, 0, 0, 0, open};
 #pragma unroll 1
-        for (int i = 0; i < C; ++i) of_cta(i).cut = f;
-      }
-      at = to;
+      for (int i = 0; i < C; ++i) of_cta(i).cut = f;
     }
   }
   together(C);
