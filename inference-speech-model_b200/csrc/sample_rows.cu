@@ -144,10 +144,11 @@ template <typename T> struct Weight {
   double t;
   bool exact;
   __device__ __forceinline__ explicit Weight(const State& st) : m(st.m), hi(st.hi), lo(st.lo), t(st.t), exact(st.exact) {}
-  __device__ __forceinline__ u64 operator()(float x) const {
-    if (exact) return exact_weight(((double)x - (double)m) / t * 1.4426950408889634074);
+  __device__ __forceinline__ u64 operator()(float x) const { return exact ? of<true>(x) : of<false>(x); }
+  template <bool EXACT> __device__ __forceinline__ u64 of(float x) const {
+    if (EXACT) return exact_weight(((double)x - (double)m) / t * 1.4426950408889634074);
     const float d = x - m;  // <= 0
-    const float n = fmaxf(rintf(d * hi), -100.f);
+    const float n = fmaxf(rintf(d * hi), -63.f);
     // f keeps what the subtraction rounded off (16-bit values: next to nothing)
     float f = fmaf(d, hi, -n), rest = d * lo;
     if constexpr (sizeof(T) == 4) {
@@ -164,8 +165,7 @@ template <typename T> struct Weight {
     q = fmaf(q, f, 0.24022650718688965f);
     q = fmaf(q, f, 0.6931471824645996f);
     const unsigned bits = (1u << 28) + (unsigned)__float2int_rn(f * q * 0x1p28f);
-    const int shift = kScale - 28 + (int)n;
-    return shift >= 0 ? (u64)bits << shift : shift > -29 ? bits >> -shift : 0;
+    return ((u64)bits << (kScale - 28)) >> -(int)n;
   }
 };
 
@@ -174,6 +174,13 @@ template <typename V> __device__ __forceinline__ V warp_total(V v) {
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
+// (of 63 bits, 21 at a time: one instruction each in place of ten)
+template <> __device__ __forceinline__ u64 warp_total<u64>(u64 v) {
+  const unsigned low = (unsigned)v & 0x1fffffu, mid = (unsigned)(v >> 21) & 0x1fffffu, high = (unsigned)(v >> 42);
+  return __reduce_add_sync(0xffffffffu, low) + ((u64)__reduce_add_sync(0xffffffffu, mid) << 21) +
+         ((u64)__reduce_add_sync(0xffffffffu, high) << 42);
+}
+template <> __device__ __forceinline__ int warp_total<int>(int v) { return (int)__reduce_add_sync(0xffffffffu, (unsigned)v); }
 template <typename V> __device__ __forceinline__ V warp_inclusive(V v) {
   const int lane = threadIdx.x & 31;
 #pragma unroll
@@ -298,23 +305,22 @@ template <typename T> __device__ __noinline__ void pass_count() {
   }, Nothing{});
 }
 // weights: above the cut's bins (chunk by chunk, too), in them (by their place) and below
-template <typename T> __device__ __noinline__ void pass_weigh() {
+template <typename T, bool EXACT> __device__ __noinline__ void pass_weigh() {
   Shared& sh = shared();
   const State& st = sh.st;
   const Weight<T> weight(st);
   const bool cut = st.top_p < 1.f;
   const float m = st.m, inv = st.inv, xt0 = st.xt0, xmin = st.xmin;
-  const int first = cut ? st.first : kFirst, last = st.last, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int first = cut ? st.first : kFirst, last = cut ? st.last : kFirst, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (cut) clear_bins();
-  u64 above = 0, inside = 0, below = 0, mine = 0;
+  u64 all = 0, above = 0, inside = 0, mine = 0;
   if (cut && xt0 > -INFINITY && st.rank == 0 && threadIdx.x == 0) {  // columns that have xt0 itself, by their number
     const int bin = bin_of(xt0, m, inv);
     const u64 w = weight(xt0) * (u64)st.ties0;
+    all = w;
     if (bin < first) {
       above = w;
-    } else if (bin > last) {
-      below = w;
-    } else {
+    } else if (bin <= last) {
       inside = w;
       put(sub_of(place_of<T>(xt0), st), (unsigned)st.ties0, w);
     }
@@ -322,15 +328,12 @@ template <typename T> __device__ __noinline__ void pass_weigh() {
   Z z(st);
   each<T>([&](int, float v) {
     z.add(v);
-    if (!(v > xt0)) return;
-    const u64 w = weight(v);
-    const int bin = cut ? bin_of(v, m, inv) : 0;
-    if (bin < first) {
-      above += w;
-      if (v >= xmin) mine += w;
-    } else if (bin > last) {
-      below += w;
-    } else {
+    const u64 w = v > xt0 ? weight.template of<EXACT>(v) : 0;
+    const int bin = bin_of(v, m, inv);  // (the last one for -inf, which weighs nothing)
+    all += w;
+    above += bin < first ? w : 0;
+    mine += bin < first && v >= xmin ? w : 0;
+    if (bin >= first && bin <= last && v > xt0) {  // few
       inside += w;
       const int sub = sub_of(place_of<T>(v), shared().st);
       if (sub >= 0) put(sub, 1, w);
@@ -341,7 +344,8 @@ template <typename T> __device__ __noinline__ void pass_weigh() {
     mine = 0;
   });
   z.keep();
-  above = warp_total(above), inside = warp_total(inside), below = warp_total(below);
+  const u64 below = warp_total(all - above - inside);
+  above = warp_total(above), inside = warp_total(inside);
   if (lane == 0) sh.sums[0][warp] = above, sh.sums[1][warp] = inside, sh.sums[2][warp] = below;
 }
 template <typename T> __device__ __noinline__ void pass_refine() {
@@ -376,9 +380,8 @@ template <typename T> __device__ __noinline__ void pass_gather() {
   Z z(st);
   each<T>([&](int c, float v) {
     z.add(v);
-    if (!(v > -INFINITY)) return;
-    if (!by_count) all += weight(v);
-    if (bin_of(v, m, inv) > last) return;
+    if (!by_count) all += v > -INFINITY ? weight.template of<false>(v) : 0;
+    if (bin_of(v, m, inv) > last || !(v > -INFINITY)) return;
     const int at = atomicAdd(&shared().listed, 1);
     if (at < kList) shared().list[0][at] = (u64)place_of<T>(v) << 32 | (unsigned)~c;
   }, Nothing{});
@@ -486,7 +489,7 @@ template <typename T> __device__ __noinline__ void after_count() {
   // between these.
   const int share = kFirst / C, per = tid * max(1, share / kThreads) < share ? max(1, share / kThreads) : 0;
   const int at0 = rank * share + tid * per;
-  const float step = (float)(1.4426950408889634 / ((double)st.inv * st.t));
+  constexpr float step = 1.4426950408889634f * 40.f / (kFirst - 1);  // of weights by a bin, as an exponent of 2
   auto most_of = [&](int bin) { return bin ? ex2_approx(-bin * step) * (1.f + 2e-5f) : 1.f; };
   const bool sure = st.sure;
   const float half = ex2_approx(-0.5f * step);  // the middle of a bin against its upper end
@@ -992,8 +995,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const SamplePa
       draw<T>();
     } else {
       const bool weigh = pass == kWeigh;
-      if (weigh) pass_weigh<T>();
-      else pass_refine<T>();
+      if (!weigh) pass_refine<T>();
+      else if (st.exact) pass_weigh<T, true>();
+      else pass_weigh<T, false>();
       if (weigh && !(st.top_p < 1.f)) {
         __syncthreads();
         if (tid == 0) st.pass = kSum;
