@@ -6,15 +6,18 @@
 //
 // What bounds it: a row is read once from memory, 2 or 4 bytes a column, and again from shared memory by each later pass;
 // the passes' instructions, some 50 a column in all, are what takes the time, and for one row the clusters' barriers
-// between them.  Nothing is sorted:
+// between them.  Rows are not sorted:
 // * A cluster of up to 8 CTAs shares a row.  A cut (the k-th largest, or the value at which the weight reaches p) is
 //   found by histograms.  The first counts columns by their distance from m (one atomic a column).  For the k-th largest
-//   the cut lies in one of its bins.  For p each bin's weight is known to within 2 %, and nearly always to within a
-//   thousandth, so the cut lies in a few; the next pass adds up the weights above, in and below these, and only the
-//   columns in them enter a histogram of weights.  (If the thousandth did not hold, which the sums show, the bins are
-//   taken anew from what is certain.  At once from that, a cut far down a flat row had a tenth of the columns to put in
-//   their bins.)  Later passes look at the order-preserving integers of the values in the bin that holds the cut, until a
-//   bin holds one value.  Equal values that the cut divides count by their place.
+//   the cut lies in one of its bins.  For p each bin's weight is known to within 2 %, and
+//   their sums, by the law of large numbers, to some hundred-thousandths, so the cut nearly always lies in one or two; the
+//   next pass adds up the weights above, in and below these, and only the columns in them enter a histogram of weights.
+//   (If it lies elsewhere, which the sums show, the bins are taken anew from what is certain.  At once from that, a cut
+//   far down a flat row had a tenth of the columns to put in their bins.)  Later passes look at the order-preserving
+//   integers of the values in the bin that holds the cut, until a bin holds one value.  Equal values that the cut
+//   divides count by their place.
+// * Where 512 columns or fewer are left, above the cut and in its bins, the first CTA gets these and puts them in order, by
+//   their ranks: cuts and the draw are then sums before a thread.
 // * Every sum of weights is an integer (units of 2^-44 of the largest weight), so no order of atomics or threads changes a
 //   result, and cumulative sums are exact in their weights.
 // * Weights are fp32 polynomials of an argument that keeps the rounding of x - m, good to 2^-23.8.  A decision that an error
@@ -485,18 +488,18 @@ template <typename T> __device__ __noinline__ void after_count() {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, C = st.ctas, rank = st.rank, k_left = st.k_left;
   const bool by_count = st.by_count;
   together(C);
-  // A thread has 4, 2 or 1 bins of the rank's share of them (or, of eight CTAs, every other thread one).  Weights of a bin:
-  // between these.
+  // A thread has 4, 2 or 1 bins of the rank's share of them (or, of eight CTAs, every other thread one).  Their weights are
+  // sums of most and least, or (not sure) in `least` of the middles and in `most` of the squares of these.
   const int share = kFirst / C, per = tid * max(1, share / kThreads) < share ? max(1, share / kThreads) : 0;
   const int at0 = rank * share + tid * per;
   constexpr float step = 1.4426950408889634f * 40.f / (kFirst - 1);  // of weights by a bin, as an exponent of 2
   auto most_of = [&](int bin) { return bin ? ex2_approx(-bin * step) * (1.f + 2e-5f) : 1.f; };
   const bool sure = st.sure;
   const float half = ex2_approx(-0.5f * step);  // the middle of a bin against its upper end
-  auto most_at = [&](int bin) { return sure || bin + 1 == kFirst ? most_of(bin) : most_of(bin) * half * 1.001f; };
   auto least_at = [&](int bin) {
-    return bin + 1 == kFirst ? 0.f : sure ? most_of(bin + 1) * (1.f - 6e-5f) : most_of(bin) * half * 0.999f;
+    return !sure ? most_of(bin) * half : bin + 1 == kFirst ? 0.f : most_of(bin + 1) * (1.f - 6e-5f);
   };
+  auto most_at = [&](int bin) { return sure ? most_of(bin) : least_at(bin) * least_at(bin); };
   int n[4], all_n = 0;
   float least = 0.f, most = 0.f;
 #pragma unroll
@@ -527,8 +530,10 @@ template <typename T> __device__ __noinline__ void after_count() {
     a_most += warp_total(lane < rank ? o_most : 0.f);
     all = warp_total(o_n), all_least = warp_total(o_least), all_most = warp_total(o_most);
   }
-  // The bins before the cut's: how many there are in all.  (Sums of fp32 here are off by less than 1e-5 of the whole.)
-  const float off = 2e-5f * all_most, t_least = st.top_p * all_least - off, t_most = st.top_p * all_most + off;
+  // The bins before the cut's: how many there are in all.  (Sums of fp32 here are off by less than 1e-5 of the whole.  A
+  // column lies off the middle of its bin by a factor whose standard deviation is 0.0057: three of the sum's are allowed.)
+  const float off = sure ? 2e-5f * all_most : 4e-5f * all_least + 3.f * 0.0057f * sqrtf(all_most);
+  const float t_least = st.top_p * all_least - off, t_most = st.top_p * (sure ? all_most : all_least) + off;
   int not_yet = 0, below_cut = 0, n_before = 0;  // n_before: columns above the cut's bin, if it is this thread's
   int n_left = 0;                                // and those above and in the cut's bins
 #pragma unroll
@@ -544,7 +549,7 @@ template <typename T> __device__ __noinline__ void after_count() {
       if (may) n_left += n[j];
       a_most += n[j] * most_at(at0 + j);
       a_least += n[j] * least_at(at0 + j);
-      not_yet += a_most < t_least || above_n + n[j] == 0;  // surely ends below it
+      not_yet += (sure ? a_most : a_least) < t_least || above_n + n[j] == 0;  // surely ends below it
     }
     above_n += n[j];
   }
