@@ -2,8 +2,8 @@
  * spd_b200.h — C ABI of the B200 (sm_100a) speech-decode hot path.
  *
  * One shared library (libspd_b200.so) exports the decode-path operations of the Whisper-class
- * serving engine, those of decoders with rotary positions, grouped heads and a 4-bit cache, and
- * error/workspace helpers.  Every entry point:
+ * serving engine, those of decoders with rotary positions, grouped heads and a 4-bit cache, those for
+ * several candidates of a request, and error/workspace helpers.  Every entry point:
  *   - takes plain device pointers, sizes and a cudaStream_t passed as `void*`
  *     (NULL = legacy default stream); no torch types cross this boundary;
  *   - returns an int status (SPD_OK == 0); on failure spd_get_last_error() gives text;
@@ -348,7 +348,7 @@ int spd_prompt_attn(const void* q, int64_t q_stride_t, int64_t q_stride_h, const
  *   q [B][Hq][D] with token and head strides in elements, D contiguous; out [B][Hq][D] contiguous (q itself may
  *      be the output); query head h reads key/value head h / (Hq / Hkv)
  *   k_pool, v_pool [num_blocks][block_size][Hkv][D]
- *   cu_groups int32 [G + 1]: group g owns sequences [cu[g], cu[g + 1]); a sequence of no group has no prefix
+ *   cu_groups int32 [G + 1], not falling: group g owns sequences [cu[g], cu[g + 1]); a sequence of no group has no prefix
  *   prefix_tables int32 [G][max_prefix_blocks], prefix_lens int32 [G]: the groups' prefixes; G == 0 or
  *      max_prefix_blocks == 0: none
  *   block_tables int32 [B][max_blocks], context_lens int32 [B]: the sequences' own tokens (<= 0: none)
@@ -371,7 +371,7 @@ int spd_shared_prefix_attn(const void* q, int64_t q_stride_t, int64_t q_stride_h
  * without a causal mask: query i of request b attends positions t < valid_lens[b] of slot slot_ids[b].
  *   q [N][Hq][D] packed, token and head strides in elements; out [N][Hq][D] contiguous (q itself may be the output)
  *   k, v: element (slot, h, t, d) at slot * kv_stride_slot + h * kv_stride_h + t * kv_stride_t + d; S slots, T positions
- *   cu_seqlens int32 [B + 1]: request b owns queries [cu[b], cu[b + 1]); NULL: N == B, one query a request
+ *   cu_seqlens int32 [B + 1], not falling: request b owns queries [cu[b], cu[b + 1]); NULL: N == B, one query a request
  *   slot_ids int32 [B], or NULL: slot b.  Two requests may share a slot.
  *   A query without any key gives zeros; rows of out that belong to no request are untouched.  A length beyond T is
  *   cut to it (flagged), a slot id out of range leaves its request without keys (flagged).
@@ -383,7 +383,7 @@ int spd_cross_attn_packed(const void* q, int64_t q_stride_t, int64_t q_stride_h,
                           int Hkv, int D, float scale, int dtype, void* workspace, size_t workspace_bytes,
                           int32_t* error_word, void* stream);
 
-/* A token a row, beside spd_argmax_rows: x [rows][ld], of which the first cols columns (up to 2^19) take part; skip_mask
+/* A token a row, beside spd_argmax_rows: x [rows][ld], of which the first cols columns (up to 2^19; 440,000 of fp32) take part; skip_mask
  * uint8 [cols] or NULL, columns that count as -inf.  temperature, top_k, top_p, min_p: [rows] device arrays, or NULL for the
  * *_all value in every row.  uniforms fp32 [rows], each in [0, 1).  With a row's largest value m and temperature t:
  *   t <= 0 (or NaN), or m not finite: the first largest column (a NaN wins), as spd_argmax_rows picks it;

@@ -584,7 +584,7 @@ def prompt_attention(
 # ----------------------------------------------------------------------------- several candidates of one request
 def shared_prefix_workspace(B: int, G: int, Hq: int, Hkv: int, D: int, block_size: int, max_prefix_blocks: int, max_blocks: int,
                             device: torch.device) -> torch.Tensor:
-    """Zero-filled workspace for ``shared_prefix_decode_attention`` (reusable on one stream)."""
+    """Zero-filled workspace for ``shared_prefix_decode_attention`` calls of this geometry (reusable on one stream)."""
     idx = device.index if device.index is not None else torch.cuda.current_device()
     n = N.load().spd_shared_prefix_attn_workspace_size(B, G, Hq, Hkv, D, block_size, max_prefix_blocks, max_blocks, idx)
     if n == 0:
@@ -593,7 +593,7 @@ def shared_prefix_workspace(B: int, G: int, Hq: int, Hkv: int, D: int, block_siz
 
 
 def cross_attn_packed_workspace(N_queries: int, Hq: int, Hkv: int, D: int, device: torch.device) -> torch.Tensor:
-    """Zero-filled workspace for ``cross_attention_packed`` (reusable on one stream)."""
+    """Zero-filled workspace for ``cross_attention_packed`` calls of this geometry (reusable on one stream)."""
     idx = device.index if device.index is not None else torch.cuda.current_device()
     n = N.load().spd_cross_attn_packed_workspace_size(N_queries, Hq, Hkv, D, idx)
     if n == 0:
@@ -621,7 +621,7 @@ def shared_prefix_decode_attention(
     q [B, Hq, D] (fp16 / bf16, D a multiple of 8 up to 128, any token and head strides that are multiples of 16
     bytes); k_pool / v_pool [num_blocks, block_size, Hkv, D] as ``rope_kv_append`` writes them (Hq a multiple of
     Hkv, block_size 8 to 128, a power of two).  Group g is the sequences [cu_groups[g], cu_groups[g + 1])
-    (int32 [G + 1]); each attends the first prefix_lens[g] tokens of prefix_tables[g] (int32 [G], [G, columns]), then
+    (int32 [G + 1], not falling); each attends the first prefix_lens[g] tokens of prefix_tables[g] (int32 [G], [G, columns]), then
     its own context_lens[b] tokens of block_tables[b] (int32 [B], [B, columns]; <= 0: none).  A sequence of no group has
     no prefix, and without the three prefix arguments (None) none has.  A sequence without any key gives
     zeros.  ``out`` may be q itself.  Device flags (a block id or length out of range, a wait that ran out)
@@ -647,7 +647,7 @@ def cross_attention_packed(
     read once for all of them (fp16 / bf16, D a multiple of 8 up to 128, Hq a multiple of Hkv).
 
     q [N, Hq, D] packed: request b owns rows [cu_seqlens[b], cu_seqlens[b + 1]) (int32 [B + 1]; None: one query a
-    request); k, v [S, Hkv, T, D] with any slot, head and row strides that are multiples of 16 bytes (the same for
+    request; not falling); k, v [S, Hkv, T, D] with any slot, head and row strides that are multiples of 16 bytes (the same for
     both); request b attends positions t < valid_lens[b] (int32 [B]) of slot slot_ids[b] (int32 [B]; None: slot
     b).  A query without any key gives zeros; rows that belong to no request are left as they are in ``out``,
     which may be q itself.  Flags as in ``shared_prefix_decode_attention``.  Returns out [N, Hq, D]."""
@@ -668,7 +668,7 @@ def sample_rows(
     logprobs: Optional[torch.Tensor] = None,
 ) -> torch.Tensor:
     """Draws a token from the first ``cols`` columns of each row of ``x`` [rows, ld] (fp32 / fp16 / bf16, unit column
-    stride) with the row's random number uniforms[r] (float32 [rows], in [0, 1)); ``skip``, a bool [cols] mask or
+    stride; up to 2^19 columns, 440,000 of fp32) with the row's random number uniforms[r] (float32 [rows], in [0, 1)); ``skip``, a bool [cols] mask or
     None, marks columns that count as -inf.
 
     temperature, top_k, top_p and min_p are numbers, or tensors with one for each row (float32, top_k int32).  With the
