@@ -20,9 +20,10 @@
 //   their ranks: cuts and the draw are then sums before a thread.
 // * Every sum of weights is an integer (units of 2^-44 of the largest weight), so no order of atomics or threads changes a
 //   result, and cumulative sums are exact in their weights.
-// * Weights are fp32 polynomials of an argument that keeps the rounding of x - m, good to 2^-23.8.  A decision that an error
-//   of 2^-22.4 of the whole could turn is taken again with weights in fp64 (one row in twenty where two hundred
-//   thousand columns weigh alike, else next to none), so that the token is the one that fp64 arithmetic gives.
+// * Weights are fp32 polynomials of an argument in two parts, good to 2^-26.4.  A decision that an error of 2^-25.4 of the
+//   whole could turn is taken again with weights in fp64 (one row in a hundred where two hundred thousand columns
+//   weigh alike, else next to none), so that the token is the one that fp64 arithmetic gives.  (With 2^-23.8, and a fifth
+//   fewer instructions a weight, it was one row in twenty, and the slowest row took twice as long.)
 // * A CTA's columns lie in its shared memory, and what is known of the row beside them: passes are functions that are
 //   called, so that none holds another's registers.  (In one function the state went to local memory, whose traffic
 //   was twice that of the columns: 87 us in place of 64 for the second case below, then.)
@@ -148,31 +149,35 @@ __device__ __noinline__ u64 exact_weight(double y) {
 }
 template <typename T> struct Weight {
   float m, hi, lo;  // the largest value, and log2(e) / t in two parts
-  double t;
+  double temperature;
   bool exact;
-  __device__ __forceinline__ explicit Weight(const State& st) : m(st.m), hi(st.hi), lo(st.lo), t(st.t), exact(st.exact) {}
+  __device__ __forceinline__ explicit Weight(const State& st)
+      : m(st.m), hi(st.hi), lo(st.lo), temperature(st.t), exact(st.exact) {}
   __device__ __forceinline__ u64 operator()(float x) const { return exact ? of<true>(x) : of<false>(x); }
   template <bool EXACT> __device__ __forceinline__ u64 of(float x) const {
-    if (EXACT) return exact_weight(((double)x - (double)m) / t * 1.4426950408889634074);
+    if (EXACT) return exact_weight(((double)x - (double)m) / temperature * 1.4426950408889634074);
     const float d = x - m;  // <= 0
-    const float n = fmaxf(rintf(d * hi), -63.f);
-    // f keeps what the subtraction rounded off (16-bit values: next to nothing)
-    float f = fmaf(d, hi, -n), rest = d * lo;
-    if constexpr (sizeof(T) == 4) {
+    // y = n + f + rest: f is exact (no contraction of its product), the rest what roundings left over
+    const float y = __fmul_rn(d, hi), n = fmaxf(rintf(y), -63.f), f = fmaxf(y - n, -1.f);
+    float rest = fmaf(d, lo, fmaf(d, hi, -y));
+    if constexpr (sizeof(T) == 4) {  // (of 16-bit values the subtraction rounds off next to nothing)
       const float b = d - x, a = d - b;
       rest = fmaf((x - a) - (m + b), hi, rest);
     }
-    f = fmaxf(f + rest, -1.f);
-    // 2^f = 1 + f q(f), q a polynomial fitted to (2^f - 1) / f on [-1/2, 1/2] (2e-10), in units of 2^-28: off by less than
-    // 2^-24.3 of itself with its roundings, 2^-23.8 with those of f
-    float q = fmaf(1.530370172986295e-05f, f, 0.00015461447765119374f);
-    q = fmaf(q, f, 0.0013333478709682822f);
-    q = fmaf(q, f, 0.009618056938052177f);
-    q = fmaf(q, f, 0.05550410971045494f);
-    q = fmaf(q, f, 0.24022650718688965f);
-    q = fmaf(q, f, 0.6931471824645996f);
-    const unsigned bits = (1u << 28) + (unsigned)__float2int_rn(f * q * 0x1p28f);
-    return ((u64)bits << (kScale - 28)) >> -(int)n;
+    // 2^f = 1 + f ln 2 + f^2 s(f), s a polynomial that interpolates (2^f - 1 - f ln 2) / f^2 at the Chebyshev nodes of
+    // [-1/2, 1/2] (4e-10), and 2^rest = 1 + rest ln 2.  f ln 2 in two parts, and what is added to 1 in units of 2^-30.
+    // Off by less than 2^-26.4 of itself (the half steps of s, f^2, the sum that holds the small terms, over 2^-1/2;
+    // 2^-26.9 at the worst of 10^8 arguments) and a unit of 2^-44 that the shift drops.
+    float s = fmaf(1.529094879515469e-05f, f, 0.00015453163359779865f);
+    s = fmaf(s, f, 0.0013333521783351898f);
+    s = fmaf(s, f, 0.009618083015084267f);
+    s = fmaf(s, f, 0.05550410971045494f);
+    s = fmaf(s, f, 0.24022650718688965f);
+    constexpr float c = 0.6931471824645996f, c_rest = -1.9046542121259336e-09f;  // ln 2
+    const float p = __fmul_rn(f, c), u = f * f, r = rest * c;
+    const float low = fmaf(f, c_rest, fmaf(f, c, -p)) + fmaf(r, fmaf(u, s, p), r), t = fmaf(u, s, low);
+    const unsigned bits = (1u << 30) + (unsigned)__float2int_rn(p * 0x1p30f) + (unsigned)__float2int_rn(t * 0x1p30f);
+    return ((u64)bits << (kScale - 30)) >> -(int)n;
   }
 };
 
@@ -437,8 +442,10 @@ __device__ __forceinline__ void again_exactly(State& st) {
   begin_cut(st, false);
   if (!(st.top_p < 1.f)) st.pass = kWeigh, st.first = kFirst;
 }
-// How far a sum and a target of it may be off: twice 2^-23.8 of the target.
-__device__ __forceinline__ double guard(const State& st, u64 whole) { return st.exact ? 0.0 : (double)whole * 0x1.78p-23; }
+// How far a sum and a target of it may be off: twice 2^-26.4 of the whole, and a unit for each column in both.
+__device__ __forceinline__ double guard(const State& st, u64 whole) {
+  return st.exact ? 0.0 : (double)whole * 0x1.84p-26 + 0x1p20;
+}
 // the largest value, and what comes first
 __device__ __noinline__ void after_max() {
   Shared& sh = shared();
