@@ -5,7 +5,7 @@
 //   its place, at which the weight left so far passes u times all of it.
 //
 // What bounds it: a row is read once from memory, 2 or 4 bytes a column, and again from shared memory by each later pass;
-// the passes' instructions, some 50 a column in all, are what takes the time, and for one row the clusters' barriers
+// the passes' instructions, some 60 a column in all, are what takes the time, and for one row the clusters' barriers
 // between them.  Rows are not sorted:
 // * A cluster of up to 8 CTAs shares a row.  A cut (the k-th largest, or the value at which the weight reaches p) is
 //   found by histograms.  The first counts columns by their distance from m (one atomic a column).  For the k-th largest
@@ -27,8 +27,8 @@
 // * A CTA's columns lie in its shared memory, and what is known of the row beside them: passes are functions that are
 //   called, so that none holds another's registers.  (In one function the state went to local memory, whose traffic
 //   was twice that of the columns: 87 us in place of 64 for the second case below, then.)
-// Measured on a B200, in CUDA graphs: one fp32 row of 51,865 columns by top-p 32 us, 64 fp16 rows of them by all settings 48,
-// 192 bf16 rows of 128,257 by top-k 98, 96 fp32 rows of 200,019 by top-p 251 (their reading alone: 0.04, 1.0, 7.5, 12).  A
+// Measured on a B200, in CUDA graphs: one fp32 row of 51,865 columns by top-p 32 us, 64 fp16 rows of them by all settings 46,
+// 192 bf16 rows of 128,257 by top-k 99, 96 fp32 rows of 200,019 by top-p 225 (their reading alone: 0.04, 1.0, 7.5, 12).  A
 // row's CTAs spend some 50,000 cycles on a cut: 4,500 until the columns are there, 6,000 to 40,000 for passes, 9,500 for
 // each barrier-bound search of a histogram.
 #include "spd_params.cuh"
@@ -493,7 +493,7 @@ __device__ __noinline__ void after_seek() {
   if (threadIdx.x == 0) sh.st.token = at, sh.st.pass = kDone;
 }
 // The bins of the first histogram that hold the cut.  Each CTA looks at a share of them and tells the others.  (With every CTA
-// reading all histograms and two barriers less, 96 rows of 200,019 took 273 us against 251, one of 51,865 34.4 against 32.3.)
+// reading all histograms and two barriers less, 96 rows of 200,019 took 273 us against 251, one of 51,865 34.4 against 32.3, then.)
 template <typename T> __device__ __noinline__ void after_count() {
   Shared& sh = shared();
   State& st = sh.st;
