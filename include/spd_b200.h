@@ -392,7 +392,8 @@ int spd_cross_attn_packed(const void* q, int64_t q_stride_t, int64_t q_stride_h,
  *   (at least one); of these min_p > 0 leaves those with x >= m + t log(min_p) (at least one).
  *   The token is the first column, by its place, at which the weight of what is left so far passes uniforms[r] times
  *   all of it.
- * Decisions are those of fp64 arithmetic; ties and order never depend on scheduling.  out int64 [rows]; logprobs fp32
+ * Decisions are those of fp64 arithmetic with weights in units of 2^-44 of the largest (columns that weigh less are not
+ * drawn); ties and order never depend on scheduling.  out int64 [rows]; logprobs fp32
  * [rows] or NULL: log softmax(x) of the token over the columns that are not skipped (temperature 1, nothing cut). */
 int spd_sample_rows(const void* x, int rows, int cols, int64_t ld, const uint8_t* skip_mask, const float* uniforms,
                     const float* temperature, float temperature_all, const int32_t* top_k, int top_k_all,

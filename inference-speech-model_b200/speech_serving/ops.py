@@ -676,8 +676,9 @@ def sample_rows(
     place); of these, in that order, top_p < 1 leaves those before which less than top_p of their weight lies; of
     these min_p > 0 leaves those with x >= m + temperature log(min_p); each leaves at least one.  The token is the
     first column, by its place, at which the weight of what is left so far passes uniforms[r] times all of it, as
-    fp64 arithmetic decides.  A temperature <= 0 picks the first largest column, and so does a row whose largest value
-    is not finite (a NaN wins), as ``argmax_rows`` does.
+    fp64 arithmetic decides, but for columns of less than 2^-44 of the largest one's weight, which are not drawn.
+    A temperature <= 0 picks the first largest column, and so does a row whose largest value is not finite (a NaN
+    wins), as ``argmax_rows`` does.
 
     Returns int64 [rows].  ``logprobs`` (float32 [rows]), if given, receives the tokens' log-probabilities under
     softmax(x) over the columns not skipped (temperature 1, nothing cut)."""

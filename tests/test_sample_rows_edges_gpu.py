@@ -92,3 +92,14 @@ def test_refusals():
     with pytest.raises(RuntimeError, match="at most"):
         ops.sample_rows(torch.zeros(1, (1 << 19) + 8, device=DEV).half(), u[:1])
     torch.cuda.synchronize()
+
+
+def test_columns_that_weigh_next_to_nothing_are_not_drawn():
+    """Not even by a random number of zero: weights are in units of 2^-44 of the largest."""
+    x = torch.full((3, 600), -100.0)
+    x[0, 300], x[1, 599], x[2, 1] = 0.0, 0.0, 0.0
+    x[2, 0] = -28.0  # 6.9e-13 of it: 12 units
+    u = torch.tensor([0.0, 0.0, 0.0], device=DEV)
+    for k, p in ((0, 1.0), (512, 1.0), (513, 1.0), (0, 0.99)):
+        want = [300, 599, 0 if p == 1.0 else 1]
+        assert ops.sample_rows(x.to(DEV), u, 1.0, k, p).tolist() == want
