@@ -150,13 +150,20 @@ __global__ void __launch_bounds__(kThreads, 3) own_attn_kernel(const OwnParams p
   };
   look_up();
 
-  // ---- the group whose prefix this sequence shares
+  // ---- the group whose prefix this sequence shares (by 32 starts at once: 1,024 groups of two 249 -> 187 us)
   int group = -1;
+  {
+    int first = 0, n = p.G;  // the groups that it may be
 #pragma unroll 1
-  for (int first = 0; first < p.G && group < 0; first += 32) {
+    while (n > 32) {  // 32 starts a step, the last that is not past it
+      const int every = (n + 31) / 32, i = lane * every;
+      const int before = __popc(__ballot_sync(0xffffffffu, i < n && p.cu_groups[first + i] <= b));
+      const int skip = max(before - 1, 0) * every;
+      first += skip;
+      n = min(every, n - skip);
+    }
     const int i = first + lane;
-    const bool in = i < p.G && p.cu_groups[i] <= b && b < p.cu_groups[i + 1];
-    const uint32_t hit = __ballot_sync(0xffffffffu, in);
+    const uint32_t hit = __ballot_sync(0xffffffffu, lane < n && p.cu_groups[i] <= b && b < p.cu_groups[i + 1]);
     if (hit) group = first + __ffs(hit) - 1;
   }
   if (group >= 0 && p.prefix_lens[group] <= 0) group = -1;

@@ -243,7 +243,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     int mine = cost_of(lane);  // of group `lane`
     unsigned sum = (unsigned)mine;
     bool over = false;
-#pragma unroll 1
+#pragma unroll 4
     for (int i = lane + 32; i < p.G; i += 32) {
       sum += (unsigned)cost_of(i);
       over |= sum >> 31;

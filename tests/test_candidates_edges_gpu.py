@@ -421,3 +421,18 @@ def test_offsets_past_32_bits():
     lens, cq = torch.tensor([2000, 1999], dtype=torch.int32, device=DEV), cu([5, 1]).to(DEV)
     got = ops.cross_attention_packed(q, kv, kv, lens, cq, lens * 0 + torch.tensor([999, 998], dtype=torch.int32, device=DEV))
     assert torch.equal(got, ops.cross_attention_packed(q, *[kv[998:].flip(0).contiguous()] * 2, lens, cq))
+
+
+@pytest.mark.parametrize("groups", [31, 32, 33, 300, 1100])
+def test_many_groups(groups):
+    """More groups than a warp looks at at once, some of them empty, and sequences before, behind and in them."""
+    g = torch.Generator().manual_seed(groups)
+    members = torch.randint(0, 3, (groups,), generator=g).tolist()
+    members[0], members[-1] = 1, 2
+    pre = torch.randint(0, 40, (groups,), generator=g).tolist()
+    mine = torch.randint(0, 4, (sum(members),), generator=g).tolist()
+    c = Prefix(groups, members, pre, mine, 4, 2, 64, torch.float16, bs=8)
+    near(prefix(*c.args()), c.want())
+    a = c.args()
+    a[5] = (a[5] + 1).clamp(max=sum(members))
+    near(prefix(*a), c.want(first=1))
