@@ -27,8 +27,8 @@
 //   belong to a block id out of range.
 // * Every wait is bounded; a CTA whose wait runs out lets its copies land before it exits.
 // Measured on a B200, in CUDA graphs, with the join: 32 requests of 5 beams over up to 1,500 positions (20 heads of 64,
-// bf16) 53 us, 0.45 of a copy's rate; 24 prompts of up to 448 tokens over them (fp16) 68 us, where the products alone would
-// take 20 and the chain of a tile (scores, maximum, exponentials, weights, product) sets the pace; one request 16 us,
+// bf16) 52 us, 0.45 of a copy's rate; 24 prompts of up to 448 tokens over them (fp16) 68 us, where the products alone would
+// take 20 and the chain of a tile (scores, maximum, exponentials, weights, product) sets the pace; one request 14 us,
 // of which 4 are the start and 3 to 4 the join.
 #include "spd_tc_attn.cuh"
 
