@@ -475,8 +475,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int it = 0; next_item(it); ++it) {
         const Steps st(w, x);
         const int q = w.pair ? x : w.q_slot;
-        // Each barrier's phases must be seen one by one.  Q: of both tiles, whoever uses them.  Rings: the one that
-        // only the other stream used is known to have landed once that stream's warp is here.
+        // Each barrier's phases must be seen one by one.  Q: of both tiles, whoever uses them; a tile that this stream
+        // does not use it gives back itself, once it has seen it.  (Were it given back by the stream that uses it, the
+        // next copy could land, and a phase pass, before this warp came to look.)  Rings: the one that only the
+        // other stream used is known to have landed once that stream's warp is here.
         if (w.pair && single_before) {
           if (lane == 0) mbar_arrive(&meet);
           if (!wait(&meet, (uint32_t)meets++)) break;
@@ -484,7 +486,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         single_before = !w.pair;
 #pragma unroll 1
         for (int r = w.pair ? 0 : q; r <= (w.pair ? 1 : q) && ok; ++r) {
-          wait(&q_full[r], q_odd >> r);
+          if (wait(&q_full[r], q_odd >> r) && lane == 0 && (r != q || st.first >= st.n)) mbar_arrive(&q_empty[r]);
           q_odd ^= 1u << r;
         }
         int k_at = w.pair ? u0 : x ? u1 : u0, v_at = w.pair ? u1 : k_at + 1;  // of the step's tiles in their rings
@@ -548,10 +550,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                          kv_desc + (uint64_t)((k_ring * C::kStages + k_slot) * kTile16 + c * kBox16), idesc_s, c != 0);
               umma_commit(&s_full[x]);
               give_back(&kv_empty[k_ring][k_slot]);
-              if (t + st.by == st.last) {
-                umma_commit(&q_empty[q]);
-                if (w.pair || st.n == 1) mbar_arrive(&q_empty[q]);  // for the stream that does not use it
-              }
+              if (t + st.by == st.last) umma_commit(&q_empty[q]);
             } else {
               umma_commit(&o_full[x]);
             }
