@@ -159,11 +159,9 @@ template <typename T> struct Weight {
     const float d = x - m;  // <= 0
     // y = n + f + rest: f is exact (no contraction of its product), the rest what roundings left over
     const float y = __fmul_rn(d, hi), n = fmaxf(rintf(y), -63.f), f = fmaxf(y - n, -1.f);
-    float rest = fmaf(d, lo, fmaf(d, hi, -y));
-    if constexpr (sizeof(T) == 4) {  // (of 16-bit values the subtraction rounds off next to nothing)
-      const float b = d - x, a = d - b;
-      rest = fmaf((x - a) - (m + b), hi, rest);
-    }
+    // (what the subtraction rounds off matters for 16-bit values too: of small ones beside m = 8 it is up to 2^-22)
+    const float b = d - x, a = d - b;
+    const float rest = fmaf((x - a) - (m + b), hi, fmaf(d, lo, fmaf(d, hi, -y)));
     // 2^f = 1 + f ln 2 + f^2 s(f), s a polynomial that interpolates (2^f - 1 - f ln 2) / f^2 at the Chebyshev nodes of
     // [-1/2, 1/2] (4e-10), and 2^rest = 1 + rest ln 2.  f ln 2 in two parts, and what is added to 1 in units of 2^-30.
     // Off by less than 2^-26.4 of itself (the half steps of s, f^2, the sum that holds the small terms, over 2^-1/2;
