@@ -69,7 +69,7 @@ constexpr int BM = 128;  // rows of a tile
 constexpr int BN = 128;  // keys of a step
 constexpr int kThreads = 384;
 constexpr int kItems = 4;       // pieces known ahead, and the present one
-constexpr int kHoles = 16;      // steps whose missing pages are remembered: more than can be under way
+constexpr int kHoles = 8;       // steps whose missing pages are remembered, of each kind (see Holes)
 // What an item costs: so much, and so much a step of it.
 constexpr int kCostItem = 4, kCostPair = 3, kCostSingle = 2;
 // of a CTA, at least (one request of 5 beams 13.0 us in place of 14.0 with 12, of 8 candidates 12.7 of 12.4; with 20 17 us each)
@@ -88,6 +88,7 @@ template <int DP> struct Cfg {
   static constexpr int kSoftmaxRegs = 208, kOtherRegs = 88;
   static constexpr int kAllRegs = 256 * kSoftmaxRegs + 128 * kOtherRegs;
   static_assert(kO + 2 * DP <= kTmemCols, "scores and outputs fit in TMEM");
+  static_assert(kStages + 2 <= kHoles, "an entry is free when it is written");
 };
 
 __device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, int x, int y, int z, int w, uint64_t* bar,
@@ -163,6 +164,24 @@ struct Steps {
       : n(w.j1 - w.j0), first(w.pair ? 0 : x), by(w.pair ? 1 : 2), last(w.pair ? n - 1 : n - 1 - ((n - 1 - x) & 1)) {}
 };
 
+// Where the missing pages of a step are remembered: single tiles' steps by stream, steps of two tiles in a third place.
+// The streams of a single tile do not wait for one another before its end, so neither may use the other's entries.  An
+// entry is read for the last time before its step's product of weights is issued.  A loader writes one when it
+// has loaded the step before, that is, when a tile kStages further back has been given back: of single tiles that
+// is a V tile, so kStages / 2 + 2 entries are in use; of two tiles' steps a K tile, given back by both streams after the
+// product of the step before it, so kStages + 2 are.
+struct Holes {
+  int own = 0, pair = 0;  // steps before this item
+  __device__ __forceinline__ int at(const Piece& w, int x, int t) const {
+    return w.pair ? 2 * kHoles + (pair + t) % kHoles : x * kHoles + (own + (t >> 1)) % kHoles;
+  }
+  __device__ __forceinline__ void next(const Piece& w, int x) {
+    const int n = w.j1 - w.j0;
+    if (w.pair) pair += n;
+    else own += (n + 1 - x) >> 1;
+  }
+};
+
 // A row's output in TMEM times f (a row a lane).
 template <int DP>
 __device__ __forceinline__ void rescale(uint32_t o_col, float f) {
@@ -187,7 +206,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ Piece items[kItems];
   __shared__ int gave_up;     // a wait has run out
   __shared__ int left[2][2];  // tiles that a loader copied into its ring ([1][1]: Q tiles), at its end
-  __shared__ volatile uint32_t holes[kHoles];  // pages of a step whose keys are left out, a bit each
+  __shared__ volatile uint32_t holes[3 * kHoles];  // pages of a step whose keys are left out, a bit each
   __shared__ float2 other[BM];                 // maximum and sum of the second stream's rows
   __shared__ __align__(8) uint64_t item_full[kItems], item_empty[kItems], other_full, other_empty;
   __shared__ __align__(8) uint64_t kv_full[2][C::kStages], kv_empty[2][C::kStages];
@@ -207,7 +226,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int Gq = p.Hq / p.Hkv;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (warp == 1) tmem_alloc(&tmem_slot, C::kTmemCols);
-  if (tid < kHoles) holes[tid] = 0;
+  if (tid < 3 * kHoles) holes[tid] = 0;
   if (tid == 0) {
     gave_up = 0;
     left[0][0] = left[0][1] = left[1][0] = left[1][1] = 0;
@@ -304,7 +323,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint64_t policy = l2_policy_evict_first();  // (the code, the pieces and the tables stay in L2)
       const int bl7 = p.bs_log2 + 7;  // log2 of a page's bytes in one box
       unsigned char* const ring = kv_tiles + x * C::kStages * C::kTile;
-      int used = 0, hole_at = 0;
+      int used = 0;
+      Holes hole;
       uint32_t q_seen = 0, q_odd = 0;  // of the Q tiles, a bit each: loaded before, an odd number of times
 
       // the share [lo, hi) of all items laid end to end: the present item starts at `at`
@@ -406,7 +426,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (bad) set_error(p.err, SPD_DEVERR_BLOCK_ID);
             bytes = (uint32_t)((pages - __popc(gone)) * C::kBoxes) << bl7;
             // known before K is armed, to all that wait for it
-            if (lane == 0 && !(w.pair && x)) holes[(hole_at + t) % kHoles] = gone;
+            if (lane == 0 && !(w.pair && x)) holes[hole.at(w, x, t)] = gone;
           }
 #pragma unroll 1
           for (int kind = w.pair ? x : 0; kind <= (w.pair ? x : 1); ++kind) {
@@ -435,7 +455,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           id = id_next;
           if (x == 0 && more && dealt < it + 3) deal();  // two ahead, between copies
         }
-        hole_at += st.n;
+        hole.next(w, x);
       }
       if (p.cta_desc && x == 0 && blockIdx.x == 0)  // what the lengths and slots have wrong
 #pragma unroll 1
@@ -462,7 +482,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                      v_desc = smem_desc_mn(kv_tiles, C::kBox);
       const bool leader = elect_one();
       uint32_t q_odd = 0, p_odd = 0, o_odd = 1;  // phases (q: a bit each)
-      int hole_at = 0, u0 = 0, u1 = 0;           // tiles of the two rings before this item
+      int u0 = 0, u1 = 0;                        // tiles of the two rings before this item
+      Holes hole;
       bool single_before = false;
       int turns = 0, meets = 0;  // steps of two tiles; times that the two warps have met
       // A tile is given back only if its products were issued: after a wait that gave up its copy may still be in
@@ -505,7 +526,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           } else {
             const int keys = w.len - (w.j0 + t) * BN;
             if (!wait(&kv_full[v_ring][v_slot], (uint32_t)(v_at / C::kStages))) break;
-            const uint32_t gone = holes[(hole_at + t) % kHoles];
+            const uint32_t gone = holes[hole.at(w, x, t)];
             if (keys < BN || gone) {
               // A weight of zero does not silence an infinity or a NaN: rows that do not count become zero.  (Of two
               // tiles of rows over one V tile both streams do so.)
@@ -565,7 +586,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         u0 += w.pair ? st.n : (st.n + 1) & ~1;
         u1 += w.pair ? st.n : st.n & ~1;
-        hole_at += st.n;
+        hole.next(w, x);
       }
       if (!ok) gave_up = 1;
       if (leader) umma_commit(&done);
@@ -581,7 +602,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t s_col = tmem + lanes + x * BN, o_col = tmem + lanes + C::kO + x * DP;
     const int row_tok = row / Gq, row_head = row % Gq;
-    int s_use = 0, others = 0, hole_at = 0;
+    int s_use = 0, others = 0;
+    Holes hole;
     uint32_t o0 = 0, o1 = 0;  // outputs completed before, of each stream
     if (p.out) {  // queries of groups without keys: zeros
       const int per = p.Hq * p.D / 8;
@@ -619,7 +641,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc_fence_after();
         uint32_t s[128];
         const int seen = w.len - (w.j0 + t) * BN;
-        const uint32_t gone = holes[(hole_at + t) % kHoles];
+        const uint32_t gone = holes[hole.at(w, x, t)];
         const bool edge = seen < BN || gone;
         if (few) {
           tmem_ld_16x256b_x8(s_col, s);
@@ -739,7 +761,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         l += t2.x + t2.y;
       }
       if (!ok) break;
-      hole_at += n;
+      hole.next(w, x);
       if (few) {  // back to a row a lane
 #pragma unroll
         for (int o = 1; o < 4; o <<= 1) {

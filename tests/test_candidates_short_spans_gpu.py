@@ -5,6 +5,7 @@ import pytest
 import torch
 
 from int4_reference import cu
+from speech_serving import _native as N
 from speech_serving import ops
 from test_candidates_gpu import DEV, EXPONENTIAL, UNIT
 
@@ -69,3 +70,33 @@ def test_prefixes_of_short_and_long_spans(kind, dtype, D, bs):
     for _ in range(40):
         assert torch.equal(ops.shared_prefix_decode_attention(*args, error_word=word), first)
     assert ops.read_error_word(word) == 0
+
+
+@pytest.mark.parametrize("kind", ["one tile", "two tiles", "both"])
+@pytest.mark.parametrize("dtype,D,bs", [(torch.float16, 64, 8), (torch.bfloat16, 128, 32)])
+def test_missing_pages_of_many_spans(kind, dtype, D, bs):
+    """Block ids out of range in spans of odd and even numbers of steps, beside spans without any: each step leaves out its own
+    pages and no other's."""
+    requests, T = 120, 3200
+    q, kv, lens, n, _ = spans(D + 2, kind, dtype, D, requests, T=T)
+    g = torch.Generator().manual_seed(8)
+    blocks = 8 * T // bs
+    pool = kv.transpose(0, 1).transpose(2, 3).reshape(2, blocks, bs, 2, D).contiguous()
+    table = torch.randint(0, blocks, (requests, T // bs), generator=g)
+    gone = (torch.rand(requests, T // bs, generator=g) < 0.3) & (torch.arange(requests) % 2 == 0)[:, None]
+    gone[:, 0] = False
+    wild = torch.where(torch.rand(table.shape, generator=g) < 0.5, torch.tensor(-1), torch.tensor(blocks))
+    B, word = q.shape[0], torch.zeros(1, dtype=torch.int32, device=DEV)
+    none = torch.zeros(B, 0, dtype=torch.int32, device=DEV), torch.zeros(B, dtype=torch.int32, device=DEV)
+    args = (q, pool[0], pool[1], torch.where(gone, wild, table).to(DEV, torch.int32), lens.to(DEV, torch.int32),
+            cu(n.tolist()).to(DEV), *none)
+
+    def keys(r):
+        left = (~gone[r]).repeat_interleave(bs)[: lens[r]].to(DEV)
+        return pool[:, table[r].to(DEV)].flatten(1, 2)[:, : lens[r]][:, left].transpose(1, 2)
+
+    first = ops.shared_prefix_decode_attention(*args, error_word=word)
+    check(first, q, keys, n)
+    for _ in range(40):
+        assert torch.equal(ops.shared_prefix_decode_attention(*args, error_word=word), first)
+    assert ops.read_error_word(word) == N.SPD_DEVERR_BLOCK_ID
