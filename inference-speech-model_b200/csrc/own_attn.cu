@@ -293,7 +293,9 @@ __global__ void __launch_bounds__(kThreads, 3) own_attn_kernel(const OwnParams p
   for (int j = 0; j < kTiles; ++j) {
     const int d = 8 * j + 2 * t;
     if constexpr (SPLIT) {
-      *reinterpret_cast<float2*>(mine + g * DP + d) = make_float2(o[j][0] + o[j][2], o[j][1] + o[j][3]);
+      // (over an infinite value a remainder, of any sign or zero, says nothing that its weight has not said)
+      auto finite = [](float x) { return fabsf(x) < INFINITY ? x : 0.f; };
+      *reinterpret_cast<float2*>(mine + g * DP + d) = make_float2(o[j][0] + finite(o[j][2]), o[j][1] + finite(o[j][3]));
     } else {
       *reinterpret_cast<float2*>(mine + g * DP + d) = make_float2(o[j][0], o[j][1]);
       *reinterpret_cast<float2*>(mine + (g + 8) * DP + d) = make_float2(o[j][2], o[j][3]);
