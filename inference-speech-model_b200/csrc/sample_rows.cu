@@ -90,7 +90,7 @@ struct State {
   int token;
   bool by_count, exact, z_due;
   bool sure, missed;      // the cut's bins are taken from certain bounds; they were not, and did not hold it
-  float m, xmin, hi, lo;  // the largest value, the least that min-p leaves, log2(e) / t in two parts
+  float m, xmin, hi, lo;  // the largest value, the least that min-p leaves, 2 log2(e) / t in two parts
   float xt, xt0, xt_k;    // what is left: values above xt, and the first `ties` columns that have it;
   int ties, ties0, ties_k;  // as the cut under way found it; as top-k left it
   // the cut under way: bins [first, last] of the first histogram, places [from, to] among them, `shift` bits of a bin's
@@ -148,7 +148,7 @@ __device__ __noinline__ u64 exact_weight(double y) {
   return down < 63 ? (bits + (1ull << (down - 1))) >> down : 0;
 }
 template <typename T> struct Weight {
-  float m, hi, lo;  // the largest value, and log2(e) / t in two parts
+  float m, hi, lo;  // the largest value, and 2 log2(e) / t in two parts
   double temperature;
   bool exact;
   __device__ __forceinline__ explicit Weight(const State& st)
@@ -156,12 +156,12 @@ template <typename T> struct Weight {
   __device__ __forceinline__ u64 operator()(float x) const { return exact ? of<true>(x) : of<false>(x); }
   template <bool EXACT> __device__ __forceinline__ u64 of(float x) const {
     if (EXACT) return exact_weight(((double)x - (double)m) / temperature * 1.4426950408889634074);
-    const float d = x - m;  // <= 0
+    const float h = 0.5f * m, d = fmaf(0.5f, x, -h);  // <= 0: half the distance, which fits where the whole one would not
     // y = n + f + rest: f is exact (no contraction of its product), the rest what roundings left over
     const float y = __fmul_rn(d, hi), n = fmaxf(rintf(y), -63.f), f = fmaxf(y - n, -1.f);
     // (what the subtraction rounds off matters for 16-bit values too: of small ones beside m = 8 it is up to 2^-22)
-    const float b = d - x, a = d - b;
-    const float rest = fmaf((x - a) - (m + b), hi, fmaf(d, lo, fmaf(d, hi, -y)));
+    const float b = fmaf(-0.5f, x, d), a = d - b;
+    const float rest = fmaf(fmaf(0.5f, x, -a) - (h + b), hi, fmaf(d, lo, fmaf(d, hi, -y)));
     // 2^f = 1 + f ln 2 + f^2 s(f), s a polynomial that interpolates (2^f - 1 - f ln 2) / f^2 at the Chebyshev nodes of
     // [-1/2, 1/2] (4e-10), and 2^rest = 1 + rest ln 2.  f ln 2 in two parts, and what is added to 1 in units of 2^-30.
     // Off by less than 2^-26.4 of itself (the half steps of s, f^2, the sum that holds the small terms, over 2^-1/2;
@@ -258,7 +258,10 @@ struct Z {
     if ((threadIdx.x & 31) == 0) shared().z[threadIdx.x >> 5] = z;
   }
 };
-__device__ __forceinline__ int bin_of(float v, float m, float inv) { return (int)fminf((m - v) * inv, (float)(kFirst - 1)); }
+// (half the distance: the whole one may be beyond fp32's range)
+__device__ __forceinline__ int bin_of(float v, float m, float inv) {
+  return (int)fminf(fmaf(-0.5f, v, 0.5f * m) * (2.f * inv), (float)(kFirst - 1));
+}
 __device__ __forceinline__ void put(int bin, unsigned n, u64 w) {
   Shared& sh = shared();
   atomicAdd(&sh.count[bin], n);
@@ -466,7 +469,7 @@ __device__ __noinline__ void after_max() {
     of_warp();
   }
   if (threadIdx.x) return;
-  const double per = 1.4426950408889634 / (double)st.t;
+  const double per = 2.0 * 1.4426950408889634 / (double)st.t;
   st.m = m;
   st.hi = (float)per;
   st.lo = (float)(per - st.hi);
