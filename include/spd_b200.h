@@ -354,7 +354,8 @@ int spd_prompt_attn(const void* q, int64_t q_stride_t, int64_t q_stride_h, const
  *   block_tables int32 [B][max_blocks], context_lens int32 [B]: the sequences' own tokens (<= 0: none)
  *   A sequence without any key gives zeros.  Lengths beyond their table are cut to it (flagged); tokens of a block
  *   whose id is out of range are left out (flagged).
- * fp32 scores, softmax statistics and accumulation; weights of prefix keys are rounded to dtype.
+ * fp32 scores, softmax statistics and accumulation; weights of prefix keys, and those of own keys with more than 8
+ * query heads a key/value head, are rounded to dtype before they meet the values.
  * Requires D % 8 == 0, D <= 128, block_size 8, 16, 32, 64 or 128, Hq / Hkv <= 128, B <= 65536, scale > 0, 16-byte aligned
  * pointers and strides.  The workspace's first header and counter bytes are zero-filled once; every call leaves the
  * counters at zero.  It serves one stream at a time. */
@@ -375,6 +376,7 @@ int spd_shared_prefix_attn(const void* q, int64_t q_stride_t, int64_t q_stride_h
  *   slot_ids int32 [B], or NULL: slot b.  Two requests may share a slot.
  *   A query without any key gives zeros; rows of out that belong to no request are untouched.  A length beyond T is
  *   cut to it (flagged), a slot id out of range leaves its request without keys (flagged).
+ * fp32 scores, softmax statistics and accumulation; weights are rounded to dtype before they meet the values.
  * Requires D % 8 == 0, D <= 128, Hq / Hkv <= 128, scale > 0, 16-byte aligned pointers and strides. */
 size_t spd_cross_attn_packed_workspace_size(int N, int Hq, int Hkv, int D, int device);
 int spd_cross_attn_packed(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k, const void* v,
@@ -394,7 +396,8 @@ int spd_cross_attn_packed(const void* q, int64_t q_stride_t, int64_t q_stride_h,
  *   all of it.
  * Decisions are those of fp64 arithmetic with weights in units of 2^-44 of the largest (columns that weigh less are not
  * drawn); ties and order never depend on scheduling.  out int64 [rows]; logprobs fp32
- * [rows] or NULL: log softmax(x) of the token over the columns that are not skipped (temperature 1, nothing cut). */
+ * [rows] or NULL: log softmax(x) of the token over the columns that are not skipped (temperature 1, nothing cut), by a sum in
+ * fp32, within 2e-6 + 1e-6 of its size. */
 int spd_sample_rows(const void* x, int rows, int cols, int64_t ld, const uint8_t* skip_mask, const float* uniforms,
                     const float* temperature, float temperature_all, const int32_t* top_k, int top_k_all,
                     const float* top_p, float top_p_all, const float* min_p, float min_p_all, int64_t* out,

@@ -8,15 +8,17 @@
 // with short contexts the latency of lengths, table, rows and join.
 // * mma.sync m16n8k16 with the group's heads as its 16 rows: at a row count of 1 to 16 the products are a
 //   small part of the time.  (tcgen05 has 128 rows.)  With up to 8 heads the other 8 rows of the weights hold
-//   their rounding remainders, so that weights keep 16 bits and more at no cost.
+//   their rounding remainders, so that weights keep 16 bits and more at no cost.  With more heads all 16 rows are
+//   heads and weights are rounded to the input's type, as span_attn.cu does: 8 heads a CTA would read the keys twice as often.
 // * A CTA takes a chunk of one sequence for one key/value head (16 heads of it), a warp every fourth step of
 //   `kKeys` keys, by cp.async into a ring of its own: any block size, rows of a block out of range as zeros.
-// * It is launched with programmatic dependent launch behind span_attn.cu, runs on what SMs that leaves, and
-//   waits for it only to join.  The chunks of a sequence are joined by the last CTA to arrive, in
-//   their order.
+// * It is launched with programmatic dependent launch behind span_attn.cu, which hides its launch: its CTAs start as
+//   those of the spans leave their SMs (which they fill with registers) and wait for the whole kernel only to join.  The
+//   chunks of a sequence are joined by the last CTA to arrive, in their order.
 // Measured on a B200, in CUDA graphs, with the prefixes' kernel: groups with ragged prefixes and own tokens 65 us (36 for
 // their bytes at a copy's rate), two groups of 64 over prefixes of 32,000 tokens 132 (83), one request's candidates
-// 12: some 8 us of dependent loads (lengths, table, rows, join) and the launches.
+// 12.7: some 8 us of dependent loads (lengths, table, rows, join) and the launches.  By itself, from cold caches: 42 us for
+// the 136 MB of the first (0.50 of a copy), 62 us for the 282 MB of the second (0.70).
 #include "spd_tc_attn.cuh"
 
 #include <algorithm>

@@ -4,9 +4,10 @@
 //   than p of their weight lies, min-p the ones with x >= m + t log(min_p); the token is the first column, by
 //   its place, at which the weight left so far passes u times all of it.
 //
-// What bounds it: a row is read once from memory, 2 or 4 bytes a column, and again from shared memory by each later pass;
-// the passes' instructions, some 60 a column in all, are what takes the time, and for one row the clusters' barriers
-// between them.  Rows are not sorted:
+// What bounds it: a row is read once from memory, 2 or 4 bytes a column, and again from shared memory by each later pass.
+// What takes the time is that a row's passes follow one another, with clusters' barriers and remote reads between them, in the
+// few rows that the SMs hold at once (37 of the last case below: three waves of them).  The passes' instructions, some 60
+// a column in all, would be 31 of its 224 us.  Rows are not sorted:
 // * A cluster of up to 8 CTAs shares a row.  A cut (the k-th largest, or the value at which the weight reaches p) is
 //   found by histograms.  The first counts columns by their distance from m (one atomic a column).  For the k-th largest
 //   the cut lies in one of its bins.  For p each bin's weight is known to within 2 %, and
@@ -27,8 +28,9 @@
 // * A CTA's columns lie in its shared memory, and what is known of the row beside them: passes are functions that are
 //   called, so that none holds another's registers.  (In one function the state went to local memory, whose traffic
 //   was twice that of the columns: 87 us in place of 64 for the second case below, then.)
-// Measured on a B200, in CUDA graphs: one fp32 row of 51,865 columns by top-p 32 us, 64 fp16 rows of them by all settings 46,
-// 192 bf16 rows of 128,257 by top-k 99, 96 fp32 rows of 200,019 by top-p 225 (their reading alone: 0.04, 1.0, 7.5, 12).  A
+// * The log-probability's sum is fp32, of special-function exponentials: some 10^-7 off.  No decision uses it.
+// Measured on a B200, in CUDA graphs: one fp32 row of 51,865 columns by top-p 33 us (29 to 37, by the row), 64 fp16 rows of
+// them by all settings 47, 192 bf16 rows of 128,257 by top-k 100, 96 fp32 rows of 200,019 by top-p 224 (their reading alone: 0.04, 1.0, 7.5, 12).  A
 // row's CTAs spend some 50,000 cycles on a cut: 4,500 until the columns are there, 6,000 to 40,000 for passes, 9,500 for
 // each barrier-bound search of a histogram.
 #include "spd_params.cuh"

@@ -26,10 +26,15 @@
 //   step ahead.  The issuing warp also zeroes the rows of V tiles that are past the span's end or
 //   belong to a block id out of range.
 // * Every wait is bounded; a CTA whose wait runs out lets its copies land before it exits.
+// * Weights go into P V in the input's type, off by half a step of it (2^-8 bf16, 2^-11 fp16); maxima, sums and outputs are
+//   fp32, and the sums take the weights unrounded.  Results are 1.3 times as far from 64 bits as with weights of
+//   32 bits (0.0022 of 0.0017 relative in bf16, 0.00028 of 0.00021 in fp16: the output's own rounding is the rest).  The
+//   remainders would take a second P V, and a second conversion and store of every weight in the chain that sets the pace.
 // Measured on a B200, in CUDA graphs, with the join: 32 requests of 5 beams over up to 1,500 positions (20 heads of 64,
 // bf16) 52 us, 0.45 of a copy's rate; 24 prompts of up to 448 tokens over them (fp16) 68 us, where the products alone would
-// take 20 and the chain of a tile (scores, maximum, exponentials, weights, product) sets the pace; one request 14 us,
-// of which 4 are the start and 3 to 4 the join.
+// take 20 and the chain of a tile (scores, maximum, exponentials, weights, product) sets the pace; one request of 5 beams 13.0 to
+// 13.7 us, of which 4 are the start and 3 to 4 the join.  Two prefixes of 32,000 tokens for 64 candidates each (bf16, 8 key/value
+// heads of 128): 83 us of this kernel alone, 27 steps of two tiles a CTA at some 5,800 cycles, of which the products are 2,050.
 #include "spd_tc_attn.cuh"
 
 #include <algorithm>
@@ -72,7 +77,7 @@ constexpr int kItems = 4;       // pieces known ahead, and the present one
 constexpr int kHoles = 8;       // steps whose missing pages are remembered, of each kind (see Holes)
 // What an item costs: so much, and so much a step of it.
 constexpr int kCostItem = 4, kCostPair = 3, kCostSingle = 2;
-// of a CTA, at least (one request of 5 beams 13.0 us in place of 14.0 with 12, of 8 candidates 12.7 of 12.4; with 20 17 us each)
+// of a CTA, at least (one request of 5 beams 13.0 to 13.7 us, with 12 14.0; of 8 candidates 12.7, with 12 12.4; with 20 17 us each)
 constexpr int kMinShare = 8;
 
 template <int DP> struct Cfg {
